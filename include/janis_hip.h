@@ -602,6 +602,120 @@ JH_API int jh_embed_norm_prepare(jh_ctx *ctx, const int32_t *ids, const uint32_t
                           float *h, void *norm_out, float *norm_stats, int rope_dims, float rope_base,
                           float rope_scale, int64_t pos, float *rope_cs);
 
+/* ---- a paged key/value cache for batches of requests ------------------------- *
+ * KVCache (qwen/cache.go) holds one sequence in one contiguous buffer. A program
+ * that serves many requests at once keeps their keys and values in pages instead:
+ *   k_pages, v_pages  [n_pages, n_kv_heads, page_size, head_dim] (JH_BF16 or
+ *                     JH_F16), page_stride elements from one page to the next
+ *                     (n_kv_heads * page_size * head_dim when dense; more where
+ *                     keys and values alternate in one buffer); page_size a power
+ *                     of two up to 65536, n_pages * page_size < 2^31
+ *   block_tables      int32 [n_req, max_blocks]: request r's key j lies in page
+ *                     block_tables[r, j / page_size], row j % page_size (its slot
+ *                     is page * page_size + row). Requests may share pages.
+ *   row_starts        int32 [n_req + 1]: request r's new tokens are the rows
+ *                     row_starts[r] .. row_starts[r+1] - 1 of the step's batch of
+ *                     n_rows rows (never decreasing; the rows from
+ *                     row_starts[n_req] on belong to nobody)
+ * all in device memory, so that one captured graph serves steps of any lengths.
+ * A step is jh_paged_plan once and, per layer, the q/k/v product
+ * (jh_quant_matmul), jh_paged_qk_norm_rope_append and jh_paged_attention. The
+ * reference has no counterpart: it decodes one session at a time. */
+
+/* *status of jh_paged_plan. */
+enum {
+    JH_PLAN_OK = 0,
+    JH_PLAN_LENGTHS = 1, /* a length below 0, or past max_blocks pages */
+    JH_PLAN_ROWS = 2,    /* more new tokens than n_rows */
+    JH_PLAN_PAGES = 3,   /* not enough free pages (or *free_count outside [0, n_pages]) */
+    JH_PLAN_TABLE = 4    /* a finished request's table, or the stack, holds a number outside
+                            [0, n_pages), or more pages come back than the stack has room for */
+};
+
+/* The bookkeeping of one step, in one launch. Per request r, new_lens[r] >= 0
+ * tokens join its kv_lens[r] keys; new_lens[r] < 0 says that it is finished.
+ * First the pages of the finished requests go onto the stack free_pages[0 ..
+ * *free_count) (request by request, in their tables' order), then the others take
+ * what their new tokens need off its top (again in order) into block_tables.
+ *   block_tables    [n_req, max_blocks], only the new pages' entries are written
+ *   free_pages      [n_pages], in place
+ *   kv_lens_out     [n_req]: kv_lens + new_lens, 0 for finished requests; may be kv_lens
+ *   free_count_out  [1]; may be free_count
+ *   row_starts      [n_req + 1]: running sums of the new tokens
+ *   positions       [n_rows]: each new token's position (kv_lens[r] + i), -1 behind the last
+ *   slots           [n_rows]: each new token's slot, -1 behind the last
+ *   status          [1]: JH_PLAN_OK, or why the step cannot be done (the first of the
+ *                   reasons above that applies). Then nothing was planned:
+ *                   block_tables and free_pages are as they were, kv_lens_out and
+ *                   free_count_out repeat their inputs, row_starts is all 0,
+ *                   positions and slots all -1, so that the step's other calls do
+ *                   nothing. With JH_CHECK_INDICES it is read back and is
+ *                   JH_ERR_INVALID here.
+ * Apart from the two aliases, outputs overlap neither inputs nor each other.
+ * n_req up to 2048 (JH_ERR_UNSUPPORTED beyond). */
+JH_API int jh_paged_plan(jh_ctx *ctx, const int32_t *new_lens, const int32_t *kv_lens, int64_t n_req,
+                         int64_t n_rows, int64_t page_size, int32_t *block_tables, int64_t max_blocks,
+                         int32_t *free_pages, int64_t n_pages, const int32_t *free_count,
+                         int32_t *kv_lens_out, int32_t *free_count_out, int32_t *row_starts,
+                         int32_t *positions, int32_t *slots, int32_t *status);
+
+/* The middle of Attention.ForwardCached (qwen/attention.go:101-122) for a batch of
+ * rows at positions of their own: from row t of the q/k/v product, q heads (RMS
+ * norm with q_norm_w, rotation by positions[t]) to q_out, k heads (k_norm_w, the
+ * same rotation) and v heads to slot slots[t] of the pages. A row whose slot is
+ * outside [0, n_pages * page_size) is skipped whole: nothing of it is written, its
+ * row of q_out stays as it was (with JH_CHECK_INDICES a slot other than -1
+ * outside is JH_ERR_INVALID). Two rows of one slot leave either one's key and value.
+ *   qkv       [n_rows, (n_heads + 2 n_kv_heads) * head_dim] of qkv_dtype (JH_BF16 or
+ *             JH_F32), qkv_stride elements from one row to the next
+ *   q_norm_w, k_norm_w  [head_dim] of w_dtype (JH_BF16, JH_F16 or JH_F32), or NULL: no norm
+ *   rotation  pairs (i, i + head_dim/2) by positions[t] * rope_scale * inv_i, inv_i =
+ *             rope_base^(-2i/head_dim), or 1 / rope_freqs[i] (fp32 [head_dim/2]) when
+ *             given; none where rope_freqs is NULL and rope_base 0. Angles are held in
+ *             double (jh_rope rounds them to fp32, which at position 10^5 is up to 0.004
+ *             of an angle off).
+ *   q_out     [n_rows, n_heads, head_dim] of the pages' dtype
+ * n_heads may be 0 (keys and values only; q_out unused). head_dim 64, 128 or 256.
+ * qkv, q_out and the pages 16-byte aligned, qkv_stride and page_stride multiples of
+ * 8. Norms and rotation in fp32, each result rounded once to the pages' dtype. */
+JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype qkv_dtype, int64_t n_rows,
+                                        int64_t qkv_stride, int64_t n_heads, int64_t n_kv_heads,
+                                        int64_t head_dim, const void *q_norm_w, const void *k_norm_w,
+                                        jh_dtype w_dtype, float eps, float rope_base, float rope_scale,
+                                        const float *rope_freqs, const int32_t *positions,
+                                        const int32_t *slots, void *k_pages, void *v_pages,
+                                        jh_dtype page_dtype, int64_t n_pages, int64_t page_size,
+                                        int64_t page_stride, void *q_out);
+
+/* Backend.SDPA (cpu/cpu_attn.go:64-119) of every request's new tokens over its
+ * pages: new token i of a request with n new tokens and kv_lens[r] = L keys (its
+ * own among them) sees keys 0 .. L - n + i, as the reference's offset causal mask
+ * has it; query head h reads kv head h / (n_heads / n_kv_heads). A row that sees no
+ * key (L < n) is zeros. Rows that belong to nobody are left as they were.
+ *   q    [n_rows, n_heads, head_dim] of the pages' dtype, q_stride elements from one
+ *        row to the next
+ *   out  [n_rows, n_heads, head_dim], dense, JH_BF16, JH_F16 or JH_F32
+ * max_new is a hint, the most new tokens any request has (1 in a decode step):
+ * it chooses the kernels, and a wrong one costs time only. head_dim 64, 128 or 256,
+ * scale finite and at least 1e-30; pointers 16-byte aligned, q_stride and
+ * page_stride multiples of 8.
+ * Scores, maxima, sums and results are fp32; the probabilities enter the product
+ * with the values in the pages' dtype: rounded once to it for 16-bit results
+ * (as the result is), as the sum of two such terms for JH_F32 ones and where a
+ * request's new rows of a kv head are at most 32.
+ * Lengths are held to their buffers (kv_lens to max_blocks pages, row_starts to
+ * n_rows); a row that sees a key whose page is outside [0, n_pages) is NaN. With
+ * JH_CHECK_INDICES those are JH_ERR_INVALID before the launch. Keys are split over
+ * blocks where rows are few, and the parts joined in a fixed order: the same
+ * call gives the same bits. The parts lie in the context's workspace. */
+JH_API int jh_paged_attention(jh_ctx *ctx, const void *q, int64_t q_stride, const void *k_pages,
+                              const void *v_pages, jh_dtype page_dtype, int64_t n_pages,
+                              int64_t page_size, int64_t page_stride, const int32_t *block_tables,
+                              int64_t max_blocks, const int32_t *row_starts, const int32_t *kv_lens,
+                              int64_t n_req, int64_t n_rows, int64_t max_new, int64_t n_heads,
+                              int64_t n_kv_heads, int64_t head_dim, float scale, void *out,
+                              jh_dtype out_dtype);
+
 #ifdef __cplusplus
 }
 #endif

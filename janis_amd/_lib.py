@@ -20,6 +20,7 @@ JH_OP_ADD, JH_OP_MUL, JH_OP_SILU, JH_OP_SILU_MUL = range(4)  # jh_op
 JH_PRO_NONE, JH_PRO_RMSNORM, JH_PRO_SILU_MUL, JH_PRO_NORMED = range(4)  # jh_prologue
 JH_EPI_STORE, JH_EPI_RESID, JH_EPI_SWIGLU, JH_EPI_RESID_NORM = range(4)  # jh_epilogue
 JH_NORM_STATS = 1024
+JH_PLAN_OK, JH_PLAN_LENGTHS, JH_PLAN_ROWS, JH_PLAN_PAGES, JH_PLAN_TABLE = range(5)  # jh_paged_plan's status
 
 EXPORTS = [
     "jh_version", "jh_create", "jh_destroy", "jh_last_error", "jh_device_info",
@@ -30,6 +31,7 @@ EXPORTS = [
     "jh_attention_decode", "jh_rope_table", "jh_norm_prepare", "jh_copy_strided", "jh_scatter_rows",
     "jh_softmax", "jh_mean", "jh_scalar", "jh_check_finite", "jh_attention_decode_noalloc",
     "jh_qkv_attention_decode", "jh_embed_norm_prepare", "jh_set_wait_limit",
+    "jh_paged_plan", "jh_paged_qk_norm_rope_append", "jh_paged_attention",
 ]
 
 _lib = None
@@ -122,6 +124,13 @@ def load() -> ctypes.CDLL:
     L.jh_scalar.argtypes = [c_ctx, i, p, i, i64, f32, p, i]
     L.jh_check_finite.argtypes = [c_ctx, p, i, i64, ctypes.POINTER(i64), ctypes.POINTER(i64)]
     for name in ("jh_softmax", "jh_mean", "jh_scalar", "jh_check_finite"):
+        getattr(L, name).restype = i
+    L.jh_paged_plan.argtypes = [c_ctx, p, p, i64, i64, i64, p, i64, p, i64, p, p, p, p, p, p, p]
+    L.jh_paged_qk_norm_rope_append.argtypes = [c_ctx, p, i, i64, i64, i64, i64, i64, p, p, i, f32, f32, f32, p, p, p,
+                                               p, p, i, i64, i64, i64, p]
+    L.jh_paged_attention.argtypes = [c_ctx, p, i64, p, p, i, i64, i64, i64, p, i64, p, p, i64, i64, i64, i64, i64, i64,
+                                     f32, p, i]
+    for name in ("jh_paged_plan", "jh_paged_qk_norm_rope_append", "jh_paged_attention"):
         getattr(L, name).restype = i
     L.jh_moe_route.argtypes = [c_ctx, p, i, i64, i64, i64, i, p, p]
     L.jh_moe_route.restype = i

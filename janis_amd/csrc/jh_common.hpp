@@ -449,6 +449,54 @@ const char* moe_unsupported(const MoeMlpArgs& a);
 size_t moe_workspace_bytes(const MoeMlpArgs& a);
 Status launch_moe_mlp(const MoeMlpArgs& a, void* workspace, hipStream_t st);
 
+// ---- paged key/value cache (paged.hip) ----
+struct PagedPlanArgs {
+    const int32_t *new_lens, *kv_lens;
+    int n_req, n_rows, page_size;  // page_size a power of two
+    int32_t* tables;
+    int max_blocks;
+    int32_t* free_pages;
+    int n_pages;
+    const int32_t* free_count;
+    int32_t *kv_out, *count_out, *row_starts, *positions, *slots, *status;
+};
+constexpr int kPlanMaxReq = 2048;
+Status launch_paged_plan(const PagedPlanArgs& a, hipStream_t st);
+struct PagedAppendArgs {
+    const void* qkv;
+    int qkv_dt;
+    int n_rows, Hq, Hk, Dh;
+    int64_t qkv_stride;
+    const void *qn_w, *kn_w;  // [Dh] or nullptr
+    int w_dt;
+    float eps, base, scale;   // base 0 without freqs: no rotation
+    const float* freqs;
+    const int32_t *positions, *slots;
+    uint16_t *k, *v;
+    int kv_f16;               // f16 pages (else bf16)
+    int n_slots, page_shift;
+    int64_t page_stride;
+    uint16_t* q_out;
+};
+Status launch_paged_append(const PagedAppendArgs& a, int num_cus, hipStream_t st);
+struct PagedAttnArgs {
+    const uint16_t* q;
+    int64_t q_stride;
+    const uint16_t *k, *v;
+    int f16;                  // f16 q and pages (else bf16)
+    int n_pages, page_shift;
+    int64_t page_stride;
+    const int32_t* tables;
+    int max_blocks;
+    const int32_t *row_starts, *kv_lens;
+    int n_req, n_rows, max_new, Hq, Hk, Dh;
+    float scale;
+    void* out;
+    int out_dt;
+};
+size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus);
+Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, hipStream_t st);
+
 // ---- operators around the products (ops.hip) ----
 // QuantMatmul with transpose = false: y [rows, m.in] = x [rows, m.rows] . Dequantize(W);
 // with idx, the gather form over a stack of n_experts (rows = the slot pairs).

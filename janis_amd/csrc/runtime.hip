@@ -1109,4 +1109,189 @@ int jh_scalar(jh_ctx* c, jh_scalar_op sop, const void* x, jh_dtype x_dtype, int6
     return check_values(c, op, y, y_dtype, n);
 }
 
+namespace {
+
+// What the operators of the paged cache share: the pages' geometry.
+int check_pages(jh_ctx* c, const char* op, jh_dtype dt, int64_t n_pages, int64_t page_size) {
+    if (dt == JH_F32) return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": the pages must be bf16 or f16");
+    if (dt != JH_BF16 && dt != JH_F16) return fail(c, JH_ERR_INVALID, std::string(op) + ": the pages must be bf16 or f16");
+    if (page_size <= 0 || page_size > 65536 || (page_size & (page_size - 1)))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": page_size must be a power of two up to 65536");
+    if (n_pages < 0 || n_pages > 0x7fffffff / page_size)
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": n_pages * page_size must be below 2^31");
+    return JH_OK;
+}
+
+int check_page_heads(jh_ctx* c, const char* op, int64_t n_kv_heads, int64_t head_dim, int64_t page_size,
+                     int64_t page_stride) {
+    if (head_dim != 64 && head_dim != 128 && head_dim != 256)
+        return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": head_dim must be 64, 128 or 256");
+    if (n_kv_heads <= 0 || n_kv_heads > 4096) return fail(c, JH_ERR_INVALID, std::string(op) + ": bad head counts");
+    if (page_stride < n_kv_heads * page_size * head_dim || page_stride % 8 || page_stride > ((int64_t)1 << 40))
+        return fail(c, JH_ERR_INVALID,
+                    std::string(op) + ": page_stride must hold a page's heads and be a multiple of 8");
+    return JH_OK;
+}
+
+// n device int32 on the host (JH_CHECK_INDICES).
+int read_ints(jh_ctx* c, const char* op, const int32_t* p, int64_t n, std::vector<int32_t>& out) {
+    if (int r = checks_not_capturing(c, op)) return r;
+    out.resize((size_t)n);
+    JH_HIP(c, hipMemcpyAsync(out.data(), p, out.size() * sizeof(int32_t), hipMemcpyDeviceToHost, c->stream));
+    JH_HIP(c, hipStreamSynchronize(c->stream));
+    return JH_OK;
+}
+
+}  // namespace
+
+int jh_paged_plan(jh_ctx* c, const int32_t* new_lens, const int32_t* kv_lens, int64_t n_req, int64_t n_rows,
+                  int64_t page_size, int32_t* block_tables, int64_t max_blocks, int32_t* free_pages, int64_t n_pages,
+                  const int32_t* free_count, int32_t* kv_lens_out, int32_t* free_count_out, int32_t* row_starts,
+                  int32_t* positions, int32_t* slots, int32_t* status) {
+    if (int r = enter(c)) return r;
+    const char* op = "jh_paged_plan";
+    if (int r = check_pages(c, op, JH_BF16, n_pages, page_size)) return r;
+    if (n_req < 0 || n_rows < 0 || n_rows > 0x7fffffff || max_blocks < 0 || max_blocks > 0x7fffffff)
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": bad shape");
+    if (n_req > jh::kPlanMaxReq)
+        return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": more than " + std::to_string(jh::kPlanMaxReq) +
+                                               " requests");
+    if (!free_count || !free_count_out || !row_starts || !status || (n_pages > 0 && !free_pages) ||
+        (n_rows > 0 && (!positions || !slots)) ||
+        (n_req > 0 && (!new_lens || !kv_lens || !kv_lens_out || (max_blocks > 0 && !block_tables))))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": null pointer");
+    if (c->checks & JH_CHECK_INDICES)
+        if (int r = checks_not_capturing(c, op)) return r;
+    jh::PagedPlanArgs a{};
+    a.new_lens = new_lens, a.kv_lens = kv_lens;
+    a.n_req = (int)n_req, a.n_rows = (int)n_rows, a.page_size = (int)page_size;
+    a.tables = block_tables, a.max_blocks = (int)max_blocks;
+    a.free_pages = free_pages, a.n_pages = (int)n_pages, a.free_count = free_count;
+    a.kv_out = kv_lens_out, a.count_out = free_count_out, a.row_starts = row_starts;
+    a.positions = positions, a.slots = slots, a.status = status;
+    if (int r = finish(c, jh::launch_paged_plan(a, c->stream), op)) return r;
+    if (c->checks & JH_CHECK_INDICES) {
+        static const char* const why[] = {"", "a length below 0 or past max_blocks pages", "more new tokens than n_rows",
+                                          "not enough free pages", "a page number outside [0, n_pages)"};
+        std::vector<int32_t> st;
+        if (int r = read_ints(c, op, status, 1, st)) return r;
+        if (st[0] != JH_PLAN_OK)
+            return fail(c, JH_ERR_INVALID, std::string(op) + ": nothing planned: " + why[st[0] >= 1 && st[0] <= 4 ? st[0] : 0]);
+    }
+    return JH_OK;
+}
+
+int jh_paged_qk_norm_rope_append(jh_ctx* c, const void* qkv, jh_dtype qkv_dtype, int64_t n_rows, int64_t qkv_stride,
+                                 int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const void* q_norm_w,
+                                 const void* k_norm_w, jh_dtype w_dtype, float eps, float rope_base, float rope_scale,
+                                 const float* rope_freqs, const int32_t* positions, const int32_t* slots, void* k_pages,
+                                 void* v_pages, jh_dtype page_dtype, int64_t n_pages, int64_t page_size,
+                                 int64_t page_stride, void* q_out) {
+    if (int r = enter(c)) return r;
+    const char* op = "jh_paged_qk_norm_rope_append";
+    if (int r = check_act_dtype(c, op, "qkv", qkv_dtype)) return r;
+    if (int r = check_pages(c, op, page_dtype, n_pages, page_size)) return r;
+    if (int r = check_page_heads(c, op, n_kv_heads, head_dim, page_size, page_stride)) return r;
+    if ((q_norm_w || k_norm_w) && w_dtype != JH_BF16 && w_dtype != JH_F16 && w_dtype != JH_F32)
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": norm weights must be bf16, f16 or f32");
+    if (n_heads < 0 || n_heads > 65536 || n_rows < 0 || n_rows > 0x7fffffff)
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": bad shape");
+    if (qkv_stride < (n_heads + 2 * n_kv_heads) * head_dim || qkv_stride % 8 || qkv_stride > ((int64_t)1 << 32))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": qkv_stride must hold a row and be a multiple of 8");
+    if (!(rope_base >= 0.0f) || !(rope_base < __builtin_inff()))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": rope_base must be finite and not below 0");
+    if (n_rows == 0) return JH_OK;
+    const bool turn = rope_freqs || rope_base != 0.0f;
+    if (!qkv || !slots || (turn && !positions) || (n_pages > 0 && (!k_pages || !v_pages)) || (n_heads > 0 && !q_out))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": null pointer");
+    if (!aligned16(qkv) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(q_out))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": qkv, q_out and the pages must be 16-byte aligned");
+    if (c->checks & JH_CHECK_INDICES) {
+        std::vector<int32_t> h;
+        if (int r = read_ints(c, op, slots, n_rows, h)) return r;
+        for (size_t i = 0; i < h.size(); i++)
+            if (h[i] < -1 || h[i] >= n_pages * page_size)
+                return fail(c, JH_ERR_INVALID, std::string(op) + ": slot " + std::to_string(h[i]) + " at " +
+                                                   std::to_string(i) + " outside [0, " +
+                                                   std::to_string(n_pages * page_size) + ")");
+    }
+    jh::PagedAppendArgs a{};
+    a.qkv = qkv, a.qkv_dt = qkv_dtype;
+    a.n_rows = (int)n_rows, a.Hq = (int)n_heads, a.Hk = (int)n_kv_heads, a.Dh = (int)head_dim;
+    a.qkv_stride = qkv_stride;
+    a.qn_w = q_norm_w, a.kn_w = k_norm_w, a.w_dt = w_dtype;
+    a.eps = eps, a.base = rope_base, a.scale = rope_scale, a.freqs = rope_freqs;
+    a.positions = positions, a.slots = slots;
+    a.k = static_cast<uint16_t*>(k_pages), a.v = static_cast<uint16_t*>(v_pages);
+    a.kv_f16 = page_dtype == JH_F16;
+    a.n_slots = (int)(n_pages * page_size), a.page_shift = __builtin_ctzll(page_size);
+    a.page_stride = page_stride;
+    a.q_out = static_cast<uint16_t*>(q_out);
+    return finish(c, jh::launch_paged_append(a, c->num_cus, c->stream), op);
+}
+
+int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                       jh_dtype page_dtype, int64_t n_pages, int64_t page_size, int64_t page_stride,
+                       const int32_t* block_tables, int64_t max_blocks, const int32_t* row_starts,
+                       const int32_t* kv_lens, int64_t n_req, int64_t n_rows, int64_t max_new, int64_t n_heads,
+                       int64_t n_kv_heads, int64_t head_dim, float scale, void* out, jh_dtype out_dtype) {
+    if (int r = enter(c)) return r;
+    const char* op = "jh_paged_attention";
+    if (int r = check_pages(c, op, page_dtype, n_pages, page_size)) return r;
+    if (int r = check_page_heads(c, op, n_kv_heads, head_dim, page_size, page_stride)) return r;
+    if (int r = check_float_dtype(c, op, "out", out_dtype)) return r;
+    if (n_heads <= 0 || n_heads > 65536 || n_heads % n_kv_heads)
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": n_heads must be a multiple of n_kv_heads");
+    if (n_req < 0 || n_rows < 0 || max_new < 0 || max_blocks < 0)
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": bad shape");
+    if (n_rows * n_heads > 0x7fffffff || n_rows > 0x7fffffff || n_req > 65536 || max_blocks > 0x7fffffff)
+        return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": too large");
+    if (q_stride < n_heads * head_dim || q_stride % 8 || q_stride > ((int64_t)1 << 32))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": q_stride must hold a row and be a multiple of 8");
+    if (!(scale >= 1e-30f) || !(scale < __builtin_inff()))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": scale must be finite and at least 1e-30");
+    if (n_rows == 0 || n_req == 0) return JH_OK;
+    if (!q || !out || !row_starts || !kv_lens || (max_blocks > 0 && !block_tables) ||
+        (n_pages > 0 && (!k_pages || !v_pages)))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": null pointer");
+    if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": q, out and the pages must be 16-byte aligned");
+    int64_t used = n_rows;
+    if (c->checks) {
+        std::vector<int32_t> st, kv, tab;
+        if (int r = read_ints(c, op, row_starts, n_req + 1, st)) return r;
+        if (c->checks & JH_CHECK_INDICES) {
+            if (int r = read_ints(c, op, kv_lens, n_req, kv)) return r;
+            if (int r = read_ints(c, op, block_tables, n_req * max_blocks, tab)) return r;
+            for (int64_t i = 0; i < n_req; i++) {
+                if (st[i] < 0 || st[i + 1] < st[i] || st[i + 1] > n_rows)
+                    return fail(c, JH_ERR_INVALID, std::string(op) + ": row_starts of request " + std::to_string(i) +
+                                                       " decrease or leave [0, n_rows]");
+                if (kv[i] < 0 || kv[i] > max_blocks * page_size)
+                    return fail(c, JH_ERR_INVALID, std::string(op) + ": kv_lens of request " + std::to_string(i) +
+                                                       " outside [0, max_blocks * page_size]");
+                for (int64_t j = 0; st[i + 1] > st[i] && j * page_size < kv[i]; j++)
+                    if (tab[i * max_blocks + j] < 0 || tab[i * max_blocks + j] >= n_pages)
+                        return fail(c, JH_ERR_INVALID, std::string(op) + ": page " +
+                                                           std::to_string(tab[i * max_blocks + j]) + " of request " +
+                                                           std::to_string(i) + " outside [0, n_pages)");
+            }
+        }
+        used = std::min<int64_t>(n_rows, std::max(0, st[n_req]));
+    }
+    jh::PagedAttnArgs a{};
+    a.q = static_cast<const uint16_t*>(q), a.q_stride = q_stride;
+    a.k = static_cast<const uint16_t*>(k_pages), a.v = static_cast<const uint16_t*>(v_pages);
+    a.f16 = page_dtype == JH_F16;
+    a.n_pages = (int)n_pages, a.page_shift = __builtin_ctzll(page_size), a.page_stride = page_stride;
+    a.tables = block_tables, a.max_blocks = (int)max_blocks;
+    a.row_starts = row_starts, a.kv_lens = kv_lens;
+    a.n_req = (int)n_req, a.n_rows = (int)n_rows, a.max_new = (int)std::min<int64_t>(max_new, n_rows);
+    a.Hq = (int)n_heads, a.Hk = (int)n_kv_heads, a.Dh = (int)head_dim;
+    a.scale = scale, a.out = out, a.out_dt = out_dtype;
+    if (int r = ensure_workspace(c, jh::paged_attn_workspace_bytes(a, c->num_cus), op)) return r;
+    if (int r = finish(c, jh::launch_paged_attn(a, c->ws, c->num_cus, c->stream), op)) return r;
+    return check_values(c, op, out, out_dtype, used * n_heads * head_dim);
+}
+
 }  // extern "C"

@@ -994,6 +994,128 @@ class HipBackend:
             k_cache.ptr, v_cache.ptr, k_cache.dtype, k_cache.shape[-2], float(scale), out.ptr, out.dtype))
         return out
 
+    # -- a paged key/value cache for batches of requests --------------------------------
+    # (include/janis_hip.h; no counterpart in the reference, which decodes one
+    # session at a time). Pages are [n_pages, Hk, page_size, Dh] in BF16 or F16,
+    # block tables I32 [n_req, max_blocks]; all bookkeeping is I32 in device memory.
+    @staticmethod
+    def _ints(op: str, **ts) -> None:
+        for name, t in ts.items():
+            if t.dtype != I32 or not t.contiguous:
+                raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: {name} must be dense I32")
+
+    @staticmethod
+    def _pages(op: str, k_pages: Tensor, v_pages: Tensor) -> tuple:
+        """(n_pages, Hk, page_size, Dh, page_stride): pages may lie apart (keys and
+        values that alternate in one buffer), their insides are dense."""
+        if k_pages.dtype != v_pages.dtype or k_pages.shape != v_pages.shape or len(k_pages.shape) != 4 \
+                or k_pages.strides != v_pages.strides:
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: k_pages and v_pages must be alike, [n_pages, Hk, page, Dh]")
+        n, hk, page, dh = k_pages.shape
+        st = k_pages.strides
+        if st[1:] != (page * dh, dh, 1):
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: the inside of a page must be dense")
+        return n, hk, page, dh, st[0]
+
+    def PagedPlan(self, newLens: Tensor, kvLens: Tensor, pageSize: int, blockTables: Tensor, freePages: Tensor,
+                  freeCount: Tensor, rows: int | None = None, out: tuple | None = None) -> tuple:
+        """One step's bookkeeping (jh_paged_plan): newLens [R] tokens join requests
+        of kvLens [R] keys (below 0: finished), pages go back to and come off the
+        stack freePages[:freeCount], blockTables [R, B] and freePages are updated in
+        place. Returns (kvLens', freeCount', rowStarts [R+1], positions [rows],
+        slots [rows], status [1]), status a JH_PLAN_* code; `out` gives these
+        tensors (the first two may be kvLens and freeCount)."""
+        op = "PagedPlan"
+        R = newLens.numel
+        if out is None:
+            if rows is None:
+                raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: rows (or out) must be given")
+            out = tuple(self.empty(I32, n) for n in (R, 1, R + 1, int(rows), int(rows), 1))
+        kv, count, starts, pos, slots, status = out
+        self._ints(op, newLens=newLens, kvLens=kvLens, blockTables=blockTables, freePages=freePages,
+                   freeCount=freeCount, kvLensOut=kv, freeCountOut=count, rowStarts=starts, positions=pos, slots=slots,
+                   status=status)
+        T = pos.numel
+        if len(blockTables.shape) != 2 or blockTables.shape[0] != R or kvLens.numel != R or kv.numel != R \
+                or starts.numel != R + 1 or slots.numel != T or not freeCount.numel == count.numel == status.numel == 1:
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: shapes do not match {R} requests and {T} rows")
+        check(self._ctx, self._L.jh_paged_plan(
+            self._ctx, newLens.ptr, kvLens.ptr, R, T, int(pageSize), blockTables.ptr, blockTables.shape[1],
+            freePages.ptr, freePages.numel, freeCount.ptr, kv.ptr, count.ptr, starts.ptr, pos.ptr, slots.ptr,
+            status.ptr))
+        return out
+
+    def PagedQKNormRoPEAppend(self, qkv: Tensor, n_heads: int, n_kv_heads: int, q_norm: Tensor | None,
+                              k_norm: Tensor | None, eps: float, base: float, rope_scale: float,
+                              positions: Tensor | None, slots: Tensor, k_pages: Tensor, v_pages: Tensor,
+                              freqs: Tensor | None = None, q_out: Tensor | None = None) -> Tensor | None:
+        """The rows of a q/k/v product [T, (Hq+2Hk)*Dh] (F32 or BF16, rows may lie
+        apart): q and k heads normalised (where weights are given) and rotated by
+        positions [T] (base 0 without freqs: not rotated), keys and values to
+        slots [T] of the pages, queries to q_out [T, Hq, Dh] in the pages' dtype,
+        which is returned (None when n_heads is 0). Rows with a slot of -1 are
+        skipped."""
+        op = "PagedQKNormRoPEAppend"
+        n, hk, page, dh, stride = self._pages(op, k_pages, v_pages)
+        T = slots.numel
+        self._ints(op, slots=slots)
+        if positions is not None:
+            self._ints(op, positions=positions)
+        if hk != n_kv_heads or len(qkv.shape) != 2 or qkv.shape != (T, (n_heads + 2 * hk) * dh) \
+                or (positions is not None and positions.numel != T):
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: qkv {list(qkv.shape)}, {T} slots and the pages do not match")
+        if qkv.strides[1] != 1:
+            qkv = self._c(qkv)
+        for w in (q_norm, k_norm):
+            if w is not None and (w.numel != dh or not w.contiguous):
+                raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: norm weights must be dense [{dh}]")
+        if q_norm is not None and k_norm is not None and q_norm.dtype != k_norm.dtype:
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: norm weights differ in dtype")
+        if freqs is not None and (freqs.dtype != F32 or freqs.numel != dh // 2 or not freqs.contiguous):
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: freqs must be dense F32 [{dh // 2}]")
+        if n_heads > 0:
+            if q_out is None:
+                q_out = self.empty(k_pages.dtype, T, n_heads, dh)
+            elif q_out.dtype != k_pages.dtype or q_out.numel != T * n_heads * dh or not q_out.contiguous:
+                raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: q_out must be dense [T, Hq, Dh] in the pages' dtype")
+        w = q_norm if q_norm is not None else k_norm
+        check(self._ctx, self._L.jh_paged_qk_norm_rope_append(
+            self._ctx, qkv.ptr, qkv.dtype, T, qkv.strides[0] if T > 1 else qkv.shape[1], n_heads, hk, dh,
+            q_norm.ptr if q_norm is not None else None, k_norm.ptr if k_norm is not None else None,
+            w.dtype if w is not None else BF16, float(eps), float(base), float(rope_scale),
+            freqs.ptr if freqs is not None else None, positions.ptr if positions is not None else None, slots.ptr,
+            k_pages.ptr, v_pages.ptr, k_pages.dtype, n, page, stride, q_out.ptr if n_heads > 0 else None))
+        return q_out if n_heads > 0 else None
+
+    def PagedAttention(self, q: Tensor, k_pages: Tensor, v_pages: Tensor, blockTables: Tensor, rowStarts: Tensor,
+                       kvLens: Tensor, scale: float, maxNew: int | None = None, out: Tensor | None = None,
+                       out_dtype: int | None = None) -> Tensor:
+        """SDPA of every request's new tokens over its pages: q [T, Hq, Dh] in the
+        pages' dtype (rows may lie apart), request r's tokens the rows
+        rowStarts[r] .. rowStarts[r+1] - 1, the last kvLens[r] - 1's position, each
+        seeing the keys up to its own. maxNew, the most tokens of a request (a
+        hint). Returns [T, Hq, Dh] (the pages' dtype unless out or out_dtype says
+        otherwise); rows past rowStarts[R] are left as they were."""
+        op = "PagedAttention"
+        n, hk, page, dh, stride = self._pages(op, k_pages, v_pages)
+        self._ints(op, blockTables=blockTables, rowStarts=rowStarts, kvLens=kvLens)
+        R = kvLens.numel
+        if q.dtype != k_pages.dtype or len(q.shape) != 3 or q.shape[2] != dh or len(blockTables.shape) != 2 \
+                or blockTables.shape[0] != R or rowStarts.numel != R + 1:
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: q {list(q.shape)}, the tables and the pages do not match")
+        T, hq = q.shape[:2]
+        if q.strides[1:] != (dh, 1):
+            q = self._c(q)
+        if out is None:
+            out = self.empty(q.dtype if out_dtype is None else out_dtype, T, hq, dh)
+        elif out.numel != T * hq * dh or not out.contiguous:
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: out must be dense [T, Hq, Dh]")
+        check(self._ctx, self._L.jh_paged_attention(
+            self._ctx, q.ptr, q.strides[0] if T > 1 else hq * dh, k_pages.ptr, v_pages.ptr, k_pages.dtype, n, page, stride,
+            blockTables.ptr, blockTables.shape[1], rowStarts.ptr, kvLens.ptr, R, T, T if maxNew is None else int(maxNew),
+            hq, hk, dh, float(scale), out.ptr, out.dtype))
+        return out
+
     def MoeRoute(self, logits: Tensor, k: int, normTopk: bool = True) -> tuple:
         """The router of MoEBlock.Forward (qwen/moe.go:455-491) on the device:
         softmax over the last axis, top-k (selection-sort ties), optional
