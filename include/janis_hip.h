@@ -697,8 +697,8 @@ JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype q
  *   out  [n_rows, n_heads, head_dim], dense, JH_BF16, JH_F16 or JH_F32
  * max_new is a hint, the most new tokens any request has (1 in a decode step):
  * it chooses the kernels, and a wrong one costs time only. head_dim 64, 128 or 256,
- * scale finite and at least 1e-30; pointers 16-byte aligned, q_stride and
- * page_stride multiples of 8.
+ * page_size at least 8, scale finite and at least 1e-30; pointers 16-byte aligned,
+ * q_stride and page_stride multiples of 8; max_blocks * page_size up to 2^30.
  * Scores, maxima, sums and results are fp32; the probabilities enter the product
  * with the values in the pages' dtype: rounded once to it for 16-bit results
  * (as the result is), as the sum of two such terms for JH_F32 ones and where a

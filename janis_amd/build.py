@@ -20,7 +20,7 @@ CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "libjanis_hip.so")
 SOURCES = ["runtime.hip", "qmv.hip", "qmm.hip", "gather.hip", "dequant.hip", "decode.hip", "attention.hip", "ops.hip",
-           "paged.hip"]
+           "paged.hip", "paged_attention.hip"]
 # bench.py's measurement kernels (plain read, copy): a library of their own,
 # outside the backend's C ABI
 BENCH_SOURCE = "bench_kernels.hip"

@@ -1,5 +1,5 @@
-// A paged key/value cache for batches of requests: the bookkeeping of a step,
-// the append of new rows, and attention over the pages.
+// A paged key/value cache for batches of requests: the bookkeeping of a step and
+// the append of new rows (attention over the pages: paged_attention.hip).
 #include "jh_common.hpp"
 
 namespace jh {
@@ -223,58 +223,6 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a) {
     }
 }
 
-// ---- attention --------------------------------------------------------------------
-template <bool F16>
-__device__ __forceinline__ float widen(uint16_t h) {
-    return F16 ? f16_to_f32(h) : bf16_to_f32(h);
-}
-
-// One wave per row and query head, one key at a time, DH / 64 features per lane.
-template <int DH, bool F16>
-__global__ __launch_bounds__(256) void paged_attn_row_kernel(PagedAttnArgs a) {
-    constexpr int kPer = DH / 64;
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const int lane = threadIdx.x & 63;
-    const int t = (int)(item / a.Hq), head = (int)(item % a.Hq);
-    if (t >= a.n_rows || t >= a.row_starts[a.n_req] || t < a.row_starts[0]) return;
-    const int r = owner_of(a.row_starts, a.n_req, t);
-    const int last = min(a.row_starts[r + 1], a.n_rows);
-    const int cap = (int)min((int64_t)a.max_blocks << a.page_shift, (int64_t)0x7fffffff);
-    const int kv = min(max(a.kv_lens[r], 0), cap);
-    const int limit = min(kv, kv - (last - t) + 1);
-    const int h = head / (a.Hq / a.Hk);
-    float q[kPer], o[kPer], m = -__builtin_inff(), sum = 0.0f;
-    for (int e = 0; e < kPer; e++) {
-        q[e] = widen<F16>(a.q[t * a.q_stride + head * DH + 64 * e + lane]);
-        o[e] = 0.0f;
-    }
-    bool bad = false;
-    for (int j = 0; j < limit; j++) {
-        const int page = a.tables[(int64_t)r * a.max_blocks + (j >> a.page_shift)];
-        if ((uint32_t)page >= (uint32_t)a.n_pages) {
-            bad = true;
-            break;
-        }
-        const int64_t at = page * a.page_stride +
-                           (((int64_t)h << a.page_shift) + (j & ((1 << a.page_shift) - 1))) * DH + lane;
-        float s = 0.0f;
-        for (int e = 0; e < kPer; e++) s = fmaf(q[e], widen<F16>(a.k[at + 64 * e]), s);
-        s = wave_sum(s) * a.scale;
-        const float mn = fmaxf(m, s), f = m == mn ? 1.0f : expf(m - mn);
-        // (every score -inf so far: a weight of 0, so that the row is 0 / 0 if it stays so)
-        const float p = mn == -__builtin_inff() ? s - s == 0.0f ? 1.0f : s == mn ? 0.0f : s : expf(s - mn);
-        sum = sum * f + p;
-        for (int e = 0; e < kPer; e++) o[e] = o[e] * f + p * widen<F16>(a.v[at + 64 * e]);
-        m = mn;
-    }
-    for (int e = 0; e < kPer; e++) {
-        const float v = bad ? __builtin_nanf("") : limit <= 0 ? 0.0f : o[e] / sum;
-        const int64_t at = ((int64_t)t * a.Hq + head) * DH + 64 * e + lane;
-        if (a.out_dt == JH_F16) static_cast<uint16_t*>(a.out)[at] = f32_to_f16(v);
-        else store_y(a.out, at, v, a.out_dt);
-    }
-}
-
 }  // namespace
 
 Status launch_paged_plan(const PagedPlanArgs& a, hipStream_t st) {
@@ -294,22 +242,6 @@ Status launch_paged_append(const PagedAppendArgs& a, int num_cus, hipStream_t st
         a.Dh == 64    ? go(paged_append_kernel<64, false>)
         : a.Dh == 128 ? go(paged_append_kernel<128, false>)
                       : go(paged_append_kernel<256, false>);
-    return Status::ok();
-}
-
-size_t paged_attn_workspace_bytes(const PagedAttnArgs&, int) { return 0; }
-
-Status launch_paged_attn(const PagedAttnArgs& a, void*, int, hipStream_t st) {
-    const dim3 grid((unsigned)(((int64_t)a.n_rows * a.Hq + 3) / 4));
-    auto go = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, st, a); };
-    if (a.f16)
-        a.Dh == 64    ? go(paged_attn_row_kernel<64, true>)
-        : a.Dh == 128 ? go(paged_attn_row_kernel<128, true>)
-                      : go(paged_attn_row_kernel<256, true>);
-    else
-        a.Dh == 64    ? go(paged_attn_row_kernel<64, false>)
-        : a.Dh == 128 ? go(paged_attn_row_kernel<128, false>)
-                      : go(paged_attn_row_kernel<256, false>);
     return Status::ok();
 }
 

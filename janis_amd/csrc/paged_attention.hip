@@ -1,0 +1,815 @@
+// Attention of every request's new tokens over a paged key/value cache (the rows of
+// jh_paged_attention) on the matrix cores: o = softmax(scale q K^T) V with an online
+// softmax, head_dim 64, 128 or 256, bf16 or f16.
+//
+// The rows of a kv head are its G query heads of each new token: row j of a request is
+// head j % G of token j / G, so the heads that share keys and values read them once.
+// Both products run transposed, S^T = K Q^T and O^T = V^T P^T: a lane holds one row
+// (lane % 32) of both accumulators, the row's maximum, sum and rescale are per-lane
+// scalars, and the scores become the second product's B operand where they are. Its
+// K order is the order the first product leaves the keys in, and the transposing LDS
+// reads (ds_read_b64_tr_b16) take V in that order straight from its rows.
+//
+// Keys and values go to LDS by loads that need no registers (global_load_lds, 1 KB per
+// wave and instruction, issued from inline asm with explicit waits): eight keys lie in
+// one page, so a group's page is looked up once, its address is scalar, and the lanes
+// add constants. 16-byte chunks are permuted within a row on the way (by the lanes'
+// source addresses), so that neither kind of LDS read meets a bank conflict. Keys past
+// the last one that a tile sees are loaded as that last one again: what lies in unused
+// slots never enters.
+//
+// Work: a block takes a tile of rows of one request and kv head and a part of its keys.
+// Lengths live on the device, so the blocks find their tile themselves, by running sums
+// over the requests; the grid is the most that the sizes known to the host allow. Keys
+// are split where that fills the GPU: all tiles' keys over as many parts as blocks are
+// resident, at least kMinUnits * 64 keys each. A request whose keys were split has its
+// parts joined, in their order, by paged_attn_merge_kernel.
+#include "jh_common.hpp"
+
+namespace jh {
+namespace {
+
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef short short4_t __attribute__((ext_vector_type(4)));
+
+constexpr float kLog2e = 1.44269504088896340736f;
+constexpr int kUnit = 64;       // keys: splits are whole units
+constexpr int kFewRows = 32;    // rows of a tile in the few-rows kernel
+constexpr int kManyRows = 128;  // ... in the many-rows kernel
+// p is held as p * 2^kPShift, and a row's maximum is moved when it grew by more than
+// kLazy (log2): f16 has nothing below 2^-24 and nothing past 2^16, so p is kept high
+// there (a weight of 2^-27 of the largest still has all its bits).
+template <bool F16>
+constexpr float kPShift = F16 ? 13.0f : 0.0f;
+template <bool F16>
+constexpr float kLazy = F16 ? 2.0f : 8.0f;
+
+__device__ __forceinline__ float ninf() { return -__builtin_inff(); }
+__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
+
+template <bool F16>
+__device__ __forceinline__ floatx16 mfma(uint4 a, uint4 b, floatx16 c) {
+    if constexpr (F16)
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8_t, a), __builtin_bit_cast(f16x8_t, b), c,
+                                                      0, 0, 0);
+    else
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
+                                                       c, 0, 0, 0);
+}
+
+// (a, b) as N packed 16-bit terms, each the nearest to what the earlier ones left.
+template <bool F16, int N>
+__device__ __forceinline__ void split_pair(float a, float b, uint32_t (&t)[N]) {
+#pragma unroll
+    for (int n = 0; n < N; n++) {
+        const f32x2_t f = {a, b};
+        if constexpr (F16) {
+            const f16x2_t v = __builtin_convertvector(f, f16x2_t);
+            t[n] = __builtin_bit_cast(uint32_t, v);
+            if (n + 1 < N) a -= (float)v.x, b -= (float)v.y;
+        } else {
+            t[n] = __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2_t));
+            if (n + 1 < N) a -= __uint_as_float(t[n] << 16), b -= __uint_as_float(t[n] & 0xFFFF0000u);
+        }
+    }
+}
+
+template <bool F16>
+__device__ __forceinline__ float2 widen2(uint32_t u) {
+    if constexpr (F16) {
+        const f16x2_t x = __builtin_bit_cast(f16x2_t, u);
+        return make_float2((float)x.x, (float)x.y);
+    }
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xFFFF0000u));
+}
+
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ int64_t uniform(int64_t v) {
+    return (int64_t)((uint64_t)(uint32_t)uniform((int)(v >> 32)) << 32 | (uint32_t)uniform((int)v));
+}
+
+// 16 bytes per lane from base + off into LDS at m0 + 16 * lane. The s_nop is the five wait
+// states between a VALU write of a scalar (a readlane into `base`) and its use by a load,
+// which the compiler does not see in here; it covers the M0 write too.
+__device__ __forceinline__ void lds_fill16(const void* base, uint32_t off, uint32_t m0) {
+    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(uniform((int64_t)base)), "{m0}"(uniform((int)m0))
+                 : "memory");
+}
+// The wave's LDS reads are done (before loads into LDS overwrite what they read).
+__device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
+__device__ __forceinline__ uint4 lds_read16(const uint8_t* p) { return *reinterpret_cast<const uint4*>(p); }
+// Four keys of one feature: in each 16 lanes, lane i's address is 4 features (8 bytes) of
+// key i / 4, and lane i receives feature i of the keys 0 .. 3.
+__device__ __forceinline__ uint2 lds_read_tr(const uint8_t* p) {
+    return __builtin_bit_cast(
+        uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) short4_t*)p));
+}
+
+// ---- finding a block's work ---------------------------------------------------------
+struct Attn {
+    PagedAttnArgs a;
+    int lo, hi;      // requests with lo < rows <= hi (rows = new tokens * G) are this launch's
+    int target;      // parts of the keys to make, per kv head
+    int min_units;   // least units of keys per part
+    float* part;     // records of split parts: [rows of a tile][DH] results, then [rows][2] maximum and sum
+};
+
+struct Request {
+    int start, n, kv;
+};
+__device__ __forceinline__ Request request(const PagedAttnArgs& a, int r) {
+    const int cap = a.max_blocks << a.page_shift;  // at most 2^30
+    Request q;
+    q.start = min(max(a.row_starts[r], 0), a.n_rows);
+    q.n = min(max(a.row_starts[r + 1], q.start), a.n_rows) - q.start;
+    q.kv = min(max(a.kv_lens[r], 0), cap);
+    return q;
+}
+
+struct Work {
+    bool ok;
+    int r, local;     // the request, and the index among its items
+    Request q;
+    int tiles, splits, per;  // row tiles; parts of the keys, `per` units each
+    int slot;         // of its first record
+};
+
+// The item `index` of all requests: tiles * splits items per request, or, with MERGE, the
+// row tiles of requests whose keys are split. By every wave of a block for itself: a lane
+// sums a run of requests, a scan over the lanes, and the run that holds the item is
+// walked by all lanes together.
+template <int TR, bool MERGE>
+__device__ __forceinline__ Work find_work(const Attn& w, int index) {
+    const PagedAttnArgs& a = w.a;
+    const int lane = threadIdx.x & 63, G = a.Hq / a.Hk, run = (a.n_req + 63) / 64;
+    auto tiles_of = [&](const Request& q) {
+        const int rows = q.n * G;
+        return rows > w.lo && rows <= w.hi ? (rows + TR - 1) / TR : 0;
+    };
+    auto units_of = [&](const Request& q) { return max(1, (q.kv + kUnit - 1) / kUnit); };
+    int64_t all = 0;
+    Request mine{0, 0, 0};
+    for (int e = 0; e < run; e++) {
+        const int r = lane * run + e;
+        if (r >= a.n_req) break;
+        const Request q = request(a, r);
+        if (e == 0) mine = q;
+        all += (int64_t)tiles_of(q) * units_of(q);
+    }
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d, 64);
+    const int64_t each = (all + w.target - 1) / w.target;
+    const int most = (int)min(max(each, (int64_t)w.min_units), (int64_t)0x40000000);  // units per part
+    auto splits_of = [&](const Request& q) { return (units_of(q) + most - 1) / most; };
+    int items = 0, slots = 0;
+    for (int e = 0; e < run; e++) {
+        const int r = lane * run + e;
+        if (r >= a.n_req) break;
+        const Request q = e == 0 ? mine : request(a, r);
+        const int t = tiles_of(q), s = splits_of(q);
+        items += MERGE ? (s > 1 ? t : 0) : t * s;
+        slots += s > 1 ? t * s : 0;
+    }
+    int upto = items, slots_upto = slots;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+        const int x = __shfl_up(upto, d, 64), y = __shfl_up(slots_upto, d, 64);
+        if (lane >= d) upto += x, slots_upto += y;
+    }
+    const uint64_t past = __ballot(upto > index);
+    Work o{};
+    if (!past) return o;
+    const int at = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
+    int left = index - __builtin_amdgcn_readlane(upto - items, at);
+    int slot = __builtin_amdgcn_readlane(slots_upto - slots, at);
+    for (int e = 0; e < run; e++) {
+        const int r = at * run + e;
+        if (r >= a.n_req) break;
+        Request q;
+        if (e == 0) {
+            q.start = __builtin_amdgcn_readlane(mine.start, at);
+            q.n = __builtin_amdgcn_readlane(mine.n, at);
+            q.kv = __builtin_amdgcn_readlane(mine.kv, at);
+        } else {
+            q = request(a, r);
+        }
+        const int t = tiles_of(q), s = splits_of(q), count = MERGE ? (s > 1 ? t : 0) : t * s;
+        if (left < count) {
+            o.ok = true, o.r = uniform(r), o.local = uniform(left), o.tiles = uniform(t), o.splits = uniform(s);
+            o.q = Request{uniform(q.start), uniform(q.n), uniform(q.kv)};
+            o.per = uniform((units_of(q) + s - 1) / s);
+            o.slot = uniform(slot);
+            // (row_starts that go up and down can make more parts than were counted)
+            if (o.splits > 1 && (o.slot < 0 || (int64_t)o.slot + (int64_t)o.tiles * o.splits > 2 * (int64_t)w.target))
+                o.ok = false;
+            return o;
+        }
+        left -= count;
+        slot += s > 1 ? t * s : 0;
+    }
+    return o;
+}
+
+// Keys that row `row` of the request sees.
+__device__ __forceinline__ int seen(const Request& q, int row, int G) { return max(0, q.kv - q.n + row / G + 1); }
+
+// ---- a row again, key by key -------------------------------------------------------
+// The products meet masked keys with p = 0, where an infinity or NaN in V gives NaN, and
+// p's lesser terms (of either sign) meet an infinity that the row does see. So a row
+// whose result is not finite is computed again here, by one wave, in fp32 and reading
+// nothing that it does not see. m is log2; the lane's features are lane + 64 e.
+template <int DH, bool F16>
+__device__ __forceinline__ void row_again(const PagedAttnArgs& a, int r, int head, int token, int kb, int lim, float& m,
+                                       float& l, float (&o)[DH / 64]) {
+    const int lane = threadIdx.x & 63, hk = head / (a.Hq / a.Hk);
+    const uint4* const q = reinterpret_cast<const uint4*>(a.q + token * a.q_stride + (int64_t)head * DH);
+    m = ninf(), l = 0.0f;
+#pragma unroll
+    for (int e = 0; e < DH / 64; e++) o[e] = 0.0f;
+    for (int k0 = kb; k0 < lim; k0 += 64) {
+        const int key = min(k0 + lane, lim - 1);
+        int page = a.tables[(int64_t)r * a.max_blocks + (key >> a.page_shift)];
+        if ((uint32_t)page >= (uint32_t)a.n_pages) page = 0;
+        const int64_t at = page * a.page_stride +
+                           (((int64_t)hk << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * DH;
+        const uint4* const k = reinterpret_cast<const uint4*>(a.k + at);
+        float s = 0.0f;
+#pragma unroll 4
+        for (int i = 0; i < DH / 8; i++) {
+            const uint4 x = q[i], y = k[i];
+            const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float2 u = widen2<F16>(xs[j]), v = widen2<F16>(ys[j]);
+                s = fmaf(u.x, v.x, s);
+                s = fmaf(u.y, v.y, s);
+            }
+        }
+        s = k0 + lane < lim ? s * (a.scale * kLog2e) : ninf();
+        const float mn = fmaxf(m, wave_max(s));
+        const float sub = mn == ninf() ? 0.0f : mn, f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - sub);
+        const float p = __builtin_amdgcn_exp2f(s - sub + kPShift<F16>);  // as the products hold it
+        l = l * f + wave_sum(p);
+#pragma unroll
+        for (int e = 0; e < DH / 64; e++) o[e] *= f;
+        m = mn;
+        for (int j = 0; j < min(64, lim - k0); j++) {
+            const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), j));
+            const int64_t row = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), j) << 32) |
+                                          (uint32_t)__builtin_amdgcn_readlane((int)at, j));
+#pragma unroll
+            for (int e = 0; e < DH / 64; e++) {
+                const uint16_t v = a.v[row + lane + 64 * e];
+                o[e] = fmaf(pj, F16 ? f16_to_f32(v) : bf16_to_f32(v), o[e]);
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ void store_out(const PagedAttnArgs& a, int64_t at, float v) {
+    if (a.out_dt == JH_F16) static_cast<uint16_t*>(a.out)[at] = f32_to_f16(v);
+    else store_y(a.out, at, v, a.out_dt);
+}
+__device__ __forceinline__ void store_out4(const PagedAttnArgs& a, int64_t at, float x, float y, float z, float w) {
+    if (a.out_dt == JH_F32) {
+        *reinterpret_cast<float4*>(static_cast<float*>(a.out) + at) = make_float4(x, y, z, w);
+        return;
+    }
+    uint32_t lo[1], hi[1];
+    if (a.out_dt == JH_F16) split_pair<true, 1>(x, y, lo), split_pair<true, 1>(z, w, hi);
+    else split_pair<false, 1>(x, y, lo), split_pair<false, 1>(z, w, hi);
+    *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at) = make_uint2(lo[0], hi[0]);
+}
+
+// Where row `row` of a request goes: element offset of its head's first feature.
+template <int DH>
+__device__ __forceinline__ int64_t out_at(const PagedAttnArgs& a, const Request& q, int row, int hk, int G) {
+    return ((int64_t)(q.start + row / G) * a.Hq + hk * G + row % G) * DH;
+}
+
+// Tiles of keys in LDS: row `key` (of the tile) holds its DH / 8 chunks of 16 bytes,
+// chunk c at place c ^ perm(key). K rows are read by 16 lanes of consecutive keys at one
+// chunk, V rows by 4 keys at 64 bytes each: over 256 bytes (all banks) none meets another.
+template <int DH>
+__device__ __forceinline__ int perm_k(int key) { return DH == 64 ? (key >> 1) & 7 : key & 15; }
+template <int DH>
+__device__ __forceinline__ int perm_v(int key) { return DH == 64 ? 4 * ((key >> 1) & 1) : 4 * (key & 3); }
+
+// Eight keys from key0 on (one page) of one head, keys or values: DH / 64 loads of 1 KB.
+// `last`: the last key that may be loaded. `g`: the group's number in its tile.
+template <int DH, bool V>
+__device__ __forceinline__ void fill_group(const uint16_t* pool, int64_t page_at, int shift, int key0, int last, int g,
+                                           uint32_t lds) {
+    const int lane = threadIdx.x & 63, first = min(key0, last), more = last - first;
+    const uint16_t* const base = pool + page_at + (int64_t)(first & ((1 << shift) - 1)) * DH;
+#pragma unroll
+    for (int u = 0; u < DH / 64; u++) {
+        const int row = (u * 64 + lane) / (DH / 8), place = (u * 64 + lane) % (DH / 8), key = 8 * g + row;
+        const int chunk = place ^ (V ? perm_v<DH>(key) : perm_k<DH>(key));
+        lds_fill16(base, (uint32_t)(min(row, more) * (2 * DH) + 16 * chunk), lds + g * (16 * DH) + u * 1024);
+    }
+}
+
+// The lane's row of q as B fragments: step kk holds features 16 kk + 8 h .. + 8.
+template <int DH>
+__device__ __forceinline__ void load_q(const PagedAttnArgs& a, const Request& q, int row, int hk, int G,
+                                       uint4 (&qf)[DH / 16]) {
+    const int h = (threadIdx.x & 63) >> 5;
+    const uint16_t* const p = a.q + (q.start + row / G) * a.q_stride + (int64_t)(hk * G + row % G) * DH + 8 * h;
+#pragma unroll
+    for (int kk = 0; kk < DH / 16; kk++) qf[kk] = *reinterpret_cast<const uint4*>(p + 16 * kk);
+}
+
+// S^T of 32 keys (their rows in LDS at kt) and the wave's 32 rows.
+template <int DH, bool F16>
+__device__ __forceinline__ floatx16 scores32(const uint8_t* kt, const uint4 (&qf)[DH / 16]) {
+    const int lane = threadIdx.x & 63, h = lane >> 5, c = lane & 31;
+    const uint8_t* const row = kt + c * (2 * DH);
+    const int x = (h ^ perm_k<DH>(c)) * 16;
+    floatx16 s;
+#pragma unroll
+    for (int r = 0; r < 16; r++) s[r] = 0.0f;
+#pragma unroll
+    for (int kk = 0; kk < DH / 16; kk++) s = mfma<F16>(lds_read16(row + (x ^ (32 * kk))), qf[kk], s);
+    return s;
+}
+
+// O^T += V^T P^T over 16 keys (their rows in LDS at vt): p as PN terms of B fragments,
+// in the order of the keys that scores32 leaves.
+template <int DH, bool F16, int PN>
+__device__ __forceinline__ void values16(const uint8_t* vt, const uint32_t (&t)[4][PN], floatx16 (&o)[DH / 32]) {
+    const int lane = threadIdx.x & 63, i = lane & 15;
+    const uint8_t* const row = vt + ((lane >> 5) * 4 + (i >> 2)) * (2 * DH) + ((lane >> 4) & 1) * 32 + (i & 3) * 8;
+    const int x = perm_v<DH>(i >> 2) / 4;
+#pragma unroll
+    for (int d = 0; d < DH / 32; d++) {
+        const uint2 lo = lds_read_tr(row + (d ^ x) * 64), hi = lds_read_tr(row + (d ^ x) * 64 + 16 * DH);
+        const uint4 vf = make_uint4(lo.x, lo.y, hi.x, hi.y);
+#pragma unroll
+        for (int n = PN - 1; n >= 0; n--) o[d] = mfma<F16>(vf, make_uint4(t[0][n], t[1][n], t[2][n], t[3][n]), o[d]);
+    }
+}
+
+// One tile of 32 * N keys (from k0) of the online softmax: scores to weights in place.
+template <int DH, bool F16, int N>
+__device__ __forceinline__ void soften(floatx16 (&s)[N], int k0, int lim, bool edge, float c, float& m, float& l,
+                                       floatx16 (&o)[DH / 32]) {
+    const int h = (threadIdx.x & 63) >> 5;
+    // register r of s[g] is key k0 + 32 g + 8 (r / 4) + 4 h + r % 4
+    if (edge) {
+#pragma unroll
+        for (int g = 0; g < N; g++)
+#pragma unroll
+            for (int r = 0; r < 16; r++)
+                if (k0 + 32 * g + 8 * (r >> 2) + 4 * h + (r & 3) >= lim) s[g][r] = ninf();
+    }
+    float mt = ninf();
+#pragma unroll
+    for (int g = 0; g < N; g++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) mt = fmaxf(mt, s[g][r]);
+    mt = pair32<true>(mt) * c;
+    if (__any(mt > m + kLazy<F16>)) {
+        const float mn = fmaxf(m, mt);
+        const float f = mn == ninf() ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+        l *= f;
+#pragma unroll
+        for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+            for (int r = 0; r < 16; r++) o[d][r] *= f;
+        m = mn;
+    }
+    const float neg = m == ninf() ? 0.0f : kPShift<F16> - m;
+#pragma unroll
+    for (int g = 0; g < N; g++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) {
+            s[g][r] = __builtin_amdgcn_exp2f(fmaf(s[g][r], c, neg));
+            l += s[g][r];
+        }
+}
+
+// The wave's rows (bit lane % 32) whose results are not finite.
+template <int DH>
+__device__ __forceinline__ uint32_t rows_again(float l, const floatx16 (&o)[DH / 32], bool live) {
+    bool bad = !finite(l);
+#pragma unroll
+    for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) bad |= !finite(o[d][r]);
+    const uint64_t votes = __ballot(bad && live);
+    return (uint32_t)votes | (uint32_t)(votes >> 32);
+}
+
+__device__ __forceinline__ int wave_min_int(int v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = min(v, __shfl_xor(v, d, 64));
+    return v;
+}
+
+// ---- few rows ------------------------------------------------------------------------
+// Tiles of 32 rows: decode (a token's G heads) and short runs of new tokens. The four
+// waves take the part's 32-key tiles in turn, each with its own buffers and no barrier:
+// while a tile's scores become weights the next tile's keys are on their way, while its
+// values are used the next values. The waves' results meet in LDS.
+template <int DH, bool F16>
+__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_few_kernel(Attn w) {
+    constexpr int kTile = 32 * DH * 2, kLoads = kTile / 1024;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[8 * kTile];
+    __shared__ float2 s_ml[4][32];
+    __shared__ int s_bad[4];
+    __shared__ uint32_t s_again[4];
+    const PagedAttnArgs& a = w.a;
+    const int hk = blockIdx.x % a.Hk, G = a.Hq / a.Hk;
+    const Work k = find_work<kFewRows, false>(w, blockIdx.x / a.Hk);
+    if (!k.ok) return;
+    const int tile = uniform(k.local / k.splits), split = k.local - tile * k.splits;
+    const Request q = k.q;
+    const int lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int w0 = tile * kFewRows, n_rows = min(kFewRows, q.n * G - w0);
+    const int kb = split * k.per * kUnit;
+    // keys this part ends at: for the tile's last row, this lane's row, the first row
+    const int end = uniform(seen(q, w0 + n_rows - 1, G));
+    const int parts = max(1, (end + k.per * kUnit - 1) / (k.per * kUnit));
+    if (split >= parts) return;
+    const int ke = min(end, kb + k.per * kUnit);
+    const int row = w0 + min(c32, n_rows - 1);
+    const int lim = min(ke, seen(q, row, G)), lim_lo = min(ke, seen(q, w0, G));
+    uint4 qf[DH / 16];
+    load_q<DH>(a, q, row, hk, G, qf);
+    const float c = a.scale * kLog2e;
+    floatx16 o[DH / 32];
+#pragma unroll
+    for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    float m = ninf(), l = 0.0f;
+    const int n_tiles = (max(0, ke - kb) + 31) / 32;
+    const uint8_t *const kt = lds + wave * 2 * kTile, *const vt = kt + kTile;
+    const uint32_t to = lds_addr(kt);
+    // pages of the wave's next 16 tiles: lane 4 j + g holds group g of its tile j's
+    int ids = 0, bad_from = 0x7fffffff;
+    auto look_up = [&](int t) {
+        const int key = kb + (t + 4 * (lane >> 2)) * 32 + (lane & 3) * 8;
+        int id = a.tables[(int64_t)k.r * a.max_blocks + (min(key, ke - 1) >> a.page_shift)];
+        if ((uint32_t)id >= (uint32_t)a.n_pages) {
+            if (key < ke) bad_from = min(bad_from, key);
+            id = 0;
+        }
+        ids = id;
+    };
+    auto page_at = [&](int j, int g) {
+        return __builtin_amdgcn_readlane(ids, 4 * j + g) * a.page_stride + (((int64_t)hk << a.page_shift) * DH);
+    };
+    auto load = [&](auto v, int t, int j) {
+        constexpr bool V = decltype(v)::value;
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            fill_group<DH, V>(V ? a.v : a.k, page_at(j, g), a.page_shift, kb + t * 32 + 8 * g, ke - 1, g, to + (V ? kTile : 0));
+    };
+    using K = std::false_type;
+    using Vals = std::true_type;
+    if (wave < n_tiles) {
+        look_up(wave);
+        load(K{}, wave, 0);
+        load(Vals{}, wave, 0);
+    }
+    int j = 0;
+    for (int t = wave; t < n_tiles; t += 4) {
+        const int k0 = kb + t * 32, next = t + 4, jn = (j + 1) & 15;
+        const bool more = next < n_tiles, edge = k0 + 32 > lim_lo;
+        wait_vmem<kLoads>();
+        floatx16 s[1] = {scores32<DH, F16>(kt, qf)};
+        wait_lds();
+        if (more) {
+            if (jn == 0) look_up(next);
+            load(K{}, next, jn);
+        }
+        soften<DH, F16, 1>(s, k0, lim, edge, c, m, l, o);
+        if (more) wait_vmem<kLoads>();
+        else wait_vmem<0>();
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            uint32_t p[4][2];
+#pragma unroll
+            for (int e = 0; e < 4; e++) split_pair<F16, 2>(s[0][8 * kk + 2 * e], s[0][8 * kk + 2 * e + 1], p[e]);
+            values16<DH, F16, 2>(vt + kk * 16 * 2 * DH, p, o);
+        }
+        wait_lds();
+        if (more) load(Vals{}, next, jn);
+        j = jn;
+    }
+    l = pair32<false>(l);
+    // the waves' results to LDS (their own buffers; the chunk of 4 features f of row c at f ^ c)
+    const int bad = wave_min_int(bad_from);
+    if (lane == 0) s_bad[wave] = bad;
+    const uint32_t mine = rows_again<DH>(l, o, c32 < n_rows);
+    if (lane == 0) s_again[wave] = mine;
+    if (h == 0) s_ml[wave][c32] = make_float2(m, l);
+    constexpr int kChunks = DH / 4;
+    static_assert(32 * DH * 4 <= 2 * kTile, "a wave's results fit its buffers");
+    if (c32 < n_rows)
+#pragma unroll
+        for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const int chunk = (8 * d + 2 * g + h) ^ (c32 & (kChunks - 1));
+                *reinterpret_cast<float4*>(lds + wave * 2 * kTile + c32 * (DH * 4) + chunk * 16) =
+                    make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+            }
+    __syncthreads();
+    const int bad_all = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
+    const int64_t slot = (int64_t)(k.slot + k.local) * a.Hk + hk;
+    float* const rec = w.part + slot * (kFewRows * (DH + 2));
+    const uint32_t again = uniform((int)(s_again[0] | s_again[1] | s_again[2] | s_again[3]));
+    if (again) {
+        for (int x = wave; x < n_rows; x += 4) {
+            if (!((again >> x) & 1u)) continue;
+            float m1, l1, o1[DH / 64];
+            const int rw = w0 + x, sees = min(ke, seen(q, rw, G));
+            row_again<DH, F16>(a, k.r, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
+            if (sees > bad_all) l1 = __builtin_nanf("");
+            if (parts > 1 && lane == 0) *reinterpret_cast<float2*>(rec + kFewRows * DH + 2 * x) = make_float2(m1, l1);
+#pragma unroll
+            for (int e = 0; e < DH / 64; e++) {
+                if (parts > 1) rec[x * DH + lane + 64 * e] = o1[e];
+                else store_out(a, out_at<DH>(a, q, rw, hk, G) + lane + 64 * e, sees ? o1[e] / l1 : 0.0f);
+            }
+        }
+    }
+    for (int i = threadIdx.x; i < n_rows * kChunks; i += 256) {
+        const int x = i / kChunks, f = i % kChunks;
+        if ((again >> x) & 1u) continue;
+        float2 ml[4];
+        float mx = ninf();
+#pragma unroll
+        for (int v = 0; v < 4; v++) ml[v] = s_ml[v][x], mx = fmaxf(mx, ml[v].x);
+        float sum = 0.0f, r0 = 0.0f, r1 = 0.0f, r2 = 0.0f, r3 = 0.0f;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            const float g = ml[v].x == ninf() ? 0.0f : __builtin_amdgcn_exp2f(ml[v].x - mx);
+            if (v >= n_tiles) break;  // a wave without keys
+            const float4 y = *reinterpret_cast<const float4*>(lds + v * 2 * kTile + x * (DH * 4) +
+                                                              (f ^ (x & (kChunks - 1))) * 16);
+            sum = fmaf(ml[v].y, ml[v].x == mx ? 1.0f : g, sum);
+            const float gg = ml[v].x == mx ? 1.0f : g;
+            r0 = fmaf(y.x, gg, r0), r1 = fmaf(y.y, gg, r1), r2 = fmaf(y.z, gg, r2), r3 = fmaf(y.w, gg, r3);
+        }
+        const int rw = w0 + x, sees = min(ke, seen(q, rw, G));
+        if (sees > bad_all) sum = __builtin_nanf("");
+        if (parts > 1) {
+            *reinterpret_cast<float4*>(rec + x * DH + 4 * f) = make_float4(r0, r1, r2, r3);
+            if (f == 0) *reinterpret_cast<float2*>(rec + kFewRows * DH + 2 * x) = make_float2(mx, sum);
+        } else if (sees) {
+            store_out4(a, out_at<DH>(a, q, rw, hk, G) + 4 * f, r0 / sum, r1 / sum, r2 / sum, r3 / sum);
+        } else {
+            store_out4(a, out_at<DH>(a, q, rw, hk, G) + 4 * f, 0.0f, 0.0f, 0.0f, 0.0f);
+        }
+    }
+}
+
+// ---- many rows -----------------------------------------------------------------------
+// Tiles of 128 rows, 32 a wave, over 64-key tiles that the waves load together into two
+// buffers: the next tile is on its way while one is used; one barrier a tile.
+template <int DH, bool F16, int PN>
+__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_many_kernel(Attn w) {
+    constexpr int kTile = 64 * DH * 2;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
+    __shared__ int s_bad[4];
+    const PagedAttnArgs& a = w.a;
+    const int hk = blockIdx.x % a.Hk, G = a.Hq / a.Hk;
+    const Work k = find_work<kManyRows, false>(w, blockIdx.x / a.Hk);
+    if (!k.ok) return;
+    // the last tiles (the longest) first
+    const int up = uniform(k.local / k.splits), tile = k.tiles - 1 - up, split = k.local - up * k.splits;
+    const Request q = k.q;
+    const int lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int rows = q.n * G, kb = split * k.per * kUnit;
+    const int end = uniform(seen(q, min(rows, (tile + 1) * kManyRows) - 1, G));
+    const int parts = max(1, (end + k.per * kUnit - 1) / (k.per * kUnit));
+    if (split >= parts) return;
+    const int ke = min(end, kb + k.per * kUnit);
+    const int w0 = tile * kManyRows + 32 * wave;  // the wave's first row
+    const int row = min(w0 + c32, rows - 1);
+    const int lim = min(ke, seen(q, row, G)), lim_lo = min(ke, seen(q, min(w0, rows - 1), G));
+    const int lim_hi = w0 < rows ? min(ke, seen(q, min(w0 + 31, rows - 1), G)) : 0;
+    uint4 qf[DH / 16];
+    load_q<DH>(a, q, row, hk, G, qf);
+    const float c = a.scale * kLog2e;
+    floatx16 o[DH / 32];
+#pragma unroll
+    for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    float m = ninf(), l = 0.0f;
+    const int n_tiles = (max(0, ke - kb) + 63) / 64;
+    // the wave loads keys 16 wave .. + 15 of a tile; lane 2 j + g holds the page of its group g in tile j
+    int ids = 0, bad_from = 0x7fffffff;
+    auto look_up = [&](int t) {
+        const int key = kb + (t + (lane >> 1)) * 64 + 16 * wave + (lane & 1) * 8;
+        int id = a.tables[(int64_t)k.r * a.max_blocks + (min(key, ke - 1) >> a.page_shift)];
+        if ((uint32_t)id >= (uint32_t)a.n_pages) {
+            if (key < ke) bad_from = min(bad_from, key);
+            id = 0;
+        }
+        ids = id;
+    };
+    auto load = [&](int t) {
+        if ((t & 31) == 0) look_up(t);
+        const uint32_t to = lds_addr(lds) + (t & 1) * 2 * kTile;
+#pragma unroll
+        for (int g = 0; g < 2; g++) {
+            const int64_t at = __builtin_amdgcn_readlane(ids, 2 * (t & 31) + g) * a.page_stride +
+                               (((int64_t)hk << a.page_shift) * DH);
+            const int key0 = kb + t * 64 + 16 * wave + 8 * g;
+            fill_group<DH, false>(a.k, at, a.page_shift, key0, ke - 1, 2 * wave + g, to);
+            fill_group<DH, true>(a.v, at, a.page_shift, key0, ke - 1, 2 * wave + g, to + kTile);
+        }
+    };
+    if (n_tiles > 0) load(0);
+    for (int t = 0; t < n_tiles; t++) {
+        const int k0 = kb + t * 64;
+        wait_vmem<0>();
+        wait_lds();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (t + 1 < n_tiles) load(t + 1);
+        if (k0 >= lim_hi) continue;
+        const uint8_t *const kt = lds + (t & 1) * 2 * kTile, *const vt = kt + kTile;
+        const bool edge = k0 + 64 > lim_lo;
+        floatx16 s[2] = {scores32<DH, F16>(kt, qf), scores32<DH, F16>(kt + 32 * 2 * DH, qf)};
+        soften<DH, F16, 2>(s, k0, lim, edge, c, m, l, o);
+#pragma unroll
+        for (int kk = 0; kk < 4; kk++) {
+            uint32_t p[4][PN];
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                split_pair<F16, PN>(s[kk >> 1][8 * (kk & 1) + 2 * e], s[kk >> 1][8 * (kk & 1) + 2 * e + 1], p[e]);
+            values16<DH, F16, PN>(vt + kk * 16 * 2 * DH, p, o);
+        }
+    }
+    l = pair32<false>(l);
+    const int bad = wave_min_int(bad_from);
+    if (lane == 0) s_bad[wave] = bad;
+    __syncthreads();
+    const int bad_all = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
+    const int64_t slot = (int64_t)(k.slot + tile * k.splits + split) * a.Hk + hk;
+    float* const rec = w.part + slot * (kManyRows * (DH + 2));
+    if (w0 >= rows) return;
+    const uint32_t again = rows_again<DH>(l, o, w0 + c32 < rows);
+    if (again) {
+        for (int x = 0; x < min(32, rows - w0); x++) {
+            if (!((again >> x) & 1u)) continue;
+            float m1, l1, o1[DH / 64];
+            const int rw = w0 + x, sees = min(ke, seen(q, rw, G)), y = 32 * wave + x;
+            row_again<DH, F16>(a, k.r, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
+            if (sees > bad_all) l1 = __builtin_nanf("");
+            if (parts > 1 && lane == 0) *reinterpret_cast<float2*>(rec + kManyRows * DH + 2 * y) = make_float2(m1, l1);
+#pragma unroll
+            for (int e = 0; e < DH / 64; e++) {
+                if (parts > 1) rec[y * DH + lane + 64 * e] = o1[e];
+                else store_out(a, out_at<DH>(a, q, rw, hk, G) + lane + 64 * e, sees ? o1[e] / l1 : 0.0f);
+            }
+        }
+    }
+    if (w0 + c32 >= rows || ((again >> c32) & 1u)) return;
+    if (lim > bad_all) l = __builtin_nanf("");
+    if (parts > 1) {
+        const int y = 32 * wave + c32;
+#pragma unroll
+        for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                *reinterpret_cast<float4*>(rec + y * DH + 32 * d + 8 * g + 4 * h) =
+                    make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+        if (h == 0) *reinterpret_cast<float2*>(rec + kManyRows * DH + 2 * y) = make_float2(m, l);
+        return;
+    }
+    const float inv = lim ? 1.0f / l : 0.0f;
+    const int64_t at = out_at<DH>(a, q, row, hk, G);
+#pragma unroll
+    for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            store_out4(a, at + 32 * d + 8 * g + 4 * h, o[d][4 * g] * inv, o[d][4 * g + 1] * inv, o[d][4 * g + 2] * inv,
+                       o[d][4 * g + 3] * inv);
+}
+
+// ---- joining the parts -----------------------------------------------------------------
+// A block takes one row tile of one kv head whose keys were split, a wave a row.
+template <int DH, int TR>
+__global__ __launch_bounds__(256) void paged_attn_merge_kernel(Attn w) {
+    const PagedAttnArgs& a = w.a;
+    const int hk = blockIdx.x % a.Hk, G = a.Hq / a.Hk;
+    const Work k = find_work<TR, true>(w, blockIdx.x / a.Hk);
+    if (!k.ok) return;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = k.local, rows = k.q.n * G;
+    const int end = seen(k.q, min(rows, (tile + 1) * TR) - 1, G);
+    const int parts = max(1, (end + k.per * kUnit - 1) / (k.per * kUnit));
+    if (parts == 1) return;
+    const int64_t size = (int64_t)TR * (DH + 2), step = a.Hk * size;
+    const float* const rec = w.part + ((int64_t)(k.slot + tile * k.splits) * a.Hk + hk) * size;
+    for (int x = wave; x < min(TR, rows - tile * TR); x += 4) {
+        const float* const ml = rec + TR * DH + 2 * x;
+        float mx = ninf();
+        for (int s = lane; s < parts; s += 64) mx = fmaxf(mx, ml[s * step]);
+        mx = wave_max(mx);
+        float l = 0.0f, o[DH / 64];
+#pragma unroll
+        for (int e = 0; e < DH / 64; e++) o[e] = 0.0f;
+        for (int s0 = 0; s0 < parts; s0 += 64) {
+            // (a part without keys of the row: a maximum of -inf, a sum of 0)
+            float f = 0.0f;
+            if (s0 + lane < parts) {
+                const float2 v = *reinterpret_cast<const float2*>(ml + (s0 + lane) * step);
+                f = v.x == mx ? 1.0f : __builtin_amdgcn_exp2f(v.x - mx);
+                l = fmaf(v.y, f, l);
+            }
+            for (int s = 0; s < min(64, parts - s0); s++) {
+                const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
+#pragma unroll
+                for (int e = 0; e < DH / 64; e++)
+                    o[e] = fmaf(rec[(s0 + s) * step + x * DH + lane + 64 * e], fs, o[e]);
+            }
+        }
+        l = wave_sum(l);
+        const int row = tile * TR + x, sees = seen(k.q, row, G);
+        const int64_t at = out_at<DH>(a, k.q, row, hk, G) + lane;
+#pragma unroll
+        for (int e = 0; e < DH / 64; e++) store_out(a, at + 64 * e, sees ? o[e] / l : 0.0f);
+    }
+}
+
+// Which kernels a call takes, and their grids. `max_new` is a hint: with at most 32 rows
+// per request as it says, the few-rows kernel takes every request (longer ones as several
+// tiles); else it takes those of at most 32 rows, the many-rows kernel the others.
+struct Launches {
+    Attn few, many;
+    int few_items, many_items;  // per kv head; 0: not launched
+    size_t few_bytes, many_bytes;
+};
+
+Launches launches(const PagedAttnArgs& a, int num_cus) {
+    const int64_t G = a.Hq / a.Hk, rows = (int64_t)a.n_rows * G;
+    Launches L{};
+    const bool only_few = std::min((int64_t)a.max_new * G, rows) <= kFewRows;
+    const int resident = num_cus * (a.Dh == 256 ? 1 : 2);
+    auto fill = [&](Attn& w, int64_t lo, int64_t hi, int min_units) {
+        w.a = a;
+        w.lo = (int)lo, w.hi = (int)std::min<int64_t>(hi, 0x7fffffff);
+        w.target = std::max(1, (resident + a.Hk - 1) / a.Hk);
+        w.min_units = min_units;
+    };
+    const int64_t requests = std::min<int64_t>(a.n_req, a.n_rows);
+    fill(L.few, 0, only_few ? rows : kFewRows, 2);
+    L.few_items = (int)(L.few.target + (only_few ? rows / kFewRows : 0) + requests);
+    fill(L.many, kFewRows, rows, 4);
+    if (!only_few)
+        L.many_items = (int)(L.many.target + rows / kManyRows + std::min(requests, rows / (kFewRows + 1)));
+    // a request of u units has ceil(u / C) <= 2 u / C parts where u > C, and all tiles' u
+    // over C are at most `target`
+    L.few_bytes = (size_t)2 * L.few.target * a.Hk * kFewRows * (a.Dh + 2) * sizeof(float);
+    L.many_bytes = only_few ? 0 : (size_t)2 * L.many.target * a.Hk * kManyRows * (a.Dh + 2) * sizeof(float);
+    return L;
+}
+
+}  // namespace
+
+size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus) {
+    const Launches L = launches(a, num_cus);
+    return L.few_bytes + L.many_bytes;
+}
+
+Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, hipStream_t st) {
+    Launches L = launches(a, num_cus);
+    L.few.part = static_cast<float*>(workspace);
+    L.many.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + L.few_bytes);
+    auto go = [&](auto kernel, const Attn& w, int64_t items) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(items * a.Hk)), dim3(256), 0, st, w);
+    };
+    auto with = [&](auto dh, auto f16) {
+        constexpr int DH = decltype(dh)::value;
+        constexpr bool F16 = decltype(f16)::value;
+        if (L.many_items) {
+            if (a.out_dt == JH_F32) go(paged_attn_many_kernel<DH, F16, 2>, L.many, L.many_items);
+            else go(paged_attn_many_kernel<DH, F16, 1>, L.many, L.many_items);
+            go(paged_attn_merge_kernel<DH, kManyRows>, L.many, L.many.target);
+        }
+        go(paged_attn_few_kernel<DH, F16>, L.few, L.few_items);
+        go(paged_attn_merge_kernel<DH, kFewRows>, L.few, L.few.target);
+    };
+    auto typed = [&](auto dh) { a.f16 ? with(dh, std::true_type{}) : with(dh, std::false_type{}); };
+    if (a.Dh == 64) typed(std::integral_constant<int, 64>{});
+    else if (a.Dh == 128) typed(std::integral_constant<int, 128>{});
+    else typed(std::integral_constant<int, 256>{});
+    return Status::ok();
+}
+
+}  // namespace jh

@@ -363,8 +363,8 @@ def check(hip, lens, Hq, Hk, D, page, dt, out_dts, pad=0, seed=0, spread=1.5):
 # single tokens: lengths around the key tiles and pages, requests without new tokens
 @pytest.mark.parametrize("lens", [[(1, 1)], [(1, 2)], [(1, 31)], [(1, 33)], [(1, 64), (1, 65)], [(1, 700)],
                                   [(1, 127), (0, 0), (1, 1), (0, 40), (1, 300)], [(1, 4099)]])
-@pytest.mark.parametrize("Hq,Hk,D,page,dt", [(8, 2, 128, 16, BF16), (4, 4, 64, 64, F16), (10, 2, 128, 4, F16),
-                                             (16, 1, 64, 1, BF16), (8, 1, 256, 16, BF16), (3, 1, 256, 128, F16)])
+@pytest.mark.parametrize("Hq,Hk,D,page,dt", [(8, 2, 128, 16, BF16), (4, 4, 64, 64, F16), (10, 2, 128, 8, F16),
+                                             (16, 1, 64, 32, BF16), (8, 1, 256, 16, BF16), (3, 1, 256, 128, F16)])
 def test_attention_one_token(hip, lens, Hq, Hk, D, page, dt):
     check(hip, lens, Hq, Hk, D, page, dt, (dt, F32), pad=len(lens) % 3)
 
@@ -373,7 +373,7 @@ def test_attention_one_token(hip, lens, Hq, Hk, D, page, dt):
 @pytest.mark.parametrize("lens", [[(2, 2)], [(4, 40)], [(5, 64), (3, 4)], [(9, 129)], [(33, 33)], [(32, 95), (1, 500), (64, 64)],
                                   [(130, 700), (2, 1200), (0, 9), (31, 31)], [(257, 257)]])
 @pytest.mark.parametrize("Hq,Hk,D,page,dt", [(8, 2, 128, 16, BF16), (4, 4, 64, 64, F16), (6, 2, 128, 8, F16),
-                                             (16, 1, 64, 2, BF16), (4, 2, 256, 32, BF16), (5, 1, 256, 16, F16)])
+                                             (16, 1, 64, 128, BF16), (4, 2, 256, 32, BF16), (5, 1, 256, 16, F16)])
 def test_attention_many_tokens(hip, lens, Hq, Hk, D, page, dt):
     check(hip, lens, Hq, Hk, D, page, dt, (BF16, F16, F32) if len(lens) < 3 else (dt, F32), pad=len(lens) % 3)
 
