@@ -113,21 +113,26 @@ __device__ __forceinline__ uint2 lds_read_tr(const uint8_t* p) {
 // ---- finding a block's work ---------------------------------------------------------
 struct Attn {
     PagedAttnArgs a;
-    int lo, hi;      // requests with lo < rows <= hi (rows = new tokens * G) are this launch's
+    int few;         // requests of at most this many rows (new tokens * G) take tiles of 32 rows, others of 128
     int target;      // parts of the keys to make, per kv head
-    int min_units;   // least units of keys per part
-    float* part;     // records of split parts: [rows of a tile][DH] results, then [rows][2] maximum and sum
+    int record;      // rows of a record
+    float* part;     // records of split parts: [record][DH] results, then [record][2] maximum and sum
 };
+// A unit of 64 keys counts kManyCost with a tile of 128 rows, 1 with one of 32.
+constexpr int kManyCost = 4;
+// Least keys of a part: 128 for tiles of 32 rows (a 32-key tile per wave), 256 for those of 128.
+constexpr int kLeastFew = 2, kLeastMany = 4;
 
 struct Request {
     int start, n, kv;
 };
 __device__ __forceinline__ Request request(const PagedAttnArgs& a, int r) {
     const int cap = a.max_blocks << a.page_shift;  // at most 2^30
+    const int from = a.row_starts[r], to = a.row_starts[r + 1], kv = a.kv_lens[r];
     Request q;
-    q.start = min(max(a.row_starts[r], 0), a.n_rows);
-    q.n = min(max(a.row_starts[r + 1], q.start), a.n_rows) - q.start;
-    q.kv = min(max(a.kv_lens[r], 0), cap);
+    q.start = min(max(from, 0), a.n_rows);
+    q.n = min(max(to, q.start), a.n_rows) - q.start;
+    q.kv = min(max(kv, 0), cap);
     return q;
 }
 
@@ -135,37 +140,67 @@ struct Work {
     bool ok;
     int r, local;     // the request, and the index among its items
     Request q;
+    bool few;
     int tiles, splits, per;  // row tiles; parts of the keys, `per` units each
     int slot;         // of its first record
 };
+
+// Sum over the lanes up to this one.
+template <class T>
+__device__ __forceinline__ T scan64(T v) {
+    auto dpp = [](T x, auto ctrl, auto rows) {
+        if constexpr (sizeof(T) == 8) {
+            const int2 u = __builtin_bit_cast(int2, x);
+            return __builtin_bit_cast(
+                T, make_int2(__builtin_amdgcn_update_dpp(0, u.x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false),
+                             __builtin_amdgcn_update_dpp(0, u.y, decltype(ctrl)::value, decltype(rows)::value, 0xF, false)));
+        } else {
+            return __builtin_amdgcn_update_dpp(0, x, decltype(ctrl)::value, decltype(rows)::value, 0xF, false);
+        }
+    };
+    v += dpp(v, std::integral_constant<int, 0x111>{}, std::integral_constant<int, 0xF>{});  // row_shr:1
+    v += dpp(v, std::integral_constant<int, 0x112>{}, std::integral_constant<int, 0xF>{});  // row_shr:2
+    v += dpp(v, std::integral_constant<int, 0x114>{}, std::integral_constant<int, 0xF>{});  // row_shr:4
+    v += dpp(v, std::integral_constant<int, 0x118>{}, std::integral_constant<int, 0xF>{});  // row_shr:8
+    v += dpp(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xA>{});  // row_bcast:15
+    v += dpp(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xC>{});  // row_bcast:31
+    return v;
+}
 
 // The item `index` of all requests: tiles * splits items per request, or, with MERGE, the
 // row tiles of requests whose keys are split. By every wave of a block for itself: a lane
 // sums a run of requests, a scan over the lanes, and the run that holds the item is
 // walked by all lanes together.
-template <int TR, bool MERGE>
+template <bool MERGE>
 __device__ __forceinline__ Work find_work(const Attn& w, int index) {
     const PagedAttnArgs& a = w.a;
     const int lane = threadIdx.x & 63, G = a.Hq / a.Hk, run = (a.n_req + 63) / 64;
     auto tiles_of = [&](const Request& q) {
         const int rows = q.n * G;
-        return rows > w.lo && rows <= w.hi ? (rows + TR - 1) / TR : 0;
+        return rows <= w.few ? (rows + kFewRows - 1) / kFewRows : (rows + kManyRows - 1) / kManyRows;
     };
     auto units_of = [&](const Request& q) { return max(1, (q.kv + kUnit - 1) / kUnit); };
-    int64_t all = 0;
+    auto cost_of = [&](const Request& q) { return q.n * G <= w.few ? 1 : kManyCost; };
+    double all = 0.0;  // exact: below 2^53
     Request mine{0, 0, 0};
     for (int e = 0; e < run; e++) {
         const int r = lane * run + e;
         if (r >= a.n_req) break;
         const Request q = request(a, r);
         if (e == 0) mine = q;
-        all += (int64_t)tiles_of(q) * units_of(q);
+        all += (double)tiles_of(q) * (double)units_of(q) * (double)cost_of(q);
     }
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) all += __shfl_xor(all, d, 64);
-    const int64_t each = (all + w.target - 1) / w.target;
-    const int most = (int)min(max(each, (int64_t)w.min_units), (int64_t)0x40000000);  // units per part
-    auto splits_of = [&](const Request& q) { return (units_of(q) + most - 1) / most; };
+    all = scan64(all);
+    const double total = __builtin_bit_cast(
+        double, make_int2(__builtin_amdgcn_readlane(__builtin_bit_cast(int2, all).x, 63),
+                          __builtin_amdgcn_readlane(__builtin_bit_cast(int2, all).y, 63)));
+    // most that a part may cost: at least total / target
+    const int most = (int)min(total / (double)w.target + 1.0, 1073741824.0);
+    auto splits_of = [&](const Request& q) {
+        const bool few = q.n * G <= w.few;
+        const int each = few ? max(most, kLeastFew) : max(most / kManyCost + 1, kLeastMany);  // units per part
+        return max(1, (units_of(q) + each / 2) / each);
+    };
     int items = 0, slots = 0;
     for (int e = 0; e < run; e++) {
         const int r = lane * run + e;
@@ -175,16 +210,11 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
         items += MERGE ? (s > 1 ? t : 0) : t * s;
         slots += s > 1 ? t * s : 0;
     }
-    int upto = items, slots_upto = slots;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int x = __shfl_up(upto, d, 64), y = __shfl_up(slots_upto, d, 64);
-        if (lane >= d) upto += x, slots_upto += y;
-    }
+    const int upto = scan64(items), slots_upto = scan64(slots);
     const uint64_t past = __ballot(upto > index);
     Work o{};
     if (!past) return o;
-    const int at = __builtin_amdgcn_readfirstlane(__ffsll((unsigned long long)past) - 1);
+    const int at = uniform(__ffsll((unsigned long long)past) - 1);
     int left = index - __builtin_amdgcn_readlane(upto - items, at);
     int slot = __builtin_amdgcn_readlane(slots_upto - slots, at);
     for (int e = 0; e < run; e++) {
@@ -202,6 +232,7 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
         if (left < count) {
             o.ok = true, o.r = uniform(r), o.local = uniform(left), o.tiles = uniform(t), o.splits = uniform(s);
             o.q = Request{uniform(q.start), uniform(q.n), uniform(q.kv)};
+            o.few = o.q.n * G <= w.few;
             o.per = uniform((units_of(q) + s - 1) / s);
             o.slot = uniform(slot);
             // (row_starts that go up and down can make more parts than were counted)
@@ -418,16 +449,13 @@ __device__ __forceinline__ int wave_min_int(int v) {
 // while a tile's scores become weights the next tile's keys are on their way, while its
 // values are used the next values. The waves' results meet in LDS.
 template <int DH, bool F16>
-__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_few_kernel(Attn w) {
+__device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, uint8_t* lds) {
     constexpr int kTile = 32 * DH * 2, kLoads = kTile / 1024;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[8 * kTile];
     __shared__ float2 s_ml[4][32];
     __shared__ int s_bad[4];
     __shared__ uint32_t s_again[4];
     const PagedAttnArgs& a = w.a;
-    const int hk = blockIdx.x % a.Hk, G = a.Hq / a.Hk;
-    const Work k = find_work<kFewRows, false>(w, blockIdx.x / a.Hk);
-    if (!k.ok) return;
+    const int G = a.Hq / a.Hk;
     const int tile = uniform(k.local / k.splits), split = k.local - tile * k.splits;
     const Request q = k.q;
     const int lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31;
@@ -526,7 +554,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_few_kernel(
     __syncthreads();
     const int bad_all = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
     const int64_t slot = (int64_t)(k.slot + k.local) * a.Hk + hk;
-    float* const rec = w.part + slot * (kFewRows * (DH + 2));
+    float *const rec = w.part + slot * (w.record * (DH + 2)), *const rec_ml = rec + w.record * DH;
     const uint32_t again = uniform((int)(s_again[0] | s_again[1] | s_again[2] | s_again[3]));
     if (again) {
         for (int x = wave; x < n_rows; x += 4) {
@@ -535,7 +563,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_few_kernel(
             const int rw = w0 + x, sees = min(ke, seen(q, rw, G));
             row_again<DH, F16>(a, k.r, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
             if (sees > bad_all) l1 = __builtin_nanf("");
-            if (parts > 1 && lane == 0) *reinterpret_cast<float2*>(rec + kFewRows * DH + 2 * x) = make_float2(m1, l1);
+            if (parts > 1 && lane == 0) *reinterpret_cast<float2*>(rec_ml + 2 * x) = make_float2(m1, l1);
 #pragma unroll
             for (int e = 0; e < DH / 64; e++) {
                 if (parts > 1) rec[x * DH + lane + 64 * e] = o1[e];
@@ -565,7 +593,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_few_kernel(
         if (sees > bad_all) sum = __builtin_nanf("");
         if (parts > 1) {
             *reinterpret_cast<float4*>(rec + x * DH + 4 * f) = make_float4(r0, r1, r2, r3);
-            if (f == 0) *reinterpret_cast<float2*>(rec + kFewRows * DH + 2 * x) = make_float2(mx, sum);
+            if (f == 0) *reinterpret_cast<float2*>(rec_ml + 2 * x) = make_float2(mx, sum);
         } else if (sees) {
             store_out4(a, out_at<DH>(a, q, rw, hk, G) + 4 * f, r0 / sum, r1 / sum, r2 / sum, r3 / sum);
         } else {
@@ -578,14 +606,11 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_few_kernel(
 // Tiles of 128 rows, 32 a wave, over 64-key tiles that the waves load together into two
 // buffers: the next tile is on its way while one is used; one barrier a tile.
 template <int DH, bool F16, int PN>
-__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_many_kernel(Attn w) {
+__device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, uint8_t* lds) {
     constexpr int kTile = 64 * DH * 2;
-    __shared__ __attribute__((aligned(16))) uint8_t lds[4 * kTile];
     __shared__ int s_bad[4];
     const PagedAttnArgs& a = w.a;
-    const int hk = blockIdx.x % a.Hk, G = a.Hq / a.Hk;
-    const Work k = find_work<kManyRows, false>(w, blockIdx.x / a.Hk);
-    if (!k.ok) return;
+    const int G = a.Hq / a.Hk;
     // the last tiles (the longest) first
     const int up = uniform(k.local / k.splits), tile = k.tiles - 1 - up, split = k.local - up * k.splits;
     const Request q = k.q;
@@ -661,7 +686,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_many_kernel
     __syncthreads();
     const int bad_all = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
     const int64_t slot = (int64_t)(k.slot + tile * k.splits + split) * a.Hk + hk;
-    float* const rec = w.part + slot * (kManyRows * (DH + 2));
+    float *const rec = w.part + slot * (w.record * (DH + 2)), *const rec_ml = rec + w.record * DH;
     if (w0 >= rows) return;
     const uint32_t again = rows_again<DH>(l, o, w0 + c32 < rows);
     if (again) {
@@ -671,7 +696,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_many_kernel
             const int rw = w0 + x, sees = min(ke, seen(q, rw, G)), y = 32 * wave + x;
             row_again<DH, F16>(a, k.r, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
             if (sees > bad_all) l1 = __builtin_nanf("");
-            if (parts > 1 && lane == 0) *reinterpret_cast<float2*>(rec + kManyRows * DH + 2 * y) = make_float2(m1, l1);
+            if (parts > 1 && lane == 0) *reinterpret_cast<float2*>(rec_ml + 2 * y) = make_float2(m1, l1);
 #pragma unroll
             for (int e = 0; e < DH / 64; e++) {
                 if (parts > 1) rec[y * DH + lane + 64 * e] = o1[e];
@@ -689,7 +714,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_many_kernel
             for (int g = 0; g < 4; g++)
                 *reinterpret_cast<float4*>(rec + y * DH + 32 * d + 8 * g + 4 * h) =
                     make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
-        if (h == 0) *reinterpret_cast<float2*>(rec + kManyRows * DH + 2 * y) = make_float2(m, l);
+        if (h == 0) *reinterpret_cast<float2*>(rec_ml + 2 * y) = make_float2(m, l);
         return;
     }
     const float inv = lim ? 1.0f / l : 0.0f;
@@ -702,108 +727,143 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_many_kernel
                        o[d][4 * g + 3] * inv);
 }
 
+// PN: terms of a probability in tiles of 128 rows; 0: a call of tiles of 32 rows alone.
+template <int DH, bool F16, int PN>
+__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_kernel(Attn w) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[8 * 32 * DH * 2];  // of either: 64 KB at a head_dim of 128
+    // heads fastest: with 8 kv heads all tiles of a head share one XCD's L2
+    const int hk = blockIdx.x % w.a.Hk;
+    const Work k = find_work<false>(w, blockIdx.x / w.a.Hk);
+    if (!k.ok) return;
+    if constexpr (PN > 0)
+        if (!k.few) {
+            many_rows<DH, F16, PN>(w, k, hk, lds);
+            return;
+        }
+    few_rows<DH, F16>(w, k, hk, lds);
+}
+
 // ---- joining the parts -----------------------------------------------------------------
-// A block takes one row tile of one kv head whose keys were split, a wave a row.
-template <int DH, int TR>
+// A block takes rows of one tile of one kv head whose keys were split: 256 / (DH / 4)
+// groups of lanes (4 features each), as many of them to a row as it has parts; they
+// meet in LDS in their order.
+template <int DH>
 __global__ __launch_bounds__(256) void paged_attn_merge_kernel(Attn w) {
+    constexpr int kLanes = DH / 4, kGroups = 256 / kLanes;
+    __shared__ float4 s_o[kGroups][kLanes];
+    __shared__ float2 s_ml[kGroups];
     const PagedAttnArgs& a = w.a;
     const int hk = blockIdx.x % a.Hk, G = a.Hq / a.Hk;
-    const Work k = find_work<TR, true>(w, blockIdx.x / a.Hk);
+    const Work k = find_work<true>(w, blockIdx.x / a.Hk);
     if (!k.ok) return;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, tile = k.local, rows = k.q.n * G;
-    const int end = seen(k.q, min(rows, (tile + 1) * TR) - 1, G);
+    const int tile = k.local, rows = k.q.n * G, tr = k.few ? kFewRows : kManyRows;
+    const int end = uniform(seen(k.q, min(rows, (tile + 1) * tr) - 1, G));
     const int parts = max(1, (end + k.per * kUnit - 1) / (k.per * kUnit));
     if (parts == 1) return;
-    const int64_t size = (int64_t)TR * (DH + 2), step = a.Hk * size;
+    const int64_t size = (int64_t)w.record * (DH + 2), step = a.Hk * size;
     const float* const rec = w.part + ((int64_t)(k.slot + tile * k.splits) * a.Hk + hk) * size;
-    for (int x = wave; x < min(TR, rows - tile * TR); x += 4) {
-        const float* const ml = rec + TR * DH + 2 * x;
-        float mx = ninf();
-        for (int s = lane; s < parts; s += 64) mx = fmaxf(mx, ml[s * step]);
-        mx = wave_max(mx);
-        float l = 0.0f, o[DH / 64];
+    const int f = threadIdx.x % kLanes, group = threadIdx.x / kLanes, count = min(tr, rows - tile * tr);
+    int each = 1;  // groups to a row
+    while (each < kGroups && each < parts) each *= 2;
+    const int sub = group % each, at_once = kGroups / each;
+    for (int x0 = blockIdx.y * at_once; x0 < count; x0 += gridDim.y * at_once) {
+        const int x = min(x0 + group / each, count - 1);
+        const float *const ml = rec + (int64_t)w.record * DH + 2 * x, *const v = rec + (int64_t)x * DH + 4 * f;
+        // (a part without keys of the row: a maximum of -inf, a sum of 0)
+        float mx = ninf(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        constexpr int kBatch = 8;  // parts requested together
+        for (int s0 = sub; s0 < parts; s0 += each * kBatch) {
+            float2 u[kBatch];
+            float4 y[kBatch];
+            float top = mx;
 #pragma unroll
-        for (int e = 0; e < DH / 64; e++) o[e] = 0.0f;
-        for (int s0 = 0; s0 < parts; s0 += 64) {
-            // (a part without keys of the row: a maximum of -inf, a sum of 0)
-            float f = 0.0f;
-            if (s0 + lane < parts) {
-                const float2 v = *reinterpret_cast<const float2*>(ml + (s0 + lane) * step);
-                f = v.x == mx ? 1.0f : __builtin_amdgcn_exp2f(v.x - mx);
-                l = fmaf(v.y, f, l);
+            for (int i = 0; i < kBatch; i++) {
+                const int64_t at = min(s0 + i * each, parts - 1) * step;
+                u[i] = *reinterpret_cast<const float2*>(ml + at);
+                y[i] = *reinterpret_cast<const float4*>(v + at);
             }
-            for (int s = 0; s < min(64, parts - s0); s++) {
-                const float fs = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), s));
 #pragma unroll
-                for (int e = 0; e < DH / 64; e++)
-                    o[e] = fmaf(rec[(s0 + s) * step + x * DH + lane + 64 * e], fs, o[e]);
+            for (int i = 0; i < kBatch; i++) top = fmaxf(top, s0 + i * each < parts ? u[i].x : top);
+            const float f = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
+            l *= f, o[0] *= f, o[1] *= f, o[2] *= f, o[3] *= f;
+            mx = top;
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) {
+                if (s0 + i * each >= parts) break;
+                const float g = u[i].x == mx ? 1.0f : __builtin_amdgcn_exp2f(u[i].x - mx);
+                l = fmaf(u[i].y, g, l);
+                o[0] = fmaf(y[i].x, g, o[0]), o[1] = fmaf(y[i].y, g, o[1]);
+                o[2] = fmaf(y[i].z, g, o[2]), o[3] = fmaf(y[i].w, g, o[3]);
             }
         }
-        l = wave_sum(l);
-        const int row = tile * TR + x, sees = seen(k.q, row, G);
-        const int64_t at = out_at<DH>(a, k.q, row, hk, G) + lane;
-#pragma unroll
-        for (int e = 0; e < DH / 64; e++) store_out(a, at + 64 * e, sees ? o[e] / l : 0.0f);
+        __syncthreads();  // (the round before has read)
+        s_o[group][f] = make_float4(o[0], o[1], o[2], o[3]);
+        if (f == 0) s_ml[group] = make_float2(mx, l);
+        __syncthreads();
+        if (sub != 0 || x0 + group / each >= count) continue;
+        for (int g = 1; g < each; g++) mx = fmaxf(mx, s_ml[group + g].x);
+        l = o[0] = o[1] = o[2] = o[3] = 0.0f;
+        for (int g = 0; g < each; g++) {
+            const float2 u = s_ml[group + g];
+            const float4 y = s_o[group + g][f];
+            const float h = u.x == mx ? 1.0f : __builtin_amdgcn_exp2f(u.x - mx);
+            l = fmaf(u.y, h, l);
+            o[0] = fmaf(y.x, h, o[0]), o[1] = fmaf(y.y, h, o[1]), o[2] = fmaf(y.z, h, o[2]), o[3] = fmaf(y.w, h, o[3]);
+        }
+        const int row = tile * tr + x;
+        const bool sees = seen(k.q, row, G) > 0;
+        store_out4(a, out_at<DH>(a, k.q, row, hk, G) + 4 * f, sees ? o[0] / l : 0.0f, sees ? o[1] / l : 0.0f,
+                   sees ? o[2] / l : 0.0f, sees ? o[3] / l : 0.0f);
     }
 }
 
-// Which kernels a call takes, and their grids. `max_new` is a hint: with at most 32 rows
-// per request as it says, the few-rows kernel takes every request (longer ones as several
-// tiles); else it takes those of at most 32 rows, the many-rows kernel the others.
-struct Launches {
-    Attn few, many;
-    int few_items, many_items;  // per kv head; 0: not launched
-    size_t few_bytes, many_bytes;
+// A call's tiles and grid. `max_new` is a hint: with at most 32 rows per request as it
+// says, every request takes tiles of 32 rows (longer ones several); else those of more
+// rows take tiles of 128.
+struct Launch {
+    Attn w;
+    bool only_few;
+    int items, merges, merge_rows;  // blocks per kv head; blocks to a joined tile
+    size_t bytes;
 };
 
-Launches launches(const PagedAttnArgs& a, int num_cus) {
-    const int64_t G = a.Hq / a.Hk, rows = (int64_t)a.n_rows * G;
-    Launches L{};
-    const bool only_few = std::min((int64_t)a.max_new * G, rows) <= kFewRows;
+Launch plan_launch(const PagedAttnArgs& a, int num_cus) {
+    const int64_t G = a.Hq / a.Hk, rows = (int64_t)a.n_rows * G, requests = std::min(a.n_req, a.n_rows);
+    Launch L{};
+    L.only_few = std::min((int64_t)a.max_new * G, rows) <= kFewRows;
     const int resident = num_cus * (a.Dh == 256 ? 1 : 2);
-    auto fill = [&](Attn& w, int64_t lo, int64_t hi, int min_units) {
-        w.a = a;
-        w.lo = (int)lo, w.hi = (int)std::min<int64_t>(hi, 0x7fffffff);
-        w.target = std::max(1, (resident + a.Hk - 1) / a.Hk);
-        w.min_units = min_units;
-    };
-    const int64_t requests = std::min<int64_t>(a.n_req, a.n_rows);
-    fill(L.few, 0, only_few ? rows : kFewRows, 2);
-    L.few_items = (int)(L.few.target + (only_few ? rows / kFewRows : 0) + requests);
-    fill(L.many, kFewRows, rows, 4);
-    if (!only_few)
-        L.many_items = (int)(L.many.target + rows / kManyRows + std::min(requests, rows / (kFewRows + 1)));
-    // a request of u units has ceil(u / C) <= 2 u / C parts where u > C, and all tiles' u
-    // over C are at most `target`
-    L.few_bytes = (size_t)2 * L.few.target * a.Hk * kFewRows * (a.Dh + 2) * sizeof(float);
-    L.many_bytes = only_few ? 0 : (size_t)2 * L.many.target * a.Hk * kManyRows * (a.Dh + 2) * sizeof(float);
+    L.w.a = a;
+    L.w.few = L.only_few ? 0x7fffffff : kFewRows;
+    L.w.target = std::max(1, (resident + a.Hk - 1) / a.Hk);
+    L.w.record = (int)(std::min<int64_t>(rows, L.only_few ? kFewRows : kManyRows) + 3) / 4 * 4;  // whole 16 bytes
+    // a request of t tiles of u units has u / C parts, rounded, at least one, and all t * u / C
+    // together are at most `target`: items are at most `target` and one for each tile,
+    // parts of split requests (u / C from 3/2 on) at most 4/3 `target`
+    const int64_t tiles = requests + rows / (L.only_few ? kFewRows : kManyRows);
+    L.items = (int)(L.w.target + tiles);
+    L.merges = (int)std::min<int64_t>(L.w.target, tiles);
+    L.merge_rows = L.only_few ? 4 : 16;
+    L.bytes = (size_t)2 * L.w.target * a.Hk * L.w.record * (a.Dh + 2) * sizeof(float);
     return L;
 }
 
 }  // namespace
 
-size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus) {
-    const Launches L = launches(a, num_cus);
-    return L.few_bytes + L.many_bytes;
-}
+size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus) { return plan_launch(a, num_cus).bytes; }
 
 Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, hipStream_t st) {
-    Launches L = launches(a, num_cus);
-    L.few.part = static_cast<float*>(workspace);
-    L.many.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + L.few_bytes);
-    auto go = [&](auto kernel, const Attn& w, int64_t items) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(items * a.Hk)), dim3(256), 0, st, w);
+    Launch L = plan_launch(a, num_cus);
+    L.w.part = static_cast<float*>(workspace);
+    auto go = [&](auto kernel, int64_t x, int y) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(x * a.Hk), (unsigned)y), dim3(256), 0, st, L.w);
     };
     auto with = [&](auto dh, auto f16) {
         constexpr int DH = decltype(dh)::value;
         constexpr bool F16 = decltype(f16)::value;
-        if (L.many_items) {
-            if (a.out_dt == JH_F32) go(paged_attn_many_kernel<DH, F16, 2>, L.many, L.many_items);
-            else go(paged_attn_many_kernel<DH, F16, 1>, L.many, L.many_items);
-            go(paged_attn_merge_kernel<DH, kManyRows>, L.many, L.many.target);
-        }
-        go(paged_attn_few_kernel<DH, F16>, L.few, L.few_items);
-        go(paged_attn_merge_kernel<DH, kFewRows>, L.few, L.few.target);
+        if (L.only_few) go(paged_attn_kernel<DH, F16, 0>, L.items, 1);
+        else if (a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2>, L.items, 1);
+        else go(paged_attn_kernel<DH, F16, 1>, L.items, 1);
+        go(paged_attn_merge_kernel<DH>, L.merges, L.merge_rows);
     };
     auto typed = [&](auto dh) { a.f16 ? with(dh, std::true_type{}) : with(dh, std::false_type{}); };
     if (a.Dh == 64) typed(std::integral_constant<int, 64>{});

@@ -1245,9 +1245,9 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
     if (n_req < 0 || n_rows < 0 || max_new < 0 || max_blocks < 0)
         return fail(c, JH_ERR_INVALID, std::string(op) + ": bad shape");
     if (page_size < 8) return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": pages of fewer than 8 keys");
-    if (n_rows > 0x7fffffff || n_rows * n_heads > 0x7fffffff || n_req > 65536 || max_blocks > ((int64_t)1 << 30) / page_size)
+    if (n_rows > (1 << 30) || n_rows * n_heads > (1 << 30) || n_req > 65536 || max_blocks > ((int64_t)1 << 30) / page_size)
         return fail(c, JH_ERR_UNSUPPORTED,
-                    std::string(op) + ": too large (n_rows * n_heads below 2^31, n_req to 65536, max_blocks * page_size to 2^30)");
+                    std::string(op) + ": too large (n_rows * n_heads to 2^30, n_req to 65536, max_blocks * page_size to 2^30)");
     if (q_stride < n_heads * head_dim || q_stride % 8 || q_stride > ((int64_t)1 << 32))
         return fail(c, JH_ERR_INVALID, std::string(op) + ": q_stride must hold a row and be a multiple of 8");
     if (!(scale >= 1e-30f) || !(scale < __builtin_inff()))
