@@ -119,9 +119,10 @@ struct Attn {
     float* part;     // records of split parts: [record][DH] results, then [record][2] maximum and sum
 };
 // A unit of 64 keys counts kManyCost with a tile of 128 rows, 1 with one of 32.
-constexpr int kManyCost = 4;
-// Least keys of a part: 128 for tiles of 32 rows (a 32-key tile per wave), 256 for those of 128.
-constexpr int kLeastFew = 2, kLeastMany = 4;
+constexpr int kManyCost = 1;
+// Least units of a part: two (a 32-key tile per wave), and one more for every kRowsPerUnit
+// rows of results that a part writes and the merge reads.
+constexpr int kLeast = 2, kRowsPerUnit = 21;
 
 struct Request {
     int start, n, kv;
@@ -197,8 +198,9 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
     // most that a part may cost: at least total / target
     const int most = (int)min(total / (double)w.target + 1.0, 1073741824.0);
     auto splits_of = [&](const Request& q) {
-        const bool few = q.n * G <= w.few;
-        const int each = few ? max(most, kLeastFew) : max(most / kManyCost + 1, kLeastMany);  // units per part
+        const int rows = q.n * G;
+        const int each = max(rows <= w.few ? most : most / kManyCost + 1,
+                             kLeast + min(rows, rows <= w.few ? kFewRows : kManyRows) / kRowsPerUnit);  // units per part
         return max(1, (units_of(q) + each / 2) / each);
     };
     int items = 0, slots = 0;
@@ -331,19 +333,51 @@ __device__ __forceinline__ int perm_k(int key) { return DH == 64 ? (key >> 1) & 
 template <int DH>
 __device__ __forceinline__ int perm_v(int key) { return DH == 64 ? 4 * ((key >> 1) & 1) : 4 * (key & 3); }
 
-// Eight keys from key0 on (one page) of one head, keys or values: DH / 64 loads of 1 KB.
-// `last`: the last key that may be loaded. `g`: the group's number in its tile.
-template <int DH, bool V>
-__device__ __forceinline__ void fill_group(const uint16_t* pool, int64_t page_at, int shift, int key0, int last, int g,
-                                           uint32_t lds) {
-    const int lane = threadIdx.x & 63, first = min(key0, last), more = last - first;
-    const uint16_t* const base = pool + page_at + (int64_t)(first & ((1 << shift) - 1)) * DH;
+// A group of eight keys (they lie in one page) of one head, keys or values, into rows
+// 8 g .. of the tile at `lds`: DH / 64 loads of 1 KB. `at`: bytes from the pool to the
+// group's first key, or to the last that may be loaded where that is an earlier one;
+// `more`: rows that follow it.
+template <int DH>
+struct Filler {
+    static constexpr int kN = DH / 64;
+    uint32_t k[kN], v[kN];  // the lane's part of the addresses in a whole group (k: of even g)
+    __device__ __forceinline__ Filler() {
+        const int lane = threadIdx.x & 63;
 #pragma unroll
-    for (int u = 0; u < DH / 64; u++) {
-        const int row = (u * 64 + lane) / (DH / 8), place = (u * 64 + lane) % (DH / 8), key = 8 * g + row;
-        const int chunk = place ^ (V ? perm_v<DH>(key) : perm_k<DH>(key));
-        lds_fill16(base, (uint32_t)(min(row, more) * (2 * DH) + 16 * chunk), lds + g * (16 * DH) + u * 1024);
+        for (int u = 0; u < kN; u++) {
+            const int row = (u * 64 + lane) / (DH / 8), place = (u * 64 + lane) % (DH / 8);
+            k[u] = row * (2 * DH) + 16 * (place ^ perm_k<DH>(row));
+            v[u] = row * (2 * DH) + 16 * (place ^ perm_v<DH>(row));
+        }
     }
+    template <bool V, bool WHOLE>
+    __device__ __forceinline__ void fill(const uint16_t* pool, int64_t at, int g, uint32_t lds, int more = 0) const {
+        const char* const base = reinterpret_cast<const char*>(pool) + at;
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int u = 0; u < kN; u++) {
+            // (eight keys on, perm_k changes by one bit)
+            uint32_t off = V ? v[u] : k[u] ^ ((g & 1) * (16 * perm_k<DH>(8)));
+            if constexpr (!WHOLE) {
+                const int row = (u * 64 + lane) / (DH / 8);
+                off -= max(0, row - more) * (2 * DH);
+            }
+            lds_fill16(base, off, lds + g * (16 * DH) + u * 1024);
+        }
+    }
+};
+
+// Bytes from a pool to key `key` of head hk; pages outside the pool give page 0.
+template <int DH>
+__device__ __forceinline__ int64_t key_at(const PagedAttnArgs& a, int r, int hk, int key, bool& outside) {
+    int id = a.tables[(int64_t)r * a.max_blocks + (key >> a.page_shift)];
+    outside = (uint32_t)id >= (uint32_t)a.n_pages;
+    if (outside) id = 0;
+    return 2 * (id * a.page_stride + (((int64_t)hk << a.page_shift) + (key & ((1 << a.page_shift) - 1))) * DH);
+}
+__device__ __forceinline__ int64_t lane_of(int64_t v, int lane) {
+    return (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32 |
+                     (uint32_t)__builtin_amdgcn_readlane((int)v, lane));
 }
 
 // The lane's row of q as B fragments: step kk holds features 16 kk + 8 h .. + 8.
@@ -388,8 +422,8 @@ __device__ __forceinline__ void values16(const uint8_t* vt, const uint32_t (&t)[
 
 // One tile of 32 * N keys (from k0) of the online softmax: scores to weights in place.
 template <int DH, bool F16, int N>
-__device__ __forceinline__ void soften(floatx16 (&s)[N], int k0, int lim, bool edge, float c, float& m, float& l,
-                                       floatx16 (&o)[DH / 32]) {
+__device__ __forceinline__ float mask_and_move(floatx16 (&s)[N], int k0, int lim, bool edge, float c, float& m, float& l,
+                                               floatx16 (&o)[DH / 32]) {
     const int h = (threadIdx.x & 63) >> 5;
     // register r of s[g] is key k0 + 32 g + 8 (r / 4) + 4 h + r % 4
     if (edge) {
@@ -415,14 +449,20 @@ __device__ __forceinline__ void soften(floatx16 (&s)[N], int k0, int lim, bool e
             for (int r = 0; r < 16; r++) o[d][r] *= f;
         m = mn;
     }
-    const float neg = m == ninf() ? 0.0f : kPShift<F16> - m;
+    return m == ninf() ? 0.0f : kPShift<F16> - m;
+}
+// (neg: mask_and_move's)
+template <int N>
+__device__ __forceinline__ void weigh(floatx16 (&s)[N], float c, float neg, float& l) {
+    float sum = 0.0f;
 #pragma unroll
     for (int g = 0; g < N; g++)
 #pragma unroll
         for (int r = 0; r < 16; r++) {
             s[g][r] = __builtin_amdgcn_exp2f(fmaf(s[g][r], c, neg));
-            l += s[g][r];
+            sum += s[g][r];
         }
+    l += sum;
 }
 
 // The wave's rows (bit lane % 32) whose results are not finite.
@@ -481,25 +521,29 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
     const int n_tiles = (max(0, ke - kb) + 31) / 32;
     const uint8_t *const kt = lds + wave * 2 * kTile, *const vt = kt + kTile;
     const uint32_t to = lds_addr(kt);
-    // pages of the wave's next 16 tiles: lane 4 j + g holds group g of its tile j's
-    int ids = 0, bad_from = 0x7fffffff;
+    // where the groups of the wave's next 16 tiles lie: lane 4 j + g holds group g of its tile j's
+    const Filler<DH> fill;
+    int64_t where = 0;
+    int bad_from = 0x7fffffff;
     auto look_up = [&](int t) {
         const int key = kb + (t + 4 * (lane >> 2)) * 32 + (lane & 3) * 8;
-        int id = a.tables[(int64_t)k.r * a.max_blocks + (min(key, ke - 1) >> a.page_shift)];
-        if ((uint32_t)id >= (uint32_t)a.n_pages) {
-            if (key < ke) bad_from = min(bad_from, key);
-            id = 0;
-        }
-        ids = id;
-    };
-    auto page_at = [&](int j, int g) {
-        return __builtin_amdgcn_readlane(ids, 4 * j + g) * a.page_stride + (((int64_t)hk << a.page_shift) * DH);
+        bool outside;
+        where = key_at<DH>(a, k.r, hk, min(key, ke - 1), outside);
+        if (outside && key < ke) bad_from = min(bad_from, key);
     };
     auto load = [&](auto v, int t, int j) {
         constexpr bool V = decltype(v)::value;
+        const int k0 = kb + t * 32;
+        const uint16_t* const pool = V ? a.v : a.k;
+        const uint32_t at = to + (V ? kTile : 0);
+        if (k0 + 32 <= ke) {
 #pragma unroll
-        for (int g = 0; g < 4; g++)
-            fill_group<DH, V>(V ? a.v : a.k, page_at(j, g), a.page_shift, kb + t * 32 + 8 * g, ke - 1, g, to + (V ? kTile : 0));
+            for (int g = 0; g < 4; g++) fill.template fill<V, true>(pool, lane_of(where, 4 * j + g), g, at);
+        } else {
+#pragma unroll
+            for (int g = 0; g < 4; g++)
+                fill.template fill<V, false>(pool, lane_of(where, 4 * j + g), g, at, max(0, ke - 1 - (k0 + 8 * g)));
+        }
     };
     using K = std::false_type;
     using Vals = std::true_type;
@@ -519,7 +563,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
             if (jn == 0) look_up(next);
             load(K{}, next, jn);
         }
-        soften<DH, F16, 1>(s, k0, lim, edge, c, m, l, o);
+        weigh<1>(s, c, mask_and_move<DH, F16, 1>(s, k0, lim, edge, c, m, l, o), l);
         if (more) wait_vmem<kLoads>();
         else wait_vmem<0>();
 #pragma unroll
@@ -635,42 +679,58 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
         for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
     float m = ninf(), l = 0.0f;
     const int n_tiles = (max(0, ke - kb) + 63) / 64;
-    // the wave loads keys 16 wave .. + 15 of a tile; lane 2 j + g holds the page of its group g in tile j
-    int ids = 0, bad_from = 0x7fffffff;
-    auto look_up = [&](int t) {
-        const int key = kb + (t + (lane >> 1)) * 64 + 16 * wave + (lane & 1) * 8;
-        int id = a.tables[(int64_t)k.r * a.max_blocks + (min(key, ke - 1) >> a.page_shift)];
-        if ((uint32_t)id >= (uint32_t)a.n_pages) {
-            if (key < ke) bad_from = min(bad_from, key);
-            id = 0;
+    // the wave loads keys 16 wave .. + 15 of a tile; lane 2 j + g holds where its group g of tile j
+    // of 32 lies, for keys and (a tile behind) for values
+    const Filler<DH> fill;
+    int64_t where[2] = {0, 0};
+    int bad_from = 0x7fffffff;
+    auto load = [&](auto vals, int t) {
+        constexpr bool V = decltype(vals)::value;
+        if (t >= n_tiles) return;
+        const int k0 = kb + t * 64 + 16 * wave;
+        if ((t & 31) == 0) {
+            const int key = k0 + (lane >> 1) * 64 + (lane & 1) * 8;
+            bool outside;
+            where[V] = key_at<DH>(a, k.r, hk, min(key, ke - 1), outside);
+            if (outside && key < ke) bad_from = min(bad_from, key);
         }
-        ids = id;
-    };
-    auto load = [&](int t) {
-        if ((t & 31) == 0) look_up(t);
-        const uint32_t to = lds_addr(lds) + (t & 1) * 2 * kTile;
+        const uint32_t to = lds_addr(lds) + ((t & 1) * 2 + V) * kTile + wave * (32 * DH);
+        const uint16_t* const pool = V ? a.v : a.k;
+        if (k0 + 16 <= ke) {
 #pragma unroll
-        for (int g = 0; g < 2; g++) {
-            const int64_t at = __builtin_amdgcn_readlane(ids, 2 * (t & 31) + g) * a.page_stride +
-                               (((int64_t)hk << a.page_shift) * DH);
-            const int key0 = kb + t * 64 + 16 * wave + 8 * g;
-            fill_group<DH, false>(a.k, at, a.page_shift, key0, ke - 1, 2 * wave + g, to);
-            fill_group<DH, true>(a.v, at, a.page_shift, key0, ke - 1, 2 * wave + g, to + kTile);
+            for (int g = 0; g < 2; g++) fill.template fill<V, true>(pool, lane_of(where[V], 2 * (t & 31) + g), g, to);
+        } else {
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+                fill.template fill<V, false>(pool, lane_of(where[V], 2 * (t & 31) + g), g, to,
+                                             max(0, ke - 1 - (k0 + 8 * g)));
         }
     };
-    if (n_tiles > 0) load(0);
-    for (int t = 0; t < n_tiles; t++) {
-        const int k0 = kb + t * 64;
+    using Keys = std::false_type;
+    using Vals = std::true_type;
+    auto meet = [&]() {
         wait_vmem<0>();
         wait_lds();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (t + 1 < n_tiles) load(t + 1);
-        if (k0 >= lim_hi) continue;
-        const uint8_t *const kt = lds + (t & 1) * 2 * kTile, *const vt = kt + kTile;
-        const bool edge = k0 + 64 > lim_lo;
-        floatx16 s[2] = {scores32<DH, F16>(kt, qf), scores32<DH, F16>(kt + 32 * 2 * DH, qf)};
-        soften<DH, F16, 2>(s, k0, lim, edge, c, m, l, o);
+    };
+    // A tile's scores are made while the one before it becomes weights: the products and the
+    // exponentials do not depend on each other.
+    load(Keys{}, 0);
+    meet();
+    load(Vals{}, 0);
+    load(Keys{}, 1);
+    auto step = [&](int t, floatx16 (&s)[2], floatx16 (&next)[2]) {
+        const int k0 = kb + t * 64;
+        meet();  // this tile's values and the next one's keys are there, the last ones are used
+        load(Vals{}, t + 1);
+        load(Keys{}, t + 2);
+        if (k0 >= lim_hi) return;
+        const uint8_t *const kt = lds + ((t + 1) & 1) * 2 * kTile, *const vt = lds + ((t & 1) * 2 + 1) * kTile;
+        const float neg = mask_and_move<DH, F16, 2>(s, k0, lim, k0 + 64 > lim_lo, c, m, l, o);
+        next[0] = scores32<DH, F16>(kt, qf);
+        next[1] = scores32<DH, F16>(kt + 32 * 2 * DH, qf);
+        weigh<2>(s, c, neg, l);
 #pragma unroll
         for (int kk = 0; kk < 4; kk++) {
             uint32_t p[4][PN];
@@ -679,6 +739,11 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
                 split_pair<F16, PN>(s[kk >> 1][8 * (kk & 1) + 2 * e], s[kk >> 1][8 * (kk & 1) + 2 * e + 1], p[e]);
             values16<DH, F16, PN>(vt + kk * 16 * 2 * DH, p, o);
         }
+    };
+    floatx16 s0[2] = {scores32<DH, F16>(lds, qf), scores32<DH, F16>(lds + 32 * 2 * DH, qf)}, s1[2];
+    for (int t = 0; t < n_tiles; t += 2) {
+        step(t, s0, s1);
+        if (t + 1 < n_tiles) step(t + 1, s1, s0);
     }
     l = pair32<false>(l);
     const int bad = wave_min_int(bad_from);
@@ -744,12 +809,13 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_kernel(Attn
 }
 
 // ---- joining the parts -----------------------------------------------------------------
-// A block takes rows of one tile of one kv head whose keys were split: 256 / (DH / 4)
-// groups of lanes (4 features each), as many of them to a row as it has parts; they
-// meet in LDS in their order.
+// A block takes rows of one tile of one kv head whose keys were split: groups of DH / 4
+// lanes, 4 features each, one to a row for every 8 parts (all requested together); a
+// row's groups meet in LDS in their order.
+constexpr int kMergeThreads = 512, kMergeBatch = 8;
 template <int DH>
-__global__ __launch_bounds__(256) void paged_attn_merge_kernel(Attn w) {
-    constexpr int kLanes = DH / 4, kGroups = 256 / kLanes;
+__global__ __launch_bounds__(kMergeThreads) void paged_attn_merge_kernel(Attn w) {
+    constexpr int kLanes = DH / 4, kGroups = kMergeThreads / kLanes, kBatch = kMergeBatch;
     __shared__ float4 s_o[kGroups][kLanes];
     __shared__ float2 s_ml[kGroups];
     const PagedAttnArgs& a = w.a;
@@ -764,14 +830,13 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(Attn w) {
     const float* const rec = w.part + ((int64_t)(k.slot + tile * k.splits) * a.Hk + hk) * size;
     const int f = threadIdx.x % kLanes, group = threadIdx.x / kLanes, count = min(tr, rows - tile * tr);
     int each = 1;  // groups to a row
-    while (each < kGroups && each < parts) each *= 2;
+    while (each < kGroups && each * kBatch < parts) each *= 2;
     const int sub = group % each, at_once = kGroups / each;
     for (int x0 = blockIdx.y * at_once; x0 < count; x0 += gridDim.y * at_once) {
         const int x = min(x0 + group / each, count - 1);
         const float *const ml = rec + (int64_t)w.record * DH + 2 * x, *const v = rec + (int64_t)x * DH + 4 * f;
         // (a part without keys of the row: a maximum of -inf, a sum of 0)
         float mx = ninf(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        constexpr int kBatch = 8;  // parts requested together
         for (int s0 = sub; s0 < parts; s0 += each * kBatch) {
             float2 u[kBatch];
             float4 y[kBatch];
@@ -796,14 +861,16 @@ __global__ __launch_bounds__(256) void paged_attn_merge_kernel(Attn w) {
                 o[2] = fmaf(y[i].z, g, o[2]), o[3] = fmaf(y[i].w, g, o[3]);
             }
         }
-        __syncthreads();  // (the round before has read)
-        s_o[group][f] = make_float4(o[0], o[1], o[2], o[3]);
-        if (f == 0) s_ml[group] = make_float2(mx, l);
-        __syncthreads();
+        if (each > 1) {
+            __syncthreads();  // (the round before has read)
+            s_o[group][f] = make_float4(o[0], o[1], o[2], o[3]);
+            if (f == 0) s_ml[group] = make_float2(mx, l);
+            __syncthreads();
+        }
         if (sub != 0 || x0 + group / each >= count) continue;
         for (int g = 1; g < each; g++) mx = fmaxf(mx, s_ml[group + g].x);
-        l = o[0] = o[1] = o[2] = o[3] = 0.0f;
-        for (int g = 0; g < each; g++) {
+        if (each > 1) l = o[0] = o[1] = o[2] = o[3] = 0.0f;
+        for (int g = 0; each > 1 && g < each; g++) {
             const float2 u = s_ml[group + g];
             const float4 y = s_o[group + g][f];
             const float h = u.x == mx ? 1.0f : __builtin_amdgcn_exp2f(u.x - mx);
@@ -831,18 +898,25 @@ Launch plan_launch(const PagedAttnArgs& a, int num_cus) {
     const int64_t G = a.Hq / a.Hk, rows = (int64_t)a.n_rows * G, requests = std::min(a.n_req, a.n_rows);
     Launch L{};
     L.only_few = std::min((int64_t)a.max_new * G, rows) <= kFewRows;
-    const int resident = num_cus * (a.Dh == 256 ? 1 : 2);
     L.w.a = a;
     L.w.few = L.only_few ? 0x7fffffff : kFewRows;
-    L.w.target = std::max(1, (resident + a.Hk - 1) / a.Hk);
+    const int64_t tiles = requests + rows / (L.only_few ? kFewRows : kManyRows);
+    // blocks resident at once (LDS; at a head_dim of 64 registers), per kv head
+    const int per_cu = a.Dh == 256 ? 1 : a.Dh == 128 ? 2 : L.only_few ? 4 : 3;
+    const int64_t room = std::max<int64_t>(1, num_cus * per_cu / a.Hk);
+    const int64_t parts = L.only_few ? (2 * tiles <= room ? room - tiles : 2 * room)
+                                     : std::max((room + 1) / 2, room - tiles / 2);
+    L.w.target = (int)std::max<int64_t>(1, parts);
     L.w.record = (int)(std::min<int64_t>(rows, L.only_few ? kFewRows : kManyRows) + 3) / 4 * 4;  // whole 16 bytes
     // a request of t tiles of u units has u / C parts, rounded, at least one, and all t * u / C
     // together are at most `target`: items are at most `target` and one for each tile,
     // parts of split requests (u / C from 3/2 on) at most 4/3 `target`
-    const int64_t tiles = requests + rows / (L.only_few ? kFewRows : kManyRows);
     L.items = (int)(L.w.target + tiles);
     L.merges = (int)std::min<int64_t>(L.w.target, tiles);
-    L.merge_rows = L.only_few ? 4 : 16;
+    // rows of a tile (as the hint says) times the groups that an average request's parts want
+    const int64_t mr = std::min<int64_t>(std::max(a.max_new, 1) * G, L.only_few ? kFewRows : kManyRows);
+    const int64_t groups = kMergeThreads / (a.Dh / 4), want = (L.w.target / tiles + kMergeBatch - 1) / kMergeBatch;
+    L.merge_rows = (int)std::max<int64_t>(1, (mr * std::max<int64_t>(1, std::min(want, groups)) + groups - 1) / groups);
     L.bytes = (size_t)2 * L.w.target * a.Hk * L.w.record * (a.Dh + 2) * sizeof(float);
     return L;
 }
@@ -854,16 +928,16 @@ size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus) { return 
 Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, hipStream_t st) {
     Launch L = plan_launch(a, num_cus);
     L.w.part = static_cast<float*>(workspace);
-    auto go = [&](auto kernel, int64_t x, int y) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(x * a.Hk), (unsigned)y), dim3(256), 0, st, L.w);
+    auto go = [&](auto kernel, int64_t x, int y, int threads) {
+        hipLaunchKernelGGL(kernel, dim3((unsigned)(x * a.Hk), (unsigned)y), dim3(threads), 0, st, L.w);
     };
     auto with = [&](auto dh, auto f16) {
         constexpr int DH = decltype(dh)::value;
         constexpr bool F16 = decltype(f16)::value;
-        if (L.only_few) go(paged_attn_kernel<DH, F16, 0>, L.items, 1);
-        else if (a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2>, L.items, 1);
-        else go(paged_attn_kernel<DH, F16, 1>, L.items, 1);
-        go(paged_attn_merge_kernel<DH>, L.merges, L.merge_rows);
+        if (L.only_few) go(paged_attn_kernel<DH, F16, 0>, L.items, 1, 256);
+        else if (a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2>, L.items, 1, 256);
+        else go(paged_attn_kernel<DH, F16, 1>, L.items, 1, 256);
+        go(paged_attn_merge_kernel<DH>, L.merges, L.merge_rows, kMergeThreads);
     };
     auto typed = [&](auto dh) { a.f16 ? with(dh, std::true_type{}) : with(dh, std::false_type{}); };
     if (a.Dh == 64) typed(std::integral_constant<int, 64>{});
