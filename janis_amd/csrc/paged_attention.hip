@@ -49,7 +49,6 @@ template <bool F16>
 constexpr float kLazy = F16 ? 2.0f : 8.0f;
 
 __device__ __forceinline__ float ninf() { return -__builtin_inff(); }
-__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7F800000u) != 0x7F800000u; }
 
 template <bool F16>
 __device__ __forceinline__ floatx16 mfma(uint4 a, uint4 b, floatx16 c) {
@@ -468,12 +467,12 @@ __device__ __forceinline__ void weigh(floatx16 (&s)[N], float c, float neg, floa
 // The wave's rows (bit lane % 32) whose results are not finite.
 template <int DH>
 __device__ __forceinline__ uint32_t rows_again(float l, const floatx16 (&o)[DH / 32], bool live) {
-    bool bad = !finite(l);
+    float z = l * 0.0f;  // NaN once something is not finite
 #pragma unroll
     for (int d = 0; d < DH / 32; d++)
 #pragma unroll
-        for (int r = 0; r < 16; r++) bad |= !finite(o[d][r]);
-    const uint64_t votes = __ballot(bad && live);
+        for (int r = 0; r < 16; r++) z = fmaf(o[d][r], 0.0f, z);
+    const uint64_t votes = __ballot(z != z && live);
     return (uint32_t)votes | (uint32_t)(votes >> 32);
 }
 
@@ -484,16 +483,16 @@ __device__ __forceinline__ int wave_min_int(int v) {
 }
 
 // ---- few rows ------------------------------------------------------------------------
-// Tiles of 32 rows: decode (a token's G heads) and short runs of new tokens. The four
+// Tiles of 32 rows: decode (a token's G heads) and short runs of new tokens. The NW
 // waves take the part's 32-key tiles in turn, each with its own buffers and no barrier:
 // while a tile's scores become weights the next tile's keys are on their way, while its
 // values are used the next values. The waves' results meet in LDS.
-template <int DH, bool F16>
+template <int DH, bool F16, int NW>
 __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, uint8_t* lds) {
     constexpr int kTile = 32 * DH * 2, kLoads = kTile / 1024;
-    __shared__ float2 s_ml[4][32];
-    __shared__ int s_bad[4];
-    __shared__ uint32_t s_again[4];
+    __shared__ float2 s_ml[NW][32];
+    __shared__ int s_bad[NW];
+    __shared__ uint32_t s_again[NW];
     const PagedAttnArgs& a = w.a;
     const int G = a.Hq / a.Hk;
     const int tile = uniform(k.local / k.splits), split = k.local - tile * k.splits;
@@ -526,7 +525,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
     int64_t where = 0;
     int bad_from = 0x7fffffff;
     auto look_up = [&](int t) {
-        const int key = kb + (t + 4 * (lane >> 2)) * 32 + (lane & 3) * 8;
+        const int key = kb + (t + NW * (lane >> 2)) * 32 + (lane & 3) * 8;
         bool outside;
         where = key_at<DH>(a, k.r, hk, min(key, ke - 1), outside);
         if (outside && key < ke) bad_from = min(bad_from, key);
@@ -553,8 +552,8 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
         load(Vals{}, wave, 0);
     }
     int j = 0;
-    for (int t = wave; t < n_tiles; t += 4) {
-        const int k0 = kb + t * 32, next = t + 4, jn = (j + 1) & 15;
+    for (int t = wave; t < n_tiles; t += NW) {
+        const int k0 = kb + t * 32, next = t + NW, jn = (j + 1) & 15;
         const bool more = next < n_tiles, edge = k0 + 32 > lim_lo;
         wait_vmem<kLoads>();
         floatx16 s[1] = {scores32<DH, F16>(kt, qf)};
@@ -596,12 +595,15 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
                     make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
             }
     __syncthreads();
-    const int bad_all = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
+    int bad_all = s_bad[0];
+    uint32_t votes = s_again[0];
+#pragma unroll
+    for (int v = 1; v < NW; v++) bad_all = min(bad_all, s_bad[v]), votes |= s_again[v];
     const int64_t slot = (int64_t)(k.slot + k.local) * a.Hk + hk;
     float *const rec = w.part + slot * (w.record * (DH + 2)), *const rec_ml = rec + w.record * DH;
-    const uint32_t again = uniform((int)(s_again[0] | s_again[1] | s_again[2] | s_again[3]));
+    const uint32_t again = uniform((int)votes);
     if (again) {
-        for (int x = wave; x < n_rows; x += 4) {
+        for (int x = wave; x < n_rows; x += NW) {
             if (!((again >> x) & 1u)) continue;
             float m1, l1, o1[DH / 64];
             const int rw = w0 + x, sees = min(ke, seen(q, rw, G));
@@ -615,16 +617,16 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
             }
         }
     }
-    for (int i = threadIdx.x; i < n_rows * kChunks; i += 256) {
+    for (int i = threadIdx.x; i < n_rows * kChunks; i += 64 * NW) {
         const int x = i / kChunks, f = i % kChunks;
         if ((again >> x) & 1u) continue;
-        float2 ml[4];
+        float2 ml[NW];
         float mx = ninf();
 #pragma unroll
-        for (int v = 0; v < 4; v++) ml[v] = s_ml[v][x], mx = fmaxf(mx, ml[v].x);
+        for (int v = 0; v < NW; v++) ml[v] = s_ml[v][x], mx = fmaxf(mx, ml[v].x);
         float sum = 0.0f, r0 = 0.0f, r1 = 0.0f, r2 = 0.0f, r3 = 0.0f;
 #pragma unroll
-        for (int v = 0; v < 4; v++) {
+        for (int v = 0; v < NW; v++) {
             const float g = ml[v].x == ninf() ? 0.0f : __builtin_amdgcn_exp2f(ml[v].x - mx);
             if (v >= n_tiles) break;  // a wave without keys
             const float4 y = *reinterpret_cast<const float4*>(lds + v * 2 * kTile + x * (DH * 4) +
@@ -647,19 +649,24 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
 }
 
 // ---- many rows -----------------------------------------------------------------------
-// Tiles of 128 rows, 32 a wave, over 64-key tiles that the waves load together into two
-// buffers: the next tile is on its way while one is used; one barrier a tile.
-template <int DH, bool F16, int PN>
+// Tiles of 128 rows, 32 a wave, over 64-key tiles that four waves load together into two
+// buffers: the next tile is on its way while one is used; one barrier a tile. Eight waves
+// are two such groups that take the tiles in turn and join their results in LDS: where a
+// CU has one tile of rows only, its keys are walked in half the time.
+template <int DH, bool F16, int PN, int NW>
 __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, uint8_t* lds) {
     constexpr int kTile = 64 * DH * 2;
-    __shared__ int s_bad[4];
+    constexpr int NG = NW / 4;
+    __shared__ int s_bad[NW];
+    __shared__ float2 s_ml[128];
     const PagedAttnArgs& a = w.a;
     const int G = a.Hq / a.Hk;
     // the last tiles (the longest) first
     const int up = uniform(k.local / k.splits), tile = k.tiles - 1 - up, split = k.local - up * k.splits;
     const Request q = k.q;
     const int lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31;
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = all_waves / 4, wave = all_waves & 3;
+    lds += group * 4 * kTile;
     const int rows = q.n * G, kb = split * k.per * kUnit;
     const int end = uniform(seen(q, min(rows, (tile + 1) * kManyRows) - 1, G));
     const int parts = max(1, (end + k.per * kUnit - 1) / (k.per * kUnit));
@@ -678,7 +685,8 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
 #pragma unroll
         for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
     float m = ninf(), l = 0.0f;
-    const int n_tiles = (max(0, ke - kb) + 63) / 64;
+    // the group's tiles, and the first group's (barriers are for all)
+    const int n_all = (max(0, ke - kb) + 63) / 64, n_tiles = max(0, (n_all - group + NG - 1) / NG), n_steps = (n_all + NG - 1) / NG;
     // the wave loads keys 16 wave .. + 15 of a tile; lane 2 j + g holds where its group g of tile j
     // of 32 lies, for keys and (a tile behind) for values
     const Filler<DH> fill;
@@ -687,9 +695,9 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
     auto load = [&](auto vals, int t) {
         constexpr bool V = decltype(vals)::value;
         if (t >= n_tiles) return;
-        const int k0 = kb + t * 64 + 16 * wave;
-        if ((t & 31) == 0) {
-            const int key = k0 + (lane >> 1) * 64 + (lane & 1) * 8;
+        const int k0 = kb + (t * NG + group) * 64 + 16 * wave;
+        if ((t & 31) == 0 && (!V || t > 0)) {
+            const int key = k0 + (lane >> 1) * (64 * NG) + (lane & 1) * 8;
             bool outside;
             where[V] = key_at<DH>(a, k.r, hk, min(key, ke - 1), outside);
             if (outside && key < ke) bad_from = min(bad_from, key);
@@ -709,23 +717,27 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
     using Keys = std::false_type;
     using Vals = std::true_type;
     auto meet = [&]() {
-        wait_vmem<0>();
         wait_lds();
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
     };
     // A tile's scores are made while the one before it becomes weights: the products and the
     // exponentials do not depend on each other.
+    constexpr int kLoads = 2 * (DH / 64);  // of a wave and tile
     load(Keys{}, 0);
-    meet();
+    where[1] = where[0];
     load(Vals{}, 0);
     load(Keys{}, 1);
+    if (n_tiles > 1) wait_vmem<2 * kLoads>();
+    else wait_vmem<kLoads>();
+    meet();
     auto step = [&](int t, floatx16 (&s)[2], floatx16 (&next)[2]) {
-        const int k0 = kb + t * 64;
+        const int k0 = kb + (t * NG + group) * 64;
+        wait_vmem<0>();
         meet();  // this tile's values and the next one's keys are there, the last ones are used
         load(Vals{}, t + 1);
         load(Keys{}, t + 2);
-        if (k0 >= lim_hi) return;
+        if (t >= n_tiles || k0 >= lim_hi) return;
         const uint8_t *const kt = lds + ((t + 1) & 1) * 2 * kTile, *const vt = lds + ((t & 1) * 2 + 1) * kTile;
         const float neg = mask_and_move<DH, F16, 2>(s, k0, lim, k0 + 64 > lim_lo, c, m, l, o);
         next[0] = scores32<DH, F16>(kt, qf);
@@ -741,15 +753,45 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
         }
     };
     floatx16 s0[2] = {scores32<DH, F16>(lds, qf), scores32<DH, F16>(lds + 32 * 2 * DH, qf)}, s1[2];
-    for (int t = 0; t < n_tiles; t += 2) {
+    for (int t = 0; t < n_steps; t += 2) {
         step(t, s0, s1);
-        if (t + 1 < n_tiles) step(t + 1, s1, s0);
+        if (t + 1 < n_steps) step(t + 1, s1, s0);
     }
     l = pair32<false>(l);
     const int bad = wave_min_int(bad_from);
-    if (lane == 0) s_bad[wave] = bad;
+    if (lane == 0) s_bad[all_waves] = bad;
     __syncthreads();
-    const int bad_all = min(min(s_bad[0], s_bad[1]), min(s_bad[2], s_bad[3]));
+    int bad_all = s_bad[0];
+#pragma unroll
+    for (int v = 1; v < NW; v++) bad_all = min(bad_all, s_bad[v]);
+    if constexpr (NG == 2) {
+        // the second group's results, as its lanes hold them
+        float4* const theirs = reinterpret_cast<float4*>(lds + (group ? 0 : 4 * kTile)) + wave * (8 * DH) + lane;
+        if (group) {
+#pragma unroll
+            for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+                for (int g = 0; g < 4; g++)
+                    theirs[(4 * d + g) * 64] = make_float4(o[d][4 * g], o[d][4 * g + 1], o[d][4 * g + 2], o[d][4 * g + 3]);
+            if (h == 0) s_ml[32 * wave + c32] = make_float2(m, l);
+        }
+        __syncthreads();
+        if (group) return;
+        const float2 ml = s_ml[32 * wave + c32];
+        const float mx = fmaxf(m, ml.x);
+        const float f0 = m == mx ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+        const float f1 = ml.x == mx ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mx);
+        m = mx;
+        l = l * f0 + ml.y * f1;
+#pragma unroll
+        for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+            for (int g = 0; g < 4; g++) {
+                const float4 y = theirs[(4 * d + g) * 64];
+                o[d][4 * g] = o[d][4 * g] * f0 + y.x * f1, o[d][4 * g + 1] = o[d][4 * g + 1] * f0 + y.y * f1;
+                o[d][4 * g + 2] = o[d][4 * g + 2] * f0 + y.z * f1, o[d][4 * g + 3] = o[d][4 * g + 3] * f0 + y.w * f1;
+            }
+    }
     const int64_t slot = (int64_t)(k.slot + tile * k.splits + split) * a.Hk + hk;
     float *const rec = w.part + slot * (w.record * (DH + 2)), *const rec_ml = rec + w.record * DH;
     if (w0 >= rows) return;
@@ -793,19 +835,19 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
 }
 
 // PN: terms of a probability in tiles of 128 rows; 0: a call of tiles of 32 rows alone.
-template <int DH, bool F16, int PN>
-__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void paged_attn_kernel(Attn w) {
-    __shared__ __attribute__((aligned(16))) uint8_t lds[8 * 32 * DH * 2];  // of either: 64 KB at a head_dim of 128
+template <int DH, bool F16, int PN, int NW>
+__global__ __launch_bounds__(64 * NW, DH == 256 || NW == 8 ? 1 : 2) void paged_attn_kernel(Attn w) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * NW * 32 * DH * 2];  // of either: 16 KB a wave at a head_dim of 128
     // heads fastest: with 8 kv heads all tiles of a head share one XCD's L2
     const int hk = blockIdx.x % w.a.Hk;
     const Work k = find_work<false>(w, blockIdx.x / w.a.Hk);
     if (!k.ok) return;
     if constexpr (PN > 0)
         if (!k.few) {
-            many_rows<DH, F16, PN>(w, k, hk, lds);
+            many_rows<DH, F16, PN, NW>(w, k, hk, lds);
             return;
         }
-    few_rows<DH, F16>(w, k, hk, lds);
+    few_rows<DH, F16, NW>(w, k, hk, lds);
 }
 
 // ---- joining the parts -----------------------------------------------------------------
@@ -889,7 +931,7 @@ __global__ __launch_bounds__(kMergeThreads) void paged_attn_merge_kernel(Attn w)
 // rows take tiles of 128.
 struct Launch {
     Attn w;
-    bool only_few;
+    bool only_few, wide;  // wide: blocks of eight waves
     int items, merges, merge_rows;  // blocks per kv head; blocks to a joined tile
     size_t bytes;
 };
@@ -901,8 +943,9 @@ Launch plan_launch(const PagedAttnArgs& a, int num_cus) {
     L.w.a = a;
     L.w.few = L.only_few ? 0x7fffffff : kFewRows;
     const int64_t tiles = requests + rows / (L.only_few ? kFewRows : kManyRows);
+    L.wide = !L.only_few && a.Dh != 256 && tiles * a.Hk <= num_cus;
     // blocks resident at once (LDS; at a head_dim of 64 registers), per kv head
-    const int per_cu = a.Dh == 256 ? 1 : a.Dh == 128 ? 2 : L.only_few ? 4 : 3;
+    const int per_cu = a.Dh == 256 || L.wide ? 1 : a.Dh == 128 ? 2 : L.only_few ? 4 : 3;
     const int64_t room = std::max<int64_t>(1, num_cus * per_cu / a.Hk);
     const int64_t parts = L.only_few ? (2 * tiles <= room ? room - tiles : 2 * room)
                                      : std::max((room + 1) / 2, room - tiles / 2);
@@ -934,9 +977,13 @@ Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, h
     auto with = [&](auto dh, auto f16) {
         constexpr int DH = decltype(dh)::value;
         constexpr bool F16 = decltype(f16)::value;
-        if (L.only_few) go(paged_attn_kernel<DH, F16, 0>, L.items, 1, 256);
-        else if (a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2>, L.items, 1, 256);
-        else go(paged_attn_kernel<DH, F16, 1>, L.items, 1, 256);
+        if (L.only_few) go(paged_attn_kernel<DH, F16, 0, 4>, L.items, 1, 256);
+        else if (!L.wide && a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2, 4>, L.items, 1, 256);
+        else if (!L.wide) go(paged_attn_kernel<DH, F16, 1, 4>, L.items, 1, 256);
+        if constexpr (DH != 256) {  // (its tiles fill the LDS)
+            if (L.wide && a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2, 8>, L.items, 1, 512);
+            else if (L.wide) go(paged_attn_kernel<DH, F16, 1, 8>, L.items, 1, 512);
+        }
         go(paged_attn_merge_kernel<DH>, L.merges, L.merge_rows, kMergeThreads);
     };
     auto typed = [&](auto dh) { a.f16 ? with(dh, std::true_type{}) : with(dh, std::false_type{}); };
