@@ -652,7 +652,7 @@ enum {
  *                   nothing. With JH_CHECK_INDICES it is read back and is
  *                   JH_ERR_INVALID here.
  * Apart from the two aliases, outputs overlap neither inputs nor each other.
- * n_req up to 2048 (JH_ERR_UNSUPPORTED beyond). */
+ * n_req up to 2048, n_rows and n_pages to 2^30 (JH_ERR_UNSUPPORTED beyond). */
 JH_API int jh_paged_plan(jh_ctx *ctx, const int32_t *new_lens, const int32_t *kv_lens, int64_t n_req,
                          int64_t n_rows, int64_t page_size, int32_t *block_tables, int64_t max_blocks,
                          int32_t *free_pages, int64_t n_pages, const int32_t *free_count,

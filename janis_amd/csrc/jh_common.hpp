@@ -468,8 +468,9 @@ struct PagedAppendArgs {
     int n_rows, Hq, Hk, Dh;
     int64_t qkv_stride;
     const void *qn_w, *kn_w;  // [Dh] or nullptr
-    int w_dt;
+    int w_dt, w_wide;         // w_wide: the weights are 16-byte aligned
     float eps, base, scale;   // base 0 without freqs: no rotation
+    double log2_step;         // log2 of base^(-2 / Dh)
     const float* freqs;
     const int32_t *positions, *slots;
     uint16_t *k, *v;

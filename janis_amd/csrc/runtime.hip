@@ -6,6 +6,7 @@
 // GatherQuantMatmul buckets by expert on the device (gather.hip).
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <cstdio>
 #include <cstring>
 #include <mutex>
@@ -1151,11 +1152,11 @@ int jh_paged_plan(jh_ctx* c, const int32_t* new_lens, const int32_t* kv_lens, in
     if (int r = enter(c)) return r;
     const char* op = "jh_paged_plan";
     if (int r = check_pages(c, op, JH_BF16, n_pages, page_size)) return r;
-    if (n_req < 0 || n_rows < 0 || n_rows > 0x7fffffff || max_blocks < 0 || max_blocks > 0x7fffffff)
+    if (n_req < 0 || n_rows < 0 || max_blocks < 0 || max_blocks > 0x7fffffff)
         return fail(c, JH_ERR_INVALID, std::string(op) + ": bad shape");
-    if (n_req > jh::kPlanMaxReq)
+    if (n_req > jh::kPlanMaxReq || n_rows > (1 << 30) || n_pages > (1 << 30))
         return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": more than " + std::to_string(jh::kPlanMaxReq) +
-                                               " requests");
+                                               " requests, or 2^30 rows or pages");
     if (!free_count || !free_count_out || !row_starts || !status || (n_pages > 0 && !free_pages) ||
         (n_rows > 0 && (!positions || !slots)) ||
         (n_req > 0 && (!new_lens || !kv_lens || !kv_lens_out || (max_blocks > 0 && !block_tables))))
@@ -1220,7 +1221,9 @@ int jh_paged_qk_norm_rope_append(jh_ctx* c, const void* qkv, jh_dtype qkv_dtype,
     a.n_rows = (int)n_rows, a.Hq = (int)n_heads, a.Hk = (int)n_kv_heads, a.Dh = (int)head_dim;
     a.qkv_stride = qkv_stride;
     a.qn_w = q_norm_w, a.kn_w = k_norm_w, a.w_dt = w_dtype;
+    a.w_wide = aligned16(q_norm_w) && aligned16(k_norm_w);
     a.eps = eps, a.base = rope_base, a.scale = rope_scale, a.freqs = rope_freqs;
+    a.log2_step = rope_base > 0.0f ? -2.0 / (double)head_dim * std::log2((double)rope_base) : 0.0;
     a.positions = positions, a.slots = slots;
     a.k = static_cast<uint16_t*>(k_pages), a.v = static_cast<uint16_t*>(v_pages);
     a.kv_f16 = page_dtype == JH_F16;
