@@ -106,7 +106,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
     else if (count < 0 || count > a.n_pages || (back_over ? about[1] > about[2] : take_over || total[1] > top))
         status = JH_PLAN_PAGES;
     else if (back_over || top > a.n_pages) status = JH_PLAN_TABLE;
-    const int n_rows = total[0], n_take = total[1], n_back = total[2];
+    const int n_rows = total[0], n_take = total[1], n_back = total[2], n_most = max(n_take, n_back);
     // the number of page `k` of those that come back, and of those that come off the stack
     auto back_of = [&](int k) {
         const int r = owner_of(s_back, R, k);
@@ -131,12 +131,13 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
 #pragma unroll
         for (int e = 0; e < kTogether; e++) {
             const int k = tid + e * kPlanThreads;
+            if (e * kPlanThreads >= n_most) break;
             back[e] = k < n_back ? back_of(k) : 0;
             take[e] = k < n_take ? take_of(k) : 0;
             out |= (uint32_t)back[e] >= (uint32_t)a.n_pages && k < n_back;
             out |= (uint32_t)take[e] >= (uint32_t)a.n_pages && k < n_take;
         }
-        for (int k = tid + kTogether * kPlanThreads; k < max(n_back, n_take); k += kPlanThreads) {
+        for (int k = tid + kTogether * kPlanThreads; k < n_most; k += kPlanThreads) {
             if (k < n_back) out |= (uint32_t)back_of(k) >= (uint32_t)a.n_pages;
             if (k < n_take) out |= (uint32_t)take_of(k) >= (uint32_t)a.n_pages;
         }
@@ -166,18 +167,20 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
 #pragma unroll
     for (int e = 0; e < kTogether; e++) {
         const int k = tid + e * kPlanThreads;
+        if (e * kPlanThreads >= n_most) break;
         if (k < n_back) a.free_pages[count + k] = back[e];
         if (k < n_take) put_taken(k, take[e]);
     }
-    for (int k = tid + kTogether * kPlanThreads; k < max(n_back, n_take); k += kPlanThreads) {
+    for (int k = tid + kTogether * kPlanThreads; k < n_most; k += kPlanThreads) {
         if (k < n_back) a.free_pages[count + k] = back_of(k);
         if (k < n_take) put_taken(k, take_of(k));
     }
-    for (int i0 = tid; i0 < a.n_rows; i0 += kTogether * kPlanThreads) {
+    for (int first = 0; first < a.n_rows; first += kTogether * kPlanThreads) {
         int pos[kTogether], page[kTogether];
 #pragma unroll
         for (int e = 0; e < kTogether; e++) {
-            const int i = i0 + e * kPlanThreads;
+            const int i = first + e * kPlanThreads + tid;
+            if (i - tid >= a.n_rows) break;
             pos[e] = page[e] = -1;
             if (i >= n_rows) continue;
             const int r = owner_of(s_row, R, i), held = blocks(s_kv[r]);
@@ -187,7 +190,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
         }
 #pragma unroll
         for (int e = 0; e < kTogether; e++) {
-            const int i = i0 + e * kPlanThreads;
+            const int i = first + e * kPlanThreads + tid;
             if (i >= a.n_rows) break;
             a.positions[i] = pos[e];
             a.slots[i] = (uint32_t)page[e] < (uint32_t)a.n_pages ? (page[e] << shift) + (pos[e] & (a.page_size - 1)) : -1;
