@@ -37,6 +37,15 @@ def _dense_strides(shape) -> tuple:
     return tuple(st)
 
 
+def _is_dense(shape, strides) -> bool:
+    acc = 1
+    for n, st in zip(reversed(shape), reversed(strides)):
+        if n != 1 and st != acc:
+            return False
+        acc *= n
+    return True
+
+
 class Tensor:
     """Device tensor: shape, dtype, device pointer, element strides (views from
     Slice/Transpose/ExpandDims are strided, as MLX's are). engine.Tensor
@@ -47,29 +56,18 @@ class Tensor:
         self._b = backend
         self.ptr = int(ptr) if ptr else 0
         self.shape = shape = tuple(map(int, shape))
+        self.numel = math.prod(shape)
         self.dtype = dtype
         self._owned = owned
         self._keep = keep  # an object whose lifetime covers the memory (non-owned views)
+        # contiguous: row-major dense (strides of length-1 axes do not matter)
         self.strides = tuple(map(int, strides)) if strides is not None else _dense_strides(shape)
+        self.contiguous = strides is None or _is_dense(shape, self.strides)
         if backend is not None and owned and backend._sweeper is not None:
             backend._sweeper.track(self)
 
-    @property
-    def contiguous(self) -> bool:
-        """Row-major dense (strides of length-1 axes do not matter)."""
-        acc = 1
-        for n, st in zip(reversed(self.shape), reversed(self.strides)):
-            if n != 1 and st != acc:
-                return False
-            acc *= n
-        return True
-
     def Shape(self) -> list:
         return list(self.shape)
-
-    @property
-    def numel(self) -> int:
-        return math.prod(self.shape)
 
     @property
     def nbytes(self) -> int:
@@ -999,10 +997,10 @@ class HipBackend:
     # session at a time). Pages are [n_pages, Hk, page_size, Dh] in BF16 or F16,
     # block tables I32 [n_req, max_blocks]; all bookkeeping is I32 in device memory.
     @staticmethod
-    def _ints(op: str, **ts) -> None:
-        for name, t in ts.items():
+    def _ints(op: str, names: str, *ts) -> None:
+        for t in ts:
             if t.dtype != I32 or not t.contiguous:
-                raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: {name} must be dense I32")
+                raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: {names} must be dense I32")
 
     @staticmethod
     def _pages(op: str, k_pages: Tensor, v_pages: Tensor) -> tuple:
@@ -1032,15 +1030,14 @@ class HipBackend:
                 raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: rows (or out) must be given")
             out = tuple(self.empty(I32, n) for n in (R, 1, R + 1, int(rows), int(rows), 1))
         kv, count, starts, pos, slots, status = out
-        self._ints(op, newLens=newLens, kvLens=kvLens, blockTables=blockTables, freePages=freePages,
-                   freeCount=freeCount, kvLensOut=kv, freeCountOut=count, rowStarts=starts, positions=pos, slots=slots,
-                   status=status)
-        T = pos.numel
-        if len(blockTables.shape) != 2 or blockTables.shape[0] != R or kvLens.numel != R or kv.numel != R \
-                or starts.numel != R + 1 or slots.numel != T or not freeCount.numel == count.numel == status.numel == 1:
+        self._ints(op, "lengths, tables, pages, counts and results", newLens, kvLens, blockTables, freePages, freeCount,
+                   *out)
+        T, tables = pos.numel, blockTables.shape
+        if len(tables) != 2 or tables[0] != R or not kvLens.numel == kv.numel == R or starts.numel != R + 1 \
+                or slots.numel != T or not freeCount.numel == count.numel == status.numel == 1:
             raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: shapes do not match {R} requests and {T} rows")
         check(self._ctx, self._L.jh_paged_plan(
-            self._ctx, newLens.ptr, kvLens.ptr, R, T, int(pageSize), blockTables.ptr, blockTables.shape[1],
+            self._ctx, newLens.ptr, kvLens.ptr, R, T, int(pageSize), blockTables.ptr, tables[1],
             freePages.ptr, freePages.numel, freeCount.ptr, kv.ptr, count.ptr, starts.ptr, pos.ptr, slots.ptr,
             status.ptr))
         return out
@@ -1058,9 +1055,7 @@ class HipBackend:
         op = "PagedQKNormRoPEAppend"
         n, hk, page, dh, stride = self._pages(op, k_pages, v_pages)
         T = slots.numel
-        self._ints(op, slots=slots)
-        if positions is not None:
-            self._ints(op, positions=positions)
+        self._ints(op, "slots and positions", slots, *(() if positions is None else (positions,)))
         if hk != n_kv_heads or len(qkv.shape) != 2 or qkv.shape != (T, (n_heads + 2 * hk) * dh) \
                 or (positions is not None and positions.numel != T):
             raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: qkv {list(qkv.shape)}, {T} slots and the pages do not match")
@@ -1098,7 +1093,7 @@ class HipBackend:
         otherwise); rows past rowStarts[R] are left as they were."""
         op = "PagedAttention"
         n, hk, page, dh, stride = self._pages(op, k_pages, v_pages)
-        self._ints(op, blockTables=blockTables, rowStarts=rowStarts, kvLens=kvLens)
+        self._ints(op, "tables, row starts and lengths", blockTables, rowStarts, kvLens)
         R = kvLens.numel
         if q.dtype != k_pages.dtype or len(q.shape) != 3 or q.shape[2] != dh or len(blockTables.shape) != 2 \
                 or blockTables.shape[0] != R or rowStarts.numel != R + 1:
