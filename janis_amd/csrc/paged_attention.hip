@@ -94,9 +94,17 @@ __device__ __forceinline__ int64_t uniform(int64_t v) {
 // 16 bytes per lane from base + off into LDS at m0 + 16 * lane. The s_nop is the five wait
 // states between a VALU write of a scalar (a readlane into `base`) and its use by a load,
 // which the compiler does not see in here; it covers the M0 write too.
+// ONCE: data that no other block reads (non-temporal).
+template <bool ONCE>
 __device__ __forceinline__ void lds_fill16(const void* base, uint32_t off, uint32_t m0) {
-    asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(uniform((int64_t)base)), "{m0}"(uniform((int)m0))
-                 : "memory");
+    if constexpr (ONCE)
+        asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1 nt" ::"v"(off), "s"(uniform((int64_t)base)),
+                     "{m0}"(uniform((int)m0))
+                     : "memory");
+    else
+        asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(uniform((int64_t)base)),
+                     "{m0}"(uniform((int)m0))
+                     : "memory");
 }
 // The wave's LDS reads are done (before loads into LDS overwrite what they read).
 __device__ __forceinline__ void wait_lds() { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
@@ -349,7 +357,7 @@ struct Filler {
             v[u] = row * (2 * DH) + 16 * (place ^ perm_v<DH>(row));
         }
     }
-    template <bool V, bool WHOLE>
+    template <bool V, bool WHOLE, bool ONCE>
     __device__ __forceinline__ void fill(const uint16_t* pool, int64_t at, int g, uint32_t lds, int more = 0) const {
         const char* const base = reinterpret_cast<const char*>(pool) + at;
         const int lane = threadIdx.x & 63;
@@ -361,7 +369,7 @@ struct Filler {
                 const int row = (u * 64 + lane) / (DH / 8);
                 off -= max(0, row - more) * (2 * DH);
             }
-            lds_fill16(base, off, lds + g * (16 * DH) + u * 1024);
+            lds_fill16<ONCE>(base, off, lds + g * (16 * DH) + u * 1024);
         }
     }
 };
@@ -537,11 +545,11 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
         const uint32_t at = to + (V ? kTile : 0);
         if (k0 + 32 <= ke) {
 #pragma unroll
-            for (int g = 0; g < 4; g++) fill.template fill<V, true>(pool, lane_of(where, 4 * j + g), g, at);
+            for (int g = 0; g < 4; g++) fill.template fill<V, true, true>(pool, lane_of(where, 4 * j + g), g, at);
         } else {
 #pragma unroll
             for (int g = 0; g < 4; g++)
-                fill.template fill<V, false>(pool, lane_of(where, 4 * j + g), g, at, max(0, ke - 1 - (k0 + 8 * g)));
+                fill.template fill<V, false, true>(pool, lane_of(where, 4 * j + g), g, at, max(0, ke - 1 - (k0 + 8 * g)));
         }
     };
     using K = std::false_type;
@@ -706,11 +714,11 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
         const uint16_t* const pool = V ? a.v : a.k;
         if (k0 + 16 <= ke) {
 #pragma unroll
-            for (int g = 0; g < 2; g++) fill.template fill<V, true>(pool, lane_of(where[V], 2 * (t & 31) + g), g, to);
+            for (int g = 0; g < 2; g++) fill.template fill<V, true, false>(pool, lane_of(where[V], 2 * (t & 31) + g), g, to);
         } else {
 #pragma unroll
             for (int g = 0; g < 2; g++)
-                fill.template fill<V, false>(pool, lane_of(where[V], 2 * (t & 31) + g), g, to,
+                fill.template fill<V, false, false>(pool, lane_of(where[V], 2 * (t & 31) + g), g, to,
                                              max(0, ke - 1 - (k0 + 8 * g)));
         }
     };
