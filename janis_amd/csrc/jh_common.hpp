@@ -379,7 +379,7 @@ size_t attn_decode_workspace_bytes(int64_t Hq, int64_t Hk, int64_t pos, int num_
 // partials be merged inside the attention launch when the GPU deals workgroups
 // to its 8 XCDs round-robin (probe_xcd_round_robin) and the kv heads are a
 // multiple of 8; otherwise a merge launch follows.
-constexpr int kAttnSyncSlots = 4096 + 64 + 32 * 512;
+constexpr int kAttnSyncSlots = 4096 + 64 + 32 * 512 + 8192;
 // The fused q/k/v + attention launch's share of them: per XCD x, the arrival
 // flags of its blocks at kAttnFlagSlot + 128 x (zero between calls).
 constexpr int kAttnFlagSlot = 1024;
@@ -394,6 +394,9 @@ constexpr int kAttnMarkerSlot = 4096;
 // kQmmSyncSlot + 32 t (one 128-byte line each) for kQmmSyncTiles tiles (zero
 // between calls).
 constexpr int kQmmSyncSlot = 4096 + 64, kQmmSyncTiles = 512;
+// jh_paged_attention's share: arrivals of a split tile's parts (zero between calls).
+constexpr int kPagedSyncSlot = kQmmSyncSlot + 32 * kQmmSyncTiles, kPagedSyncSlots = 8192;
+static_assert(kPagedSyncSlot + kPagedSyncSlots == kAttnSyncSlots, "the shares fill the array");
 // Polls of the arrival flags before a fused launch's wait gives up (the default
 // of jh_set_wait_limit).
 constexpr uint32_t kDefaultWaitPolls = 1u << 22;
@@ -496,7 +499,9 @@ struct PagedAttnArgs {
     int out_dt;
 };
 size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus);
-Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, hipStream_t st);
+// `sync`: kPagedSyncSlots of the context's zeroed counters where launches keep the
+// round-robin placement, or nullptr.
+Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, int* sync, hipStream_t st);
 
 // ---- operators around the products (ops.hip) ----
 // QuantMatmul with transpose = false: y [rows, m.in] = x [rows, m.rows] . Dequantize(W);

@@ -120,9 +120,13 @@ __device__ __forceinline__ uint2 lds_read_tr(const uint8_t* p) {
 // ---- finding a block's work ---------------------------------------------------------
 struct Attn {
     PagedAttnArgs a;
+    int G;           // Hq / Hk
+    double per_target;  // 1 / target
     int few;         // requests of at most this many rows (new tokens * G) take tiles of 32 rows, others of 128
     int target;      // parts of the keys to make, per kv head
     int record;      // rows of a record
+    int* sync;       // arrivals at [kv head][slot of a split tile's first record], zero between calls; nullptr: a
+                     // merge launch joins the parts
     float* part;     // records of split parts: [record][DH] results, then [record][2] maximum and sum
 };
 // A unit of 64 keys counts kManyCost with a tile of 128 rows, 1 with one of 32.
@@ -182,7 +186,7 @@ __device__ __forceinline__ T scan64(T v) {
 template <bool MERGE>
 __device__ __forceinline__ Work find_work(const Attn& w, int index) {
     const PagedAttnArgs& a = w.a;
-    const int lane = threadIdx.x & 63, G = a.Hq / a.Hk, run = (a.n_req + 63) / 64;
+    const int lane = threadIdx.x & 63, G = w.G, run = (a.n_req + 63) / 64;
     auto tiles_of = [&](const Request& q) {
         const int rows = q.n * G;
         return rows <= w.few ? (rows + kFewRows - 1) / kFewRows : (rows + kManyRows - 1) / kManyRows;
@@ -203,19 +207,23 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
         double, make_int2(__builtin_amdgcn_readlane(__builtin_bit_cast(int2, all).x, 63),
                           __builtin_amdgcn_readlane(__builtin_bit_cast(int2, all).y, 63)));
     // most that a part may cost: at least total / target
-    const int most = (int)min(total / (double)w.target + 1.0, 1073741824.0);
+    const int most = (int)min(fma(total, w.per_target, 1.0), 1073741824.0);
     auto splits_of = [&](const Request& q) {
-        const int rows = q.n * G;
-        const int each = max(rows <= w.few ? most : most / kManyCost + 1,
-                             kLeast + min(rows, rows <= w.few ? kFewRows : kManyRows) / kRowsPerUnit);  // units per part
-        return max(1, (units_of(q) + each / 2) / each);
+        const int rows = q.n * G, units = units_of(q);
+        int each = max(rows <= w.few ? most : most / kManyCost + 1,
+                       kLeast + min(rows, rows <= w.few ? kFewRows : kManyRows) / kRowsPerUnit);  // units per part
+        // joined by one block, a part costs about a ninth of a unit: least of C + units / C / 9
+        if (w.sync) each = max(each, (int)sqrtf((float)units * (1.0f / 9.0f)));
+        // (a rounded quotient: any count near it will do, the same in every block)
+        return max(1, (int)((float)(units + each / 2) * __builtin_amdgcn_rcpf((float)each)));
     };
-    int items = 0, slots = 0;
+    int items = 0, slots = 0, my_tiles = 0, my_splits = 1;
     for (int e = 0; e < run; e++) {
         const int r = lane * run + e;
         if (r >= a.n_req) break;
         const Request q = e == 0 ? mine : request(a, r);
         const int t = tiles_of(q), s = splits_of(q);
+        if (e == 0) my_tiles = t, my_splits = s;
         items += MERGE ? (s > 1 ? t : 0) : t * s;
         slots += s > 1 ? t * s : 0;
     }
@@ -230,14 +238,18 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
         const int r = at * run + e;
         if (r >= a.n_req) break;
         Request q;
+        int t, s;
         if (e == 0) {
+            t = __builtin_amdgcn_readlane(my_tiles, at);
+            s = __builtin_amdgcn_readlane(my_splits, at);
             q.start = __builtin_amdgcn_readlane(mine.start, at);
             q.n = __builtin_amdgcn_readlane(mine.n, at);
             q.kv = __builtin_amdgcn_readlane(mine.kv, at);
         } else {
             q = request(a, r);
+            t = tiles_of(q), s = splits_of(q);
         }
-        const int t = tiles_of(q), s = splits_of(q), count = MERGE ? (s > 1 ? t : 0) : t * s;
+        const int count = MERGE ? (s > 1 ? t : 0) : t * s;
         if (left < count) {
             o.ok = true, o.r = uniform(r), o.local = uniform(left), o.tiles = uniform(t), o.splits = uniform(s);
             o.q = Request{uniform(q.start), uniform(q.n), uniform(q.kv)};
@@ -264,9 +276,9 @@ __device__ __forceinline__ int seen(const Request& q, int row, int G) { return m
 // whose result is not finite is computed again here, by one wave, in fp32 and reading
 // nothing that it does not see. m is log2; the lane's features are lane + 64 e.
 template <int DH, bool F16>
-__device__ __forceinline__ void row_again(const PagedAttnArgs& a, int r, int head, int token, int kb, int lim, float& m,
+__device__ __forceinline__ void row_again(const PagedAttnArgs& a, int r, int hk, int head, int token, int kb, int lim, float& m,
                                        float& l, float (&o)[DH / 64]) {
-    const int lane = threadIdx.x & 63, hk = head / (a.Hq / a.Hk);
+    const int lane = threadIdx.x & 63;
     const uint4* const q = reinterpret_cast<const uint4*>(a.q + token * a.q_stride + (int64_t)head * DH);
     m = ninf(), l = 0.0f;
 #pragma unroll
@@ -490,6 +502,86 @@ __device__ __forceinline__ int wave_min_int(int v) {
     return v;
 }
 
+// ---- joining the parts -----------------------------------------------------------------
+// Rows of one tile of one kv head whose keys were split, `first`, first + stride, ...
+// times the rows at once: groups of DH / 4 lanes, 4 features each, one to a row for every
+// 8 parts (all requested together); a row's groups meet in LDS in their order. L2: the
+// records were stored by this launch on this XCD (device-coherent loads: past the CU's L1).
+constexpr int kJoinBatch = 8;
+template <int DH, int NT, bool L2>
+__device__ __forceinline__ void join_rows(const Attn& w, const Work& k, int hk, int tile, int parts, int first, int stride,
+                                          float4* s_o, float2* s_ml) {
+    constexpr int kLanes = DH / 4, kGroups = NT / kLanes, kBatch = kJoinBatch;
+    const PagedAttnArgs& a = w.a;
+    const int G = w.G, rows = k.q.n * G, tr = k.few ? kFewRows : kManyRows;
+    const int64_t size = (int64_t)w.record * (DH + 2), step = a.Hk * size;
+    const float* const rec = w.part + ((int64_t)(k.slot + tile * k.splits) * a.Hk + hk) * size;
+    const auto rsrc = make_rsrc(rec, 0x7FFFFFFFu);  // (L2: the launch keeps the records below 2^31 bytes)
+    const int f = threadIdx.x % kLanes, group = threadIdx.x / kLanes, count = min(tr, rows - tile * tr);
+    // groups to a row: for its parts, as long as the block's rows find room beside each other
+    const int here = (count + stride - 1) / stride;
+    int each = 1;
+    while (each * kBatch < parts && 2 * each * here <= kGroups) each *= 2;
+    const int sub = group % each, at_once = kGroups / each;
+    for (int x0 = first * at_once; x0 < count; x0 += stride * at_once) {
+        const int x = min(x0 + group / each, count - 1);
+        // (a part without keys of the row: a maximum of -inf, a sum of 0)
+        float mx = ninf(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s0 = sub; s0 < parts; s0 += each * kBatch) {
+            float2 u[kBatch];
+            float4 y[kBatch];
+            float top = mx;
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) {
+                const int64_t at = min(s0 + i * each, parts - 1) * step;
+                if constexpr (L2) {
+                    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+                    u[i] = __builtin_bit_cast(float2, (u32x2_t)__builtin_amdgcn_raw_buffer_load_b64(
+                                                          rsrc, (uint32_t)(at + w.record * DH + 2 * x) * 4, 0, kAuxSc1));
+                    y[i] = __builtin_bit_cast(float4, (u32x4_t)__builtin_amdgcn_raw_buffer_load_b128(
+                                                          rsrc, (uint32_t)(at + x * DH + 4 * f) * 4, 0, kAuxSc1));
+                } else {
+                    u[i] = *reinterpret_cast<const float2*>(rec + at + (int64_t)w.record * DH + 2 * x);
+                    y[i] = *reinterpret_cast<const float4*>(rec + at + (int64_t)x * DH + 4 * f);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) top = fmaxf(top, s0 + i * each < parts ? u[i].x : top);
+            const float g0 = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
+            l *= g0, o[0] *= g0, o[1] *= g0, o[2] *= g0, o[3] *= g0;
+            mx = top;
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) {
+                if (s0 + i * each >= parts) break;
+                const float g = u[i].x == mx ? 1.0f : __builtin_amdgcn_exp2f(u[i].x - mx);
+                l = fmaf(u[i].y, g, l);
+                o[0] = fmaf(y[i].x, g, o[0]), o[1] = fmaf(y[i].y, g, o[1]);
+                o[2] = fmaf(y[i].z, g, o[2]), o[3] = fmaf(y[i].w, g, o[3]);
+            }
+        }
+        if (each > 1) {
+            __syncthreads();  // (the round before has read)
+            s_o[group * kLanes + f] = make_float4(o[0], o[1], o[2], o[3]);
+            if (f == 0) s_ml[group] = make_float2(mx, l);
+            __syncthreads();
+        }
+        if (sub != 0 || x0 + group / each >= count) continue;
+        for (int g = 1; g < each; g++) mx = fmaxf(mx, s_ml[group + g].x);
+        if (each > 1) l = o[0] = o[1] = o[2] = o[3] = 0.0f;
+        for (int g = 0; each > 1 && g < each; g++) {
+            const float2 u = s_ml[group + g];
+            const float4 y = s_o[(group + g) * kLanes + f];
+            const float h = u.x == mx ? 1.0f : __builtin_amdgcn_exp2f(u.x - mx);
+            l = fmaf(u.y, h, l);
+            o[0] = fmaf(y.x, h, o[0]), o[1] = fmaf(y.y, h, o[1]), o[2] = fmaf(y.z, h, o[2]), o[3] = fmaf(y.w, h, o[3]);
+        }
+        const int row = tile * tr + x;
+        const bool sees = seen(k.q, row, G) > 0;
+        store_out4(a, out_at<DH>(a, k.q, row, hk, G) + 4 * f, sees ? o[0] / l : 0.0f, sees ? o[1] / l : 0.0f,
+                   sees ? o[2] / l : 0.0f, sees ? o[3] / l : 0.0f);
+    }
+}
+
 // ---- few rows ------------------------------------------------------------------------
 // Tiles of 32 rows: decode (a token's G heads) and short runs of new tokens. The NW
 // waves take the part's 32-key tiles in turn, each with its own buffers and no barrier:
@@ -502,7 +594,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
     __shared__ int s_bad[NW];
     __shared__ uint32_t s_again[NW];
     const PagedAttnArgs& a = w.a;
-    const int G = a.Hq / a.Hk;
+    const int G = w.G;
     const int tile = uniform(k.local / k.splits), split = k.local - tile * k.splits;
     const Request q = k.q;
     const int lane = threadIdx.x & 63, h = lane >> 5, c32 = lane & 31;
@@ -615,7 +707,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
             if (!((again >> x) & 1u)) continue;
             float m1, l1, o1[DH / 64];
             const int rw = w0 + x, sees = min(ke, seen(q, rw, G));
-            row_again<DH, F16>(a, k.r, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
+            row_again<DH, F16>(a, k.r, hk, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
             if (sees > bad_all) l1 = __builtin_nanf("");
             if (parts > 1 && lane == 0) *reinterpret_cast<float2*>(rec_ml + 2 * x) = make_float2(m1, l1);
 #pragma unroll
@@ -654,6 +746,20 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
             store_out4(a, out_at<DH>(a, q, rw, hk, G) + 4 * f, 0.0f, 0.0f, 0.0f, 0.0f);
         }
     }
+    if (!w.sync || parts == 1) return;
+    // The part that arrives last joins them. All parts of a kv head run on one XCD (the grid
+    // deals head h to XCD h % 8) and meet in its L2: the records' stores are done before the
+    // arrival is counted there, and are read past this CU's L1 after it.
+    __shared__ int s_last;
+    wait_vmem<0>();
+    __syncthreads();
+    int* const arrivals = w.sync + (int64_t)hk * (2 * w.target) + k.slot + tile * k.splits;
+    if (threadIdx.x == 0)
+        s_last = __hip_atomic_fetch_add(arrivals, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
+    __syncthreads();
+    if (!s_last) return;
+    join_rows<DH, 64 * NW, true>(w, k, hk, tile, parts, 0, 1, reinterpret_cast<float4*>(lds), &s_ml[0][0]);
+    if (threadIdx.x == 0) __hip_atomic_store(arrivals, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
 // ---- many rows -----------------------------------------------------------------------
@@ -668,7 +774,7 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
     __shared__ int s_bad[NW];
     __shared__ float2 s_ml[128];
     const PagedAttnArgs& a = w.a;
-    const int G = a.Hq / a.Hk;
+    const int G = w.G;
     // the last tiles (the longest) first
     const int up = uniform(k.local / k.splits), tile = k.tiles - 1 - up, split = k.local - up * k.splits;
     const Request q = k.q;
@@ -809,7 +915,7 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
             if (!((again >> x) & 1u)) continue;
             float m1, l1, o1[DH / 64];
             const int rw = w0 + x, sees = min(ke, seen(q, rw, G)), y = 32 * wave + x;
-            row_again<DH, F16>(a, k.r, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
+            row_again<DH, F16>(a, k.r, hk, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
             if (sees > bad_all) l1 = __builtin_nanf("");
             if (parts > 1 && lane == 0) *reinterpret_cast<float2*>(rec_ml + 2 * y) = make_float2(m1, l1);
 #pragma unroll
@@ -846,9 +952,9 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
 template <int DH, bool F16, int PN, int NW>
 __global__ __launch_bounds__(64 * NW, DH == 256 || NW == 8 ? 1 : 2) void paged_attn_kernel(Attn w) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * NW * 32 * DH * 2];  // of either: 16 KB a wave at a head_dim of 128
-    // heads fastest: with 8 kv heads all tiles of a head share one XCD's L2
-    const int hk = blockIdx.x % w.a.Hk;
-    const Work k = find_work<false>(w, blockIdx.x / w.a.Hk);
+    // (the grid's fastest axis: with 8 kv heads all tiles of a head share one XCD's L2)
+    const int hk = blockIdx.x;
+    const Work k = find_work<false>(w, blockIdx.z * gridDim.y + blockIdx.y);
     if (!k.ok) return;
     if constexpr (PN > 0)
         if (!k.few) {
@@ -858,80 +964,18 @@ __global__ __launch_bounds__(64 * NW, DH == 256 || NW == 8 ? 1 : 2) void paged_a
     few_rows<DH, F16, NW>(w, k, hk, lds);
 }
 
-// ---- joining the parts -----------------------------------------------------------------
-// A block takes rows of one tile of one kv head whose keys were split: groups of DH / 4
-// lanes, 4 features each, one to a row for every 8 parts (all requested together); a
-// row's groups meet in LDS in their order.
-constexpr int kMergeThreads = 512, kMergeBatch = 8;
+constexpr int kMergeThreads = 512;
 template <int DH>
 __global__ __launch_bounds__(kMergeThreads) void paged_attn_merge_kernel(Attn w) {
-    constexpr int kLanes = DH / 4, kGroups = kMergeThreads / kLanes, kBatch = kMergeBatch;
-    __shared__ float4 s_o[kGroups][kLanes];
-    __shared__ float2 s_ml[kGroups];
-    const PagedAttnArgs& a = w.a;
-    const int hk = blockIdx.x % a.Hk, G = a.Hq / a.Hk;
-    const Work k = find_work<true>(w, blockIdx.x / a.Hk);
+    __shared__ float4 s_o[kMergeThreads];
+    __shared__ float2 s_ml[kMergeThreads / (DH / 4)];
+    const int hk = blockIdx.x, G = w.G;
+    const Work k = find_work<true>(w, blockIdx.y);
     if (!k.ok) return;
-    const int tile = k.local, rows = k.q.n * G, tr = k.few ? kFewRows : kManyRows;
-    const int end = uniform(seen(k.q, min(rows, (tile + 1) * tr) - 1, G));
+    const int tile = k.local, tr = k.few ? kFewRows : kManyRows;
+    const int end = uniform(seen(k.q, min(k.q.n * G, (tile + 1) * tr) - 1, G));
     const int parts = max(1, (end + k.per * kUnit - 1) / (k.per * kUnit));
-    if (parts == 1) return;
-    const int64_t size = (int64_t)w.record * (DH + 2), step = a.Hk * size;
-    const float* const rec = w.part + ((int64_t)(k.slot + tile * k.splits) * a.Hk + hk) * size;
-    const int f = threadIdx.x % kLanes, group = threadIdx.x / kLanes, count = min(tr, rows - tile * tr);
-    int each = 1;  // groups to a row
-    while (each < kGroups && each * kBatch < parts) each *= 2;
-    const int sub = group % each, at_once = kGroups / each;
-    for (int x0 = blockIdx.y * at_once; x0 < count; x0 += gridDim.y * at_once) {
-        const int x = min(x0 + group / each, count - 1);
-        const float *const ml = rec + (int64_t)w.record * DH + 2 * x, *const v = rec + (int64_t)x * DH + 4 * f;
-        // (a part without keys of the row: a maximum of -inf, a sum of 0)
-        float mx = ninf(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s0 = sub; s0 < parts; s0 += each * kBatch) {
-            float2 u[kBatch];
-            float4 y[kBatch];
-            float top = mx;
-#pragma unroll
-            for (int i = 0; i < kBatch; i++) {
-                const int64_t at = min(s0 + i * each, parts - 1) * step;
-                u[i] = *reinterpret_cast<const float2*>(ml + at);
-                y[i] = *reinterpret_cast<const float4*>(v + at);
-            }
-#pragma unroll
-            for (int i = 0; i < kBatch; i++) top = fmaxf(top, s0 + i * each < parts ? u[i].x : top);
-            const float f = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
-            l *= f, o[0] *= f, o[1] *= f, o[2] *= f, o[3] *= f;
-            mx = top;
-#pragma unroll
-            for (int i = 0; i < kBatch; i++) {
-                if (s0 + i * each >= parts) break;
-                const float g = u[i].x == mx ? 1.0f : __builtin_amdgcn_exp2f(u[i].x - mx);
-                l = fmaf(u[i].y, g, l);
-                o[0] = fmaf(y[i].x, g, o[0]), o[1] = fmaf(y[i].y, g, o[1]);
-                o[2] = fmaf(y[i].z, g, o[2]), o[3] = fmaf(y[i].w, g, o[3]);
-            }
-        }
-        if (each > 1) {
-            __syncthreads();  // (the round before has read)
-            s_o[group][f] = make_float4(o[0], o[1], o[2], o[3]);
-            if (f == 0) s_ml[group] = make_float2(mx, l);
-            __syncthreads();
-        }
-        if (sub != 0 || x0 + group / each >= count) continue;
-        for (int g = 1; g < each; g++) mx = fmaxf(mx, s_ml[group + g].x);
-        if (each > 1) l = o[0] = o[1] = o[2] = o[3] = 0.0f;
-        for (int g = 0; each > 1 && g < each; g++) {
-            const float2 u = s_ml[group + g];
-            const float4 y = s_o[group + g][f];
-            const float h = u.x == mx ? 1.0f : __builtin_amdgcn_exp2f(u.x - mx);
-            l = fmaf(u.y, h, l);
-            o[0] = fmaf(y.x, h, o[0]), o[1] = fmaf(y.y, h, o[1]), o[2] = fmaf(y.z, h, o[2]), o[3] = fmaf(y.w, h, o[3]);
-        }
-        const int row = tile * tr + x;
-        const bool sees = seen(k.q, row, G) > 0;
-        store_out4(a, out_at<DH>(a, k.q, row, hk, G) + 4 * f, sees ? o[0] / l : 0.0f, sees ? o[1] / l : 0.0f,
-                   sees ? o[2] / l : 0.0f, sees ? o[3] / l : 0.0f);
-    }
+    if (parts > 1) join_rows<DH, kMergeThreads, false>(w, k, hk, tile, parts, blockIdx.z, gridDim.z, s_o, s_ml);
 }
 
 // A call's tiles and grid. `max_new` is a hint: with at most 32 rows per request as it
@@ -944,11 +988,12 @@ struct Launch {
     size_t bytes;
 };
 
-Launch plan_launch(const PagedAttnArgs& a, int num_cus) {
+Launch plan_launch(const PagedAttnArgs& a, int num_cus, int* sync) {
     const int64_t G = a.Hq / a.Hk, rows = (int64_t)a.n_rows * G, requests = std::min(a.n_req, a.n_rows);
     Launch L{};
     L.only_few = std::min((int64_t)a.max_new * G, rows) <= kFewRows;
     L.w.a = a;
+    L.w.G = (int)G;
     L.w.few = L.only_few ? 0x7fffffff : kFewRows;
     const int64_t tiles = requests + rows / (L.only_few ? kFewRows : kManyRows);
     L.wide = !L.only_few && a.Dh != 256 && tiles * a.Hk <= num_cus;
@@ -958,6 +1003,7 @@ Launch plan_launch(const PagedAttnArgs& a, int num_cus) {
     const int64_t parts = L.only_few ? (2 * tiles <= room ? room - tiles : 2 * room)
                                      : std::max((room + 1) / 2, room - tiles / 2);
     L.w.target = (int)std::max<int64_t>(1, parts);
+    L.w.per_target = 1.0 / L.w.target;
     L.w.record = (int)(std::min<int64_t>(rows, L.only_few ? kFewRows : kManyRows) + 3) / 4 * 4;  // whole 16 bytes
     // a request of t tiles of u units has u / C parts, rounded, at least one, and all t * u / C
     // together are at most `target`: items are at most `target` and one for each tile,
@@ -966,33 +1012,39 @@ Launch plan_launch(const PagedAttnArgs& a, int num_cus) {
     L.merges = (int)std::min<int64_t>(L.w.target, tiles);
     // rows of a tile (as the hint says) times the groups that an average request's parts want
     const int64_t mr = std::min<int64_t>(std::max(a.max_new, 1) * G, L.only_few ? kFewRows : kManyRows);
-    const int64_t groups = kMergeThreads / (a.Dh / 4), want = (L.w.target / tiles + kMergeBatch - 1) / kMergeBatch;
+    const int64_t groups = kMergeThreads / (a.Dh / 4), want = (L.w.target / tiles + kJoinBatch - 1) / kJoinBatch;
     L.merge_rows = (int)std::max<int64_t>(1, (mr * std::max<int64_t>(1, std::min(want, groups)) + groups - 1) / groups);
     L.bytes = (size_t)2 * L.w.target * a.Hk * L.w.record * (a.Dh + 2) * sizeof(float);
+    // (heads dealt to the XCDs in turn, counters for every slot, 32-bit offsets)
+    if (L.only_few && a.Hk % 8 == 0 && (int64_t)2 * L.w.target * a.Hk <= kPagedSyncSlots && L.bytes < (1u << 31))
+        L.w.sync = sync;
     return L;
 }
 
 }  // namespace
 
-size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus) { return plan_launch(a, num_cus).bytes; }
+size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus) { return plan_launch(a, num_cus, nullptr).bytes; }
 
-Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, hipStream_t st) {
-    Launch L = plan_launch(a, num_cus);
+Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, int* sync, hipStream_t st) {
+    Launch L = plan_launch(a, num_cus, sync);
     L.w.part = static_cast<float*>(workspace);
-    auto go = [&](auto kernel, int64_t x, int y, int threads) {
-        hipLaunchKernelGGL(kernel, dim3((unsigned)(x * a.Hk), (unsigned)y), dim3(threads), 0, st, L.w);
+    // heads fastest: block b takes kv head b % Hk; z: items past 2^15, and a merge's shares of rows
+    auto go = [&](auto kernel, int64_t items, int shares, int threads) {
+        const int64_t y = std::min<int64_t>(items, 1 << 15);
+        const dim3 grid((unsigned)a.Hk, (unsigned)y, (unsigned)(shares ? shares : (items + y - 1) / y));
+        hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, L.w);
     };
     auto with = [&](auto dh, auto f16) {
         constexpr int DH = decltype(dh)::value;
         constexpr bool F16 = decltype(f16)::value;
-        if (L.only_few) go(paged_attn_kernel<DH, F16, 0, 4>, L.items, 1, 256);
-        else if (!L.wide && a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2, 4>, L.items, 1, 256);
-        else if (!L.wide) go(paged_attn_kernel<DH, F16, 1, 4>, L.items, 1, 256);
+        if (L.only_few) go(paged_attn_kernel<DH, F16, 0, 4>, L.items, 0, 256);
+        else if (!L.wide && a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2, 4>, L.items, 0, 256);
+        else if (!L.wide) go(paged_attn_kernel<DH, F16, 1, 4>, L.items, 0, 256);
         if constexpr (DH != 256) {  // (its tiles fill the LDS)
-            if (L.wide && a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2, 8>, L.items, 1, 512);
-            else if (L.wide) go(paged_attn_kernel<DH, F16, 1, 8>, L.items, 1, 512);
+            if (L.wide && a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2, 8>, L.items, 0, 512);
+            else if (L.wide) go(paged_attn_kernel<DH, F16, 1, 8>, L.items, 0, 512);
         }
-        go(paged_attn_merge_kernel<DH>, L.merges, L.merge_rows, kMergeThreads);
+        if (!L.w.sync) go(paged_attn_merge_kernel<DH>, L.merges, L.merge_rows, kMergeThreads);
     };
     auto typed = [&](auto dh) { a.f16 ? with(dh, std::true_type{}) : with(dh, std::false_type{}); };
     if (a.Dh == 64) typed(std::integral_constant<int, 64>{});

@@ -1295,7 +1295,8 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
     a.Hq = (int)n_heads, a.Hk = (int)n_kv_heads, a.Dh = (int)head_dim;
     a.scale = scale, a.out = out, a.out_dt = out_dtype;
     if (int r = ensure_workspace(c, jh::paged_attn_workspace_bytes(a, c->num_cus), op)) return r;
-    if (int r = finish(c, jh::launch_paged_attn(a, c->ws, c->num_cus, c->stream), op)) return r;
+    int* const sync = xcd_sync(c) ? xcd_sync(c) + jh::kPagedSyncSlot : nullptr;
+    if (int r = finish(c, jh::launch_paged_attn(a, c->ws, c->num_cus, sync, c->stream), op)) return r;
     return check_values(c, op, out, out_dtype, used * n_heads * head_dim);
 }
 

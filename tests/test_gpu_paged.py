@@ -378,6 +378,15 @@ def test_attention_many_tokens(hip, lens, Hq, Hk, D, page, dt):
     check(hip, lens, Hq, Hk, D, page, dt, (BF16, F16, F32) if len(lens) < 3 else (dt, F32), pad=len(lens) % 3)
 
 
+# 8 and 16 kv heads: the parts of split keys are joined inside the launch
+@pytest.mark.parametrize("lens", [[(1, 700)], [(1, 4099), (0, 3), (1, 129), (2, 1500)], [(1, 9001)], [(3, 2000)]])
+@pytest.mark.parametrize("Hq,Hk,D,page,dt", [(32, 8, 128, 16, BF16), (8, 8, 64, 64, F16), (24, 8, 128, 32, F16), (16, 16, 64, 16, BF16),
+                                             (16, 8, 256, 16, BF16)])
+def test_attention_joined_in_the_launch(hip, lens, Hq, Hk, D, page, dt):
+    c = check(hip, lens, Hq, Hk, D, page, dt, (dt, F32), pad=1)
+    assert np.array_equal(c.run(F32), c.run(F32))  # counters are left at zero, parts joined in order
+
+
 def test_attention_many_requests(hip):
     """More requests than lanes of a wave, of every length."""
     rng = np.random.default_rng(3)
@@ -394,12 +403,12 @@ def test_attention_rows_without_keys(hip):
 
 
 @pytest.mark.parametrize("dt", [BF16, F16])
-@pytest.mark.parametrize("n,kv", [(1, 500), (6, 500), (90, 300), (90, 2500)])
-def test_attention_not_finite(hip, dt, n, kv):
+@pytest.mark.parametrize("n,kv,Hk", [(1, 500, 2), (6, 500, 2), (90, 300, 2), (90, 2500, 2), (1, 700, 8), (7, 700, 8)])
+def test_attention_not_finite(hip, dt, n, kv, Hk):
     """Infinities and NaN in keys and values reach the rows that see them, and
     no others of the same tile; scores of -inf weigh nothing; a row of them alone
     is NaN, as 0 / 0 is."""
-    Hq, Hk, D = 4, 2, 128
+    Hq, D = 2 * Hk, 128
     rng = np.random.default_rng(n + kv)
     k = [rounded(rng.standard_normal((Hk, kv, D)), dt)]
     v = [rounded(rng.standard_normal((Hk, kv, D)), dt)]
