@@ -120,9 +120,11 @@ JH_API void *jh_get_stream(const jh_ctx *ctx);
 
 /* Read-back checks, the equivalent of janis's JANIS_GGML_CHECK
  * (ggml/ggml.go:622-677), off by default. flags is a combination of:
- *   JH_CHECK_INDICES  jh_gather_quant_matmul, jh_moe_swiglu and jh_take_rows
+ *   JH_CHECK_INDICES  jh_gather_quant_matmul, jh_moe_swiglu, jh_take_rows and the
+ *                     operators of the paged cache
  *                     copy their indices to the host and reject an out-of-range
- *                     one with JH_ERR_INVALID before launching. When off, an
+ *                     one with JH_ERR_INVALID before launching (jh_paged_plan after
+ *                     it, by its status). When off, an
  *                     out-of-range expert index yields a row of NaN (a row id,
  *                     a row of zeros) and no memory outside the table is read.
  *   JH_CHECK_VALUES   after each operator with a float result (the quantized
@@ -677,7 +679,8 @@ JH_API int jh_paged_plan(jh_ctx *ctx, const int32_t *new_lens, const int32_t *kv
  *   q_out     [n_rows, n_heads, head_dim] of the pages' dtype
  * n_heads may be 0 (keys and values only; q_out unused). head_dim 64, 128 or 256.
  * qkv, q_out and the pages 16-byte aligned, qkv_stride and page_stride multiples of
- * 8. Norms and rotation in fp32, each result rounded once to the pages' dtype. */
+ * 8; q_out and the pages overlap no input. Norms and rotation in fp32, each result rounded
+ * once to the pages' dtype. No value checks (JH_CHECK_VALUES) run here. */
 JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype qkv_dtype, int64_t n_rows,
                                         int64_t qkv_stride, int64_t n_heads, int64_t n_kv_heads,
                                         int64_t head_dim, const void *q_norm_w, const void *k_norm_w,
@@ -697,7 +700,7 @@ JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype q
  *   out  [n_rows, n_heads, head_dim], dense, JH_BF16, JH_F16 or JH_F32
  * max_new is a hint, the most new tokens any request has (1 in a decode step):
  * it chooses the kernels, and a wrong one costs time only. head_dim 64, 128 or 256,
- * page_size at least 8, scale finite and at least 1e-30; pointers 16-byte aligned,
+ * page_size at least 8, scale in [1e-30, 1e30]; pointers 16-byte aligned,
  * q_stride and page_stride multiples of 8; max_blocks * page_size up to 2^30.
  * Scores, maxima, sums and results are fp32; the probabilities enter the product
  * with the values in the pages' dtype: rounded once to it for 16-bit results
@@ -705,9 +708,15 @@ JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype q
  * request's new rows of a kv head are at most 32.
  * Lengths are held to their buffers (kv_lens to max_blocks pages, row_starts to
  * n_rows); a row that sees a key whose page is outside [0, n_pages) is NaN. With
- * JH_CHECK_INDICES those are JH_ERR_INVALID before the launch. Keys are split over
- * blocks where rows are few, and the parts joined in a fixed order: the same
- * call gives the same bits. The parts lie in the context's workspace. */
+ * JH_CHECK_INDICES those, and row_starts that decrease, are JH_ERR_INVALID before
+ * the launch (without, decreasing row_starts leave rows unwritten). out overlaps none of
+ * the inputs. Keys are split over blocks where rows are few, and the parts, which lie in
+ * the context's workspace, joined in a fixed order: the same call gives the same
+ * bits. Where the workspace cannot grow (a capture, no memory) keys are not split, so that
+ * the speed and the rounding of a captured call depend on whether the same call ran
+ * before the capture. With n_kv_heads a multiple of 8 and at most 32 rows of a kv head
+ * per request the parts are joined inside the launch, by the last of them, through
+ * counters of the context that every call leaves at zero. */
 JH_API int jh_paged_attention(jh_ctx *ctx, const void *q, int64_t q_stride, const void *k_pages,
                               const void *v_pages, jh_dtype page_dtype, int64_t n_pages,
                               int64_t page_size, int64_t page_stride, const int32_t *block_tables,

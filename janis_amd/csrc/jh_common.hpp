@@ -497,6 +497,7 @@ struct PagedAttnArgs {
     float scale;
     void* out;
     int out_dt;
+    int whole;                // keys are not split (no workspace)
 };
 size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus);
 // `sync`: kPagedSyncSlots of the context's zeroed counters where launches keep the

@@ -194,20 +194,25 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
     auto units_of = [&](const Request& q) { return max(1, (q.kv + kUnit - 1) / kUnit); };
     auto cost_of = [&](const Request& q) { return q.n * G <= w.few ? 1 : kManyCost; };
     double all = 0.0;  // exact: below 2^53
+    float new_rows = 0.0f;
     Request mine{0, 0, 0};
     for (int e = 0; e < run; e++) {
         const int r = lane * run + e;
         if (r >= a.n_req) break;
         const Request q = request(a, r);
         if (e == 0) mine = q;
+        new_rows += (float)q.n;
         all += (double)tiles_of(q) * (double)units_of(q) * (double)cost_of(q);
     }
+    // row_starts that go up and down, so that requests overlap: more items than the grid was
+    // made for (it has room for 0.1 %), and nothing is done
+    if (wave_sum(new_rows) > 1.001f * (float)a.n_rows) return Work{};
     all = scan64(all);
     const double total = __builtin_bit_cast(
         double, make_int2(__builtin_amdgcn_readlane(__builtin_bit_cast(int2, all).x, 63),
                           __builtin_amdgcn_readlane(__builtin_bit_cast(int2, all).y, 63)));
     // most that a part may cost: at least total / target
-    const int most = (int)min(fma(total, w.per_target, 1.0), 1073741824.0);
+    const int most = a.whole ? 1 << 30 : (int)min(fma(total, w.per_target, 1.0), 1073741824.0);
     auto splits_of = [&](const Request& q) {
         const int rows = q.n * G, units = units_of(q);
         int each = max(rows <= w.few ? most : most / kManyCost + 1,
@@ -256,9 +261,6 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
             o.few = o.q.n * G <= w.few;
             o.per = uniform((units_of(q) + s - 1) / s);
             o.slot = uniform(slot);
-            // (row_starts that go up and down can make more parts than were counted)
-            if (o.splits > 1 && (o.slot < 0 || (int64_t)o.slot + (int64_t)o.tiles * o.splits > 2 * (int64_t)w.target))
-                o.ok = false;
             return o;
         }
         left -= count;
@@ -995,7 +997,7 @@ Launch plan_launch(const PagedAttnArgs& a, int num_cus, int* sync) {
     L.w.a = a;
     L.w.G = (int)G;
     L.w.few = L.only_few ? 0x7fffffff : kFewRows;
-    const int64_t tiles = requests + rows / (L.only_few ? kFewRows : kManyRows);
+    const int64_t full = rows / (L.only_few ? kFewRows : kManyRows), tiles = requests + full + full / 512;
     L.wide = !L.only_few && a.Dh != 256 && tiles * a.Hk <= num_cus;
     // blocks resident at once (LDS; at a head_dim of 64 registers), per kv head
     const int per_cu = a.Dh == 256 || L.wide ? 1 : a.Dh == 128 ? 2 : L.only_few ? 4 : 3;
@@ -1016,7 +1018,7 @@ Launch plan_launch(const PagedAttnArgs& a, int num_cus, int* sync) {
     L.merge_rows = (int)std::max<int64_t>(1, (mr * std::max<int64_t>(1, std::min(want, groups)) + groups - 1) / groups);
     L.bytes = (size_t)2 * L.w.target * a.Hk * L.w.record * (a.Dh + 2) * sizeof(float);
     // (heads dealt to the XCDs in turn, counters for every slot, 32-bit offsets)
-    if (L.only_few && a.Hk % 8 == 0 && (int64_t)2 * L.w.target * a.Hk <= kPagedSyncSlots && L.bytes < (1u << 31))
+    if (L.only_few && !a.whole && a.Hk % 8 == 0 && (int64_t)2 * L.w.target * a.Hk <= kPagedSyncSlots && L.bytes < (1u << 31))
         L.w.sync = sync;
     return L;
 }
@@ -1044,7 +1046,7 @@ Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, i
             if (L.wide && a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2, 8>, L.items, 0, 512);
             else if (L.wide) go(paged_attn_kernel<DH, F16, 1, 8>, L.items, 0, 512);
         }
-        if (!L.w.sync) go(paged_attn_merge_kernel<DH>, L.merges, L.merge_rows, kMergeThreads);
+        if (!L.w.sync && !a.whole) go(paged_attn_merge_kernel<DH>, L.merges, L.merge_rows, kMergeThreads);
     };
     auto typed = [&](auto dh) { a.f16 ? with(dh, std::true_type{}) : with(dh, std::false_type{}); };
     if (a.Dh == 64) typed(std::integral_constant<int, 64>{});

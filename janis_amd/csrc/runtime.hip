@@ -1253,8 +1253,8 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
                     std::string(op) + ": too large (n_rows * n_heads to 2^30, n_req to 65536, max_blocks * page_size to 2^30)");
     if (q_stride < n_heads * head_dim || q_stride % 8 || q_stride > ((int64_t)1 << 32))
         return fail(c, JH_ERR_INVALID, std::string(op) + ": q_stride must hold a row and be a multiple of 8");
-    if (!(scale >= 1e-30f) || !(scale < __builtin_inff()))
-        return fail(c, JH_ERR_INVALID, std::string(op) + ": scale must be finite and at least 1e-30");
+    if (!(scale >= 1e-30f && scale <= 1e30f))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": scale must lie in [1e-30, 1e30]");
     if (n_rows == 0 || n_req == 0) return JH_OK;
     if (n_pages == 0) return fail(c, JH_ERR_INVALID, std::string(op) + ": no pages");
     if (!q || !out || !row_starts || !kv_lens || (max_blocks > 0 && !block_tables) || !k_pages || !v_pages)
@@ -1294,7 +1294,13 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
     a.n_req = (int)n_req, a.n_rows = (int)n_rows, a.max_new = (int)std::min<int64_t>(max_new, n_rows);
     a.Hq = (int)n_heads, a.Hk = (int)n_kv_heads, a.Dh = (int)head_dim;
     a.scale = scale, a.out = out, a.out_dt = out_dtype;
-    if (int r = ensure_workspace(c, jh::paged_attn_workspace_bytes(a, c->num_cus), op)) return r;
+    // the parts of split keys need a workspace; where it cannot grow (a stream under capture,
+    // no memory) the keys stay whole
+    if (int r = ensure_workspace(c, jh::paged_attn_workspace_bytes(a, c->num_cus), op)) {
+        if (r != JH_ERR_INVALID && r != JH_ERR_OOM) return r;
+        c->err.clear();
+        a.whole = 1;
+    }
     int* const sync = xcd_sync(c) ? xcd_sync(c) + jh::kPagedSyncSlot : nullptr;
     if (int r = finish(c, jh::launch_paged_attn(a, c->ws, c->num_cus, sync, c->stream), op)) return r;
     return check_values(c, op, out, out_dtype, used * n_heads * head_dim);

@@ -568,11 +568,137 @@ def test_attention_far_page(hip):
     big.free()
 
 
+def test_attention_rows_that_overlap(hip):
+    """row_starts that go up and down: no fault, and the calls after it are right
+    (the counters of the joined parts stay at zero)."""
+    c = Paged(hip, [(1, 3000), (1, 900), (2, 50), (1, 4000)], 32, 8, 128, 16, BF16)
+    want, bar = c.ref(BF16)
+    good = c.ST
+    for bad in ([0, 5, 0, 5, 0], [0, 5, 1, 5, 5], [5, 0, 5, 0, 5], [0, 1, 2, 9, 5]):
+        c.ST = ints(hip, bad)
+        step(f"jh_paged_attention row_starts {bad}")
+        hip.PagedAttention(c.Q, c.K, c.V, c.TAB, c.ST, c.KV, c.scale, maxNew=2)
+        c.ST = good
+        for _ in range(2):
+            close(c.run(BF16), want, bar, c.T)
+
+
+def test_attention_captured_without_workspace():
+    """A call whose keys would be split still captures on a context whose workspace
+    was never sized (they stay whole), and replays to its result."""
+    b = HipBackend(0)
+    for n in (1, 50):
+        c = Paged(b, [(n, 1500), (1, 40)], 8, 8, 64, 16, F16)
+        out = up(b, np.zeros((c.T, 8, 64)), F32)
+        step(f"jh_paged_attention captured first n={n}")
+        g = Graph(b, lambda: b.PagedAttention(c.Q, c.K, c.V, c.TAB, c.ST, c.KV, c.scale, maxNew=n, out=out))
+        want, bar = c.ref(F32)
+        for _ in range(3):
+            put(b, out, np.zeros((c.T, 8, 64), np.float32))
+            g.replay()
+            close(b.Floats(out), want, bar, c.T)
+        g.close()
+    b.Close()
+
+
+def test_attention_two_contexts_and_streams():
+    """Calls of two contexts in flight together on one GPU, and one on a caller's
+    stream, each with its own workspace and counters."""
+    import torch
+
+    bs = [HipBackend(0), HipBackend(0)]
+    stream = torch.cuda.Stream()
+    bs[1].SetStream(stream.cuda_stream)
+    cs = [Paged(b, [(1, 5000), (3, 700), (1, 9)], 16, 8, 128, 16, BF16, seed=i) for i, b in enumerate(bs)]
+    refs = [c.ref(BF16) for c in cs]
+    outs = [up(c.hip, np.full((c.T, 16, 128), 7.0), BF16) for c in cs]
+    for b in bs:
+        b.Sync()
+    step("jh_paged_attention on two contexts at once")
+    for _ in range(20):
+        for c, o in zip(cs, outs):
+            c.hip.PagedAttention(c.Q, c.K, c.V, c.TAB, c.ST, c.KV, c.scale, maxNew=3, out=o)
+    for c, o, (want, bar) in zip(cs, outs, refs):
+        close(c.hip.Floats(o), want, bar, c.T)
+    for b in bs:
+        b.Close()
+
+
 def test_attention_repeats_bits(hip):
     c = Paged(hip, [(1, 3000), (20, 900), (1, 50)], 8, 2, 128, 16, BF16)
     step("jh_paged_attention twice")
     a, b = c.run(F32), c.run(F32)
     assert np.array_equal(a, b)
+
+
+# ---- refusals of the C entries --------------------------------------------------------------
+
+def refused(hip, name, good, changes):
+    """The entry with `good` arguments (by name, in order) and each change: its code."""
+    fn, L = getattr(hip._L, name), hip._L
+    for code, change in changes:
+        args = dict(good, **change)
+        step(f"{name} refuses {change}")
+        assert set(change) <= set(good)
+        assert fn(hip._ctx, *args.values()) == code, (change, L.jh_last_error(hip._ctx))
+        assert name.encode() in L.jh_last_error(hip._ctx)
+
+
+def test_refusals(hip):
+    INVALID, UNSUPPORTED = _lib.JH_ERR_INVALID, _lib.JH_ERR_UNSUPPORTED
+    t = hip.empty(F32, 1 << 16)
+    p = t.ptr
+    good = dict(new=p, kv=p + 64, R=2, T=4, page=16, tab=p + 1024, blocks=4, free=p + 2048, pages=8, count=p + 4096, kvo=p + 64,
+                co=p + 4096, starts=p + 5000 * 4, pos=p + 6000 * 4, slots=p + 7000 * 4, status=p + 8000 * 4)
+    refused(hip, "jh_paged_plan", good, [
+        (INVALID, dict(page=0)), (INVALID, dict(page=24)), (INVALID, dict(page=1 << 17)), (INVALID, dict(R=-1)), (INVALID, dict(T=-1)),
+        (INVALID, dict(blocks=-1)), (INVALID, dict(pages=-1)), (INVALID, dict(pages=1 << 28)), (UNSUPPORTED, dict(R=2049)),
+        (UNSUPPORTED, dict(T=(1 << 30) + 1))] + [(INVALID, {k: None}) for k in
+                                                 ("new", "kv", "tab", "free", "count", "kvo", "co", "starts", "pos", "slots", "status")])
+    good = dict(qkv=p, dt=F32, T=2, stride=6 * 64, hq=2, hk=2, d=64, qw=p, kw=p, wdt=F32, eps=1e-6, base=1e4, scale=1.0, freqs=None,
+                pos=p, slots=p, k=p, v=p, pdt=BF16, pages=2, page=16, pstride=2 * 16 * 64, qo=p)
+    refused(hip, "jh_paged_qk_norm_rope_append", good, [
+        (INVALID, dict(dt=F16)), (INVALID, dict(wdt=I32)), (UNSUPPORTED, dict(pdt=F32)), (INVALID, dict(pdt=I32)),
+        (UNSUPPORTED, dict(d=96)), (UNSUPPORTED, dict(d=512)), (INVALID, dict(hk=0)), (INVALID, dict(hq=-1)), (INVALID, dict(T=-1)),
+        (INVALID, dict(stride=6 * 64 - 8)), (INVALID, dict(stride=6 * 64 + 4)), (INVALID, dict(pstride=2 * 16 * 64 - 8)),
+        (INVALID, dict(pstride=2 * 16 * 64 + 2)), (INVALID, dict(page=12)), (INVALID, dict(pages=1 << 28)), (INVALID, dict(base=-1.0)),
+        (INVALID, dict(base=float("nan"))), (INVALID, dict(base=float("inf"))), (INVALID, dict(qkv=p + 4)), (INVALID, dict(qo=p + 8)),
+        (INVALID, dict(k=p + 2)), (INVALID, dict(v=p + 2))] + [(INVALID, {k: None}) for k in ("qkv", "pos", "slots", "k", "v", "qo")])
+    good = dict(q=p, qs=2 * 64, k=p, v=p, pdt=BF16, pages=2, page=16, pstride=2 * 16 * 64, tab=p, blocks=2, starts=p, kv=p, R=1, T=2,
+                new=1, hq=2, hk=2, d=64, scale=0.1, out=p, odt=BF16)
+    refused(hip, "jh_paged_attention", good, [
+        (UNSUPPORTED, dict(pdt=F32)), (INVALID, dict(pdt=I32)), (INVALID, dict(odt=I32)), (INVALID, dict(pages=0)), (INVALID, dict(pages=-1)),
+        (INVALID, dict(page=0)), (INVALID, dict(page=20)), (UNSUPPORTED, dict(page=4)), (INVALID, dict(hq=3)), (INVALID, dict(hq=0)),
+        (INVALID, dict(hk=0)), (UNSUPPORTED, dict(d=32)), (INVALID, dict(qs=64)), (INVALID, dict(qs=2 * 64 + 4)), (INVALID, dict(pstride=64)),
+        (INVALID, dict(R=-1)), (INVALID, dict(T=-1)), (INVALID, dict(new=-1)), (INVALID, dict(blocks=-1)), (UNSUPPORTED, dict(R=65537)),
+        (UNSUPPORTED, dict(T=1 << 30)), (UNSUPPORTED, dict(blocks=(1 << 26) + 1)), (INVALID, dict(scale=0.0)), (INVALID, dict(scale=-1.0)),
+        (INVALID, dict(scale=float("nan"))), (INVALID, dict(scale=float("inf"))), (INVALID, dict(q=p + 8)), (INVALID, dict(out=p + 4)),
+        (INVALID, dict(k=p + 2))] + [(INVALID, {k: None}) for k in ("q", "k", "v", "tab", "starts", "kv", "out")])
+
+
+def test_nothing_to_do(hip):
+    """No rows or no requests: a success that touches nothing (null buffers among them)."""
+    L, c = hip._L, hip._ctx
+    assert L.jh_paged_attention(c, None, 64, None, None, BF16, 1, 16, 1024, None, 0, None, None, 1, 0, 0, 1, 1, 64, 0.1, None, BF16) == 0
+    assert L.jh_paged_attention(c, None, 64, None, None, BF16, 1, 16, 1024, None, 0, None, None, 0, 3, 1, 1, 1, 64, 0.1, None, BF16) == 0
+    assert L.jh_paged_qk_norm_rope_append(c, None, F32, 0, 192, 1, 1, 64, None, None, F32, 0.0, 0.0, 1.0, None, None, None, None, None,
+                                          BF16, 0, 16, 1024, None) == 0
+
+
+def test_values_checked(hip):
+    """JH_CHECK_VALUES names the operator whose result holds a NaN, and does not look
+    at the rows behind the last."""
+    c = Paged(hip, [(1, 40), (2, 30)], 4, 2, 64, 16, BF16, pad=2)
+    fill = up(hip, np.full((c.T, 4, 64), np.nan), BF16)
+    hip.SetChecks(_lib.JH_CHECK_VALUES)
+    try:
+        hip.PagedAttention(c.Q, c.K, c.V, c.TAB, c.ST, c.KV, c.scale, maxNew=2, out=fill)
+        c.tables[1, 0] = 2 ** 30
+        with pytest.raises(JanisHipError, match="jh_paged_attention") as e:
+            hip.PagedAttention(c.Q, c.K, c.V, ints(hip, c.tables), c.ST, c.KV, c.scale, maxNew=2, out=fill)
+        assert e.value.code == _lib.JH_ERR_NONFINITE
+    finally:
+        hip.SetChecks(False)
 
 
 # ---- a step of them together ------------------------------------------------------------
