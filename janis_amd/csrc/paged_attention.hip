@@ -40,6 +40,7 @@ constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kUnit = 64;       // keys: splits are whole units
 constexpr int kFewRows = 32;    // rows of a tile in the few-rows kernel
 constexpr int kManyRows = 128;  // ... in the many-rows kernel
+constexpr int kFewLimit = 64;   // requests of up to this many rows take tiles of 32
 // p is held as p * 2^kPShift, and a row's maximum is moved when it grew by more than
 // kLazy (log2): f16 has nothing below 2^-24 and nothing past 2^16, so p is kept high
 // there (a weight of 2^-27 of the largest still has all its bits).
@@ -993,17 +994,21 @@ struct Launch {
 Launch plan_launch(const PagedAttnArgs& a, int num_cus, int* sync) {
     const int64_t G = a.Hq / a.Hk, rows = (int64_t)a.n_rows * G, requests = std::min(a.n_req, a.n_rows);
     Launch L{};
-    L.only_few = std::min((int64_t)a.max_new * G, rows) <= kFewRows;
+    // (heads dealt to the XCDs in turn)
+    const bool join = sync && !a.whole && a.Hk % 8 == 0;
+    L.only_few = std::min((int64_t)a.max_new * G, rows) <= (join ? kFewLimit : kFewRows);
     L.w.a = a;
     L.w.G = (int)G;
-    L.w.few = L.only_few ? 0x7fffffff : kFewRows;
-    const int64_t full = rows / (L.only_few ? kFewRows : kManyRows), tiles = requests + full + full / 512;
-    L.wide = !L.only_few && a.Dh != 256 && tiles * a.Hk <= num_cus;
+    L.w.few = L.only_few ? 0x7fffffff : kFewLimit;
+    const int64_t full = rows / (L.only_few ? kFewRows : kManyRows), about = requests + full;
+    // at most: a request of few rows may have a second tile, and overlapping rows (0.1 %)
+    const int64_t tiles = about + (L.only_few ? 0 : std::min(requests, rows / (kFewRows + 1))) + full / 512;
+    L.wide = !L.only_few && a.Dh != 256 && about * a.Hk <= num_cus;
     // blocks resident at once (LDS; at a head_dim of 64 registers), per kv head
     const int per_cu = a.Dh == 256 || L.wide ? 1 : a.Dh == 128 ? 2 : L.only_few ? 4 : 3;
     const int64_t room = std::max<int64_t>(1, num_cus * per_cu / a.Hk);
-    const int64_t parts = L.only_few ? (2 * tiles <= room ? room - tiles : 2 * room)
-                                     : std::max((room + 1) / 2, room - tiles / 2);
+    const int64_t parts = L.only_few ? (2 * about <= room ? room - about : 2 * room)
+                                     : std::max((room + 1) / 2, room - about / 2);
     L.w.target = (int)std::max<int64_t>(1, parts);
     L.w.per_target = 1.0 / L.w.target;
     L.w.record = (int)(std::min<int64_t>(rows, L.only_few ? kFewRows : kManyRows) + 3) / 4 * 4;  // whole 16 bytes
@@ -1017,9 +1022,7 @@ Launch plan_launch(const PagedAttnArgs& a, int num_cus, int* sync) {
     const int64_t groups = kMergeThreads / (a.Dh / 4), want = (L.w.target / tiles + kJoinBatch - 1) / kJoinBatch;
     L.merge_rows = (int)std::max<int64_t>(1, (mr * std::max<int64_t>(1, std::min(want, groups)) + groups - 1) / groups);
     L.bytes = (size_t)2 * L.w.target * a.Hk * L.w.record * (a.Dh + 2) * sizeof(float);
-    // (heads dealt to the XCDs in turn, counters for every slot, 32-bit offsets)
-    if (L.only_few && !a.whole && a.Hk % 8 == 0 && (int64_t)2 * L.w.target * a.Hk <= kPagedSyncSlots && L.bytes < (1u << 31))
-        L.w.sync = sync;
+    if (join && L.only_few && (int64_t)2 * L.w.target * a.Hk <= kPagedSyncSlots && L.bytes < (1u << 31)) L.w.sync = sync;
     return L;
 }
 
