@@ -499,10 +499,11 @@ struct PagedAttnArgs {
     int out_dt;
     int whole;                // keys are not split (no workspace)
 };
-size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus);
 // `sync`: kPagedSyncSlots of the context's zeroed counters where launches keep the
-// round-robin placement, or nullptr.
-Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, int* sync, hipStream_t st);
+// round-robin placement, or nullptr; the same in both.
+size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus, int* sync);
+Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, size_t workspace_bytes, int num_cus, int* sync,
+                         hipStream_t st);
 
 // ---- operators around the products (ops.hip) ----
 // QuantMatmul with transpose = false: y [rows, m.in] = x [rows, m.rows] . Dequantize(W);

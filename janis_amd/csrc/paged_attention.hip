@@ -1028,10 +1028,15 @@ Launch plan_launch(const PagedAttnArgs& a, int num_cus, int* sync) {
 
 }  // namespace
 
-size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus) { return plan_launch(a, num_cus, nullptr).bytes; }
+size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus, int* sync) {
+    return plan_launch(a, num_cus, sync).bytes;
+}
 
-Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, int num_cus, int* sync, hipStream_t st) {
+Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, size_t workspace_bytes, int num_cus, int* sync,
+                         hipStream_t st) {
     Launch L = plan_launch(a, num_cus, sync);
+    if (!a.whole && L.bytes > workspace_bytes)
+        return Status::fail(JH_ERR_INVALID, "jh_paged_attention: the workspace does not hold the parts");
     L.w.part = static_cast<float*>(workspace);
     // heads fastest: block b takes kv head b % Hk; z: items past 2^15, and a merge's shares of rows
     auto go = [&](auto kernel, int64_t items, int shares, int threads) {

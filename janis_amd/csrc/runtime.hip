@@ -1296,13 +1296,13 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
     a.scale = scale, a.out = out, a.out_dt = out_dtype;
     // the parts of split keys need a workspace; where it cannot grow (a stream under capture,
     // no memory) the keys stay whole
-    if (int r = ensure_workspace(c, jh::paged_attn_workspace_bytes(a, c->num_cus), op)) {
+    int* const sync = xcd_sync(c) ? xcd_sync(c) + jh::kPagedSyncSlot : nullptr;
+    if (int r = ensure_workspace(c, jh::paged_attn_workspace_bytes(a, c->num_cus, sync), op)) {
         if (r != JH_ERR_INVALID && r != JH_ERR_OOM) return r;
         c->err.clear();
         a.whole = 1;
     }
-    int* const sync = xcd_sync(c) ? xcd_sync(c) + jh::kPagedSyncSlot : nullptr;
-    if (int r = finish(c, jh::launch_paged_attn(a, c->ws, c->num_cus, sync, c->stream), op)) return r;
+    if (int r = finish(c, jh::launch_paged_attn(a, c->ws, c->ws_bytes, c->num_cus, sync, c->stream), op)) return r;
     return check_values(c, op, out, out_dtype, used * n_heads * head_dim);
 }
 

@@ -303,15 +303,12 @@ class Paged:
         self.TAB, self.ST = ints(hip, self.tables), ints(hip, self.starts)
         self.KV = ints(hip, [kv for _, kv in lens])
 
-    def ref(self, out_dt, few=None):
+    def ref(self, out_dt):
         """(expected, bar) [T, Hq, D]; rows behind the last: NaN."""
         G = self.Hq // self.Hk
         want, bar = np.full((2, self.T, self.Hq, self.D), np.nan)
         for r, (n, kv) in enumerate(self.lens):
-            two = out_dt == F32 or n * G <= 32 if few is None else few
-            p_half = HALF[self.dt] ** 2 if two else HALF[self.dt]
-            if out_dt != F32 and not two:
-                p_half = HALF[self.dt]
+            p_half = HALF[self.dt] ** 2 if out_dt == F32 or n * G <= 64 else HALF[self.dt]
             for i in range(n):
                 seen = kv - n + i + 1
                 t = self.starts[r] + i
@@ -599,6 +596,16 @@ def test_attention_captured_without_workspace():
             close(b.Floats(out), want, bar, c.T)
         g.close()
     b.Close()
+
+
+def test_attention_sizes_its_workspace():
+    """The first call of a context sizes the workspace for exactly its parts (a call
+    that needs more than it was given says so)."""
+    for lens, Hq, Hk, D in (([(9, 900)], 32, 8, 128), ([(1, 5000)], 32, 8, 128), ([(12, 3000), (1, 40)], 32, 8, 64), ([(200, 900)], 8, 2, 64),
+                            ([(5, 2000)], 16, 2, 128), ([(40, 700)], 8, 8, 256), ([(64, 400)], 8, 8, 64), ([(1, 300)] * 70, 8, 8, 64)):
+        b = HipBackend(0)
+        check(b, lens, Hq, Hk, D, 16, BF16, (BF16,))
+        b.Close()
 
 
 def test_attention_two_contexts_and_streams():
