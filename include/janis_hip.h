@@ -705,7 +705,7 @@ JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype q
  * Scores, maxima, sums and results are fp32; the probabilities enter the product
  * with the values in the pages' dtype: rounded once to it for 16-bit results
  * (as the result is), as the sum of two such terms for JH_F32 ones and where a
- * request's new rows of a kv head are at most 32.
+ * request has at most 64 rows of a kv head.
  * Lengths are held to their buffers (kv_lens to max_blocks pages, row_starts to
  * n_rows); a row that sees a key whose page is outside [0, n_pages) is NaN. With
  * JH_CHECK_INDICES those, and row_starts that decrease, are JH_ERR_INVALID before
@@ -714,8 +714,8 @@ JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype q
  * the context's workspace, joined in a fixed order: the same call gives the same
  * bits. Where the workspace cannot grow (a capture, no memory) keys are not split, so that
  * the speed and the rounding of a captured call depend on whether the same call ran
- * before the capture. With n_kv_heads a multiple of 8 and at most 32 rows of a kv head
- * per request the parts are joined inside the launch, by the last of them, through
+ * before the capture. With n_kv_heads a multiple of 8 and max_new * n_heads / n_kv_heads
+ * at most 64 the parts are joined inside the launch, by the last of them, through
  * counters of the context that every call leaves at zero. */
 JH_API int jh_paged_attention(jh_ctx *ctx, const void *q, int64_t q_stride, const void *k_pages,
                               const void *v_pages, jh_dtype page_dtype, int64_t n_pages,

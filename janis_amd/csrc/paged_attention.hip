@@ -21,9 +21,24 @@
 // Work: a block takes a tile of rows of one request and kv head and a part of its keys.
 // Lengths live on the device, so the blocks find their tile themselves, by running sums
 // over the requests; the grid is the most that the sizes known to the host allow. Keys
-// are split where that fills the GPU: all tiles' keys over as many parts as blocks are
-// resident, at least kMinUnits * 64 keys each. A request whose keys were split has its
-// parts joined, in their order, by paged_attn_merge_kernel.
+// are split where that fills the GPU: all tiles' keys over about as many parts as blocks
+// are resident, none so small that its records cost more than its keys. The parts of a
+// tile are joined in their order: by a launch that follows, or, where rows are few and
+// all blocks of a kv head run on one XCD (heads a multiple of 8), by the last of them.
+//
+// What bounds it, and figures on MI355X (calls in a row, their launches' gaps included;
+// 32 query heads over 8 of 128 unless said):
+//   few rows: HBM. 32 tokens of 8000 bf16 keys 167 us (6.3 TB/s), 64 of 100 to 8000
+//     87 us (5.7), one of 100001 f16 keys over 4 heads 43 us (4.7 TB/s). Loads are
+//     non-temporal: 32 of 8000 take 189 us without. Short ones are chains of
+//     round trips (lengths, tables, keys, records): 1 token of 64 keys 6 us, of 700 9 to 10;
+//     with a launch of its own for the join 9 and 11 us.
+//   many rows: 2000 tokens of 8000 bf16 keys 240-250 us (920-950 TFLOP/s, where a large
+//     bf16 product of the library reaches 1180). By counters the MFMA pipes are busy 44 %
+//     of the time at 1.9 GHz and VALU 44 %; of 250 us on one device it takes 224
+//     without the exponentials, 183 without the second product, 220 without loads, 247
+//     without the LDS reads of V and 213 of K: no unit alone bounds it. 513 tokens of
+//     513 21 to 22 us: a tile's keys are walked in order, 1.5 us a step.
 #include "jh_common.hpp"
 
 namespace jh {
@@ -38,9 +53,12 @@ typedef short short4_t __attribute__((ext_vector_type(4)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr int kUnit = 64;       // keys: splits are whole units
-constexpr int kFewRows = 32;    // rows of a tile in the few-rows kernel
-constexpr int kManyRows = 128;  // ... in the many-rows kernel
-constexpr int kFewLimit = 64;   // requests of up to this many rows take tiles of 32
+constexpr int kFewRows = 32;    // rows of a tile where rows are few
+constexpr int kManyRows = 128;  // ... and many
+// Requests of up to this many rows take tiles of 32, which read keys once per tile but
+// leave no wave idle: 16 runs of 2 to 7 tokens (8 rows each) 26.5 us, 28.9 with a limit of
+// 32; a run beyond takes tiles of 128 (two pieces of prompts beside 22 tokens 34.9 us).
+constexpr int kFewLimit = 64;
 // p is held as p * 2^kPShift, and a row's maximum is moved when it grew by more than
 // kLazy (log2): f16 has nothing below 2^-24 and nothing past 2^16, so p is kept high
 // there (a weight of 2^-27 of the largest still has all its bits).
@@ -982,8 +1000,14 @@ __global__ __launch_bounds__(kMergeThreads) void paged_attn_merge_kernel(Attn w)
 }
 
 // A call's tiles and grid. `max_new` is a hint: with at most 32 rows per request as it
-// says, every request takes tiles of 32 rows (longer ones several); else those of more
-// rows take tiles of 128.
+// says (64 where the parts are joined in the launch), every request takes tiles of 32
+// rows; else those of more than kFewLimit rows take tiles of 128. `wide`: blocks of eight
+// waves where that many still find a CU each (mixed lengths 36.8 us, 46.5 without; a
+// prompt of 64 to 256 tokens loses 0.9 to 1.5 us, one of 1024 nothing). `parts`: with few tiles so many that all
+// blocks are resident at once (1 of 700 keys 11.5 us, 12.4 with one block more per head),
+// with many twice the room (64 of 100-8000: 102 us, 108 with the room alone, 103 with
+// three times); for long runs, whose records are large, fewer (2000 of 8000 249 us, 253
+// with the room, 288 with twice).
 struct Launch {
     Attn w;
     bool only_few, wide;  // wide: blocks of eight waves
