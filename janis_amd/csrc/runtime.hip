@@ -1137,7 +1137,11 @@ int check_page_heads(jh_ctx* c, const char* op, int64_t n_kv_heads, int64_t head
 // n device int32 on the host (JH_CHECK_INDICES).
 int read_ints(jh_ctx* c, const char* op, const int32_t* p, int64_t n, std::vector<int32_t>& out) {
     if (int r = checks_not_capturing(c, op)) return r;
-    out.resize((size_t)n);
+    try {
+        out.resize((size_t)n);
+    } catch (const std::exception&) {
+        return fail(c, JH_ERR_OOM, std::string(op) + ": no host memory to check " + std::to_string(n) + " indices");
+    }
     JH_HIP(c, hipMemcpyAsync(out.data(), p, out.size() * sizeof(int32_t), hipMemcpyDeviceToHost, c->stream));
     JH_HIP(c, hipStreamSynchronize(c->stream));
     return JH_OK;
@@ -1267,7 +1271,6 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
         if (int r = read_ints(c, op, row_starts, n_req + 1, st)) return r;
         if (c->checks & JH_CHECK_INDICES) {
             if (int r = read_ints(c, op, kv_lens, n_req, kv)) return r;
-            if (int r = read_ints(c, op, block_tables, n_req * max_blocks, tab)) return r;
             for (int64_t i = 0; i < n_req; i++) {
                 if (st[i] < 0 || st[i + 1] < st[i] || st[i + 1] > n_rows)
                     return fail(c, JH_ERR_INVALID, std::string(op) + ": row_starts of request " + std::to_string(i) +
@@ -1275,10 +1278,12 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
                 if (kv[i] < 0 || kv[i] > max_blocks * page_size)
                     return fail(c, JH_ERR_INVALID, std::string(op) + ": kv_lens of request " + std::to_string(i) +
                                                        " outside [0, max_blocks * page_size]");
-                for (int64_t j = 0; st[i + 1] > st[i] && j * page_size < kv[i]; j++)
-                    if (tab[i * max_blocks + j] < 0 || tab[i * max_blocks + j] >= n_pages)
-                        return fail(c, JH_ERR_INVALID, std::string(op) + ": page " +
-                                                           std::to_string(tab[i * max_blocks + j]) + " of request " +
+                const int64_t pages = st[i + 1] > st[i] ? (kv[i] + page_size - 1) / page_size : 0;
+                if (pages == 0) continue;
+                if (int r = read_ints(c, op, block_tables + i * max_blocks, pages, tab)) return r;
+                for (int64_t j = 0; j < pages; j++)
+                    if (tab[j] < 0 || tab[j] >= n_pages)
+                        return fail(c, JH_ERR_INVALID, std::string(op) + ": page " + std::to_string(tab[j]) + " of request " +
                                                            std::to_string(i) + " outside [0, n_pages)");
             }
         }
