@@ -144,6 +144,8 @@ struct Attn {
     int few;         // requests of at most this many rows (new tokens * G) take tiles of 32 rows, others of 128
     int target;      // parts of the keys to make, per kv head
     int record;      // rows of a record
+    int size;        // floats of a record: whole 128-byte lines, so that no two XCDs write one
+    int arrivals;    // of a kv head, in `sync` (whole lines too)
     int* sync;       // arrivals at [kv head][slot of a split tile's first record], zero between calls; nullptr: a
                      // merge launch joins the parts
     float* part;     // records of split parts: [record][DH] results, then [record][2] maximum and sum
@@ -535,8 +537,8 @@ __device__ __forceinline__ void join_rows(const Attn& w, const Work& k, int hk, 
     constexpr int kLanes = DH / 4, kGroups = NT / kLanes, kBatch = kJoinBatch;
     const PagedAttnArgs& a = w.a;
     const int G = w.G, rows = k.q.n * G, tr = k.few ? kFewRows : kManyRows;
-    const int64_t size = (int64_t)w.record * (DH + 2), step = a.Hk * size;
-    const float* const rec = w.part + ((int64_t)(k.slot + tile * k.splits) * a.Hk + hk) * size;
+    const int64_t step = (int64_t)a.Hk * w.size;
+    const float* const rec = w.part + ((int64_t)(k.slot + tile * k.splits) * a.Hk + hk) * w.size;
     const auto rsrc = make_rsrc(rec, 0x7FFFFFFFu);  // (L2: the launch keeps the records below 2^31 bytes)
     const int f = threadIdx.x % kLanes, group = threadIdx.x / kLanes, count = min(tr, rows - tile * tr);
     // groups to a row: for its parts, as long as the block's rows find room beside each other
@@ -721,7 +723,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
 #pragma unroll
     for (int v = 1; v < NW; v++) bad_all = min(bad_all, s_bad[v]), votes |= s_again[v];
     const int64_t slot = (int64_t)(k.slot + k.local) * a.Hk + hk;
-    float *const rec = w.part + slot * (w.record * (DH + 2)), *const rec_ml = rec + w.record * DH;
+    float *const rec = w.part + slot * w.size, *const rec_ml = rec + w.record * DH;
     const uint32_t again = uniform((int)votes);
     if (again) {
         for (int x = wave; x < n_rows; x += NW) {
@@ -774,7 +776,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
     __shared__ int s_last;
     wait_vmem<0>();
     __syncthreads();
-    int* const arrivals = w.sync + (int64_t)hk * (2 * w.target) + k.slot + tile * k.splits;
+    int* const arrivals = w.sync + hk * w.arrivals + k.slot + tile * k.splits;
     if (threadIdx.x == 0)
         s_last = __hip_atomic_fetch_add(arrivals, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
     __syncthreads();
@@ -928,7 +930,7 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
             }
     }
     const int64_t slot = (int64_t)(k.slot + tile * k.splits + split) * a.Hk + hk;
-    float *const rec = w.part + slot * (w.record * (DH + 2)), *const rec_ml = rec + w.record * DH;
+    float *const rec = w.part + slot * w.size, *const rec_ml = rec + w.record * DH;
     if (w0 >= rows) return;
     const uint32_t again = rows_again<DH>(l, o, w0 + c32 < rows);
     if (again) {
@@ -1045,8 +1047,10 @@ Launch plan_launch(const PagedAttnArgs& a, int num_cus, int* sync) {
     const int64_t mr = std::min<int64_t>(std::max(a.max_new, 1) * G, L.only_few ? kFewRows : kManyRows);
     const int64_t groups = kMergeThreads / (a.Dh / 4), want = (L.w.target / tiles + kJoinBatch - 1) / kJoinBatch;
     L.merge_rows = (int)std::max<int64_t>(1, (mr * std::max<int64_t>(1, std::min(want, groups)) + groups - 1) / groups);
-    L.bytes = (size_t)2 * L.w.target * a.Hk * L.w.record * (a.Dh + 2) * sizeof(float);
-    if (join && L.only_few && (int64_t)2 * L.w.target * a.Hk <= kPagedSyncSlots && L.bytes < (1u << 31)) L.w.sync = sync;
+    L.w.size = (L.w.record * (a.Dh + 2) + 31) / 32 * 32;
+    L.w.arrivals = (2 * L.w.target + 31) / 32 * 32;
+    L.bytes = (size_t)2 * L.w.target * a.Hk * L.w.size * sizeof(float);
+    if (join && L.only_few && (int64_t)L.w.arrivals * a.Hk <= kPagedSyncSlots && L.bytes < (1u << 31)) L.w.sync = sync;
     return L;
 }
 
