@@ -641,6 +641,9 @@ enum {
  * what their new tokens need off its top (again in order) into block_tables.
  *   block_tables    [n_req, max_blocks], only the new pages' entries are written
  *   free_pages      [n_pages], in place
+ *                   (a page that requests share would come back once for each of them:
+ *                   their tables hold pages of their own here, or the caller does the
+ *                   bookkeeping)
  *   kv_lens_out     [n_req]: kv_lens + new_lens, 0 for finished requests; may be kv_lens
  *   free_count_out  [1]; may be free_count
  *   row_starts      [n_req + 1]: running sums of the new tokens
@@ -716,7 +719,10 @@ JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype q
  * the speed and the rounding of a captured call depend on whether the same call ran
  * before the capture. With n_kv_heads a multiple of 8 and max_new * n_heads / n_kv_heads
  * at most 64 the parts are joined inside the launch, by the last of them, through
- * counters of the context that every call leaves at zero. */
+ * counters of the context that every call leaves at zero. A row whose result is not
+ * finite (a NaN or infinity among its keys or values, or in masked places that share a
+ * product with it) is computed a second time, key by key: right, but slow (all of 2000
+ * rows over 8000 keys: 50 ms). */
 JH_API int jh_paged_attention(jh_ctx *ctx, const void *q, int64_t q_stride, const void *k_pages,
                               const void *v_pages, jh_dtype page_dtype, int64_t n_pages,
                               int64_t page_size, int64_t page_stride, const int32_t *block_tables,
