@@ -16,7 +16,9 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 // rows, new pages and pages that come back are running sums in LDS (one scan of up to
 // 2048 requests over 1024 threads), and a row or page finds its request by bisection,
 // kTogether of them to a thread at once. Bound: latency -- the lengths' round trip, the
-// scan's barriers, the pages' round trip, the tables' and the stores.
+// scan's barriers, the pages' round trip, the tables' and the stores. MI355X: 64 requests
+// of one new token 5.2 us, 700 requests with 8192 rows 14.0 us (16.0 with one row or page
+// to a thread at a time, 14.4 with two, 13.9 with eight, where 64 requests take 1 us more).
 constexpr int kPlanThreads = 1024, kTogether = 4;
 static_assert(kPlanMaxReq % kPlanThreads == 0, "requests per thread");
 
@@ -231,6 +233,10 @@ __device__ __forceinline__ float group_sum(float x) {
 // while they are on their way the lanes evaluate the rotation's factors, a pair each:
 // the angle in double, its whole turns taken off there, sine and cosine of the rest in
 // fp32 (within 2^-23). Calls of few rows share a row's heads among `share` waves.
+// Bound: many rows, HBM; few, the round trips of slot, position and row. MI355X, 32 and 8
+// heads of 128: 1 bf16 row 3.2 us, 4001 rows 22 us (98 MB, 4.4 TB/s; a block to a row
+// took 35 us). kAhead: one 3.1 and 23.9 us, three 3.6 and 22.6; at 8000 rows one
+// loses 4 us.
 constexpr int kAhead = 2;
 template <int DH, bool F16, bool F32>
 __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, int share) {

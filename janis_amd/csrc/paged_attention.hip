@@ -29,7 +29,7 @@
 // What bounds it, and figures on MI355X (calls in a row, their launches' gaps included;
 // 32 query heads over 8 of 128 unless said):
 //   few rows: HBM. 32 tokens of 8000 bf16 keys 167 us (6.3 TB/s), 64 of 100 to 8000
-//     87 us (5.7), one of 100001 f16 keys over 4 heads 43 us (4.7 TB/s). Loads are
+//     87 us (5.7), one of 100001 f16 keys over 4 heads 43 us (36 and 7 for the join). Loads are
 //     non-temporal: 32 of 8000 take 189 us without. Short ones are chains of
 //     round trips (lengths, tables, keys, records): 1 token of 64 keys 6 us, of 700 9 to 10;
 //     with a launch of its own for the join 9 and 11 us.
