@@ -608,6 +608,41 @@ def test_attention_sizes_its_workspace():
         b.Close()
 
 
+def test_attention_graphs_share_workspace_and_counters():
+    """Two captured calls of different sizes whose parts are joined in their launch, in
+    turn, eager calls of other head counts between them, and again after a call that grew
+    the workspace: the eager bits each time."""
+    b = HipBackend(0)
+    cases = [Paged(b, [(1, 3000), (1, 90)], 32, 8, 128, 16, BF16, seed=1), Paged(b, [(7, 900)] * 3, 64, 16, 64, 32, F16, seed=2)]
+    other = Paged(b, [(1, 2000)], 16, 4, 128, 16, BF16, seed=3)
+    big = Paged(b, [(400, 2500)] * 4, 8, 8, 128, 16, BF16, seed=4)
+    outs = [up(b, np.zeros((c.T, c.Hq, c.D)), F32) for c in cases]
+
+    def call(i):
+        c = cases[i]
+        b.PagedAttention(c.Q, c.K, c.V, c.TAB, c.ST, c.KV, c.scale, maxNew=max(n for n, _ in c.lens), out=outs[i])
+
+    wants = []
+    for i, c in enumerate(cases):  # (sizes the workspace)
+        step(f"jh_paged_attention eager, then captured: {c.lens}")
+        call(i)
+        want, bar = c.ref(F32)
+        wants.append(b.Floats(outs[i]))
+        close(wants[i], want, bar, c.T)
+    graphs = [Graph(b, lambda i=i: call(i)) for i in range(2)]
+    for turn in range(4):
+        if turn == 2:
+            big.run(F32)
+        for i, c in enumerate(cases):
+            put(b, outs[i], np.zeros((c.T, c.Hq, c.D), np.float32))
+            graphs[i].replay()
+            assert np.array_equal(b.Floats(outs[i]), wants[i]), (turn, i)
+            other.run(F32)
+    for g in graphs:
+        g.close()
+    b.Close()
+
+
 def test_attention_two_contexts_and_streams():
     """Calls of two contexts in flight together on one GPU, and one on a caller's
     stream, each with its own workspace and counters."""
