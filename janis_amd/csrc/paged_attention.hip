@@ -33,7 +33,7 @@
 //     non-temporal: 32 of 8000 take 189 us without. Short ones are chains of
 //     round trips (lengths, tables, keys, records): 1 token of 64 keys 6 us, of 700 9 to 10;
 //     with a launch of its own for the join 9 and 11 us.
-//   many rows: 2000 tokens of 8000 bf16 keys 240-250 us (920-950 TFLOP/s, where a large
+//   many rows: 2000 tokens of 8000 bf16 keys 237-250 us (920-966 TFLOP/s, where a large
 //     bf16 product of the library reaches 1180). By counters the MFMA pipes are busy 44 %
 //     of the time at 1.9 GHz and VALU 44 %; of 250 us on one device it takes 224
 //     without the exponentials, 183 without the second product, 220 without loads, 247
