@@ -702,13 +702,12 @@ JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype q
  *        row to the next
  *   out  [n_rows, n_heads, head_dim], dense, JH_BF16, JH_F16 or JH_F32
  * max_new is a hint, the most new tokens any request has (1 in a decode step):
- * it chooses the kernels, and a wrong one costs time only. head_dim 64, 128 or 256,
+ * it chooses the kernels; a wrong one costs time, and changes the order of fp32 sums. head_dim 64, 128 or 256,
  * page_size at least 8, scale in [1e-30, 1e30]; pointers 16-byte aligned,
  * q_stride and page_stride multiples of 8; max_blocks * page_size up to 2^30.
- * Scores, maxima, sums and results are fp32; the probabilities enter the product
- * with the values in the pages' dtype: rounded once to it for 16-bit results
- * (as the result is), as the sum of two such terms for JH_F32 ones and where a
- * request has at most 64 rows of a kv head.
+ * Scores, maxima, sums and results are fp32; a probability enters the product with
+ * the values as the sum of two terms of the pages' dtype (off by at most 2^-16 of itself
+ * in bf16, 2^-22 in f16), and a 16-bit result is rounded once.
  * Lengths are held to their buffers (kv_lens to max_blocks pages, row_starts to
  * n_rows); a row that sees a key whose page is outside [0, n_pages) is NaN. With
  * JH_CHECK_INDICES those, and row_starts that decrease, are JH_ERR_INVALID before

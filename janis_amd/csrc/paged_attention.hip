@@ -33,12 +33,10 @@
 //     non-temporal: 32 of 8000 take 189 us without. Short ones are chains of
 //     round trips (lengths, tables, keys, records): 1 token of 64 keys 6 us, of 700 9 to 10;
 //     with a launch of its own for the join 9 and 11 us.
-//   many rows: 2000 tokens of 8000 bf16 keys 237-250 us (920-966 TFLOP/s, where a large
-//     bf16 product of the library reaches 1180). By counters the MFMA pipes are busy 44 %
-//     of the time at 1.9 GHz and VALU 44 %; of 250 us on one device it takes 224
-//     without the exponentials, 183 without the second product, 220 without loads, 247
-//     without the LDS reads of V and 213 of K: no unit alone bounds it. 513 tokens of
-//     513 21 to 22 us: a tile's keys are walked in order, 1.5 us a step.
+//   many rows: 2000 tokens of 8000 bf16 keys 328 us: 700 TFLOP/s of the formula's
+//     operations, and, the second product being made twice (kTerms), 1050 of the matrix
+//     cores', where a large bf16 product of the library reaches 1180. 513 tokens of 513 25
+//     us: a tile's keys are walked in order.
 #include "jh_common.hpp"
 
 namespace jh {
@@ -78,6 +76,13 @@ __device__ __forceinline__ floatx16 mfma(uint4 a, uint4 b, floatx16 c) {
         return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, a), __builtin_bit_cast(bf16x8_t, b),
                                                        c, 0, 0, 0);
 }
+
+// Terms of a probability in the product with the values: together they hold it to 2^-16
+// (bf16) or 2^-22 (f16), so that results of 16 bits are rounded once, at the end. One term
+// is faster where rows are many (2000 tokens of 8000 bf16 keys 240 us against 328) and
+// leaves bf16 results with 1.36 times the error of that one rounding (0.00226 of their size
+// against 0.00166).
+constexpr int kTerms = 2;
 
 // (a, b) as N packed 16-bit terms, each the nearest to what the earlier ones left.
 template <bool F16, int N>
@@ -446,10 +451,10 @@ __device__ __forceinline__ floatx16 scores32(const uint8_t* kt, const uint4 (&qf
     return s;
 }
 
-// O^T += V^T P^T over 16 keys (their rows in LDS at vt): p as PN terms of B fragments,
+// O^T += V^T P^T over 16 keys (their rows in LDS at vt): p as kTerms terms of B fragments,
 // in the order of the keys that scores32 leaves.
-template <int DH, bool F16, int PN>
-__device__ __forceinline__ void values16(const uint8_t* vt, const uint32_t (&t)[4][PN], floatx16 (&o)[DH / 32]) {
+template <int DH, bool F16>
+__device__ __forceinline__ void values16(const uint8_t* vt, const uint32_t (&t)[4][kTerms], floatx16 (&o)[DH / 32]) {
     const int lane = threadIdx.x & 63, i = lane & 15;
     const uint8_t* const row = vt + ((lane >> 5) * 4 + (i >> 2)) * (2 * DH) + ((lane >> 4) & 1) * 32 + (i & 3) * 8;
     const int x = perm_v<DH>(i >> 2) / 4;
@@ -458,7 +463,7 @@ __device__ __forceinline__ void values16(const uint8_t* vt, const uint32_t (&t)[
         const uint2 lo = lds_read_tr(row + (d ^ x) * 64), hi = lds_read_tr(row + (d ^ x) * 64 + 16 * DH);
         const uint4 vf = make_uint4(lo.x, lo.y, hi.x, hi.y);
 #pragma unroll
-        for (int n = PN - 1; n >= 0; n--) o[d] = mfma<F16>(vf, make_uint4(t[0][n], t[1][n], t[2][n], t[3][n]), o[d]);
+        for (int n = kTerms - 1; n >= 0; n--) o[d] = mfma<F16>(vf, make_uint4(t[0][n], t[1][n], t[2][n], t[3][n]), o[d]);
     }
 }
 
@@ -690,10 +695,10 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
         else wait_vmem<0>();
 #pragma unroll
         for (int kk = 0; kk < 2; kk++) {
-            uint32_t p[4][2];
+            uint32_t p[4][kTerms];
 #pragma unroll
-            for (int e = 0; e < 4; e++) split_pair<F16, 2>(s[0][8 * kk + 2 * e], s[0][8 * kk + 2 * e + 1], p[e]);
-            values16<DH, F16, 2>(vt + kk * 16 * 2 * DH, p, o);
+            for (int e = 0; e < 4; e++) split_pair<F16, kTerms>(s[0][8 * kk + 2 * e], s[0][8 * kk + 2 * e + 1], p[e]);
+            values16<DH, F16>(vt + kk * 16 * 2 * DH, p, o);
         }
         wait_lds();
         if (more) load(Vals{}, next, jn);
@@ -790,7 +795,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
 // buffers: the next tile is on its way while one is used; one barrier a tile. Eight waves
 // are two such groups that take the tiles in turn and join their results in LDS: where a
 // CU has one tile of rows only, its keys are walked in half the time.
-template <int DH, bool F16, int PN, int NW>
+template <int DH, bool F16, int NW>
 __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, uint8_t* lds) {
     constexpr int kTile = 64 * DH * 2;
     constexpr int NG = NW / 4;
@@ -882,11 +887,11 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
         weigh<2>(s, c, neg, l);
 #pragma unroll
         for (int kk = 0; kk < 4; kk++) {
-            uint32_t p[4][PN];
+            uint32_t p[4][kTerms];
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                split_pair<F16, PN>(s[kk >> 1][8 * (kk & 1) + 2 * e], s[kk >> 1][8 * (kk & 1) + 2 * e + 1], p[e]);
-            values16<DH, F16, PN>(vt + kk * 16 * 2 * DH, p, o);
+                split_pair<F16, kTerms>(s[kk >> 1][8 * (kk & 1) + 2 * e], s[kk >> 1][8 * (kk & 1) + 2 * e + 1], p[e]);
+            values16<DH, F16>(vt + kk * 16 * 2 * DH, p, o);
         }
     };
     floatx16 s0[2] = {scores32<DH, F16>(lds, qf), scores32<DH, F16>(lds + 32 * 2 * DH, qf)}, s1[2];
@@ -971,17 +976,17 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
                        o[d][4 * g + 3] * inv);
 }
 
-// PN: terms of a probability in tiles of 128 rows; 0: a call of tiles of 32 rows alone.
-template <int DH, bool F16, int PN, int NW>
+// MIXED: tiles of 128 rows and of 32; else of 32 alone.
+template <int DH, bool F16, bool MIXED, int NW>
 __global__ __launch_bounds__(64 * NW, DH == 256 || NW == 8 ? 1 : 2) void paged_attn_kernel(Attn w) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * NW * 32 * DH * 2];  // of either: 16 KB a wave at a head_dim of 128
     // (the grid's fastest axis: with 8 kv heads all tiles of a head share one XCD's L2)
     const int hk = blockIdx.x;
     const Work k = find_work<false>(w, blockIdx.z * gridDim.y + blockIdx.y);
     if (!k.ok) return;
-    if constexpr (PN > 0)
+    if constexpr (MIXED)
         if (!k.few) {
-            many_rows<DH, F16, PN, NW>(w, k, hk, lds);
+            many_rows<DH, F16, NW>(w, k, hk, lds);
             return;
         }
     few_rows<DH, F16, NW>(w, k, hk, lds);
@@ -1075,13 +1080,10 @@ Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, size_t workspa
     auto with = [&](auto dh, auto f16) {
         constexpr int DH = decltype(dh)::value;
         constexpr bool F16 = decltype(f16)::value;
-        if (L.only_few) go(paged_attn_kernel<DH, F16, 0, 4>, L.items, 0, 256);
-        else if (!L.wide && a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2, 4>, L.items, 0, 256);
-        else if (!L.wide) go(paged_attn_kernel<DH, F16, 1, 4>, L.items, 0, 256);
-        if constexpr (DH != 256) {  // (its tiles fill the LDS)
-            if (L.wide && a.out_dt == JH_F32) go(paged_attn_kernel<DH, F16, 2, 8>, L.items, 0, 512);
-            else if (L.wide) go(paged_attn_kernel<DH, F16, 1, 8>, L.items, 0, 512);
-        }
+        if (L.only_few) go(paged_attn_kernel<DH, F16, false, 4>, L.items, 0, 256);
+        else if (!L.wide) go(paged_attn_kernel<DH, F16, true, 4>, L.items, 0, 256);
+        if constexpr (DH != 256)  // (its tiles fill the LDS)
+            if (L.wide) go(paged_attn_kernel<DH, F16, true, 8>, L.items, 0, 512);
         if (!L.w.sync && !a.whole) go(paged_attn_merge_kernel<DH>, L.merges, L.merge_rows, kMergeThreads);
     };
     auto typed = [&](auto dh) { a.f16 ? with(dh, std::true_type{}) : with(dh, std::false_type{}); };

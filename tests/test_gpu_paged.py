@@ -820,3 +820,26 @@ def test_step_captured(hip):
         hip.Floats(hip.Add(up(hip, np.ones(300), F32), up(hip, np.ones(300), F32)))
     g.close()
     b.Close()
+
+
+# ---- probabilities in two terms, whatever the result's type --------------------------------
+
+def fp32_bar(c, out_dt):
+    """(expected, bar): the bar of fp32 results, whose probabilities are two terms of the
+    pages' dtype, and one rounding of the result to out_dt."""
+    want, bar = c.ref(F32)
+    return want, bar + HALF[out_dt] * np.abs(want) * 1.01 + (2.0 ** -25 if out_dt == F16 else 0)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("lens,Hq,Hk,D", [([(70, 300)], 4, 2, 64), ([(257, 257), (3, 90)], 8, 2, 128), ([(40, 2500), (1, 70)], 8, 2, 128),
+                                          ([(50, 200)], 4, 2, 256)])
+def test_attention_probabilities_are_not_rounded(hip, dt, lens, Hq, Hk, D):
+    """Results of 16 bits in tiles of 128 rows are as near as fp32's, rounded once, also
+    where they have more bits than the pages; the hint chooses kernels of the same precision."""
+    c = Paged(hip, lens, Hq, Hk, D, 16, dt, spread=0.25)
+    for out_dt in (BF16, F16):
+        want, bar = fp32_bar(c, out_dt)
+        for max_new in (lens[0][0], 1):
+            step(f"jh_paged_attention two terms {lens} D={D} dt={dt} out={out_dt} hint={max_new}")
+            close(c.run(out_dt, max_new=max_new), want, bar, c.starts[-1])
