@@ -630,8 +630,9 @@ enum {
     JH_PLAN_LENGTHS = 1, /* a length below 0, or past max_blocks pages */
     JH_PLAN_ROWS = 2,    /* more new tokens than n_rows */
     JH_PLAN_PAGES = 3,   /* not enough free pages (or *free_count outside [0, n_pages]) */
-    JH_PLAN_TABLE = 4    /* a finished request's table, or the stack, holds a number outside
-                            [0, n_pages), or more pages come back than the stack has room for */
+    JH_PLAN_TABLE = 4    /* a page number that the step uses lies outside [0, n_pages): a finished
+                            request's, one off the stack, or that of a partly filled page which new
+                            tokens go on filling; or more pages come back than the stack has room for */
 };
 
 /* The bookkeeping of one step, in one launch. Per request r, new_lens[r] >= 0

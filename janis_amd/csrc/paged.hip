@@ -17,8 +17,9 @@ typedef float f32x2_t __attribute__((ext_vector_type(2)));
 // 2048 requests over 1024 threads), and a row or page finds its request by bisection,
 // kTogether of them to a thread at once. Bound: latency -- the lengths' round trip, the
 // scan's barriers, the pages' round trip, the tables' and the stores. MI355X: 64 requests
-// of one new token 5.2 us, 700 requests with 8192 rows 14.0 us (16.0 with one row or page
-// to a thread at a time, 14.4 with two, 13.9 with eight, where 64 requests take 1 us more).
+// of one new token 5.7 us, 700 requests with 8192 rows 14.6 us, of which 0.15 and 0.5 are
+// the look at the pages that requests go on filling. Without it 14.1, where one row or page
+// to a thread at a time took 16.0, two 14.4 and eight 13.9 (64 requests then 1 us more).
 constexpr int kPlanThreads = 1024, kTogether = 4;
 static_assert(kPlanMaxReq % kPlanThreads == 0, "requests per thread");
 
@@ -64,7 +65,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
     int kv[kPer], n[kPer], add[kPer][3];
     int run[3] = {0, 0, 0};           // rows, pages to take, pages that come back
     float about[3] = {0.0f, 0.0f, 0.0f};  // the same, where 32 bits may not hold them
-    bool bad = false;
+    bool bad = false, out = false;  // out: a page number that is used lies outside the pool
+    int last[kPer];
 #pragma unroll
     for (int e = 0; e < kPer; e++) {
         const int r = tid * kPer + e;
@@ -76,6 +78,9 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
         const bool wrong = kv[e] < 0 || kv[e] > limit || (int64_t)kv[e] + max(n[e], 0) > limit;
         bad |= wrong;
         const int held = wrong ? 0 : blocks(kv[e]);
+        // new tokens that begin inside the last page held: its number is on its way beside the scan
+        last[e] = !wrong && n[e] > 0 && (kv[e] & (a.page_size - 1))
+                      ? a.tables[(int64_t)(tid * kPer + e) * a.max_blocks + held - 1] : 0;
         add[e][0] = wrong ? 0 : max(n[e], 0);
         add[e][1] = wrong || n[e] < 0 ? 0 : blocks((int64_t)kv[e] + n[e]) - held;
         add[e][2] = n[e] < 0 ? held : 0;
@@ -129,7 +134,8 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             for (int c = 0; c < 3; c++) run[c] += add[e][c];
         }
         __syncthreads();
-        bool out = false;
+#pragma unroll
+        for (int e = 0; e < kPer; e++) out |= (uint32_t)last[e] >= (uint32_t)a.n_pages && n[e] > 0;
 #pragma unroll
         for (int e = 0; e < kTogether; e++) {
             const int k = tid + e * kPlanThreads;
@@ -195,7 +201,7 @@ __global__ __launch_bounds__(kPlanThreads) void paged_plan_kernel(PagedPlanArgs 
             const int i = first + e * kPlanThreads + tid;
             if (i >= a.n_rows) break;
             a.positions[i] = pos[e];
-            a.slots[i] = (uint32_t)page[e] < (uint32_t)a.n_pages ? (page[e] << shift) + (pos[e] & (a.page_size - 1)) : -1;
+            a.slots[i] = pos[e] >= 0 ? (page[e] << shift) + (pos[e] & (a.page_size - 1)) : -1;
         }
     }
 }

@@ -843,3 +843,35 @@ def test_attention_probabilities_are_not_rounded(hip, dt, lens, Hq, Hk, D):
         for max_new in (lens[0][0], 1):
             step(f"jh_paged_attention two terms {lens} D={D} dt={dt} out={out_dt} hint={max_new}")
             close(c.run(out_dt, max_new=max_new), want, bar, c.starts[-1])
+
+
+# ---- the plan: pages that requests go on filling ----------------------------------------------
+
+@pytest.mark.parametrize("bad", [-1, 7, 2 ** 30])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_plan_page_in_use_outside(hip, bad, in_place):
+    """New tokens that begin inside a page whose number is outside the pool: nothing is
+    planned. Such numbers where no token goes (a request without new tokens, a last page
+    that is full, earlier pages) are not looked at."""
+    page, rows, n_pages = 16, 8, 7
+    kv, free, count = np.array([20, 16, 40, 5], np.int32), np.array([5, 6, -1, -1, -1, -1, -1], np.int32), 2
+    tables = np.array([[0, 1, -1, -1], [2, -1, -1, -1], [bad, bad, 3, -1], [4, -1, -1, -1]], np.int32)
+    new = np.array([2, 1, 3, 0], np.int32)
+    tables[1, 0] = tables[3, 0] = bad
+    step(f"jh_paged_plan page {bad} where no token goes, in_place={in_place}")
+    want = plan_ref(new, kv, page, tables, free, count, rows, n_pages)
+    assert want[5] == 0 and (want[4][:6] >= 0).all()
+    same_plan(run_plan(hip, new, kv, page, tables, free, count, rows, in_place), want)
+    for r, at in ((0, 1), (2, 2), (3, 0)):
+        t, n = tables.copy(), new.copy()
+        t[r, at], n[r] = bad, 1
+        none = np.full(rows, -1, np.int32)
+        step(f"jh_paged_plan page {bad} in use by request {r}")
+        same_plan(run_plan(hip, n, kv, page, t, free, count, rows, in_place),
+                  (kv, count, np.zeros(5, np.int32), none, none, _lib.JH_PLAN_TABLE, t, free))
+    hip.SetChecks(True)
+    try:
+        with pytest.raises(JanisHipError, match="page number"):
+            run_plan(hip, n, kv, page, t, free, count, rows)
+    finally:
+        hip.SetChecks(False)
