@@ -617,8 +617,8 @@ JH_API int jh_embed_norm_prepare(jh_ctx *ctx, const int32_t *ids, const uint32_t
  *                     is page * page_size + row). Requests may share pages.
  *   row_starts        int32 [n_req + 1]: request r's new tokens are the rows
  *                     row_starts[r] .. row_starts[r+1] - 1 of the step's batch of
- *                     n_rows rows (never decreasing; the rows from
- *                     row_starts[n_req] on belong to nobody)
+ *                     n_rows rows (never decreasing; rows before
+ *                     row_starts[0] and from row_starts[n_req] on belong to nobody)
  * all in device memory, so that one captured graph serves steps of any lengths.
  * A step is jh_paged_plan once and, per layer, the q/k/v product
  * (jh_quant_matmul), jh_paged_qk_norm_rope_append and jh_paged_attention. The

@@ -260,15 +260,17 @@ int count_nonfinite(jh_ctx* c, const char* op, const void* p, int dt, int64_t n,
 // With JH_CHECK_VALUES, an operator's result is counted for NaN/Inf after it
 // runs, as JANIS_GGML_CHECK reads every fp32 result back (ggml/ggml.go:622-677);
 // any found is JH_ERR_NONFINITE, naming the operator, the count and the first
-// index. The reference exits the process there; here the caller decides.
-int check_values(jh_ctx* c, const char* op, const void* y, int dt, int64_t n) {
+// index. The reference exits the process there; here the caller decides. The n
+// values from y[from] on are looked at.
+int check_values(jh_ctx* c, const char* op, const void* y, int dt, int64_t n, int64_t from = 0) {
     if (!(c->checks & JH_CHECK_VALUES) || n <= 0) return JH_OK;
     int64_t bad = 0, first = 0;
-    if (int r = count_nonfinite(c, op, y, dt, n, &bad, &first)) return r;
+    const void* const at = static_cast<const char*>(y) + from * (dt == JH_F32 ? 4 : 2);
+    if (int r = count_nonfinite(c, op, at, dt, n, &bad, &first)) return r;
     if (bad)
         return fail(c, JH_ERR_NONFINITE, std::string(op) + ": " + std::to_string(bad) + " of " + std::to_string(n) +
                                              " values NaN/Inf in the result, the first at index " +
-                                             std::to_string(first));
+                                             std::to_string(from + first));
     return JH_OK;
 }
 
@@ -1265,7 +1267,7 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
         return fail(c, JH_ERR_INVALID, std::string(op) + ": null pointer");
     if (!aligned16(q) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out))
         return fail(c, JH_ERR_INVALID, std::string(op) + ": q, out and the pages must be 16-byte aligned");
-    int64_t used = n_rows;
+    int64_t from = 0, used = n_rows;  // the rows that belong to requests: what a value check looks at
     if (c->checks) {
         std::vector<int32_t> st, kv, tab;
         if (int r = read_ints(c, op, row_starts, n_req + 1, st)) return r;
@@ -1287,7 +1289,8 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
                                                            std::to_string(i) + " outside [0, n_pages)");
             }
         }
-        used = std::min<int64_t>(n_rows, std::max(0, st[n_req]));
+        from = std::min<int64_t>(n_rows, std::max(0, st[0]));
+        used = std::min<int64_t>(n_rows, std::max(0, st[n_req])) - from;
     }
     jh::PagedAttnArgs a{};
     a.q = static_cast<const uint16_t*>(q), a.q_stride = q_stride;
@@ -1308,7 +1311,8 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
         a.whole = 1;
     }
     if (int r = finish(c, jh::launch_paged_attn(a, c->ws, c->ws_bytes, c->num_cus, sync, c->stream), op)) return r;
-    return check_values(c, op, out, out_dtype, used * n_heads * head_dim);
+    const int64_t row = n_heads * head_dim;
+    return check_values(c, op, out, out_dtype, used * row, from * row);
 }
 
 }  // extern "C"

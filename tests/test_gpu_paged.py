@@ -875,3 +875,27 @@ def test_plan_page_in_use_outside(hip, bad, in_place):
             run_plan(hip, n, kv, page, t, free, count, rows)
     finally:
         hip.SetChecks(False)
+
+
+def test_values_checked_between_the_ends(hip):
+    """Rows before the first request's belong to nobody: left as they were, and not
+    looked at by JH_CHECK_VALUES, whose index counts from the result's start."""
+    c = Paged(hip, [(2, 40), (3, 30)], 4, 2, 64, 16, BF16, pad=4)
+    want, bar = c.ref(BF16)
+    shift = 3
+    Q = np.zeros_like(c.q)
+    Q[shift:shift + 5] = c.q[:5]
+    Q, ST = up(hip, Q, BF16), ints(hip, c.starts + shift)
+    fill = up(hip, np.full((c.T, 4, 64), np.nan), BF16)
+    hip.SetChecks(_lib.JH_CHECK_INDICES | _lib.JH_CHECK_VALUES)
+    try:
+        step("jh_paged_attention checked, rows of nobody at both ends")
+        got = hip.Floats(hip.PagedAttention(Q, c.K, c.V, c.TAB, ST, c.KV, c.scale, maxNew=3, out=fill))
+        assert np.isnan(got[:shift]).all() and np.isnan(got[shift + 5:]).all()
+        close(got[shift:], want, bar, 5)
+        hip.SetChecks(_lib.JH_CHECK_VALUES)
+        c.tables[1, 0] = 2 ** 30
+        with pytest.raises(JanisHipError, match=f"index {(shift + 2) * 4 * 64}"):
+            hip.PagedAttention(Q, c.K, c.V, ints(hip, c.tables), ST, c.KV, c.scale, maxNew=3, out=fill)
+    finally:
+        hip.SetChecks(False)
