@@ -219,13 +219,28 @@ _engine = []
 
 
 def _backend():
-    """The program's one backend and the stream it works on."""
+    """The program's one backend and its stream, which torch's work goes to from then
+    on: inputs are ready when the backend reads them, and what reads its results waits."""
     if not _engine:
         from janis_amd.engine import HipBackend
         b, stream = HipBackend(0), torch.cuda.Stream()
         b.SetStream(stream.cuda_stream)
-        _engine.extend((b, stream))
-    return _engine[0]
+        stream.wait_stream(torch.cuda.current_stream())
+        torch.cuda.set_stream(stream)
+        _engine.extend((b, stream, stream.cuda_stream))
+    return _engine
+
+
+def _ordered(call, c, s):
+    """One of the calls below, in the order of the caller's stream where that is another one."""
+    b, stream, handle = _backend()
+    if torch._C._cuda_getCurrentRawStream(0) == handle:
+        return call(b, c, s)
+    caller = torch.cuda.current_stream()
+    stream.wait_stream(caller)
+    out = call(b, c, s)
+    caller.wait_stream(stream)
+    return out
 
 
 def _handles(b, s):
@@ -237,24 +252,21 @@ def _handles(b, s):
     return s["handles"]
 
 
-def _own_plan(c, s):
-    b = _backend()
+def _own_plan(b, c, s):
     h = _handles(b, s)
     b.PagedPlan(h["new"], h["kv"], c["page"], h["tables"], h["free"], h["count"],
                 out=(h["kv_out"], h["count_out"], h["starts"], h["pos"], h["slots"], h["status"]))
     return _plan_out(s["kv_out"], s["count_out"], s["starts"], s["pos"], s["slots"], s["status"], s["tables"], s["free"])
 
 
-def _own_append(c, s):
-    b = _backend()
+def _own_append(b, c, s):
     h = _handles(b, s)
     b.PagedQKNormRoPEAppend(h["qkv"], c["heads"], c["kv"], h["q_norm"], h["k_norm"], EPS, THETA, 1.0, h["pos"], h["slots"], h["k_pages"],
                             h["v_pages"], q_out=h["q_out"])
     return {"q": s["q_out"], "k_pages": s["k_pages"], "v_pages": s["v_pages"]}
 
 
-def _own_attention(c, s):
-    b = _backend()
+def _own_attention(b, c, s):
     h = _handles(b, s)
     b.PagedAttention(h["q"], h["k_pages"], h["v_pages"], h["tables"], h["starts"], h["kv"], c["dim"] ** -0.5, maxNew=s["max_new"], out=h["out"])
     return {"out": s["out"]}
@@ -346,7 +358,7 @@ def _plain_attention(c, s):
 def run(s):
     c = s["case"]
     if own:
-        return {"plan": _own_plan, "append": _own_append, "attention": _own_attention}[c["kind"]](c, s)
+        return _ordered({"plan": _own_plan, "append": _own_append, "attention": _own_attention}[c["kind"]], c, s)
     return {"plan": _plain_plan, "append": _plain_append, "attention": _plain_attention}[c["kind"]](c, s)
 
 
