@@ -681,8 +681,8 @@ JH_API int jh_paged_plan(jh_ctx *ctx, const int32_t *new_lens, const int32_t *kv
  *             double (jh_rope rounds them to fp32, which at position 10^5 is up to 0.004
  *             of an angle off).
  *   q_out     [n_rows, n_heads, head_dim] of the pages' dtype
- * n_heads may be 0 (keys and values only; q_out unused). head_dim 64, 128 or 256.
- * qkv, q_out and the pages 16-byte aligned, qkv_stride and page_stride multiples of
+ * n_heads may be 0 (keys and values only; q_out unused). head_dim 64, 128 or 256, n_rows
+ * up to 2^25 (JH_ERR_UNSUPPORTED beyond). qkv, q_out and the pages 16-byte aligned, qkv_stride and page_stride multiples of
  * 8; q_out and the pages overlap no input. Norms and rotation in fp32, each result rounded
  * once to the pages' dtype. No value checks (JH_CHECK_VALUES) run here. */
 JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype qkv_dtype, int64_t n_rows,

@@ -482,6 +482,8 @@ struct PagedAppendArgs {
     int64_t page_stride;
     uint16_t* q_out;
 };
+// A wave per row, four to a block: the grid's threads stay below 2^32.
+constexpr int64_t kAppendMaxRows = 1 << 25;
 Status launch_paged_append(const PagedAppendArgs& a, int num_cus, hipStream_t st);
 struct PagedAttnArgs {
     const uint16_t* q;

@@ -1201,8 +1201,10 @@ int jh_paged_qk_norm_rope_append(jh_ctx* c, const void* qkv, jh_dtype qkv_dtype,
     if (int r = check_page_heads(c, op, n_kv_heads, head_dim, page_size, page_stride)) return r;
     if ((q_norm_w || k_norm_w) && w_dtype != JH_BF16 && w_dtype != JH_F16 && w_dtype != JH_F32)
         return fail(c, JH_ERR_INVALID, std::string(op) + ": norm weights must be bf16, f16 or f32");
-    if (n_heads < 0 || n_heads > 65536 || n_rows < 0 || n_rows > 0x7fffffff)
-        return fail(c, JH_ERR_INVALID, std::string(op) + ": bad shape");
+    if (n_heads < 0 || n_heads > 65536 || n_rows < 0) return fail(c, JH_ERR_INVALID, std::string(op) + ": bad shape");
+    if (n_rows > jh::kAppendMaxRows)
+        return fail(c, JH_ERR_UNSUPPORTED,
+                    std::string(op) + ": more than " + std::to_string(jh::kAppendMaxRows) + " rows in one call");
     if (qkv_stride < (n_heads + 2 * n_kv_heads) * head_dim || qkv_stride % 8 || qkv_stride > ((int64_t)1 << 32))
         return fail(c, JH_ERR_INVALID, std::string(op) + ": qkv_stride must hold a row and be a multiple of 8");
     if (!(rope_base >= 0.0f) || !(rope_base < __builtin_inff()))

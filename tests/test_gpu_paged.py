@@ -899,3 +899,12 @@ def test_values_checked_between_the_ends(hip):
             hip.PagedAttention(Q, c.K, c.V, ints(hip, c.tables), ST, c.KV, c.scale, maxNew=3, out=fill)
     finally:
         hip.SetChecks(False)
+
+
+def test_refusal_of_rows_past_the_grid(hip):
+    """A wave per row: more rows than a grid has room for are refused before the launch."""
+    t = hip.empty(F32, 1 << 12)
+    p = t.ptr
+    good = dict(qkv=p, dt=F32, T=0, stride=6 * 64, hq=2, hk=2, d=64, qw=p, kw=p, wdt=F32, eps=1e-6, base=1e4, scale=1.0, freqs=None,
+                pos=p, slots=p, k=p, v=p, pdt=BF16, pages=2, page=16, pstride=2 * 16 * 64, qo=p)
+    refused(hip, "jh_paged_qk_norm_rope_append", good, [(_lib.JH_ERR_UNSUPPORTED, dict(T=T)) for T in ((1 << 25) + 1, 1 << 31, 1 << 62)])
