@@ -1005,14 +1005,18 @@ class HipBackend:
     @staticmethod
     def _pages(op: str, k_pages: Tensor, v_pages: Tensor) -> tuple:
         """(n_pages, Hk, page_size, Dh, page_stride): pages may lie apart (keys and
-        values that alternate in one buffer), their insides are dense."""
-        if k_pages.dtype != v_pages.dtype or k_pages.shape != v_pages.shape or len(k_pages.shape) != 4 \
-                or k_pages.strides != v_pages.strides:
+        values that alternate in one buffer), their insides are dense (strides of
+        length-1 axes do not matter)."""
+        shape, st, vst = k_pages.shape, k_pages.strides, v_pages.strides
+        if k_pages.dtype != v_pages.dtype or shape != v_pages.shape or len(shape) != 4:
             raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: k_pages and v_pages must be alike, [n_pages, Hk, page, Dh]")
-        n, hk, page, dh = k_pages.shape
-        st = k_pages.strides
-        if st[1:] != (page * dh, dh, 1):
+        n, hk, page, dh = shape
+        if (st != vst or st[1:] != (page * dh, dh, 1)) and not (_is_dense(shape[1:], st[1:]) and _is_dense(shape[1:], vst[1:])):
             raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: the inside of a page must be dense")
+        if n == 1:
+            return n, hk, page, dh, hk * page * dh
+        if st[0] != vst[0]:
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: k_pages and v_pages must be alike, pages as far apart")
         return n, hk, page, dh, st[0]
 
     def PagedPlan(self, newLens: Tensor, kvLens: Tensor, pageSize: int, blockTables: Tensor, freePages: Tensor,

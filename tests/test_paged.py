@@ -131,3 +131,25 @@ def test_what_is_passed_on(b):
     assert b.PagedPlan(**a) is a["out"]
     (name, c), = b._L.made
     assert name == "jh_paged_plan" and c[3:6] == (R, T, PAGE) and c[7] == B and c[9] == P
+
+
+def test_pages_that_are_dense_whatever_their_strides_say(b):
+    """Strides of axes of length 1 do not matter: pages that hold [page, heads, dim] with one
+    head, pages of one key, a pool of one page."""
+    one_head = b.Transpose(tensor(b, (P, PAGE, 1, D), F16), 0, 2, 1, 3)
+    one_page = b._view(tensor(b, (HK, PAGE, D), F16), (1, HK, PAGE, D), (0, PAGE * D, D, 1))
+    for pages, hq, stride in ((one_head, HQ, PAGE * D), (one_page, HQ, HK * PAGE * D)):
+        a = attention_args(b)
+        a["k_pages"] = a["v_pages"] = pages
+        assert b.PagedAttention(**a) is a["out"]
+        assert b._L.made.pop()[1][5:9] == (F16, pages.shape[0], PAGE, stride)
+    one_key = b.Transpose(tensor(b, (P, 1, HK, D), BF16), 0, 2, 1, 3)
+    a = append_args(b)
+    a["k_pages"], a["v_pages"] = one_key, tensor(b, (P, HK, 1, D), BF16)
+    assert b.PagedQKNormRoPEAppend(**a) is a["q_out"]
+    assert b._L.made.pop()[1][19:23] == (BF16, P, 1, HK * D)
+    # keys and values whose pages lie apart differently are still refused
+    a["v_pages"] = b.Slice(tensor(b, (P, 2 * HK, 1, D), BF16), 1, 0, HK)
+    with pytest.raises(JanisHipError, match="alike"):
+        b.PagedQKNormRoPEAppend(**a)
+    assert not b._L.made
