@@ -908,3 +908,179 @@ def test_refusal_of_rows_past_the_grid(hip):
     good = dict(qkv=p, dt=F32, T=0, stride=6 * 64, hq=2, hk=2, d=64, qw=p, kw=p, wdt=F32, eps=1e-6, base=1e4, scale=1.0, freqs=None,
                 pos=p, slots=p, k=p, v=p, pdt=BF16, pages=2, page=16, pstride=2 * 16 * 64, qo=p)
     refused(hip, "jh_paged_qk_norm_rope_append", good, [(_lib.JH_ERR_UNSUPPORTED, dict(T=T)) for T in ((1 << 25) + 1, 1 << 31, 1 << 62)])
+
+
+# ---- long walks: what a block looks up, shares out or repeats more than once --------------------
+
+def expected(c, out_dt, tokens=None):
+    """(tokens, expected, bar) as Paged.ref gives them for fp32 results, then one rounding
+    to out_dt, for some tokens; keys with a score of -inf weigh nothing, and nothing of
+    them enters the bar."""
+    G = c.Hq // c.Hk
+    owner = [(r, i) for r, (n, _) in enumerate(c.lens) for i in range(n)]
+    tokens = list(range(len(owner))) if tokens is None else sorted(set(tokens))
+    want, bar = np.zeros((2, len(tokens), c.Hq, c.D))
+    for at, t in enumerate(tokens):
+        r, i = owner[t]
+        n, kv = c.lens[r]
+        seen = kv - n + i + 1
+        for h in range(c.Hk):
+            k, v = c.k[r][h, :seen].astype(np.float64), c.v[r][h, :seen].astype(np.float64)
+            q = c.q[t, h * G:(h + 1) * G].astype(np.float64)
+            s = q @ k.T * c.scale
+            live = np.isfinite(s).all(0)
+            assert (s[:, ~live] == -np.inf).all() and live.any()
+            k, v, s = k[live], v[live], s[:, live]
+            rest = (np.abs(q) @ np.abs(k).T).max(-1) * c.scale
+            w = np.exp(s - s.max(-1, keepdims=True))
+            w /= w.sum(-1, keepdims=True)
+            o, A = w @ v, w @ np.abs(v)
+            d = c.D * 2.0 ** -24 * rest + 2.0 ** -22 * (1 + np.abs(s).max(-1))
+            rel = 2 * np.expm1(2 * d) + HALF[c.dt] ** 2 + (seen / 64 + 128) * 2.0 ** -24
+            want[at, h * G:(h + 1) * G] = o
+            bar[at, h * G:(h + 1) * G] = A * rel[:, None] * 1.01
+    bar += (HALF[out_dt] + 2.0 ** -24) * 1.01 * np.abs(want) + (2.0 ** -25 if out_dt == F16 else 0)
+    assert np.isfinite(want).all() and np.isfinite(bar).all()
+    return tokens, want, bar
+
+
+def near(got, e):
+    tokens, want, bar = e
+    off = np.abs(got[tokens].astype(np.float64) - want) - bar
+    assert (off <= 0).all(), (np.unravel_index(np.argmax(off), off.shape), float(off.max()))
+
+
+def sharing(hip, R, new, kv, Hq, Hk, D, page, dt, seed=0):
+    """R requests of `new` tokens over the same kv keys and pages, queries of their own."""
+    c = Paged(hip, [(new, kv)], Hq, Hk, D, page, dt, seed=seed, pad=(R - 1) * new)
+    c.lens, c.k, c.v = [(new, kv)] * R, c.k * R, c.v * R
+    c.tables, c.starts = np.repeat(c.tables, R, 0), np.arange(R + 1, dtype=np.int32) * new
+    c.TAB, c.ST, c.KV = ints(hip, c.tables), ints(hip, c.starts), ints(hip, [kv] * R)
+    return c
+
+
+def captured_whole(lens, Hq, Hk, D, page, dt, out_dt, seed=0):
+    """The call captured on a context without a workspace, where keys are not split."""
+    b = HipBackend(0)
+    c = Paged(b, lens, Hq, Hk, D, page, dt, seed=seed)
+    n = max(n for n, _ in lens)
+    out = up(b, np.zeros((c.T, Hq, D)), out_dt)
+    step(f"jh_paged_attention whole keys {str(lens)[:50]} Hq={Hq} Hk={Hk} D={D} dt={dt} out={out_dt}")
+    g = Graph(b, lambda: b.PagedAttention(c.Q, c.K, c.V, c.TAB, c.ST, c.KV, c.scale, maxNew=n, out=out))
+    e = expected(c, out_dt, [t for t in range(c.T) if t < 3 or t > c.T - 4 or t % 23 == 0])
+    for _ in range(2):
+        put(b, out, np.zeros((c.T, Hq, D), np.float32 if out_dt == F32 else np.uint16))
+        g.replay()
+        near(b.Floats(out), e)
+    g.close()
+    b.Close()
+
+
+CUS = 256  # of an MI355X
+
+
+@pytest.mark.parametrize("dt,D,page", [(BF16, 128, 16), (F16, 128, 32), (BF16, 64, 8), (F16, 256, 64)])
+def test_attention_few_rows_look_up_pages_again(dt, D, page):
+    """A part of more than 16 tiles of 32 keys for each of four waves, three times over."""
+    kv = 5003
+    assert kv > 2 * 16 * 4 * 32
+    captured_whole([(1, kv), (3, 2100)], 4, 2, D, page, dt, dt)
+
+
+@pytest.mark.parametrize("Hk,D", [(64, 64), (32, 128)])
+def test_attention_split_parts_look_up_pages_again(hip, Hk, D):
+    """The same in split parts that are joined inside the launch: a decode batch whose
+    parts have more than 2048 keys each."""
+    R, kv = 16, 17000 if Hk == 32 else 9000
+    room = CUS * (4 if D == 64 else 2) // Hk  # blocks at once, per kv head; split over at most twice that
+    assert R * kv / (2 * room + R) > 16 * 4 * 32
+    c = sharing(hip, R, 1, kv, Hk, Hk, D, 16, BF16)
+    step(f"jh_paged_attention parts of many keys Hk={Hk} D={D}")
+    near(c.run(BF16), expected(c, BF16, [0, 7, 15]))
+
+
+@pytest.mark.parametrize("dt,D,page,out_dt", [(BF16, 128, 16, BF16), (F16, 64, 32, F16), (F16, 128, 64, F32), (BF16, 256, 16, BF16)])
+@pytest.mark.parametrize("others", [0, 8])
+def test_attention_many_rows_look_up_pages_again(dt, D, page, out_dt, others):
+    """More than 32 tiles of 64 keys for each group of waves: alone, where eight waves are
+    two groups (one of four at a head_dim of 256), and beside so many requests that blocks
+    have four."""
+    kv, Hk, G = 4700, 32 if others else 2, 2
+    tiles = 1 + others + (70 * G + others * 66 * G) // 128
+    assert (tiles * Hk > CUS) == bool(others) and kv > (2 if others or D == 256 else 1) * 32 * 64 * (1 if others or D == 256 else 2)
+    captured_whole([(70, kv)] + [(66, 67)] * others, Hk * G, Hk, D, page, dt, out_dt)
+
+
+@pytest.mark.parametrize("dt", [BF16, F16])
+@pytest.mark.parametrize("Hq,Hk,D,lens", [(256, 32, 128, [(130, 300)]), (256, 32, 64, [(130, 300)]), (64, 32, 128, [(70, 90)] * 4 + [(200, 400), (1, 900), (0, 5)]),
+                                          (48, 16, 64, [(90, 500)] * 9 + [(1, 70)] * 3), (32, 8, 128, [(1030, 1203)]), (32, 8, 64, [(1030, 1030)])])
+def test_attention_more_tiles_than_cus(hip, dt, Hq, Hk, D, lens):
+    """Long runs in so many tiles that blocks have four waves: all result types."""
+    rows = sum(n for n, _ in lens) * (Hq // Hk)
+    assert (min(len(lens), rows) + rows // 128) * Hk > CUS
+    c = Paged(hip, lens, Hq, Hk, D, 16, dt, pad=2)
+    T = int(c.starts[-1])
+    some = [t for t in range(T) if t < 2 or t > T - 3 or t % 41 == 0] + [int(s) for s in c.starts[:-1] if s < T] + [int(s) - 1 for s in c.starts if s > 0]
+    for out_dt in (BF16, F16, F32):
+        step(f"jh_paged_attention four waves Hq={Hq} Hk={Hk} D={D} lens={str(lens)[:40]} dt={dt} out={out_dt}")
+        near(c.run(out_dt), expected(c, out_dt, some))
+
+
+@pytest.mark.parametrize("n,kv,Hk", [(1, 500, 2), (6, 500, 2), (90, 300, 2), (90, 2500, 2), (1, 700, 8), (130, 200, 32)])
+@pytest.mark.parametrize("dt", [BF16, F16])
+def test_attention_scores_of_minus_infinity(hip, dt, n, kv, Hk):
+    """Keys whose scores are -inf weigh nothing; the others' results keep their bar. Half
+    of the keys, whole tiles of them, and a first tile without any other."""
+    Hq, D = 2 * Hk, 128
+    rng = np.random.default_rng(n + kv + Hk)
+    k, v = (rounded(rng.standard_normal((Hk, kv, D)), dt) for _ in range(2))
+    k[0, 1::2, 7] = -np.inf
+    k[1, :kv - n, 7] = -np.inf
+    if kv - n > 130:
+        k[1, 100, 7] = 0.5
+    c = Paged(hip, [(n, kv)], Hq, Hk, D, 16, dt, k=[k], v=[v])
+    c.q[:] = rounded(np.abs(c.q) + 0.125, dt)
+    c.Q = up(hip, c.q, dt)
+    for out_dt in (dt, F32):
+        step(f"jh_paged_attention scores of -inf n={n} kv={kv} Hk={Hk} dt={dt} out={out_dt}")
+        near(c.run(out_dt), expected(c, out_dt))
+
+
+@pytest.mark.parametrize("page,done,fresh", [(1, 30, 7000), (1, 45, 4500), (8, 30, 40000)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_plan_of_many_pages(hip, page, done, fresh, in_place):
+    """More pages than one round of the block takes (four for each of 1024 threads) come
+    back and are taken: past what came back into the stack, and not."""
+    rng = np.random.default_rng(fresh)
+    R = 60
+    kv = (rng.integers(150, 250, R) * page + rng.integers(0, page, R)).astype(np.int32)
+    new = np.ones(R, np.int32)
+    new[rng.permutation(R)[:done]] = -1
+    left = np.flatnonzero(new > 0)
+    new[left[0]], new[left[1]] = fresh // 3, fresh - fresh // 3
+    rows = int(np.maximum(new, 0).sum()) + 9
+    blocks = -(-kv // page)
+    back = int(blocks[new < 0].sum())
+    take = int((-(-(kv + np.maximum(new, 0)) // page) - blocks)[new >= 0].sum())
+    assert back > 4096 and take > 4096 and (take > back) == (fresh == 7000)
+    spare = 3000
+    n_pages = int(blocks.sum()) + spare
+    order = rng.permutation(n_pages).astype(np.int32)
+    tables = np.full((R, int((-(-(kv + np.maximum(new, 0)) // page)).max()) + 1), -7, np.int32)
+    at = 0
+    for r in range(R):
+        tables[r, :blocks[r]] = order[at:at + blocks[r]]
+        at += blocks[r]
+    free = np.full(n_pages, -9, np.int32)
+    free[:spare] = order[at:]
+    step(f"jh_paged_plan page={page}: {back} pages back, {take} taken, {rows} rows, in_place={in_place}")
+    want = plan_ref(new, kv, page, tables, free, spare, rows, n_pages)
+    assert want[5] == 0
+    same_plan(run_plan(hip, new, kv, page, tables, free, spare, rows, in_place), want)
+    # a bad number among those of the later rounds: nothing is planned
+    t = tables.copy()
+    last = int(np.flatnonzero(new < 0)[-1])
+    t[last, blocks[last] - 1] = n_pages
+    want = plan_ref(new, kv, page, t, free, spare, rows, n_pages)
+    assert want[5] == _lib.JH_PLAN_TABLE
+    same_plan(run_plan(hip, new, kv, page, t, free, spare, rows, in_place), want)
