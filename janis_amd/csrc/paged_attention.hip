@@ -155,8 +155,6 @@ struct Attn {
                      // merge launch joins the parts
     float* part;     // records of split parts: [record][DH] results, then [record][2] maximum and sum
 };
-// A unit of 64 keys counts kManyCost with a tile of 128 rows, 1 with one of 32.
-constexpr int kManyCost = 1;
 // Least units of a part: two (a 32-key tile per wave), and one more for every kRowsPerUnit
 // rows of results that a part writes and the merge reads.
 constexpr int kLeast = 2, kRowsPerUnit = 21;
@@ -218,7 +216,6 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
         return rows <= w.few ? (rows + kFewRows - 1) / kFewRows : (rows + kManyRows - 1) / kManyRows;
     };
     auto units_of = [&](const Request& q) { return max(1, (q.kv + kUnit - 1) / kUnit); };
-    auto cost_of = [&](const Request& q) { return q.n * G <= w.few ? 1 : kManyCost; };
     double all = 0.0;  // exact: below 2^53
     float new_rows = 0.0f;
     Request mine{0, 0, 0};
@@ -228,7 +225,7 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
         const Request q = request(a, r);
         if (e == 0) mine = q;
         new_rows += (float)q.n;
-        all += (double)tiles_of(q) * (double)units_of(q) * (double)cost_of(q);
+        all += (double)tiles_of(q) * (double)units_of(q);
     }
     // row_starts that go up and down, so that requests overlap: more items than the grid was
     // made for (it has room for 0.1 %), and nothing is done
@@ -237,12 +234,11 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
     const double total = __builtin_bit_cast(
         double, make_int2(__builtin_amdgcn_readlane(__builtin_bit_cast(int2, all).x, 63),
                           __builtin_amdgcn_readlane(__builtin_bit_cast(int2, all).y, 63)));
-    // most that a part may cost: at least total / target
+    // least units of a part that leave at most `target` of them
     const int most = a.whole ? 1 << 30 : (int)min(fma(total, w.per_target, 1.0), 1073741824.0);
     auto splits_of = [&](const Request& q) {
         const int rows = q.n * G, units = units_of(q);
-        int each = max(rows <= w.few ? most : most / kManyCost + 1,
-                       kLeast + min(rows, rows <= w.few ? kFewRows : kManyRows) / kRowsPerUnit);  // units per part
+        int each = max(most, kLeast + min(rows, rows <= w.few ? kFewRows : kManyRows) / kRowsPerUnit);  // units per part
         // joined by one block, a part costs about a ninth of a unit: least of C + units / C / 9
         if (w.sync) each = max(each, (int)sqrtf((float)units * (1.0f / 9.0f)));
         // (a rounded quotient: any count near it will do, the same in every block)
