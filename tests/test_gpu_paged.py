@@ -1084,3 +1084,16 @@ def test_plan_of_many_pages(hip, page, done, fresh, in_place):
     want = plan_ref(new, kv, page, t, free, spare, rows, n_pages)
     assert want[5] == _lib.JH_PLAN_TABLE
     same_plan(run_plan(hip, new, kv, page, t, free, spare, rows, in_place), want)
+
+
+@pytest.mark.parametrize("n,kv", [(1, 300), (6, 300), (90, 200)])
+def test_attention_values_below_the_normal_numbers(hip, n, kv):
+    """f16 values of a few of its least steps (2^-24) are used as they are, not as zeros."""
+    Hq, Hk, D = 4, 2, 128
+    rng = np.random.default_rng(n)
+    k = [rounded(0.5 * rng.standard_normal((Hk, kv, D)), F16)]
+    v = [(rng.integers(-300, 300, (Hk, kv, D)) * 2.0 ** -24).astype(np.float32)]
+    assert np.array_equal(rounded(v[0], F16), v[0])
+    c = Paged(hip, [(n, kv)], Hq, Hk, D, 16, F16, k=k, v=v)
+    step(f"jh_paged_attention small values n={n}")
+    near(c.run(F32), expected(c, F32))
