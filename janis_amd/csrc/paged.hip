@@ -301,7 +301,10 @@ __global__ __launch_bounds__(256) void paged_append_kernel(PagedAppendArgs a, in
             sincospif(2.0f * (float)(turns - rint(turns)), &s, &co);
             s_turn[wave][i] = make_float2(co, s);
         }
+        // (the lanes read each other's factors)
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
         __builtin_amdgcn_wave_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     }
 #pragma unroll
     for (int e = 0; e < 8; e++) {
