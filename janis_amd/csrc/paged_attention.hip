@@ -33,10 +33,12 @@
 //     non-temporal: 32 of 8000 take 189 us without. Short ones are chains of
 //     round trips (lengths, tables, keys, records): 1 token of 64 keys 6 us, of 700 9 to 10;
 //     with a launch of its own for the join 9 and 11 us.
-//   many rows: 2000 tokens of 8000 bf16 keys 328 us: 700 TFLOP/s of the formula's
-//     operations, and, the second product being made twice (kTerms), 1050 of the matrix
-//     cores', where a large bf16 product of the library reaches 1180. 513 tokens of 513 25
-//     us: a tile's keys are walked in order.
+//   many rows: 2000 tokens of 8000 bf16 keys 328 to 348 us, by device: 660 to 700 TFLOP/s
+//     of the formula's operations, and, the second product being made twice (kTerms), 990
+//     to 1050 of the matrix cores', where a large bf16 product of the library reaches 1180
+//     to 1350. By counters the MFMA pipes are busy 52 % of the time at 1.8 GHz and VALU
+//     47 %. Built with 256 registers, 8 of them spilled. 513 tokens of 513 24 us, of which
+//     4 are a merge launch that finds nothing to join: 136 blocks walk five steps of keys.
 #include "jh_common.hpp"
 
 namespace jh {
@@ -54,8 +56,8 @@ constexpr int kUnit = 64;       // keys: splits are whole units
 constexpr int kFewRows = 32;    // rows of a tile where rows are few
 constexpr int kManyRows = 128;  // ... and many
 // Requests of up to this many rows take tiles of 32, which read keys once per tile but
-// leave no wave idle: 16 runs of 2 to 7 tokens (8 rows each) 26.5 us, 28.9 with a limit of
-// 32; a run beyond takes tiles of 128 (two pieces of prompts beside 22 tokens 34.9 us).
+// leave no wave idle: 16 runs of 2 to 7 tokens (8 rows each) 26.7 us, 32.5 with a limit of
+// 32; a run beyond takes tiles of 128 (two pieces of prompts beside 22 tokens 42 us).
 constexpr int kFewLimit = 64;
 // p is held as p * 2^kPShift, and a row's maximum is moved when it grew by more than
 // kLazy (log2): f16 has nothing below 2^-24 and nothing past 2^16, so p is kept high
@@ -1004,13 +1006,15 @@ __global__ __launch_bounds__(kMergeThreads) void paged_attn_merge_kernel(Attn w)
 
 // A call's tiles and grid. `max_new` is a hint: with at most 32 rows per request as it
 // says (64 where the parts are joined in the launch), every request takes tiles of 32
-// rows; else those of more than kFewLimit rows take tiles of 128. `wide`: blocks of eight
-// waves where that many still find a CU each (mixed lengths 36.8 us, 46.5 without; a
-// prompt of 64 to 256 tokens loses 0.9 to 1.5 us, one of 1024 nothing). `parts`: with few tiles so many that all
-// blocks are resident at once (1 of 700 keys 11.5 us, 12.4 with one block more per head),
-// with many twice the room (64 of 100-8000: 102 us, 108 with the room alone, 103 with
-// three times); for long runs, whose records are large, fewer (2000 of 8000 249 us, 253
-// with the room, 288 with twice).
+// rows; else those of more than kFewLimit rows take tiles of 128. Runs of 2 to 7 tokens of
+// 8 heads: with a merge launch 16 of them 26.8 us in blocks made for both tiles, 29.0 in
+// blocks for tiles of 32; joined in the launch 64 of them 64 and 59, but 16 of 500 to 5000
+// keys 40 and 49. `wide`: blocks of eight waves where that many still find a CU each (mixed
+// lengths 42.5 us, 53 without; a prompt of 64 tokens loses 1.5 us, of 128 1.0, of 256 0.3,
+// of 1024 nothing). `parts`: with few tiles so many that all blocks are resident at once,
+// with many twice the room (64 of 100-8000: 87.9 us, 92.5 with the room alone, 88.1 with
+// three times); for long runs, whose records are large, fewer (2000 of 8000 348 us, 351
+// with the room, 395 with twice; a prompt of 1024 41, 47 and 47).
 struct Launch {
     Attn w;
     bool only_few, wide;  // wide: blocks of eight waves
