@@ -686,278 +686,6 @@ JH_API int jh_paged_plan(jh_ctx *ctx, const int32_t *new_lens, const int32_t *kv
  * up to 2^25 (JH_ERR_UNSUPPORTED beyond). qkv, q_out and the pages 16-byte aligned,
  * qkv_stride and page_stride multiples of 8; q_out and the pages overlap no input. Norms
  * and rotation in fp32, each result rounded once to the pages' dtype. No value checks (JH_CHECK_VALUES) run here. */
-JH_API int jh_attention_decode_noalloc(jh_ctx *ctx, const void *qkv, jh_dtype qkv_dtype, int64_t n_heads,
-                                       int64_t n_kv_heads, int64_t head_dim, const void *q_norm_w,
-                                       const void *k_norm_w, jh_dtype w_dtype, float eps, float rope_base,
-                                       float rope_scale, const float *rope_cs, int64_t pos, void *k_cache,
-                                       void *v_cache, jh_dtype cache_dtype, int64_t capacity, float scale,
-                                       void *out, jh_dtype out_dtype);
-
-/* The RoPE factors at one position, for callers that rotate many heads there
- * (the RoPE angles of cpu/cpu_attn.go:13-34): out[i] = cos(theta_i) and
- * out[dims/2 + i] = sin(theta_i), theta_i = pos * scale * inv_i, inv_i =
- * base^(-2i/dims) or 1/freqs[i] (freqs fp32 [dims/2], may be NULL); pow, cos
- * and sin in double, rounded to fp32, as jh_rope evaluates them. out is fp32
- * [dims], device. Computed once per decode step, it serves every layer's
- * jh_attention_decode (rope_cs), which otherwise evaluates them in each block. */
-JH_API int jh_rope_table(jh_ctx *ctx, int dims, float base, float scale, int64_t pos, const float *freqs,
-                  float *out);
-
-/* The router of MoEBlock.Forward (qwen/moe.go:455-491) on the device, for a
- * backend that offers it: per token, softmax over the n_experts logits
- * (cpu/cpu.go:461-499), the k largest by the reference's selection sort
- * (qwen/moe.go:420-444, ties as it breaks them), and with norm_topk != 0 the k
- * scores divided by their sum (NormTopk, :472-481). The reference copies the
- * probabilities to the host for this (the per-layer sync at :459); here the
- * indices and scores stay on the device for jh_moe_swiglu or
- * jh_gather_quant_matmul. Bit-identical to the CPU backend: the same fp32 order
- * of operations and exp evaluated in double.
- *   logits       [n_tok, n_experts] of logits_dtype (JH_F32 or JH_BF16), device
- *   rhs_indices  int32 [n_tok, k] (global expert ids), device
- *   scores       fp32 [n_tok, k], device
- * n_experts up to 4096. */
-JH_API int jh_moe_route(jh_ctx *ctx, const void *logits, jh_dtype logits_dtype, int64_t n_tok,
-                 int64_t n_experts, int64_t k, int norm_topk, int32_t *rhs_indices, float *scores);
-
-/* The expert MLP of moeApply (qwen/moe.go:501-511) in one call, for a backend
- * that offers it (the engine's optional-capability pattern,
- * engine/backend.go:38-112). The reference composes it from three
- * GatherQuantMatmul calls and four element-wise operators:
- *   g = gather(x, gate), u = gather(x, up)      one vector per token (A = 1)
- *   h = SiLU(g) * u                              SiLU(v) = v / (1 + exp(-v))
- *   d = gather(h, down)                          one vector per slot (A = k_slots)
- *   out[t, :] = mean_k(d[t, k, :] * scores[t, k]) * k_slots
- * Here it is two launches: gate+up with the SiLU*mul epilogue (h stays on the
- * device in bf16), then the down product with the score-weighted sum taken in
- * a fixed order (slot order, then a fixed tree of four partial sums) and
- * written once; calls of more than 32 (token, slot) pairs add a bucketing
- * launch and a launch that sums each token's weighted slot rows in slot order.
- * No atomics: repeated calls give the same bits.
- *   x            bf16 [n_tok, hidden] (x_dtype must be JH_BF16)
- *   gate, up     stacked [n_experts, intermediate, hidden * bits / 32] with
- *                scales/biases [n_experts, intermediate, hidden / group_size]
- *   down         stacked [n_experts, hidden, intermediate * bits / 32] with
- *                scales/biases [n_experts, hidden, intermediate / group_size]
- *   rhs_indices  int32 [n_tok, k_slots] and scores fp32 [n_tok, k_slots], device memory
- *   out          [n_tok, hidden] of out_dtype (JH_F32 or JH_BF16)
- * A token with an index outside [0, n_experts)
- * gets a row of NaN (or JH_ERR_INVALID when jh_set_checks is on). Shapes
- * outside the expert tiles (hidden and intermediate in {256, 512, 768, 1024,
- * 1536, 2048, 3072, 4096, 6144, 8192, 12288}, group_size 32/64/128, 16-bit
- * scales shared by the three stacks) return JH_ERR_UNSUPPORTED; callers then
- * compose it from jh_gather_quant_matmul as the reference does. */
-JH_API int jh_moe_swiglu(jh_ctx *ctx, const void *x, jh_dtype x_dtype, int64_t n_tok,
-                  const uint32_t *w_gate, const void *s_gate, const void *b_gate,
-                  const uint32_t *w_up, const void *s_up, const void *b_up,
-                  const uint32_t *w_down, const void *s_down, const void *b_down,
-                  jh_dtype sb_dtype, int64_t n_experts, int64_t hidden, int64_t intermediate,
-                  const int32_t *rhs_indices, const float *scores, int64_t k_slots,
-                  int group_size, int bits, void *out, jh_dtype out_dtype);
-
-/* Backend.Softmax (engine/backend.go:241-242; cpu/cpu.go:461-499) along the
- * middle axis of x viewed as [outer, len, inner] (axis a of a shape d: outer =
- * d0..d(a-1), len = d(a), inner = d(a+1)..): the maximum, e = exp(x - max) in
- * double rounded to fp32, e / sum(e), with the CPU backend's sequential fp32
- * sum for len <= 8192 (bit-identical; longer lines sum in a tree). y is fp32
- * of x's shape. The router softmax of MoEBlock.Forward (qwen/moe.go:458). */
-JH_API int jh_softmax(jh_ctx *ctx, const void *x, jh_dtype x_dtype, int64_t outer, int64_t len, int64_t inner,
-                      float *y);
-
-/* Backend.Mean (engine/backend.go:186; cpu/cpu_ops.go:113-142) over the middle
- * axis of [outer, len, inner]: y [outer, inner] fp32, each the sequential fp32
- * sum along the axis divided by len (bit-identical to the CPU backend). */
-JH_API int jh_mean(jh_ctx *ctx, const void *x, jh_dtype x_dtype, int64_t outer, int64_t len, int64_t inner,
-                   float *y);
-
-/* Backend.ScalarMul / ScalarAdd (engine/backend.go:250-252; cpu/cpu_misc.go:24-30). */
-typedef enum {
-    JH_SCALAR_MUL = 0, /* y = x * v */
-    JH_SCALAR_ADD = 1  /* y = x + v */
-} jh_scalar_op;
-JH_API int jh_scalar(jh_ctx *ctx, jh_scalar_op op, const void *x, jh_dtype x_dtype, int64_t n, float v, void *y,
-                     jh_dtype y_dtype);
-
-/* Prologues and epilogues of jh_quant_matvec_fused. */
-typedef enum {
-    JH_PRO_NONE = 0,     /* x_in = x */
-    JH_PRO_RMSNORM = 1,  /* x_in = RMSNorm(x, norm_w, eps): Block.ForwardCached's InputNorm /
-                            PostNorm feeding q/k/v and gate/up (qwen/block.go:59-60), and the
-                            final norm feeding the LM head (qwen/model.go:294-303) */
-    JH_PRO_SILU_MUL = 2, /* x holds [gate | up] (2 * in_features): x_in = SiLU(gate) * up,
-                            MLP.Forward's input to Down (qwen/mlp.go:33-35) */
-    JH_PRO_NORMED = 3    /* the same RMSNorm, prepared by the producer of x: x is the bf16
-                            norm_out and norm_stats the statistics that a JH_EPI_RESID_NORM
-                            call (or jh_norm_prepare) wrote; the product is scaled by
-                            1 / sqrt(sum(norm_stats) / in_features + eps) */
-} jh_prologue;
-
-typedef enum {
-    JH_EPI_STORE = 0,    /* y = x_in . W^T */
-    JH_EPI_RESID = 1,    /* y = resid + x_in . W^T in fp32 (y_dtype JH_F32; resid may be y):
-                            the residual adds of Block.ForwardCached (qwen/block.go:59-60) */
-    JH_EPI_SWIGLU = 2,   /* W holds 2 * out_features rows, the Gate rows then the Up rows
-                            (scales/biases likewise): y[j] = SiLU(g_j) * u_j with
-                            g = x_in . Gate^T, u = x_in . Up^T in fp32 (MLP.Forward's
-                            Mul(SiLU(Gate.Forward(x)), Up.Forward(x)), qwen/mlp.go:33-35) */
-    JH_EPI_RESID_NORM = 3 /* JH_EPI_RESID, and the input of the NEXT RMSNorm'd product:
-                            norm_out = bf16(y * norm_w) with norm_w that norm's weight
-                            [out_features], and norm_stats (JH_NORM_STATS fp32) the sum of
-                            y^2 split in partials; pass both to that product with
-                            JH_PRO_NORMED */
-} jh_epilogue;
-
-/* fp32 slots of the statistics buffer of JH_EPI_RESID_NORM / JH_PRO_NORMED. */
-#define JH_NORM_STATS 1024
-
-/* One decode product with the operators on either side of it, for a backend
- * that offers it (the engine's optional-capability pattern,
- * engine/backend.go:38-112). It replaces the reference's sequences
- *   RMSNorm -> QuantMatmul                 (prologue JH_PRO_RMSNORM)
- *   Mul(SiLU(gate), up) -> QuantMatmul      (prologue JH_PRO_SILU_MUL)
- *   QuantMatmul -> Add(resid, .)            (epilogue JH_EPI_RESID)
- *   QuantMatmul(Gate), QuantMatmul(Up) -> Mul(SiLU(.), .)  (epilogue JH_EPI_SWIGLU)
- * for one row (rows == 1 of jh_quant_matmul, transpose = true):
- *   x_in = bf16(prologue(x))  (as jh_rms_norm / jh_elementwise with a bf16 out)
- *   the product with fp32 accumulation (as jh_quant_matmul), then the epilogue.
- * On the one-launch path RMSNorm is applied as (bf16(x * norm_w) . W^T) /
- * sqrt(mean(x^2) + eps): the same value up to where the bf16 rounding of the
- * product's input falls (the product is linear in it), with no reduction
- * ahead of the weight stream.
- * One launch where the decode tiles take the shape (4-bit weights, group size
- * 32/64/128, bf16 scales, K = in_features in {256, 512, 768, 1024, 1536, 2048,
- * 3072, 4096, 6144, 8192, 12288, 16384}) and
- *   JH_PRO_NONE with JH_EPI_STORE or JH_EPI_RESID, x bf16, or
- *   JH_PRO_RMSNORM with JH_EPI_STORE or JH_EPI_SWIGLU, x fp32, norm_w bf16:
- * each block normalises its own copy of x in registers (no normalised copy
- * goes through HBM) and the add or SwiGLU happens in the product's epilogue.
- * Everything else runs the same arithmetic as separate launches through the
- * context's workspace.
- *   x       [in_features] ([2 * in_features] for JH_PRO_SILU_MUL), device
- *   resid   fp32 [out_features] for JH_EPI_RESID / JH_EPI_RESID_NORM, else ignored
- *   y       [out_features] of y_dtype
- *   norm_stats, norm_out   for JH_PRO_NORMED (stats in) and JH_EPI_RESID_NORM
- *           (stats and bf16 [out_features] out); a call cannot use both
- * The split RMSNorm (JH_EPI_RESID_NORM then JH_PRO_NORMED) moves the x * w part
- * of the norm into the epilogue of the product that makes x, so the product
- * that consumes it reads bf16 x like a plain one: y = (bf16(x * w) . W^T) /
- * sqrt(mean(x^2) + eps), with mean(x^2) summed from per-block partials in a
- * fixed order. It needs the one-launch tiles (and bf16 norm weights); other
- * shapes run as jh_norm_prepare-style and separate launches. */
-JH_API int jh_quant_matvec_fused(jh_ctx *ctx, jh_prologue prologue, const void *x, jh_dtype x_dtype,
-                          const void *norm_w, jh_dtype norm_w_dtype, float eps, const uint32_t *w,
-                          const void *scales, const void *biases, jh_dtype sb_dtype,
-                          int64_t out_features, int64_t in_features, int group_size, int bits,
-                          jh_epilogue epilogue, const float *resid, void *y, jh_dtype y_dtype,
-                          float *norm_stats, void *norm_out);
-
-/* The producer half of a split RMSNorm for a row the caller already holds (the
- * embedding row that enters the first block): norm_out = bf16(x * norm_w) [d]
- * and norm_stats (JH_NORM_STATS fp32) = the sum of x^2 in partials (the rest 0), for a
- * jh_quant_matvec_fused call with JH_PRO_NORMED. */
-JH_API int jh_norm_prepare(jh_ctx *ctx, const void *x, jh_dtype x_dtype, int64_t d, const void *norm_w,
-                    jh_dtype norm_w_dtype, void *norm_out, float *norm_stats);
-
-/* The decode step's entry into the first block, one launch: h = the embedding
- * row of token ids[0] (QuantEmbedding.Forward, qwen/embed.go:78-83: TakeAxis of
- * the packed table, its scales and biases, then Dequantize, cpu/cpu_misc.go:
- * 134-161; zeros for an id outside [0, vocab), as jh_take_rows gives), then
- * jh_norm_prepare on h with norm_w (the first block's InputNorm), and, when
- * rope_cs is not NULL, jh_rope_table(rope_dims, rope_base, rope_scale, pos)
- * into rope_cs. Every output is bit-identical to those separate calls.
- *   ids      int32 [1], device (the previous step's jh_argmax output)
- *   w/scales/biases  the [vocab, dims] table (bits 2, 4 or 8)
- *   h        F32 [dims]; norm_out bf16 [dims]; norm_stats JH_NORM_STATS fp32
- * No counterpart call in the reference: it fuses the three its decode step makes
- * (qwen/model.go:294-303 embedding, qwen/block.go:58 InputNorm, and the RoPE
- * factors every Attention.ForwardCached call evaluates). */
-JH_API int jh_embed_norm_prepare(jh_ctx *ctx, const int32_t *ids, const uint32_t *w, const void *scales,
-                          const void *biases, jh_dtype sb_dtype, int64_t vocab, int64_t dims,
-                          int group_size, int bits, const void *norm_w, jh_dtype norm_w_dtype,
-                          float *h, void *norm_out, float *norm_stats, int rope_dims, float rope_base,
-                          float rope_scale, int64_t pos, float *rope_cs);
-
-/* ---- a paged key/value cache for batches of requests ------------------------- *
- * KVCache (qwen/cache.go) holds one sequence in one contiguous buffer. A program
- * that serves many requests at once keeps their keys and values in pages instead:
- *   k_pages, v_pages  [n_pages, n_kv_heads, page_size, head_dim] (JH_BF16 or
- *                     JH_F16), page_stride elements from one page to the next
- *                     (n_kv_heads * page_size * head_dim when dense; more where
- *                     keys and values alternate in one buffer); page_size a power
- *                     of two up to 65536, n_pages * page_size < 2^31
- *   block_tables      int32 [n_req, max_blocks]: request r's key j lies in page
- *                     block_tables[r, j / page_size], row j % page_size (its slot
- *                     is page * page_size + row). Requests may share pages.
- *   row_starts        int32 [n_req + 1]: request r's new tokens are the rows
- *                     row_starts[r] .. row_starts[r+1] - 1 of the step's batch of
- *                     n_rows rows (never decreasing; rows before
- *                     row_starts[0] and from row_starts[n_req] on belong to nobody)
- * all in device memory, so that one captured graph serves steps of any lengths.
- * A step is jh_paged_plan once and, per layer, the q/k/v product
- * (jh_quant_matmul), jh_paged_qk_norm_rope_append and jh_paged_attention. The
- * reference has no counterpart: it decodes one session at a time. */
-
-/* *status of jh_paged_plan. */
-enum {
-    JH_PLAN_OK = 0,
-    JH_PLAN_LENGTHS = 1, /* a length below 0, or past max_blocks pages */
-    JH_PLAN_ROWS = 2,    /* more new tokens than n_rows */
-    JH_PLAN_PAGES = 3,   /* not enough free pages (or *free_count outside [0, n_pages]) */
-    JH_PLAN_TABLE = 4    /* a page number that the step uses lies outside [0, n_pages): a finished
-                            request's, one off the stack, or that of a partly filled page which new
-                            tokens go on filling; or more pages come back than the stack has room for */
-};
-
-/* The bookkeeping of one step, in one launch. Per request r, new_lens[r] >= 0
- * tokens join its kv_lens[r] keys; new_lens[r] < 0 says that it is finished.
- * First the pages of the finished requests go onto the stack free_pages[0 ..
- * *free_count) (request by request, in their tables' order), then the others take
- * what their new tokens need off its top (again in order) into block_tables.
- *   block_tables    [n_req, max_blocks], only the new pages' entries are written
- *   free_pages      [n_pages], in place
- *                   (a page that requests share would come back once for each of them:
- *                   their tables hold pages of their own here, or the caller does the
- *                   bookkeeping)
- *   kv_lens_out     [n_req]: kv_lens + new_lens, 0 for finished requests; may be kv_lens
- *   free_count_out  [1]; may be free_count
- *   row_starts      [n_req + 1]: running sums of the new tokens
- *   positions       [n_rows]: each new token's position (kv_lens[r] + i), -1 behind the last
- *   slots           [n_rows]: each new token's slot, -1 behind the last
- *                   (and nowhere else: a token whose page is not one is JH_PLAN_TABLE)
- *   status          [1]: JH_PLAN_OK, or why the step cannot be done (the first of the
- *                   reasons above that applies). Then nothing was planned:
- *                   block_tables and free_pages are as they were, kv_lens_out and
- *                   free_count_out repeat their inputs, row_starts is all 0,
- *                   positions and slots all -1, so that the step's other calls do
- *                   nothing. With JH_CHECK_INDICES it is read back and is
- *                   JH_ERR_INVALID here.
- * Apart from the two aliases, outputs overlap neither inputs nor each other.
- * n_req up to 2048, n_rows and n_pages to 2^30 (JH_ERR_UNSUPPORTED beyond). */
-JH_API int jh_paged_plan(jh_ctx *ctx, const int32_t *new_lens, const int32_t *kv_lens, int64_t n_req,
-                         int64_t n_rows, int64_t page_size, int32_t *block_tables, int64_t max_blocks,
-                         int32_t *free_pages, int64_t n_pages, const int32_t *free_count,
-                         int32_t *kv_lens_out, int32_t *free_count_out, int32_t *row_starts,
-                         int32_t *positions, int32_t *slots, int32_t *status);
-
-/* The middle of Attention.ForwardCached (qwen/attention.go:101-122) for a batch of
- * rows at positions of their own: from row t of the q/k/v product, q heads (RMS
- * norm with q_norm_w, rotation by positions[t]) to q_out, k heads (k_norm_w, the
- * same rotation) and v heads to slot slots[t] of the pages. A row whose slot is
- * outside [0, n_pages * page_size) is skipped whole: nothing of it is written, its
- * row of q_out stays as it was (with JH_CHECK_INDICES a slot other than -1
- * outside is JH_ERR_INVALID). Two rows of one slot leave a mix of their keys and values.
- *   qkv       [n_rows, (n_heads + 2 n_kv_heads) * head_dim] of qkv_dtype (JH_BF16 or
- *             JH_F32), qkv_stride elements from one row to the next
- *   q_norm_w, k_norm_w  [head_dim] of w_dtype (JH_BF16, JH_F16 or JH_F32), or NULL: no norm
- *   rotation  pairs (i, i + head_dim/2) by positions[t] * rope_scale * inv_i, inv_i =
- *             rope_base^(-2i/head_dim), or 1 / rope_freqs[i] (fp32 [head_dim/2]) when
- *             given; none where rope_freqs is NULL and rope_base 0. Angles are held in
- *             double (jh_rope rounds them to fp32, which at position 10^5 is up to 0.004
- *             of an angle off).
- *   q_out     [n_rows, n_heads, head_dim] of the pages' dtype
- * n_heads may be 0 (keys and values only; q_out unused). head_dim 64, 128 or 256, n_rows
- * up to 2^25 (JH_ERR_UNSUPPORTED beyond). qkv, q_out and the pages 16-byte aligned, qkv_stride and page_stride multiples of
- * 8; q_out and the pages overlap no input. Norms and rotation in fp32, each result rounded
- * once to the pages' dtype. No value checks (JH_CHECK_VALUES) run here. */
 JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype qkv_dtype, int64_t n_rows,
                                         int64_t qkv_stride, int64_t n_heads, int64_t n_kv_heads,
                                         int64_t head_dim, const void *q_norm_w, const void *k_norm_w,
