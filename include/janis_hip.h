@@ -685,7 +685,8 @@ JH_API int jh_paged_plan(jh_ctx *ctx, const int32_t *new_lens, const int32_t *kv
  * n_heads may be 0 (keys and values only; q_out unused). head_dim 64, 128 or 256, n_rows
  * up to 2^25 (JH_ERR_UNSUPPORTED beyond). qkv, q_out and the pages 16-byte aligned,
  * qkv_stride and page_stride multiples of 8; q_out and the pages overlap no input. Norms
- * and rotation in fp32, each result rounded once to the pages' dtype. No value checks (JH_CHECK_VALUES) run here. */
+ * and rotation in fp32, each result rounded once to the pages' dtype. No value checks
+ * (JH_CHECK_VALUES) run here. */
 JH_API int jh_paged_qk_norm_rope_append(jh_ctx *ctx, const void *qkv, jh_dtype qkv_dtype, int64_t n_rows,
                                         int64_t qkv_stride, int64_t n_heads, int64_t n_kv_heads,
                                         int64_t head_dim, const void *q_norm_w, const void *k_norm_w,
