@@ -306,12 +306,12 @@ def _ordered(call, c, s):
 def _handles(b, s):
     """The engine's handles on the state's buffers, made once as a program keeps them."""
     if "handles" not in s:
-        from janis_amd.engine import BF16, F16, F32, I32
+        from janis_amd.engine import BF16, F16, F32, I32, PagedLayers
         code = {torch.bfloat16: BF16, torch.float16: F16, torch.float32: F32, torch.int32: I32}
         h = {k: b.Wrap(t.data_ptr(), tuple(t.shape), code[t.dtype], keep=t) for k, t in s.items() if isinstance(t, torch.Tensor)}
         if s["case"]["kind"] == "commit":
-            for k in ("k_pages", "v_pages"):  # one cache to a layer
-                h[k] = [b.Wrap(t.data_ptr(), tuple(t.shape), code[t.dtype], keep=t) for t in s[k]]
+            caches = [[b.Wrap(t.data_ptr(), tuple(t.shape), code[t.dtype], keep=t) for t in s[k]] for k in ("k_pages", "v_pages")]
+            h["layers"] = PagedLayers(*caches)  # a cache to a layer
         s["handles"] = h
     return s["handles"]
 
@@ -339,7 +339,7 @@ def _own_logprobs(b, c, s):
 def _own_commit(b, c, s):
     h = _handles(b, s)
     b.PagedTreeCommit(h["parents"], h["tokens"], h["chosen"], h["starts"], h["kv"], c["words"], c["page"], h["tables"], h["free"], h["count"], h["slots"],
-                      h["k_pages"], h["v_pages"], known=h["known"],
+                      layers=h["layers"], known=h["known"],
                       out=(h["kv_out"], h["count_out"], h["accepted"], h["path"], h["next"], h["status"]))
     return _commit_out(s["kv_out"], s["count_out"], s["accepted"], s["path"], s["next"], s["status"], s["free"], s["k_pages"], s["v_pages"])
 
