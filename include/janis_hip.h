@@ -737,6 +737,142 @@ JH_API int jh_paged_attention(jh_ctx *ctx, const void *q, int64_t q_stride, cons
                               int64_t n_kv_heads, int64_t head_dim, float scale, void *out,
                               jh_dtype out_dtype);
 
+/* ---- trees of drafted tokens over the paged cache ------------------------------ *
+ * Speculative decoding: a small model drafts several continuations of every request
+ * as a tree of tokens, the large model looks at all of them in one step, and the path
+ * that it agrees with is kept. Row i of a request (the first is 0) is a token that is
+ * known (the last one sampled) or drafted; parents[t], int32 per row of the batch,
+ * says which earlier row of its request it follows (-1: it follows the request's
+ * committed keys). All rows are new tokens of jh_paged_plan, so a tree of n rows takes
+ * n slots behind the committed keys, whatever its shape.
+ *   jh_paged_plan             slots for all rows of the trees
+ *   jh_paged_tree_plan        positions and masks, once a step
+ *   per layer: jh_quant_matmul, jh_paged_qk_norm_rope_append, jh_paged_tree_attention
+ *   jh_argmax, jh_token_logprobs, or a sampler: the large model's token after each row
+ *   jh_paged_tree_commit      the path it agrees with; lengths, pages, keys and values
+ * A mask is mask_words (1 to JH_TREE_WORDS) 32-bit words per row, bit b % 32 of word
+ * b / 32 for row b of its request. A request of more than 32 * mask_words rows is an
+ * ordinary run (a prompt's piece in the same batch): a chain, causal, whose parents and
+ * masks are not looked at. The reference has no counterpart: it decodes one token of
+ * one session at a time. */
+#define JH_TREE_WORDS 16
+
+/* The positions and masks of one step's trees, in one launch.
+ *   parents     [n_rows]; a parent outside [-1, i) counts as -1 (with JH_CHECK_INDICES
+ *               it is JH_ERR_INVALID)
+ *   row_starts, kv_lens   as jh_paged_plan wrote them (kv_lens[r] with the new tokens)
+ *   positions   [n_rows]: kv_lens[r] - n + the row's depth (0 without a parent); may be
+ *               jh_paged_plan's positions, which number the rows one after the other
+ *   tree_mask   [n_rows, mask_words]: the row itself and the rows on its way up
+ * A run of more rows than bits has the positions of a chain and masks of 0; rows that
+ * belong to nobody have positions of -1 and masks of 0. Outputs overlap neither inputs
+ * nor each other. n_req up to 65536, n_rows to 2^30 (JH_ERR_UNSUPPORTED beyond). */
+JH_API int jh_paged_tree_plan(jh_ctx *ctx, const int32_t *parents, const int32_t *row_starts,
+                              const int32_t *kv_lens, int64_t n_req, int64_t n_rows, int64_t mask_words,
+                              int32_t *positions, uint32_t *tree_mask);
+
+/* jh_paged_attention where a new token sees the committed keys of its request, 0 ..
+ * L - n - 1, and of its n new ones those whose bits its mask has: key L - n + b for bit
+ * b < n. Any mask will do, a tree's or another (a row need not see itself); a row that
+ * sees no key (an empty mask and L <= n) is zeros. Requests of more than 32 *
+ * mask_words new tokens are causal, as in jh_paged_attention.
+ *   tree_mask  [n_rows, mask_words]
+ * Everything else is as there: types, sizes, strides, precision, the workspace, splits
+ * and their joining, max_new (a hint), rows without a request, checks. A row is NaN if
+ * a page of its request that holds a key up to the last one that it sees lies outside
+ * the pool. */
+JH_API int jh_paged_tree_attention(jh_ctx *ctx, const void *q, int64_t q_stride, const void *k_pages,
+                                   const void *v_pages, jh_dtype page_dtype, int64_t n_pages,
+                                   int64_t page_size, int64_t page_stride, const int32_t *block_tables,
+                                   int64_t max_blocks, const int32_t *row_starts, const int32_t *kv_lens,
+                                   const uint32_t *tree_mask, int64_t mask_words, int64_t n_req,
+                                   int64_t n_rows, int64_t max_new, int64_t n_heads, int64_t n_kv_heads,
+                                   int64_t head_dim, float scale, void *out, jh_dtype out_dtype);
+
+/* The path that the large model agrees with, request by request, in at most one launch
+ * for the bookkeeping and one for every 64 layers. The first known[r] rows of a request
+ * (held to 1 .. n; 1 where known is NULL) are tokens that are kept whatever the model
+ * says, a chain whose parents are not looked at: the last token sampled, or a prompt's
+ * end. From the last of them on, the row whose parent is the one before it and whose
+ * token is the model's choice there is kept too (of several the first), until there is
+ * none. A run of more than 32 * mask_words rows is kept whole.
+ *   parents      [n_rows]; parents outside [-1, i) belong to no path
+ *   tokens       int32 [n_rows]: each row's token
+ *   chosen       int32, chosen[t * chosen_stride]: the model's token after row t
+ *   known        int32 [n_req] or NULL
+ *   row_starts, kv_lens, block_tables, slots   as jh_paged_plan wrote them
+ *   free_pages   [n_pages], *free_count of them: pages that hold no kept token any more
+ *                go back onto the stack (request by request, in their tables' order).
+ *                A page that requests share would come back too, as there.
+ *   kv_lens_out  [n_req]: kv_lens without the rows that are not kept; may be kv_lens
+ *   free_count_out  [1]; may be free_count
+ *   accepted     [n_req]: rows kept, the known ones among them
+ *   path         [n_rows]: from row_starts[r] on, the kept rows of request r (numbers of
+ *                the batch's rows, increasing), then -1; -1 where rows belong to nobody
+ *   next_tokens  [n_req]: the model's token after the last kept row, -1 for a request
+ *                without rows
+ *   status       [1]: JH_PLAN_OK, or why nothing was done: JH_PLAN_LENGTHS (kv_lens[r]
+ *                below the request's rows, or past max_blocks pages), JH_PLAN_ROWS
+ *                (row_starts that decrease or leave [0, n_rows]), JH_PLAN_PAGES
+ *                (*free_count outside [0, n_pages]) or JH_PLAN_TABLE (a page that comes
+ *                back lies outside [0, n_pages), or the stack has no room for it). Then
+ *                kv_lens_out and free_count_out repeat their inputs, accepted is 0,
+ *                path and next_tokens are -1, free_pages, keys and values are as they
+ *                were. With JH_CHECK_INDICES it is read back and is JH_ERR_INVALID here.
+ *   k_pages, v_pages   HOST arrays of n_layers device pointers, each a layer's pages:
+ *                keys and values of the kept rows move to the request's first slots, so
+ *                that they lie one after the other behind the committed ones. (A row
+ *                whose slot is outside the pages is left out.) n_layers may be 0: the
+ *                caller moves them, from slots[path[j]] to slots[j].
+ * Apart from the two aliases, outputs overlap neither inputs nor each other. n_req up to
+ * 2048, n_rows and n_pages to 2^30, n_layers to 65536 (JH_ERR_UNSUPPORTED beyond).
+ * head_dim 64, 128 or 256; pages 16-byte aligned, page_stride a multiple of 8. */
+JH_API int jh_paged_tree_commit(jh_ctx *ctx, const int32_t *parents, const int32_t *tokens,
+                                const int32_t *chosen, int64_t chosen_stride, const int32_t *known,
+                                const int32_t *row_starts, const int32_t *kv_lens, int64_t n_req,
+                                int64_t n_rows, int64_t mask_words, int64_t page_size,
+                                const int32_t *block_tables, int64_t max_blocks, int32_t *free_pages,
+                                int64_t n_pages, const int32_t *free_count, const int32_t *slots,
+                                int32_t *kv_lens_out, int32_t *free_count_out, int32_t *accepted,
+                                int32_t *path, int32_t *next_tokens, int32_t *status,
+                                void *const *k_pages, void *const *v_pages, int64_t n_layers,
+                                jh_dtype page_dtype, int64_t n_kv_heads, int64_t head_dim,
+                                int64_t page_stride);
+
+/* ---- log probabilities ------------------------------------------------------------ */
+
+/* Most alternatives, and most given tokens, of a row of jh_token_logprobs. */
+#define JH_LOGPROBS_TOP 32
+#define JH_LOGPROBS_TOKENS 64
+
+/* Per row x of logits, with p = softmax(scale * x) over the vocabulary: the log
+ * probabilities of given tokens, the entropy of p, and the likeliest tokens, what the
+ * logprobs and top_logprobs of a completion report and what a draft is judged by. The
+ * reference copies the logits to the host and has neither (qwen/model.go:57-165 samples
+ * there).
+ *   logits       [rows, vocab] of logits_dtype (JH_BF16 or JH_F32), row_stride elements
+ *                from one row to the next, 16-byte aligned
+ *   tokens       int32 [rows, n_tokens], or NULL with n_tokens 0 (up to JH_LOGPROBS_TOKENS)
+ *   logprobs     fp32 [rows, n_tokens]: scale * (x[token] - max x) - ln sum e^(scale (x - max x));
+ *                NaN for a token outside [0, vocab) (with JH_CHECK_INDICES one other than
+ *                -1 is JH_ERR_INVALID)
+ *   entropy      fp32 [rows], in nats, or NULL
+ *   top_ids, top_logprobs  int32 and fp32 [rows, top_k] (top_k up to JH_LOGPROBS_TOP and
+ *                vocab; 0: neither): the largest logits in their order, of equal ones the
+ *                lower token first
+ * A logit of -inf (a token that a grammar leaves out) has probability 0, log probability
+ * -inf, and adds nothing to the entropy. A row that holds a NaN or +inf, or nothing but
+ * -inf, has no distribution: its values are NaN, its top_ids those of its largest
+ * logits, where a NaN counts as -inf. Sums and results are fp32, the sums of a row made
+ * in a fixed order: the same call gives the same bits. scale in [1e-30, 1e30], vocab up
+ * to 2^28, rows to 2^24 (JH_ERR_UNSUPPORTED beyond). Rows may be split over blocks,
+ * whose parts lie in the context's workspace. Outputs overlap neither inputs nor each
+ * other. No value checks (JH_CHECK_VALUES) run here. */
+JH_API int jh_token_logprobs(jh_ctx *ctx, const void *logits, jh_dtype logits_dtype, int64_t rows,
+                             int64_t vocab, int64_t row_stride, float scale, const int32_t *tokens,
+                             int64_t n_tokens, int64_t top_k, float *logprobs, float *entropy,
+                             int32_t *top_ids, float *top_logprobs);
+
 #ifdef __cplusplus
 }
 #endif

@@ -21,6 +21,7 @@ JH_PRO_NONE, JH_PRO_RMSNORM, JH_PRO_SILU_MUL, JH_PRO_NORMED = range(4)  # jh_pro
 JH_EPI_STORE, JH_EPI_RESID, JH_EPI_SWIGLU, JH_EPI_RESID_NORM = range(4)  # jh_epilogue
 JH_NORM_STATS = 1024
 JH_PLAN_OK, JH_PLAN_LENGTHS, JH_PLAN_ROWS, JH_PLAN_PAGES, JH_PLAN_TABLE = range(5)  # jh_paged_plan's status
+JH_TREE_WORDS, JH_LOGPROBS_TOP, JH_LOGPROBS_TOKENS = 16, 32, 64  # limits of the drafted trees and of jh_token_logprobs
 
 EXPORTS = [
     "jh_version", "jh_create", "jh_destroy", "jh_last_error", "jh_device_info",
@@ -32,6 +33,7 @@ EXPORTS = [
     "jh_softmax", "jh_mean", "jh_scalar", "jh_check_finite", "jh_attention_decode_noalloc",
     "jh_qkv_attention_decode", "jh_embed_norm_prepare", "jh_set_wait_limit",
     "jh_paged_plan", "jh_paged_qk_norm_rope_append", "jh_paged_attention",
+    "jh_paged_tree_plan", "jh_paged_tree_attention", "jh_paged_tree_commit", "jh_token_logprobs",
 ]
 
 _lib = None
@@ -130,7 +132,14 @@ def load() -> ctypes.CDLL:
                                                p, p, i, i64, i64, i64, p]
     L.jh_paged_attention.argtypes = [c_ctx, p, i64, p, p, i, i64, i64, i64, p, i64, p, p, i64, i64, i64, i64, i64, i64,
                                      f32, p, i]
-    for name in ("jh_paged_plan", "jh_paged_qk_norm_rope_append", "jh_paged_attention"):
+    L.jh_paged_tree_plan.argtypes = [c_ctx, p, p, p, i64, i64, i64, p, p]
+    L.jh_paged_tree_attention.argtypes = [c_ctx, p, i64, p, p, i, i64, i64, i64, p, i64, p, p, p, i64, i64, i64, i64,
+                                          i64, i64, i64, f32, p, i]
+    L.jh_paged_tree_commit.argtypes = [c_ctx, p, p, p, i64, p, p, p, i64, i64, i64, i64, p, i64, p, i64, p, p, p, p, p,
+                                       p, p, p, p, p, i64, i, i64, i64, i64]
+    L.jh_token_logprobs.argtypes = [c_ctx, p, i, i64, i64, i64, f32, p, i64, i64, p, p, p, p]
+    for name in ("jh_paged_plan", "jh_paged_qk_norm_rope_append", "jh_paged_attention", "jh_paged_tree_plan",
+                 "jh_paged_tree_attention", "jh_paged_tree_commit", "jh_token_logprobs"):
         getattr(L, name).restype = i
     L.jh_moe_route.argtypes = [c_ctx, p, i, i64, i64, i64, i, p, p]
     L.jh_moe_route.restype = i

@@ -500,12 +500,61 @@ struct PagedAttnArgs {
     void* out;
     int out_dt;
     int whole;                // keys are not split (no workspace)
+    const uint32_t* mask;     // jh_paged_tree_attention's, or nullptr
+    int mask_words;
 };
 // `sync`: kPagedSyncSlots of the context's zeroed counters where launches keep the
 // round-robin placement, or nullptr; the same in both.
 size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus, int* sync);
 Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, size_t workspace_bytes, int num_cus, int* sync,
                          hipStream_t st);
+
+// ---- trees of drafted tokens (tree.hip) ----
+struct TreePlanArgs {
+    const int32_t *parents, *row_starts, *kv_lens;
+    int n_req, n_rows, words;
+    int32_t* positions;
+    uint32_t* mask;
+};
+Status launch_tree_plan(const TreePlanArgs& a, hipStream_t st);
+struct TreeCommitArgs {
+    const int32_t *parents, *tokens, *chosen;
+    int64_t chosen_stride;
+    const int32_t *known, *row_starts, *kv_lens;
+    int n_req, n_rows, tree_rows, page_shift;  // tree_rows: a request of more is a run
+    const int32_t* tables;
+    int max_blocks;
+    int32_t* free_pages;
+    int n_pages;
+    const int32_t* free_count;
+    int32_t *kv_out, *count_out, *accepted, *path, *next_tokens, *status;
+};
+Status launch_tree_commit(const TreeCommitArgs& a, hipStream_t st);
+// Pointers travel in the launch's arguments: so many layers a launch.
+constexpr int kMoveLayers = 64;
+struct TreeMoveArgs {
+    const int32_t *row_starts, *accepted, *path, *slots;
+    int n_req, n_rows, n_slots, page_shift, Hk, Dh, layers;
+    int64_t page_stride;
+    uint16_t *k[kMoveLayers], *v[kMoveLayers];
+};
+Status launch_tree_move(const TreeMoveArgs& a, hipStream_t st);
+
+// ---- log probabilities (logprobs.hip) ----
+struct LogProbsArgs {
+    const void* x;
+    int f32;          // fp32 logits (else bf16)
+    int rows, vocab;
+    int64_t stride;   // elements from one row to the next
+    float scale;
+    const int32_t* tokens;
+    int n_tokens, top_k;
+    float *logprobs, *entropy;
+    int32_t* top_ids;
+    float* top_logprobs;
+};
+size_t logprobs_workspace_bytes(const LogProbsArgs& a, int num_cus);
+Status launch_logprobs(const LogProbsArgs& a, void* workspace, int num_cus, hipStream_t st);
 
 // ---- operators around the products (ops.hip) ----
 // QuantMatmul with transpose = false: y [rows, m.in] = x [rows, m.rows] . Dequantize(W);

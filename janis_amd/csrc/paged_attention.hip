@@ -296,14 +296,60 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
 // Keys that row `row` of the request sees.
 __device__ __forceinline__ int seen(const Request& q, int row, int G) { return max(0, q.kv - q.n + row / G + 1); }
 
+// With TREE the new tokens of a request see each other by the bits of a mask (those of a
+// run longer than the mask's bits up to their own, as above): key kv - n + b by bit b.
+__device__ __forceinline__ bool is_tree(const PagedAttnArgs& a, const Request& q) { return q.n <= 32 * a.mask_words; }
+// Keys up to the last one that the row sees.
+template <bool TREE>
+__device__ __forceinline__ int reach(const PagedAttnArgs& a, const Request& q, int row, int G) {
+    if constexpr (TREE)
+        if (is_tree(a, q)) {
+            const uint32_t* const m = a.mask + (int64_t)(q.start + row / G) * a.mask_words;
+            int top = 0;
+            for (int w = (q.n - 1) / 32; w >= 0 && top == 0; w--) {
+                const uint32_t bits = q.n - 32 * w < 32 ? m[w] & ((1u << (q.n - 32 * w)) - 1) : m[w];
+                if (bits) top = 32 * w + 32 - __clz((int)bits);
+            }
+            return max(0, q.kv - q.n + top);
+        }
+    return seen(q, row, G);
+}
+// The same over rows up to `last` of a request, where their first `all` is what all see.
+template <bool TREE>
+__device__ __forceinline__ int reach_of_tile(const PagedAttnArgs& a, const Request& q, int last, int G) {
+    if constexpr (TREE)
+        if (is_tree(a, q)) return q.kv;
+    return seen(q, last, G);
+}
+template <bool TREE>
+__device__ __forceinline__ int seen_by_all(const PagedAttnArgs& a, const Request& q, int first, int G) {
+    if constexpr (TREE)
+        if (is_tree(a, q)) return max(0, q.kv - q.n);
+    return seen(q, first, G);
+}
+// Of the 32 keys from k0 on those that the row sees, as bits; `lim`: its reach.
+__device__ __forceinline__ uint32_t sees32(const PagedAttnArgs& a, const Request& q, int row, int G, int k0, int lim) {
+    uint32_t bits = 0xFFFFFFFFu;
+    if (is_tree(a, q)) {
+        const int j = k0 - (q.kv - q.n), w = j >> 5;
+        const uint32_t* const m = a.mask + (int64_t)(q.start + row / G) * a.mask_words;
+        // (words before the first: committed keys, which all rows see)
+        const uint32_t lo = w < 0 ? 0xFFFFFFFFu : w < a.mask_words ? m[w] : 0u;
+        const uint32_t hi = w + 1 < 0 ? 0xFFFFFFFFu : w + 1 < a.mask_words ? m[w + 1] : 0u;
+        bits = __builtin_amdgcn_alignbit(hi, lo, (uint32_t)j & 31u);
+    }
+    const int left = lim - k0;
+    return left >= 32 ? bits : left <= 0 ? 0u : bits & ((1u << left) - 1);
+}
+
 // ---- a row again, key by key -------------------------------------------------------
 // The products meet masked keys with p = 0, where an infinity or NaN in V gives NaN, and
 // p's lesser terms (of either sign) meet an infinity that the row does see. So a row
 // whose result is not finite is computed again here, by one wave, in fp32 and reading
 // nothing that it does not see. m is log2; the lane's features are lane + 64 e.
-template <int DH, bool F16>
-__device__ __forceinline__ void row_again(const PagedAttnArgs& a, int r, int hk, int head, int token, int kb, int lim, float& m,
-                                       float& l, float (&o)[DH / 64]) {
+template <int DH, bool F16, bool TREE>
+__device__ __forceinline__ void row_again(const PagedAttnArgs& a, const Request& rq, int r, int hk, int head, int token, int kb, int lim,
+                                       float& m, float& l, float (&o)[DH / 64]) {
     const int lane = threadIdx.x & 63;
     const uint4* const q = reinterpret_cast<const uint4*>(a.q + token * a.q_stride + (int64_t)head * DH);
     m = ninf(), l = 0.0f;
@@ -328,7 +374,10 @@ __device__ __forceinline__ void row_again(const PagedAttnArgs& a, int r, int hk,
                 s = fmaf(u.y, v.y, s);
             }
         }
-        s = k0 + lane < lim ? s * (a.scale * kLog2e) : ninf();
+        bool sees = k0 + lane < lim;
+        if constexpr (TREE) sees = sees32(a, rq, token - rq.start, 1, k0 + (lane & 32), lim) >> (lane & 31) & 1u;
+        s = sees ? s * (a.scale * kLog2e) : ninf();
+        const uint64_t votes = __ballot(sees);
         const float mn = fmaxf(m, wave_max(s));
         const float sub = mn == ninf() ? 0.0f : mn, f = m == mn ? 1.0f : __builtin_amdgcn_exp2f(m - sub);
         const float p = __builtin_amdgcn_exp2f(s - sub + kPShift<F16>);  // as the products hold it
@@ -337,6 +386,7 @@ __device__ __forceinline__ void row_again(const PagedAttnArgs& a, int r, int hk,
         for (int e = 0; e < DH / 64; e++) o[e] *= f;
         m = mn;
         for (int j = 0; j < min(64, lim - k0); j++) {
+            if (TREE && !(votes >> j & 1u)) continue;
             const float pj = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(p), j));
             const int64_t row = (int64_t)(((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(at >> 32), j) << 32) |
                                           (uint32_t)__builtin_amdgcn_readlane((int)at, j));
@@ -466,12 +516,22 @@ __device__ __forceinline__ void values16(const uint8_t* vt, const uint32_t (&t)[
 }
 
 // One tile of 32 * N keys (from k0) of the online softmax: scores to weights in place.
-template <int DH, bool F16, int N>
-__device__ __forceinline__ float mask_and_move(floatx16 (&s)[N], int k0, int lim, bool edge, float c, float& m, float& l,
+// sees(k): with TREE, of the 32 keys from k on those that the lane's row sees.
+template <int DH, bool F16, bool TREE, int N, class Sees>
+__device__ __forceinline__ float mask_and_move(floatx16 (&s)[N], int k0, int lim, bool edge, Sees sees, float c, float& m, float& l,
                                                floatx16 (&o)[DH / 32]) {
     const int h = (threadIdx.x & 63) >> 5;
     // register r of s[g] is key k0 + 32 g + 8 (r / 4) + 4 h + r % 4
-    if (edge) {
+    if constexpr (TREE) {
+        if (edge)
+#pragma unroll
+            for (int g = 0; g < N; g++) {
+                const uint32_t bits = sees(k0 + 32 * g) >> (4 * h);
+#pragma unroll
+                for (int r = 0; r < 16; r++)
+                    if (!(bits & (1u << (8 * (r >> 2) + (r & 3))))) s[g][r] = ninf();
+            }
+    } else if (edge) {
 #pragma unroll
         for (int g = 0; g < N; g++)
 #pragma unroll
@@ -534,7 +594,7 @@ __device__ __forceinline__ int wave_min_int(int v) {
 // 8 parts (all requested together); a row's groups meet in LDS in their order. L2: the
 // records were stored by this launch on this XCD (device-coherent loads: past the CU's L1).
 constexpr int kJoinBatch = 8;
-template <int DH, int NT, bool L2>
+template <int DH, int NT, bool L2, bool TREE>
 __device__ __forceinline__ void join_rows(const Attn& w, const Work& k, int hk, int tile, int parts, int first, int stride,
                                           float4* s_o, float2* s_ml) {
     constexpr int kLanes = DH / 4, kGroups = NT / kLanes, kBatch = kJoinBatch;
@@ -602,7 +662,7 @@ __device__ __forceinline__ void join_rows(const Attn& w, const Work& k, int hk, 
             o[0] = fmaf(y.x, h, o[0]), o[1] = fmaf(y.y, h, o[1]), o[2] = fmaf(y.z, h, o[2]), o[3] = fmaf(y.w, h, o[3]);
         }
         const int row = tile * tr + x;
-        const bool sees = seen(k.q, row, G) > 0;
+        const bool sees = reach<TREE>(a, k.q, row, G) > 0;
         store_out4(a, out_at<DH>(a, k.q, row, hk, G) + 4 * f, sees ? o[0] / l : 0.0f, sees ? o[1] / l : 0.0f,
                    sees ? o[2] / l : 0.0f, sees ? o[3] / l : 0.0f);
     }
@@ -613,12 +673,13 @@ __device__ __forceinline__ void join_rows(const Attn& w, const Work& k, int hk, 
 // waves take the part's 32-key tiles in turn, each with its own buffers and no barrier:
 // while a tile's scores become weights the next tile's keys are on their way, while its
 // values are used the next values. The waves' results meet in LDS.
-template <int DH, bool F16, int NW>
+template <int DH, bool F16, int NW, bool TREE>
 __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, uint8_t* lds) {
     constexpr int kTile = 32 * DH * 2, kLoads = kTile / 1024;
     __shared__ float2 s_ml[NW][32];
     __shared__ int s_bad[NW];
     __shared__ uint32_t s_again[NW];
+    __shared__ int s_lim[TREE ? 32 : 1];  // the rows' reach within the part
     const PagedAttnArgs& a = w.a;
     const int G = w.G;
     const int tile = uniform(k.local / k.splits), split = k.local - tile * k.splits;
@@ -628,12 +689,15 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
     const int w0 = tile * kFewRows, n_rows = min(kFewRows, q.n * G - w0);
     const int kb = split * k.per * kUnit;
     // keys this part ends at: for the tile's last row, this lane's row, the first row
-    const int end = uniform(seen(q, w0 + n_rows - 1, G));
+    const int end = uniform(reach_of_tile<TREE>(a, q, w0 + n_rows - 1, G));
     const int parts = max(1, (end + k.per * kUnit - 1) / (k.per * kUnit));
     if (split >= parts) return;
     const int ke = min(end, kb + k.per * kUnit);
     const int row = w0 + min(c32, n_rows - 1);
-    const int lim = min(ke, seen(q, row, G)), lim_lo = min(ke, seen(q, w0, G));
+    const int lim = min(ke, reach<TREE>(a, q, row, G)), lim_lo = min(ke, seen_by_all<TREE>(a, q, w0, G));
+    if (TREE && threadIdx.x < n_rows) s_lim[threadIdx.x] = lim;
+    auto sees_at = [&](int x) { return TREE ? s_lim[x] : min(ke, seen(q, w0 + x, G)); };
+    auto sees_from = [&](int k) { return sees32(a, q, row, G, k, lim); };
     uint4 qf[DH / 16];
     load_q<DH>(a, q, row, hk, G, qf);
     const float c = a.scale * kLog2e;
@@ -688,7 +752,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
             if (jn == 0) look_up(next);
             load(K{}, next, jn);
         }
-        weigh<1>(s, c, mask_and_move<DH, F16, 1>(s, k0, lim, edge, c, m, l, o), l);
+        weigh<1>(s, c, mask_and_move<DH, F16, TREE, 1>(s, k0, lim, edge, sees_from, c, m, l, o), l);
         if (more) wait_vmem<kLoads>();
         else wait_vmem<0>();
 #pragma unroll
@@ -732,8 +796,8 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
         for (int x = wave; x < n_rows; x += NW) {
             if (!((again >> x) & 1u)) continue;
             float m1, l1, o1[DH / 64];
-            const int rw = w0 + x, sees = min(ke, seen(q, rw, G));
-            row_again<DH, F16>(a, k.r, hk, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
+            const int rw = w0 + x, sees = uniform(sees_at(x));
+            row_again<DH, F16, TREE>(a, q, k.r, hk, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
             if (sees > bad_all) l1 = __builtin_nanf("");
             if (parts > 1 && lane == 0) *reinterpret_cast<float2*>(rec_ml + 2 * x) = make_float2(m1, l1);
 #pragma unroll
@@ -761,7 +825,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
             const float gg = ml[v].x == mx ? 1.0f : g;
             r0 = fmaf(y.x, gg, r0), r1 = fmaf(y.y, gg, r1), r2 = fmaf(y.z, gg, r2), r3 = fmaf(y.w, gg, r3);
         }
-        const int rw = w0 + x, sees = min(ke, seen(q, rw, G));
+        const int rw = w0 + x, sees = sees_at(x);
         if (sees > bad_all) sum = __builtin_nanf("");
         if (parts > 1) {
             *reinterpret_cast<float4*>(rec + x * DH + 4 * f) = make_float4(r0, r1, r2, r3);
@@ -784,7 +848,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
         s_last = __hip_atomic_fetch_add(arrivals, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == parts - 1;
     __syncthreads();
     if (!s_last) return;
-    join_rows<DH, 64 * NW, true>(w, k, hk, tile, parts, 0, 1, reinterpret_cast<float4*>(lds), &s_ml[0][0]);
+    join_rows<DH, 64 * NW, true, TREE>(w, k, hk, tile, parts, 0, 1, reinterpret_cast<float4*>(lds), &s_ml[0][0]);
     if (threadIdx.x == 0) __hip_atomic_store(arrivals, 0, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
 
@@ -793,7 +857,7 @@ __device__ __forceinline__ void few_rows(const Attn& w, const Work& k, int hk, u
 // buffers: the next tile is on its way while one is used; one barrier a tile. Eight waves
 // are two such groups that take the tiles in turn and join their results in LDS: where a
 // CU has one tile of rows only, its keys are walked in half the time.
-template <int DH, bool F16, int NW>
+template <int DH, bool F16, int NW, bool TREE>
 __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, uint8_t* lds) {
     constexpr int kTile = 64 * DH * 2;
     constexpr int NG = NW / 4;
@@ -808,14 +872,15 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
     const int all_waves = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), group = all_waves / 4, wave = all_waves & 3;
     lds += group * 4 * kTile;
     const int rows = q.n * G, kb = split * k.per * kUnit;
-    const int end = uniform(seen(q, min(rows, (tile + 1) * kManyRows) - 1, G));
+    const int end = uniform(reach_of_tile<TREE>(a, q, min(rows, (tile + 1) * kManyRows) - 1, G));
     const int parts = max(1, (end + k.per * kUnit - 1) / (k.per * kUnit));
     if (split >= parts) return;
     const int ke = min(end, kb + k.per * kUnit);
     const int w0 = tile * kManyRows + 32 * wave;  // the wave's first row
     const int row = min(w0 + c32, rows - 1);
-    const int lim = min(ke, seen(q, row, G)), lim_lo = min(ke, seen(q, min(w0, rows - 1), G));
-    const int lim_hi = w0 < rows ? min(ke, seen(q, min(w0 + 31, rows - 1), G)) : 0;
+    const int lim = min(ke, reach<TREE>(a, q, row, G)), lim_lo = min(ke, seen_by_all<TREE>(a, q, min(w0, rows - 1), G));
+    const int lim_hi = w0 < rows ? min(ke, reach_of_tile<TREE>(a, q, min(w0 + 31, rows - 1), G)) : 0;
+    auto sees_from = [&](int k) { return sees32(a, q, row, G, k, lim); };
     uint4 qf[DH / 16];
     load_q<DH>(a, q, row, hk, G, qf);
     const float c = a.scale * kLog2e;
@@ -879,7 +944,7 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
         load(Keys{}, t + 2);
         if (t >= n_tiles || k0 >= lim_hi) return;
         const uint8_t *const kt = lds + ((t + 1) & 1) * 2 * kTile, *const vt = lds + ((t & 1) * 2 + 1) * kTile;
-        const float neg = mask_and_move<DH, F16, 2>(s, k0, lim, k0 + 64 > lim_lo, c, m, l, o);
+        const float neg = mask_and_move<DH, F16, TREE, 2>(s, k0, lim, k0 + 64 > lim_lo, sees_from, c, m, l, o);
         next[0] = scores32<DH, F16>(kt, qf);
         next[1] = scores32<DH, F16>(kt + 32 * 2 * DH, qf);
         weigh<2>(s, c, neg, l);
@@ -940,8 +1005,8 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
         for (int x = 0; x < min(32, rows - w0); x++) {
             if (!((again >> x) & 1u)) continue;
             float m1, l1, o1[DH / 64];
-            const int rw = w0 + x, sees = min(ke, seen(q, rw, G)), y = 32 * wave + x;
-            row_again<DH, F16>(a, k.r, hk, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
+            const int rw = w0 + x, sees = min(ke, reach<TREE>(a, q, rw, G)), y = 32 * wave + x;
+            row_again<DH, F16, TREE>(a, q, k.r, hk, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1);
             if (sees > bad_all) l1 = __builtin_nanf("");
             if (parts > 1 && lane == 0) *reinterpret_cast<float2*>(rec_ml + 2 * y) = make_float2(m1, l1);
 #pragma unroll
@@ -975,7 +1040,7 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
 }
 
 // MIXED: tiles of 128 rows and of 32; else of 32 alone.
-template <int DH, bool F16, bool MIXED, int NW>
+template <int DH, bool F16, bool MIXED, int NW, bool TREE>
 __global__ __launch_bounds__(64 * NW, DH == 256 || NW == 8 ? 1 : 2) void paged_attn_kernel(Attn w) {
     __shared__ __attribute__((aligned(16))) uint8_t lds[2 * NW * 32 * DH * 2];  // of either: 16 KB a wave at a head_dim of 128
     // (the grid's fastest axis: with 8 kv heads all tiles of a head share one XCD's L2)
@@ -984,14 +1049,14 @@ __global__ __launch_bounds__(64 * NW, DH == 256 || NW == 8 ? 1 : 2) void paged_a
     if (!k.ok) return;
     if constexpr (MIXED)
         if (!k.few) {
-            many_rows<DH, F16, NW>(w, k, hk, lds);
+            many_rows<DH, F16, NW, TREE>(w, k, hk, lds);
             return;
         }
-    few_rows<DH, F16, NW>(w, k, hk, lds);
+    few_rows<DH, F16, NW, TREE>(w, k, hk, lds);
 }
 
 constexpr int kMergeThreads = 512;
-template <int DH>
+template <int DH, bool TREE>
 __global__ __launch_bounds__(kMergeThreads) void paged_attn_merge_kernel(Attn w) {
     __shared__ float4 s_o[kMergeThreads];
     __shared__ float2 s_ml[kMergeThreads / (DH / 4)];
@@ -999,9 +1064,9 @@ __global__ __launch_bounds__(kMergeThreads) void paged_attn_merge_kernel(Attn w)
     const Work k = find_work<true>(w, blockIdx.y);
     if (!k.ok) return;
     const int tile = k.local, tr = k.few ? kFewRows : kManyRows;
-    const int end = uniform(seen(k.q, min(k.q.n * G, (tile + 1) * tr) - 1, G));
+    const int end = uniform(reach_of_tile<TREE>(w.a, k.q, min(k.q.n * G, (tile + 1) * tr) - 1, G));
     const int parts = max(1, (end + k.per * kUnit - 1) / (k.per * kUnit));
-    if (parts > 1) join_rows<DH, kMergeThreads, false>(w, k, hk, tile, parts, blockIdx.z, gridDim.z, s_o, s_ml);
+    if (parts > 1) join_rows<DH, kMergeThreads, false, TREE>(w, k, hk, tile, parts, blockIdx.z, gridDim.z, s_o, s_ml);
 }
 
 // A call's tiles and grid. `max_new` is a hint: with at most 32 rows per request as it
@@ -1077,16 +1142,17 @@ Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, size_t workspa
         const dim3 grid((unsigned)a.Hk, (unsigned)y, (unsigned)(shares ? shares : (items + y - 1) / y));
         hipLaunchKernelGGL(kernel, grid, dim3(threads), 0, st, L.w);
     };
-    auto with = [&](auto dh, auto f16) {
+    auto with = [&](auto dh, auto f16, auto tree) {
         constexpr int DH = decltype(dh)::value;
-        constexpr bool F16 = decltype(f16)::value;
-        if (L.only_few) go(paged_attn_kernel<DH, F16, false, 4>, L.items, 0, 256);
-        else if (!L.wide) go(paged_attn_kernel<DH, F16, true, 4>, L.items, 0, 256);
+        constexpr bool F16 = decltype(f16)::value, TREE = decltype(tree)::value;
+        if (L.only_few) go(paged_attn_kernel<DH, F16, false, 4, TREE>, L.items, 0, 256);
+        else if (!L.wide) go(paged_attn_kernel<DH, F16, true, 4, TREE>, L.items, 0, 256);
         if constexpr (DH != 256)  // (its tiles fill the LDS)
-            if (L.wide) go(paged_attn_kernel<DH, F16, true, 8>, L.items, 0, 512);
-        if (!L.w.sync && !a.whole) go(paged_attn_merge_kernel<DH>, L.merges, L.merge_rows, kMergeThreads);
+            if (L.wide) go(paged_attn_kernel<DH, F16, true, 8, TREE>, L.items, 0, 512);
+        if (!L.w.sync && !a.whole) go(paged_attn_merge_kernel<DH, TREE>, L.merges, L.merge_rows, kMergeThreads);
     };
-    auto typed = [&](auto dh) { a.f16 ? with(dh, std::true_type{}) : with(dh, std::false_type{}); };
+    auto kind = [&](auto dh, auto f16) { a.mask ? with(dh, f16, std::true_type{}) : with(dh, f16, std::false_type{}); };
+    auto typed = [&](auto dh) { a.f16 ? kind(dh, std::true_type{}) : kind(dh, std::false_type{}); };
     if (a.Dh == 64) typed(std::integral_constant<int, 64>{});
     else if (a.Dh == 128) typed(std::integral_constant<int, 128>{});
     else typed(std::integral_constant<int, 256>{});

@@ -1241,13 +1241,15 @@ int jh_paged_qk_norm_rope_append(jh_ctx* c, const void* qkv, jh_dtype qkv_dtype,
     return finish(c, jh::launch_paged_append(a, c->num_cus, c->stream), op);
 }
 
-int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
-                       jh_dtype page_dtype, int64_t n_pages, int64_t page_size, int64_t page_stride,
-                       const int32_t* block_tables, int64_t max_blocks, const int32_t* row_starts,
-                       const int32_t* kv_lens, int64_t n_req, int64_t n_rows, int64_t max_new, int64_t n_heads,
-                       int64_t n_kv_heads, int64_t head_dim, float scale, void* out, jh_dtype out_dtype) {
+namespace {
+
+// jh_paged_attention, and with a mask jh_paged_tree_attention.
+int paged_attention(jh_ctx* c, const char* op, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                    jh_dtype page_dtype, int64_t n_pages, int64_t page_size, int64_t page_stride,
+                    const int32_t* block_tables, int64_t max_blocks, const int32_t* row_starts, const int32_t* kv_lens,
+                    const uint32_t* mask, int64_t mask_words, int64_t n_req, int64_t n_rows, int64_t max_new,
+                    int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, float scale, void* out, jh_dtype out_dtype) {
     if (int r = enter(c)) return r;
-    const char* op = "jh_paged_attention";
     if (int r = check_pages(c, op, page_dtype, n_pages, page_size)) return r;
     if (int r = check_page_heads(c, op, n_kv_heads, head_dim, page_size, page_stride)) return r;
     if (int r = check_float_dtype(c, op, "out", out_dtype)) return r;
@@ -1304,6 +1306,7 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
     a.n_req = (int)n_req, a.n_rows = (int)n_rows, a.max_new = (int)std::min<int64_t>(max_new, n_rows);
     a.Hq = (int)n_heads, a.Hk = (int)n_kv_heads, a.Dh = (int)head_dim;
     a.scale = scale, a.out = out, a.out_dt = out_dtype;
+    a.mask = mask, a.mask_words = (int)mask_words;
     // the parts of split keys need a workspace; where it cannot grow (a stream under capture,
     // no memory) the keys stay whole
     int* const sync = xcd_sync(c) ? xcd_sync(c) + jh::kPagedSyncSlot : nullptr;
@@ -1315,6 +1318,176 @@ int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k
     if (int r = finish(c, jh::launch_paged_attn(a, c->ws, c->ws_bytes, c->num_cus, sync, c->stream), op)) return r;
     const int64_t row = n_heads * head_dim;
     return check_values(c, op, out, out_dtype, used * row, from * row);
+}
+
+int check_mask_words(jh_ctx* c, const char* op, int64_t mask_words) {
+    if (mask_words < 1) return fail(c, JH_ERR_INVALID, std::string(op) + ": mask_words must be at least 1");
+    if (mask_words > JH_TREE_WORDS)
+        return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": more than " + std::to_string(JH_TREE_WORDS) + " mask_words");
+    return JH_OK;
+}
+
+}  // namespace
+
+int jh_paged_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                       jh_dtype page_dtype, int64_t n_pages, int64_t page_size, int64_t page_stride,
+                       const int32_t* block_tables, int64_t max_blocks, const int32_t* row_starts,
+                       const int32_t* kv_lens, int64_t n_req, int64_t n_rows, int64_t max_new, int64_t n_heads,
+                       int64_t n_kv_heads, int64_t head_dim, float scale, void* out, jh_dtype out_dtype) {
+    return paged_attention(c, "jh_paged_attention", q, q_stride, k_pages, v_pages, page_dtype, n_pages, page_size, page_stride,
+                           block_tables, max_blocks, row_starts, kv_lens, nullptr, 0, n_req, n_rows, max_new, n_heads,
+                           n_kv_heads, head_dim, scale, out, out_dtype);
+}
+
+int jh_paged_tree_attention(jh_ctx* c, const void* q, int64_t q_stride, const void* k_pages, const void* v_pages,
+                            jh_dtype page_dtype, int64_t n_pages, int64_t page_size, int64_t page_stride,
+                            const int32_t* block_tables, int64_t max_blocks, const int32_t* row_starts,
+                            const int32_t* kv_lens, const uint32_t* tree_mask, int64_t mask_words, int64_t n_req,
+                            int64_t n_rows, int64_t max_new, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim,
+                            float scale, void* out, jh_dtype out_dtype) {
+    if (!c) return JH_ERR_INVALID;
+    const char* op = "jh_paged_tree_attention";
+    c->err.clear();
+    if (int r = check_mask_words(c, op, mask_words)) return r;
+    if (!tree_mask && n_rows > 0 && n_req > 0) return fail(c, JH_ERR_INVALID, std::string(op) + ": null pointer");
+    return paged_attention(c, op, q, q_stride, k_pages, v_pages, page_dtype, n_pages, page_size, page_stride, block_tables,
+                           max_blocks, row_starts, kv_lens, tree_mask, mask_words, n_req, n_rows, max_new, n_heads,
+                           n_kv_heads, head_dim, scale, out, out_dtype);
+}
+
+int jh_paged_tree_plan(jh_ctx* c, const int32_t* parents, const int32_t* row_starts, const int32_t* kv_lens,
+                       int64_t n_req, int64_t n_rows, int64_t mask_words, int32_t* positions, uint32_t* tree_mask) {
+    if (int r = enter(c)) return r;
+    const char* op = "jh_paged_tree_plan";
+    if (int r = check_mask_words(c, op, mask_words)) return r;
+    if (n_req < 0 || n_rows < 0) return fail(c, JH_ERR_INVALID, std::string(op) + ": bad shape");
+    if (n_rows > (1 << 30) || n_req > 65536)
+        return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": too large (n_rows to 2^30, n_req to 65536)");
+    if (n_rows == 0) return JH_OK;
+    if (!parents || !row_starts || !positions || !tree_mask || (n_req > 0 && !kv_lens))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": null pointer");
+    if (c->checks & JH_CHECK_INDICES) {
+        std::vector<int32_t> st, par;
+        if (int r = read_ints(c, op, row_starts, n_req + 1, st)) return r;
+        if (int r = read_ints(c, op, parents, n_rows, par)) return r;
+        for (int64_t r = 0; r < n_req; r++) {
+            if (st[r] < 0 || st[r + 1] < st[r] || st[r + 1] > n_rows)
+                return fail(c, JH_ERR_INVALID, std::string(op) + ": row_starts of request " + std::to_string(r) +
+                                                   " decrease or leave [0, n_rows]");
+            const int64_t n = st[r + 1] - st[r];
+            for (int64_t i = 0; n <= 32 * mask_words && i < n; i++)
+                if (par[st[r] + i] < -1 || par[st[r] + i] >= i)
+                    return fail(c, JH_ERR_INVALID, std::string(op) + ": parent " + std::to_string(par[st[r] + i]) +
+                                                       " of row " + std::to_string(i) + " of request " +
+                                                       std::to_string(r) + " is not an earlier row of it");
+        }
+    }
+    jh::TreePlanArgs a{parents, row_starts, kv_lens, (int)n_req, (int)n_rows, (int)mask_words, positions, tree_mask};
+    return finish(c, jh::launch_tree_plan(a, c->stream), op);
+}
+
+int jh_paged_tree_commit(jh_ctx* c, const int32_t* parents, const int32_t* tokens, const int32_t* chosen,
+                         int64_t chosen_stride, const int32_t* known, const int32_t* row_starts, const int32_t* kv_lens,
+                         int64_t n_req, int64_t n_rows, int64_t mask_words, int64_t page_size,
+                         const int32_t* block_tables, int64_t max_blocks, int32_t* free_pages, int64_t n_pages,
+                         const int32_t* free_count, const int32_t* slots, int32_t* kv_lens_out, int32_t* free_count_out,
+                         int32_t* accepted, int32_t* path, int32_t* next_tokens, int32_t* status, void* const* k_pages,
+                         void* const* v_pages, int64_t n_layers, jh_dtype page_dtype, int64_t n_kv_heads,
+                         int64_t head_dim, int64_t page_stride) {
+    if (int r = enter(c)) return r;
+    const char* op = "jh_paged_tree_commit";
+    if (int r = check_mask_words(c, op, mask_words)) return r;
+    if (int r = check_pages(c, op, n_layers > 0 ? page_dtype : JH_BF16, n_pages, page_size)) return r;
+    if (n_layers > 0)
+        if (int r = check_page_heads(c, op, n_kv_heads, head_dim, page_size, page_stride)) return r;
+    if (n_req < 0 || n_rows < 0 || n_layers < 0 || max_blocks < 0 || max_blocks > 0x7fffffff || chosen_stride < 1 ||
+        chosen_stride > ((int64_t)1 << 32))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": bad shape");
+    if (n_req > jh::kPlanMaxReq || n_rows > (1 << 30) || n_pages > (1 << 30) || n_layers > 65536)
+        return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": more than " + std::to_string(jh::kPlanMaxReq) +
+                                               " requests, 2^30 rows or pages, or 65536 layers");
+    if (!row_starts || !free_count || !free_count_out || !status || (n_pages > 0 && !free_pages) ||
+        (n_rows > 0 && (!parents || !tokens || !chosen || !path || !slots)) ||
+        (n_req > 0 && (!kv_lens || !kv_lens_out || !accepted || !next_tokens || (max_blocks > 0 && !block_tables))) ||
+        (n_layers > 0 && (!k_pages || !v_pages)))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": null pointer");
+    for (int64_t i = 0; i < n_layers && n_pages > 0; i++) {
+        if (!k_pages[i] || !v_pages[i]) return fail(c, JH_ERR_INVALID, std::string(op) + ": null pages of layer " + std::to_string(i));
+        if (!aligned16(k_pages[i]) || !aligned16(v_pages[i]))
+            return fail(c, JH_ERR_INVALID, std::string(op) + ": pages of layer " + std::to_string(i) + " not 16-byte aligned");
+    }
+    if (c->checks & JH_CHECK_INDICES)
+        if (int r = checks_not_capturing(c, op)) return r;
+    jh::TreeCommitArgs a{};
+    a.parents = parents, a.tokens = tokens, a.chosen = chosen, a.chosen_stride = chosen_stride, a.known = known;
+    a.row_starts = row_starts, a.kv_lens = kv_lens;
+    a.n_req = (int)n_req, a.n_rows = (int)n_rows, a.tree_rows = (int)(32 * mask_words), a.page_shift = __builtin_ctzll(page_size);
+    a.tables = block_tables, a.max_blocks = (int)max_blocks;
+    a.free_pages = free_pages, a.n_pages = (int)n_pages, a.free_count = free_count;
+    a.kv_out = kv_lens_out, a.count_out = free_count_out, a.accepted = accepted, a.path = path;
+    a.next_tokens = next_tokens, a.status = status;
+    if (int r = finish(c, jh::launch_tree_commit(a, c->stream), op)) return r;
+    if (n_layers > 0 && n_req > 0 && n_rows > 0 && n_pages > 0) {
+        jh::TreeMoveArgs m{};
+        m.row_starts = row_starts, m.accepted = accepted, m.path = path, m.slots = slots;
+        m.n_req = (int)n_req, m.n_rows = (int)n_rows, m.n_slots = (int)(n_pages * page_size);
+        m.page_shift = a.page_shift, m.Hk = (int)n_kv_heads, m.Dh = (int)head_dim, m.page_stride = page_stride;
+        for (int64_t i = 0; i < n_layers; i += jh::kMoveLayers) {
+            m.layers = (int)std::min<int64_t>(jh::kMoveLayers, n_layers - i);
+            for (int j = 0; j < m.layers; j++)
+                m.k[j] = static_cast<uint16_t*>(k_pages[i + j]), m.v[j] = static_cast<uint16_t*>(v_pages[i + j]);
+            if (int r = finish(c, jh::launch_tree_move(m, c->stream), op)) return r;
+        }
+    }
+    if (c->checks & JH_CHECK_INDICES) {
+        static const char* const why[] = {"", "a request of fewer keys than rows, or more than max_blocks pages",
+                                          "row_starts that decrease or leave [0, n_rows]", "*free_count outside [0, n_pages]",
+                                          "a page that comes back lies outside [0, n_pages), or the stack is full"};
+        std::vector<int32_t> st;
+        if (int r = read_ints(c, op, status, 1, st)) return r;
+        if (st[0] != JH_PLAN_OK)
+            return fail(c, JH_ERR_INVALID, std::string(op) + ": nothing done: " + why[st[0] >= 1 && st[0] <= 4 ? st[0] : 0]);
+    }
+    return JH_OK;
+}
+
+int jh_token_logprobs(jh_ctx* c, const void* logits, jh_dtype logits_dtype, int64_t rows, int64_t vocab,
+                      int64_t row_stride, float scale, const int32_t* tokens, int64_t n_tokens, int64_t top_k,
+                      float* logprobs, float* entropy, int32_t* top_ids, float* top_logprobs) {
+    if (int r = enter(c)) return r;
+    const char* op = "jh_token_logprobs";
+    if (int r = check_act_dtype(c, op, "logits", logits_dtype)) return r;
+    if (rows < 0 || vocab <= 0 || n_tokens < 0 || top_k < 0) return fail(c, JH_ERR_INVALID, std::string(op) + ": bad shape");
+    if (rows > (1 << 24) || vocab > (1 << 28))
+        return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": too large (rows to 2^24, vocab to 2^28)");
+    if (n_tokens > JH_LOGPROBS_TOKENS || top_k > JH_LOGPROBS_TOP)
+        return fail(c, JH_ERR_UNSUPPORTED, std::string(op) + ": more than " + std::to_string(JH_LOGPROBS_TOKENS) +
+                                               " tokens or " + std::to_string(JH_LOGPROBS_TOP) + " alternatives of a row");
+    if (top_k > vocab) return fail(c, JH_ERR_INVALID, std::string(op) + ": top_k past the vocabulary");
+    if (row_stride < vocab || row_stride > ((int64_t)1 << 32))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": row_stride must hold a row");
+    if (!(scale >= 1e-30f && scale <= 1e30f))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": scale must lie in [1e-30, 1e30]");
+    if (rows == 0) return JH_OK;
+    if (!logits || (n_tokens > 0 && (!tokens || !logprobs)) || (top_k > 0 && (!top_ids || !top_logprobs)))
+        return fail(c, JH_ERR_INVALID, std::string(op) + ": null pointer");
+    if (!aligned16(logits)) return fail(c, JH_ERR_INVALID, std::string(op) + ": logits must be 16-byte aligned");
+    if (n_tokens == 0 && top_k == 0 && !entropy) return JH_OK;
+    if ((c->checks & JH_CHECK_INDICES) && n_tokens > 0) {
+        std::vector<int32_t> h;
+        if (int r = read_ints(c, op, tokens, rows * n_tokens, h)) return r;
+        for (size_t i = 0; i < h.size(); i++)
+            if (h[i] < -1 || h[i] >= vocab)
+                return fail(c, JH_ERR_INVALID, std::string(op) + ": token " + std::to_string(h[i]) + " at " +
+                                                   std::to_string(i) + " outside [0, " + std::to_string(vocab) + ")");
+    }
+    jh::LogProbsArgs a{};
+    a.x = logits, a.f32 = logits_dtype == JH_F32, a.rows = (int)rows, a.vocab = (int)vocab, a.stride = row_stride, a.scale = scale;
+    a.tokens = tokens, a.n_tokens = (int)n_tokens, a.top_k = (int)top_k;
+    a.logprobs = logprobs, a.entropy = entropy, a.top_ids = top_ids, a.top_logprobs = top_logprobs;
+    if (const size_t need = jh::logprobs_workspace_bytes(a, c->num_cus))
+        if (int r = ensure_workspace(c, need, op)) return r;
+    return finish(c, jh::launch_logprobs(a, c->ws, c->num_cus, c->stream), op);
 }
 
 }  // extern "C"

@@ -132,6 +132,26 @@ class _Sweeper:
         return freed
 
 
+class PagedLayers:
+    """The caches of a model's layers, [n_pages, Hk, page, Dh] each and alike, as
+    HipBackend.PagedTreeCommit takes them: made once beside the caches, which it keeps."""
+
+    def __init__(self, k_pages, v_pages):
+        op = "PagedLayers"
+        self.tensors = tuple(k_pages), tuple(v_pages)
+        if len(self.tensors[0]) != len(self.tensors[1]) or not self.tensors[0]:
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: as many layers of values as of keys, and at least one")
+        seen = set()
+        for k, v in zip(*self.tensors):
+            n, hk, page, dh, stride = HipBackend._pages(op, k, v)
+            seen.add((n, page, (k.dtype, hk, dh, stride)))
+        if len(seen) != 1:
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: the layers' pages must be alike")
+        (self.n_pages, self.page, self.geometry), = seen
+        self.n = len(self.tensors[0])
+        self.k, self.v = ((ctypes.c_void_p * self.n)(*(t.ptr for t in ts)) for ts in self.tensors)
+
+
 class HipBackend:
     """engine.Backend subset on one MI355X (gfx950)."""
 
@@ -1095,7 +1115,10 @@ class HipBackend:
         seeing the keys up to its own. maxNew, the most tokens of a request (a
         hint). Returns [T, Hq, Dh] (the pages' dtype unless out or out_dtype says
         otherwise); rows past rowStarts[R] are left as they were."""
-        op = "PagedAttention"
+        return self._paged_attention("PagedAttention", q, k_pages, v_pages, blockTables, rowStarts, kvLens, None, scale, maxNew, out,
+                                     out_dtype)
+
+    def _paged_attention(self, op, q, k_pages, v_pages, blockTables, rowStarts, kvLens, mask, scale, maxNew, out, out_dtype) -> Tensor:
         n, hk, page, dh, stride = self._pages(op, k_pages, v_pages)
         self._ints(op, "tables, row starts and lengths", blockTables, rowStarts, kvLens)
         R = kvLens.numel
@@ -1109,10 +1132,125 @@ class HipBackend:
             out = self.empty(q.dtype if out_dtype is None else out_dtype, T, hq, dh)
         elif out.numel != T * hq * dh or not out.contiguous:
             raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: out must be dense [T, Hq, Dh]")
-        check(self._ctx, self._L.jh_paged_attention(
-            self._ctx, q.ptr, q.strides[0] if T > 1 else hq * dh, k_pages.ptr, v_pages.ptr, k_pages.dtype, n, page, stride,
-            blockTables.ptr, blockTables.shape[1], rowStarts.ptr, kvLens.ptr, R, T, T if maxNew is None else int(maxNew),
-            hq, hk, dh, float(scale), out.ptr, out.dtype))
+        pages = (self._ctx, q.ptr, q.strides[0] if T > 1 else hq * dh, k_pages.ptr, v_pages.ptr, k_pages.dtype, n, page, stride,
+                 blockTables.ptr, blockTables.shape[1], rowStarts.ptr, kvLens.ptr)
+        sizes = (R, T, T if maxNew is None else int(maxNew), hq, hk, dh, float(scale), out.ptr, out.dtype)
+        if mask is None:
+            check(self._ctx, self._L.jh_paged_attention(*pages, *sizes))
+        else:
+            check(self._ctx, self._L.jh_paged_tree_attention(*pages, mask.ptr, self._mask(op, mask, T), *sizes))
+        return out
+
+    # -- trees of drafted tokens over the paged cache (include/janis_hip.h) ----------------
+    def _mask(self, op: str, mask: Tensor, rows: int) -> int:
+        """The words per row of a tree mask [rows, W] (I32 or U32)."""
+        if len(mask.shape) != 2 or mask.shape[0] != rows or mask.dtype not in (I32, U32) or not mask.contiguous:
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: the mask must be dense U32 or I32 [{rows}, words]")
+        return mask.shape[1]
+
+    def PagedTreePlan(self, parents: Tensor, rowStarts: Tensor, kvLens: Tensor, maskWords: int | None = None,
+                      out: tuple | None = None) -> tuple:
+        """Positions and masks of one step's trees (jh_paged_tree_plan): parents [T],
+        each the number of an earlier row of its request or -1; rowStarts [R+1] and
+        kvLens [R] from PagedPlan. Returns (positions [T] I32, mask [T, maskWords]
+        U32); `out` gives these tensors (positions may be PagedPlan's)."""
+        op = "PagedTreePlan"
+        T, R = parents.numel, kvLens.numel
+        if out is None:
+            if maskWords is None:
+                raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: maskWords (or out) must be given")
+            out = (self.empty(I32, T), self.empty(U32, T, int(maskWords)))
+        pos, mask = out
+        W = self._mask(op, mask, T)
+        self._ints(op, "parents, row starts, lengths and positions", parents, rowStarts, kvLens, pos)
+        if rowStarts.numel != R + 1 or pos.numel != T or (maskWords is not None and maskWords != W):
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: shapes do not match {R} requests and {T} rows")
+        check(self._ctx, self._L.jh_paged_tree_plan(self._ctx, parents.ptr, rowStarts.ptr, kvLens.ptr, R, T, W, pos.ptr,
+                                                    mask.ptr))
+        return out
+
+    def PagedTreeAttention(self, q: Tensor, k_pages: Tensor, v_pages: Tensor, blockTables: Tensor, rowStarts: Tensor,
+                           kvLens: Tensor, mask: Tensor, scale: float, maxNew: int | None = None,
+                           out: Tensor | None = None, out_dtype: int | None = None) -> Tensor:
+        """PagedAttention in which a new token sees its request's committed keys and,
+        of the new ones, those whose bits mask [T, W] has (jh_paged_tree_attention)."""
+        return self._paged_attention("PagedTreeAttention", q, k_pages, v_pages, blockTables, rowStarts, kvLens, mask, scale,
+                                     maxNew, out, out_dtype)
+
+    def PagedTreeCommit(self, parents: Tensor, tokens: Tensor, chosen: Tensor, rowStarts: Tensor, kvLens: Tensor,
+                        maskWords: int, pageSize: int, blockTables: Tensor, freePages: Tensor, freeCount: Tensor,
+                        slots: Tensor, layers: "PagedLayers | None" = None, known: Tensor | None = None,
+                        out: tuple | None = None) -> tuple:
+        """The path that the model agrees with (jh_paged_tree_commit): tokens [T] of the
+        rows, chosen [T] or [T, n] the model's token after each (of [T, n] the first
+        column, as TokenLogProbs returns its likeliest), known [R] rows of each request
+        that are kept anyway (1 without it). Pages that are not needed go back to
+        freePages[:freeCount] in place, and the kept rows' keys and values in `layers`
+        move together. Returns (kvLens', freeCount', accepted [R], path [T], next [R],
+        status [1]); `out` gives these tensors (the first two may be kvLens and
+        freeCount)."""
+        op = "PagedTreeCommit"
+        T, R = parents.numel, kvLens.numel
+        if out is None:
+            out = tuple(self.empty(I32, n) for n in (R, 1, R, T, R, 1))
+        kv, count, accepted, path, following, status = out
+        self._ints(op, "rows, lengths, tables, pages, counts and results", parents, tokens, rowStarts, kvLens, blockTables,
+                   freePages, freeCount, slots, *(() if known is None else (known,)), *out)
+        if chosen.dtype != I32 or len(chosen.shape) not in (1, 2) or chosen.shape[0] != T \
+                or (len(chosen.shape) == 2 and chosen.shape[1] < 1):
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: chosen must be I32 [{T}] or [{T}, n]")
+        tables = blockTables.shape
+        if len(tables) != 2 or tables[0] != R or not kv.numel == accepted.numel == following.numel == R \
+                or not tokens.numel == slots.numel == path.numel == T or rowStarts.numel != R + 1 \
+                or not freeCount.numel == count.numel == status.numel == 1 or (known is not None and known.numel != R):
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: shapes do not match {R} requests and {T} rows")
+        if layers is None:
+            ks, vs, n, geometry = None, None, 0, (BF16, 1, 64, 64 * int(pageSize))
+        else:
+            ks, vs, n, geometry = layers.k, layers.v, layers.n, layers.geometry
+            if (layers.n_pages, layers.page) != (freePages.numel, int(pageSize)):
+                raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: the layers have {layers.n_pages} pages of {layers.page}, not "
+                                                         f"{freePages.numel} of {pageSize}")
+        check(self._ctx, self._L.jh_paged_tree_commit(
+            self._ctx, parents.ptr, tokens.ptr, chosen.ptr, chosen.strides[0] if T > 1 else 1,
+            known.ptr if known is not None else None, rowStarts.ptr, kvLens.ptr, R, T, int(maskWords), int(pageSize),
+            blockTables.ptr, tables[1], freePages.ptr, freePages.numel, freeCount.ptr, slots.ptr, kv.ptr, count.ptr,
+            accepted.ptr, path.ptr, following.ptr, status.ptr, ks, vs, n, *geometry))
+        return out
+
+    def TokenLogProbs(self, logits: Tensor, tokens: Tensor | None = None, topK: int = 0, scale: float = 1.0,
+                      entropy: bool = True, out: tuple | None = None) -> tuple:
+        """Log probabilities of rows of logits [.., V] (F32 or BF16) under
+        softmax(scale * logits) (jh_token_logprobs): of tokens [.., n] I32 (or [..], one
+        to a row), the entropy, and the topK likeliest tokens (equal logits: the lower
+        token first). Returns (logprobs F32 of tokens' shape, entropy F32 [..], ids I32
+        [.., topK], their logprobs F32 [.., topK]), None for what is not asked for; `out`
+        gives these tensors (None: not wanted)."""
+        op = "TokenLogProbs"
+        V, lead = logits.shape[-1], logits.shape[:-1]
+        T = math.prod(lead)
+        if len(logits.shape) != 2 or logits.strides[1] != 1:
+            logits = self._c(logits)
+        n = 0
+        if tokens is not None:
+            self._ints(op, "tokens", tokens)
+            if tokens.shape != lead and tokens.shape[:-1] != lead:
+                raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: tokens {list(tokens.shape)} for logits of {list(lead)} rows")
+            n = 1 if tokens.shape == lead else tokens.shape[-1]
+        topK = int(topK)
+        if out is None:
+            out = (self.empty(F32, *tokens.shape) if tokens is not None else None, self.empty(F32, *lead) if entropy else None,
+                   self.empty(I32, *lead, topK) if topK else None, self.empty(F32, *lead, topK) if topK else None)
+        lp, ent, ids, top = out
+        for t, dt, count in ((lp, F32, T * n), (ent, F32, T), (ids, I32, T * topK), (top, F32, T * topK)):
+            if t is not None and (t.dtype != dt or t.numel != count or not t.contiguous):
+                raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: a result must be dense {DTYPE_NAME[dt]} of {count} elements")
+        if (lp is None) != (tokens is None) or (topK > 0) != (ids is not None) or (topK > 0) != (top is not None):
+            raise JanisHipError(_lib.JH_ERR_INVALID, f"{op}: results for tokens and alternatives, where they are asked for")
+        ptr = lambda t: t.ptr if t is not None else None  # noqa: E731
+        check(self._ctx, self._L.jh_token_logprobs(
+            self._ctx, logits.ptr, logits.dtype, T, V, logits.strides[0] if len(logits.shape) == 2 and T > 1 else V,
+            float(scale), ptr(tokens), n, topK, ptr(lp), ptr(ent), ptr(ids), ptr(top)))
         return out
 
     def MoeRoute(self, logits: Tensor, k: int, normTopk: bool = True) -> tuple:
