@@ -379,7 +379,7 @@ size_t attn_decode_workspace_bytes(int64_t Hq, int64_t Hk, int64_t pos, int num_
 // partials be merged inside the attention launch when the GPU deals workgroups
 // to its 8 XCDs round-robin (probe_xcd_round_robin) and the kv heads are a
 // multiple of 8; otherwise a merge launch follows.
-constexpr int kAttnSyncSlots = 4096 + 64 + 32 * 512 + 8192;
+constexpr int kAttnSyncSlots = 4096 + 64 + 32 * 512 + 8192 + 1024;
 // The fused q/k/v + attention launch's share of them: per XCD x, the arrival
 // flags of its blocks at kAttnFlagSlot + 128 x (zero between calls).
 constexpr int kAttnFlagSlot = 1024;
@@ -396,7 +396,10 @@ constexpr int kAttnMarkerSlot = 4096;
 constexpr int kQmmSyncSlot = 4096 + 64, kQmmSyncTiles = 512;
 // jh_paged_attention's share: arrivals of a split tile's parts (zero between calls).
 constexpr int kPagedSyncSlot = kQmmSyncSlot + 32 * kQmmSyncTiles, kPagedSyncSlots = 8192;
-static_assert(kPagedSyncSlot + kPagedSyncSlots == kAttnSyncSlots, "the shares fill the array");
+// jh_token_logprobs' share: arrivals of a row's parts (zero between calls), kLogProbsRows rows
+// to an XCD.
+constexpr int kLogProbsSyncSlot = kPagedSyncSlot + kPagedSyncSlots, kLogProbsRows = 128;
+static_assert(kLogProbsSyncSlot + 8 * kLogProbsRows == kAttnSyncSlots, "the shares fill the array");
 // Polls of the arrival flags before a fused launch's wait gives up (the default
 // of jh_set_wait_limit).
 constexpr uint32_t kDefaultWaitPolls = 1u << 22;
@@ -554,7 +557,8 @@ struct LogProbsArgs {
     float* top_logprobs;
 };
 size_t logprobs_workspace_bytes(const LogProbsArgs& a, int num_cus);
-Status launch_logprobs(const LogProbsArgs& a, void* workspace, int num_cus, hipStream_t st);
+// `sync`: 8 * kLogProbsRows of the context's zeroed counters, or nullptr.
+Status launch_logprobs(const LogProbsArgs& a, void* workspace, int num_cus, int* sync, hipStream_t st);
 
 // ---- operators around the products (ops.hip) ----
 // QuantMatmul with transpose = false: y [rows, m.in] = x [rows, m.rows] . Dequantize(W);

@@ -1487,7 +1487,8 @@ int jh_token_logprobs(jh_ctx* c, const void* logits, jh_dtype logits_dtype, int6
     a.logprobs = logprobs, a.entropy = entropy, a.top_ids = top_ids, a.top_logprobs = top_logprobs;
     if (const size_t need = jh::logprobs_workspace_bytes(a, c->num_cus))
         if (int r = ensure_workspace(c, need, op)) return r;
-    return finish(c, jh::launch_logprobs(a, c->ws, c->num_cus, c->stream), op);
+    int* const sync = xcd_sync(c) ? xcd_sync(c) + jh::kLogProbsSyncSlot : nullptr;
+    return finish(c, jh::launch_logprobs(a, c->ws, c->num_cus, sync, c->stream), op);
 }
 
 }  // extern "C"

@@ -303,3 +303,28 @@ def test_refusals(hip):
             Graph(hip, lambda: hip.TokenLogProbs(X, tok, out=(out, None, None, None)))
         finally:
             hip.SetChecks(False)
+
+
+def test_logprobs_on_a_stream_without_all_cus():
+    """A stream that leaves a CU out does not keep blocks on the XCDs as the join in the
+    launch needs it: the parts are joined by a second one, to the same bits."""
+    import ctypes
+
+    from tests.conftest import hip_runtime
+
+    b, rt = HipBackend(0), hip_runtime()
+    rng = np.random.default_rng(12)
+    cases = [(some(rng, 1, 151936, F32), F32, 20), (some(rng, 40, 50021, BF16), BF16, 5), (some(rng, 9, 151936, BF16), BF16, 0)]
+    Xs = [up(b, x, dt) for x, dt, _ in cases]
+    read = lambda out: [b.Floats(out[1])] + ([b.Ints(out[2]), b.Floats(out[3])] if out[2] is not None else [])  # noqa: E731
+    wants = [read(b.TokenLogProbs(X, topK=k)) for X, (_, _, k) in zip(Xs, cases)]
+    mask = (ctypes.c_uint32 * 8)(*([0xFFFFFFFF] * 7 + [0x7FFFFFFF]))
+    stream = ctypes.c_void_p()
+    assert rt.hipExtStreamCreateWithCUMask(ctypes.byref(stream), 8, mask) == 0
+    b.SetStream(stream.value)
+    for X, (x, dt, k), want in zip(Xs, cases, wants):
+        step(f"jh_token_logprobs {x.shape} joined by a second launch")
+        assert all(np.array_equal(g, w) for g, w in zip(read(b.TokenLogProbs(X, topK=k)), want))
+    b.SetStream(None)
+    b.Close()
+    assert rt.hipStreamDestroy(stream) == 0
