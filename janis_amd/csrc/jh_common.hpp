@@ -511,6 +511,9 @@ struct PagedAttnArgs {
 size_t paged_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus, int* sync);
 Status launch_paged_attn(const PagedAttnArgs& a, void* workspace, size_t workspace_bytes, int num_cus, int* sync,
                          hipStream_t st);
+// With a mask.
+size_t paged_tree_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus);
+Status launch_paged_tree_attn(const PagedAttnArgs& a, void* workspace, size_t workspace_bytes, int num_cus, hipStream_t st);
 
 // ---- trees of drafted tokens (tree.hip) ----
 struct TreePlanArgs {

@@ -1,0 +1,813 @@
+// Attention of trees of drafted tokens over a paged key/value cache (jh_paged_tree_attention),
+// on the parts that it shares with jh_paged_attention: there, what a tile does with a part of
+// its keys is described. Here a new token sees the committed keys of its request and, of the
+// new ones, those whose bits its mask has; the tiles that meet new keys take the bits of 32
+// keys as one word per row.
+//
+// Trees have some dozens to hundreds of rows (new tokens times the query heads of a kv head)
+// over caches of very different lengths, which is too few tiles to fill the GPU and too
+// unequal to deal them out. So the work is dealt out instead: all tiles of a kv head, each
+// its 64-key units times what a unit of its kind costs, stand in one line, which is cut into
+// as many equal pieces as blocks are resident. A block finds its piece by running sums over
+// the requests and walks it: the end of one tile, whole ones, the beginning of another. A
+// tile that is cut leaves parts, which a launch that follows joins in their order (joined by
+// the part that arrives last, the largest tiles, of 128 rows in 30 parts, held one block for
+// 170 us, and the launch is 4 to 9). A cut near a tile's end is moved there.
+#include "paged_attention.hpp"
+
+namespace jh {
+namespace {
+
+// Kinds of tiles, by rows: 128 (four waves of 32 share 64 keys), 64 (two pairs of waves,
+// 32 keys each), 32 (each wave takes 32 keys of its own).
+struct TreeAttn {
+    PagedAttnArgs a;
+    int G;            // Hq / Hk
+    int blocks;       // most pieces of a kv head's line
+    int record, size; // rows and floats (whole 128-byte lines) of a record
+    struct Split* split;  // of block b: the tile that begins there and goes on in the next; nullptr: keys stay whole
+    float* part;      // records: [blocks] of the tiles that go on in a block, [blocks] of those that begin there
+};
+// Cost of a unit of 64 keys, by the tile's rows: with all blocks at work one took 2.7, 3.1, 3.8 and
+// 4.3 us for tiles of 32, 64, 96 and 128 rows (bf16, head_dim 128). And of a tile (its queries, its
+// results): 4 to 8 us.
+__device__ __forceinline__ int cost_of(int rows) { return 4 + (rows + 31) / 32; }
+constexpr int kCostTile = 12;
+// The least cost of a piece, below which a block costs more to begin than it saves: 16 tokens over
+// 700 keys (32 heads on 8) took 16.7, 19.1 and 21.1 us with 12, 24 and 36; larger calls the same.
+constexpr double kLeastPiece = 12;
+// The least units of a part: a cut nearer a tile's end is moved there. 16 requests of 8 to 32
+// tokens over 500 to 5000 keys took 60, 58 and 63 us with 1, 2 and 4.
+constexpr int kLeastUnits = 2;
+
+struct Split {
+    int parts;        // 0: no such tile
+    Request q;
+    int row0, rows;
+};
+struct Shape {
+    int whole, rest;     // tiles of 128 rows, and rows behind them
+    int rest_tiles;      // 0 or 1
+    int units;
+    double tile, cost;   // of a tile of 128 rows; of the request
+};
+__device__ __forceinline__ Shape shape_of(const Request& q, int G) {
+    Shape s;
+    const int rows = q.n * G;
+    s.whole = rows / kManyRows, s.rest = rows % kManyRows, s.rest_tiles = s.rest > 0;
+    s.units = max(1, (q.kv + kUnit - 1) / kUnit);
+    s.tile = (double)s.units * cost_of(kManyRows) + kCostTile;
+    s.cost = s.whole * s.tile + (s.rest ? (double)s.units * cost_of(s.rest) + kCostTile : 0.0);
+    return s;
+}
+
+// A place on the line: before unit `unit` of tile `tile` of request r, which begins at `begin`.
+struct Place {
+    int r, tile, unit;
+    double begin;
+    Request q;
+};
+// The line's cuts: all a block keeps of it (in scalar registers).
+struct Cuts {
+    double each;   // cost of a piece
+    int pieces;
+    // Where piece j (not the first behind the last) begins.
+    __device__ __forceinline__ double at(int j) const { return floor(each * j); }
+};
+// A wave's view of the line: a lane sums a run of requests.
+struct Line {
+    Cuts cuts;
+    double before; // the lane's run's beginning (exact, as are all sums: below 2^53)
+    double mine;   // its cost
+    Request first; // its first request
+    int run;
+};
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const int2 u = __builtin_bit_cast(int2, v);
+    return __builtin_bit_cast(double, make_int2(__builtin_amdgcn_readlane(u.x, lane), __builtin_amdgcn_readlane(u.y, lane)));
+}
+__device__ __forceinline__ double uniform(double v) { return lane_of(v, 0); }
+__device__ __forceinline__ Line line_of(const TreeAttn& w) {
+    const PagedAttnArgs& a = w.a;
+    Line l;
+    l.run = (a.n_req + 63) / 64;
+    l.mine = 0.0;
+    l.first = Request{0, 0, 0};
+    float rows = 0.0f;
+    for (int e = 0; e < l.run; e++) {
+        const int r = (threadIdx.x & 63) * l.run + e;
+        if (r >= a.n_req) break;
+        const Request q = request(a, r);
+        if (e == 0) l.first = q;
+        l.mine += shape_of(q, w.G).cost;
+        rows += (float)q.n;
+    }
+    const double upto = scan64(l.mine);
+    l.before = upto - l.mine;
+    // row_starts that go up and down, so that requests overlap: nothing is done
+    const bool overlap = wave_sum(rows) > 1.001f * (float)a.n_rows;
+    const double total = overlap ? 0.0 : lane_of(upto, 63);
+    l.cuts.pieces = uniform(total > 0.0 ? max(1, (int)fmin((double)w.blocks, total / kLeastPiece)) : 0);
+    l.cuts.each = uniform(total / max(1, l.cuts.pieces));
+    return l;
+}
+
+// A tile of a request, and its beginning counted from the request's.
+struct Tile {
+    int row0, rows, kind;  // kind: 128, 64 or 32 rows
+    double at;
+};
+__device__ __forceinline__ Tile tile_of(const Shape& s, int tile) {
+    Tile t;
+    t.row0 = tile * kManyRows;
+    t.at = tile * s.tile;
+    t.rows = tile < s.whole ? kManyRows : s.rest;
+    t.kind = t.rows > 64 ? 128 : t.rows > 32 ? 64 : 32;
+    return t;
+}
+// The unit at which a cut `x` behind the tile's beginning divides it: 0 and `units` where it
+// does not (near its ends, and where keys stay whole).
+__device__ __forceinline__ int unit_at(const TreeAttn& w, double x, int units, int rows) {
+    const int per = cost_of(rows);
+    const int u = ((int)fmin(fmax(x, 0.0), (double)units * per + kCostTile) - kCostTile) / per;
+    if (w.a.whole || u < kLeastUnits) return 0;
+    return u > units - kLeastUnits ? units : u;
+}
+
+// The place of cut x (below the line's total).
+__device__ __forceinline__ Place place_of(const TreeAttn& w, const Line& l, double x) {
+    const uint64_t past = __ballot(l.before + l.mine > x);
+    const int at = uniform(__ffsll((unsigned long long)past) - 1);
+    double begin = lane_of(l.before, at);
+    int r = at * l.run;
+    Request q{__builtin_amdgcn_readlane(l.first.start, at), __builtin_amdgcn_readlane(l.first.n, at),
+              __builtin_amdgcn_readlane(l.first.kv, at)};
+    Shape s = shape_of(q, w.G);
+    while (begin + s.cost <= x) {
+        begin += s.cost;
+        q = request(w.a, ++r);
+        s = shape_of(q, w.G);
+    }
+    x -= begin;
+    const int tiles = s.whole + s.rest_tiles, tile = tiles == 1 ? 0 : min(tiles - 1, (int)floor(x / s.tile));
+    const Tile t = tile_of(s, tile);
+    const int u = unit_at(w, x - t.at, s.units, t.rows);
+    const bool next = u == s.units;
+    return Place{uniform(r), uniform(next ? tile + 1 : tile), uniform(next ? 0 : u), uniform(begin), q};
+}
+
+// A record holds results as the lanes have them: of 32 rows at a time and features 8 i .. + 7, the 4
+// features of lane 32 h + row (h: 0 and 1) one after the other, so that a wave stores and loads 1 KB at
+// once; behind them [record][2] maximum and sum.
+template <int DH>
+__device__ __forceinline__ int64_t in_record(int row, int feature) {
+    return ((row >> 5) * (DH / 8) + (feature >> 3)) * 256 + ((feature >> 2) & 1) * 128 + (row & 31) * 4 + (feature & 3);
+}
+
+// A part of a tile's keys.
+struct Segment {
+    Request q;
+    int r, row0, rows;
+    int kb, ke;      // keys
+    float* rec;      // nullptr: all of the tile's keys
+};
+
+// ---- tiles of 32 rows ------------------------------------------------------------------
+// The four waves take the 32-key tiles in turn, each with its own buffers and no barrier:
+// while a tile's scores become weights the next tile's keys are on their way, while its
+// values are used the next values. The waves' results meet in LDS.
+template <int DH, bool F16>
+__device__ __forceinline__ void rows32(const TreeAttn& w, const Segment& g, int hk, uint8_t* lds, int tid) {
+    constexpr int NW = 4, kTile = 32 * DH * 2, kLoads = kTile / 1024;
+    __shared__ float2 s_ml[NW][32];
+    __shared__ int s_bad[NW];
+    __shared__ uint32_t s_again[NW];
+    __shared__ int s_lim[32];  // the rows' reach within the part
+    const PagedAttnArgs& a = w.a;
+    const int G = w.G;
+    const Request q = g.q;
+    const int lane = tid & 63, h = lane >> 5, c32 = lane & 31;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int w0 = g.row0, n_rows = g.rows, kb = g.kb, ke = g.ke;
+    const int row = w0 + min(c32, n_rows - 1);
+    const int lim = min(ke, reach<true>(a, q, row, G)), lim_lo = min(ke, seen_by_all<true>(a, q, w0, G));
+    if (tid < n_rows) s_lim[tid] = lim;
+    auto sees_from = [&](int k) { return sees32(a, q, row, G, k, lim); };
+    uint4 qf[DH / 16];
+    load_q<DH>(a, q, row, hk, G, qf, lane);
+    const float c = a.scale * kLog2e;
+    floatx16 o[DH / 32];
+#pragma unroll
+    for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    float m = ninf(), l = 0.0f;
+    const int n_tiles = (max(0, ke - kb) + 31) / 32;
+    const uint8_t *const kt = lds + wave * 2 * kTile, *const vt = kt + kTile;
+    const uint32_t to = lds_addr(kt);
+    // where the groups of the wave's next 16 tiles lie: lane 4 j + g holds group g of its tile j's
+    const Filler<DH> fill(lane);
+    int64_t where = 0;
+    int bad_from = 0x7fffffff;
+    auto look_up = [&](int t) {
+        const int key = kb + (t + NW * (lane >> 2)) * 32 + (lane & 3) * 8;
+        bool outside;
+        where = key_at<DH>(a, g.r, hk, min(key, ke - 1), outside);
+        if (outside && key < ke) bad_from = min(bad_from, key);
+    };
+    auto load = [&](auto v, int t, int j) {
+        constexpr bool V = decltype(v)::value;
+        const int k0 = kb + t * 32;
+        const uint16_t* const pool = V ? a.v : a.k;
+        const uint32_t at = to + (V ? kTile : 0);
+        if (k0 + 32 <= ke) {
+#pragma unroll
+            for (int n = 0; n < 4; n++) fill.template fill<V, true, true>(pool, lane_of(where, 4 * j + n), n, at);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+                fill.template fill<V, false, true>(pool, lane_of(where, 4 * j + n), n, at, max(0, ke - 1 - (k0 + 8 * n)));
+        }
+    };
+    using K = std::false_type;
+    using Vals = std::true_type;
+    if (wave < n_tiles) {
+        look_up(wave);
+        load(K{}, wave, 0);
+        load(Vals{}, wave, 0);
+    }
+    int j = 0;
+    for (int t = wave; t < n_tiles; t += NW) {
+        const int k0 = kb + t * 32, next = t + NW, jn = (j + 1) & 15;
+        const bool more = next < n_tiles, edge = k0 + 32 > lim_lo;
+        wait_vmem<kLoads>();
+        floatx16 s[1] = {scores32<DH, F16>(kt, qf, lane)};
+        wait_lds();
+        if (more) {
+            if (jn == 0) look_up(next);
+            load(K{}, next, jn);
+        }
+        weigh<1>(s, c, mask_and_move<DH, F16, true, 1>(s, k0, lim, edge, sees_from, c, m, l, o, lane), l);
+        if (more) wait_vmem<kLoads>();
+        else wait_vmem<0>();
+#pragma unroll
+        for (int kk = 0; kk < 2; kk++) {
+            uint32_t p[4][kTerms];
+#pragma unroll
+            for (int e = 0; e < 4; e++) split_pair<F16, kTerms>(s[0][8 * kk + 2 * e], s[0][8 * kk + 2 * e + 1], p[e]);
+            values16<DH, F16>(vt + kk * 16 * 2 * DH, p, o, lane);
+        }
+        wait_lds();
+        if (more) load(Vals{}, next, jn);
+        j = jn;
+    }
+    l = pair32<false>(l);
+    // the waves' results to LDS (their own buffers; the chunk of 4 features f of row c at f ^ c)
+    const int bad = wave_min_int(bad_from);
+    if (lane == 0) s_bad[wave] = bad;
+    const uint32_t mine = rows_again<DH>(l, o, c32 < n_rows);
+    if (lane == 0) s_again[wave] = mine;
+    if (h == 0) s_ml[wave][c32] = make_float2(m, l);
+    constexpr int kChunks = DH / 4;
+    static_assert(32 * DH * 4 <= 2 * kTile, "a wave's results fit its buffers");
+    if (c32 < n_rows)
+#pragma unroll
+        for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const int chunk = (8 * d + 2 * n + h) ^ (c32 & (kChunks - 1));
+                *reinterpret_cast<float4*>(lds + wave * 2 * kTile + c32 * (DH * 4) + chunk * 16) =
+                    make_float4(o[d][4 * n], o[d][4 * n + 1], o[d][4 * n + 2], o[d][4 * n + 3]);
+            }
+    __syncthreads();
+    int bad_all = s_bad[0];
+    uint32_t votes = s_again[0];
+#pragma unroll
+    for (int v = 1; v < NW; v++) bad_all = min(bad_all, s_bad[v]), votes |= s_again[v];
+    float* const rec_ml = g.rec + w.record * DH;
+    const uint32_t again = uniform((int)votes);
+    if (again) {
+        for (int x = wave; x < n_rows; x += NW) {
+            if (!((again >> x) & 1u)) continue;
+            float m1, l1, o1[DH / 64];
+            const int rw = w0 + x, sees = uniform(s_lim[x]);
+            row_again<DH, F16, true>(a, q, g.r, hk, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1, lane);
+            if (sees > bad_all) l1 = __builtin_nanf("");
+            if (g.rec && lane == 0) *reinterpret_cast<float2*>(rec_ml + 2 * x) = make_float2(m1, l1);
+#pragma unroll
+            for (int e = 0; e < DH / 64; e++) {
+                if (g.rec) g.rec[in_record<DH>(x, lane + 64 * e)] = o1[e];
+                else store_out(a, out_at<DH>(a, q, rw, hk, G) + lane + 64 * e, sees ? o1[e] / l1 : 0.0f);
+            }
+        }
+    }
+    for (int i = tid; i < 32 * kChunks; i += 64 * NW) {
+        // a record's 32 rows side by side, else a row's features
+        const int x = g.rec ? i % 32 : i / kChunks, f = g.rec ? i / 32 : i % kChunks;
+        if (x >= n_rows || ((again >> x) & 1u)) continue;
+        float2 ml[NW];
+        float mx = ninf();
+#pragma unroll
+        for (int v = 0; v < NW; v++) ml[v] = s_ml[v][x], mx = fmaxf(mx, ml[v].x);
+        float sum = 0.0f, r0 = 0.0f, r1 = 0.0f, r2 = 0.0f, r3 = 0.0f;
+#pragma unroll
+        for (int v = 0; v < NW; v++) {
+            if (v >= n_tiles) break;  // a wave without keys
+            const float e = ml[v].x == mx ? 1.0f : __builtin_amdgcn_exp2f(ml[v].x - mx);
+            const float4 y = *reinterpret_cast<const float4*>(lds + v * 2 * kTile + x * (DH * 4) +
+                                                              (f ^ (x & (kChunks - 1))) * 16);
+            sum = fmaf(ml[v].y, e, sum);
+            r0 = fmaf(y.x, e, r0), r1 = fmaf(y.y, e, r1), r2 = fmaf(y.z, e, r2), r3 = fmaf(y.w, e, r3);
+        }
+        const int rw = w0 + x, sees = s_lim[x];
+        if (sees > bad_all) sum = __builtin_nanf("");
+        if (g.rec) {
+            *reinterpret_cast<float4*>(g.rec + in_record<DH>(x, 4 * f)) = make_float4(r0, r1, r2, r3);
+            if (f == 0) *reinterpret_cast<float2*>(rec_ml + 2 * x) = make_float2(mx, sum);
+        } else {
+            const float inv = sees ? 1.0f / sum : 0.0f;
+            store_out4(a, out_at<DH>(a, q, rw, hk, G) + 4 * f, sees ? r0 * inv : 0.0f, sees ? r1 * inv : 0.0f,
+                       sees ? r2 * inv : 0.0f, sees ? r3 * inv : 0.0f);
+        }
+    }
+}
+
+// Products and exponentials use different units, but only as far as their instructions
+// alternate; the order here is the source's (sched_barrier), with operands read two products ahead.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// scores32 of a tile of 32 N keys into `next`, and weigh of the tile before it.
+template <int DH, bool F16, int N>
+__device__ __forceinline__ void scores_and_weigh(const uint8_t* kt, const uint4 (&qf)[DH / 16], floatx16 (&next)[N],
+                                                 floatx16 (&s)[N], float c, float neg, float& l, int lane) {
+    constexpr int kSteps = N * DH / 16, kEach = 16 * N / kSteps;
+    const int row = lane & 31, x = ((lane >> 5) ^ perm_k<DH>(row)) * 16;
+    const uint8_t* const at = kt + row * (2 * DH);
+    auto key = [&](int i) { return lds_read16(at + (i % N) * 64 * DH + (x ^ (32 * (i / N)))); };
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) next[n][r] = 0.0f;
+    uint4 k[3] = {key(0), key(1), key(0)};
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+        if (i + 2 < kSteps) k[(i + 2) % 3] = key(i + 2);
+        next[i % N] = mfma<F16>(k[i % 3], qf[i / N], next[i % N]);
+#pragma unroll
+        for (int e = i * kEach; e < (i + 1) * kEach; e++) {
+            s[e >> 4][e & 15] = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], c, neg));
+            sum += s[e >> 4][e & 15];
+        }
+        in_order();
+    }
+    l += sum;
+}
+// values16 over 32 N keys.
+template <int DH, bool F16, int N>
+__device__ __forceinline__ void values(const uint8_t* vt, const floatx16 (&s)[N], floatx16 (&o)[DH / 32], int lane) {
+    constexpr int kD = DH / 32, kSteps = 2 * N * kD;
+    const int i16 = lane & 15, x = perm_v<DH>(i16 >> 2) / 4;
+    const uint8_t* const at = vt + ((lane >> 5) * 4 + (i16 >> 2)) * (2 * DH) + ((lane >> 4) & 1) * 32 + (i16 & 3) * 8;
+    auto value = [&](int i) {
+        const uint8_t* const p = at + (i / kD) * 32 * DH + ((i % kD) ^ x) * 64;
+        const uint2 lo = lds_read_tr(p), hi = lds_read_tr(p + 16 * DH);
+        return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    };
+    uint32_t p[2][4][kTerms];
+    auto split = [&](int kk, int e) {
+        split_pair<F16, kTerms>(s[kk >> 1][8 * (kk & 1) + 2 * e], s[kk >> 1][8 * (kk & 1) + 2 * e + 1], p[kk & 1][e]);
+    };
+    uint4 v[2] = {value(0), value(0)};
+#pragma unroll
+    for (int e = 0; e < 4; e++) split(0, e);
+    in_order();
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+        const int kk = i / kD, d = i % kD;
+        if (i + 1 < kSteps) v[(i + 1) & 1] = value(i + 1);
+#pragma unroll
+        for (int n = kTerms - 1; n >= 0; n--)
+            o[d] = mfma<F16>(v[i & 1], make_uint4(p[kk & 1][0][n], p[kk & 1][1][n], p[kk & 1][2][n], p[kk & 1][3][n]), o[d]);
+        if (kk + 1 < 2 * N)
+#pragma unroll
+            for (int e = d * 4 / kD; e < (d + 1) * 4 / kD; e++) split(kk + 1, e);
+        in_order();
+    }
+}
+
+// ---- tiles of 64 and 128 rows ----------------------------------------------------------
+// WR waves of 32 rows share tiles of 16 WR keys that they load together into two buffers:
+// the next tile is on its way while one is used; one barrier a tile. With WR = 2 the block
+// is two such groups that take the tiles in turn and join their results in LDS.
+template <int DH, bool F16, int WR>
+__device__ __forceinline__ void rows_shared(const TreeAttn& w, const Segment& g, int hk, uint8_t* lds, int tid) {
+    constexpr int NW = 4, NG = NW / WR, TK = 64 / NG, kTile = TK * DH * 2, N = TK / 32;
+    __shared__ int s_bad[NW];
+    __shared__ float2 s_ml[64];
+    const PagedAttnArgs& a = w.a;
+    const int G = w.G;
+    const Request q = g.q;
+    const int lane = tid & 63, h = lane >> 5, c32 = lane & 31;
+    const int all_waves = __builtin_amdgcn_readfirstlane(tid >> 6), group = all_waves / WR, wave = all_waves % WR;
+    lds += group * 4 * kTile;
+    const int last = g.row0 + g.rows, kb = g.kb, ke = g.ke;
+    const int w0 = g.row0 + 32 * wave;  // the wave's first row
+    const int row = min(w0 + c32, last - 1);
+    const float c = a.scale * kLog2e;
+    // the group's tiles, and the first group's (barriers are for all)
+    const int n_all = (max(0, ke - kb) + TK - 1) / TK, n_tiles = max(0, (n_all - group + NG - 1) / NG), n_steps = (n_all + NG - 1) / NG;
+    // the wave loads keys 16 wave .. + 15 of a tile; lane 2 j + n holds where its group n of tile j
+    // of 32 lies, for keys and (a tile behind) for values
+    const Filler<DH> fill(lane);
+    int64_t where[2] = {0, 0};
+    int bad_from = 0x7fffffff;
+    auto load = [&](auto vals, int t) {
+        constexpr bool V = decltype(vals)::value;
+        if (t >= n_tiles) return;
+        const int k0 = kb + (t * NG + group) * TK + 16 * wave;
+        if ((t & 31) == 0 && (!V || t > 0)) {
+            const int key = k0 + (lane >> 1) * (TK * NG) + (lane & 1) * 8;
+            bool outside;
+            where[V] = key_at<DH>(a, g.r, hk, min(key, ke - 1), outside);
+            if (outside && key < ke) bad_from = min(bad_from, key);
+        }
+        const uint32_t to = lds_addr(lds) + ((t & 1) * 2 + V) * kTile + wave * (32 * DH);
+        const uint16_t* const pool = V ? a.v : a.k;
+        if (k0 + 16 <= ke) {
+#pragma unroll
+            for (int n = 0; n < 2; n++) fill.template fill<V, true, false>(pool, lane_of(where[V], 2 * (t & 31) + n), n, to);
+        } else {
+#pragma unroll
+            for (int n = 0; n < 2; n++)
+                fill.template fill<V, false, false>(pool, lane_of(where[V], 2 * (t & 31) + n), n, to,
+                                             max(0, ke - 1 - (k0 + 8 * n)));
+        }
+    };
+    using Keys = std::false_type;
+    using Vals = std::true_type;
+    auto meet = [&]() {
+        wait_lds();
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+    };
+    // A tile's scores are made while the one before it becomes weights: the products and the
+    // exponentials do not depend on each other.
+    constexpr int kLoads = 2 * (DH / 64);  // of a wave and tile
+    load(Keys{}, 0);
+    where[1] = where[0];
+    load(Vals{}, 0);
+    load(Keys{}, 1);
+    // (the first keys and values are on their way)
+    const int lim = min(ke, reach<true>(a, q, row, G)), lim_lo = min(ke, seen_by_all<true>(a, q, min(w0, last - 1), G));
+    const int lim_hi = w0 < last ? min(ke, reach_of_tile<true>(a, q, min(w0 + 31, last - 1), G)) : 0;
+    auto sees_from = [&](int k) { return sees32(a, q, row, G, k, lim); };
+    uint4 qf[DH / 16];
+    load_q<DH>(a, q, row, hk, G, qf, lane);
+    floatx16 o[DH / 32];
+#pragma unroll
+    for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) o[d][r] = 0.0f;
+    float m = ninf(), l = 0.0f;
+    if (n_tiles > 1) wait_vmem<2 * kLoads>();
+    else wait_vmem<kLoads>();
+    meet();
+    auto scores = [&](const uint8_t* kt, floatx16 (&s)[N]) {
+#pragma unroll
+        for (int n = 0; n < N; n++) s[n] = scores32<DH, F16>(kt + n * 32 * 2 * DH, qf, lane);
+    };
+    auto step = [&](int t, floatx16 (&s)[N], floatx16 (&next)[N]) {
+        const int k0 = kb + (t * NG + group) * TK;
+        wait_vmem<0>();
+        meet();  // this tile's values and the next one's keys are there, the last ones are used
+        load(Vals{}, t + 1);
+        load(Keys{}, t + 2);
+        if (t >= n_tiles || k0 >= lim_hi) return;
+        const uint8_t *const kt = lds + ((t + 1) & 1) * 2 * kTile, *const vt = lds + ((t & 1) * 2 + 1) * kTile;
+        const float neg = mask_and_move<DH, F16, true, N>(s, k0, lim, k0 + TK > lim_lo, sees_from, c, m, l, o, lane);
+        scores_and_weigh<DH, F16, N>(kt, qf, next, s, c, neg, l, lane);
+        values<DH, F16, N>(vt, s, o, lane);
+    };
+    floatx16 s0[N], s1[N];
+    scores(lds, s0);
+    for (int t = 0; t < n_steps; t += 2) {
+        step(t, s0, s1);
+        if (t + 1 < n_steps) step(t + 1, s1, s0);
+    }
+    l = pair32<false>(l);
+    const int bad = wave_min_int(bad_from);
+    if (lane == 0) s_bad[all_waves] = bad;
+    __syncthreads();
+    int bad_all = s_bad[0];
+#pragma unroll
+    for (int v = 1; v < NW; v++) bad_all = min(bad_all, s_bad[v]);
+    if constexpr (NG == 2) {
+        // the second group's results, as its lanes hold them
+        float4* const theirs = reinterpret_cast<float4*>(lds + (group ? 0 : 4 * kTile)) + wave * (8 * DH) + lane;
+        if (group) {
+#pragma unroll
+            for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+                    theirs[(4 * d + n) * 64] = make_float4(o[d][4 * n], o[d][4 * n + 1], o[d][4 * n + 2], o[d][4 * n + 3]);
+            if (h == 0) s_ml[32 * wave + c32] = make_float2(m, l);
+        }
+        __syncthreads();
+        if (group) return;
+        const float2 ml = s_ml[32 * wave + c32];
+        const float mx = fmaxf(m, ml.x);
+        const float f0 = m == mx ? 1.0f : __builtin_amdgcn_exp2f(m - mx);
+        const float f1 = ml.x == mx ? 1.0f : __builtin_amdgcn_exp2f(ml.x - mx);
+        m = mx;
+        l = l * f0 + ml.y * f1;
+#pragma unroll
+        for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+            for (int n = 0; n < 4; n++) {
+                const float4 y = theirs[(4 * d + n) * 64];
+                o[d][4 * n] = o[d][4 * n] * f0 + y.x * f1, o[d][4 * n + 1] = o[d][4 * n + 1] * f0 + y.y * f1;
+                o[d][4 * n + 2] = o[d][4 * n + 2] * f0 + y.z * f1, o[d][4 * n + 3] = o[d][4 * n + 3] * f0 + y.w * f1;
+            }
+    }
+    if (w0 >= last) return;
+    float* const rec_ml = g.rec + w.record * DH;
+    const uint32_t again = rows_again<DH>(l, o, w0 + c32 < last);
+    if (again) {
+        for (int x = 0; x < min(32, last - w0); x++) {
+            if (!((again >> x) & 1u)) continue;
+            float m1, l1, o1[DH / 64];
+            const int rw = w0 + x, sees = min(ke, reach<true>(a, q, rw, G)), y = 32 * wave + x;
+            row_again<DH, F16, true>(a, q, g.r, hk, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1, lane);
+            if (sees > bad_all) l1 = __builtin_nanf("");
+            if (g.rec && lane == 0) *reinterpret_cast<float2*>(rec_ml + 2 * y) = make_float2(m1, l1);
+#pragma unroll
+            for (int e = 0; e < DH / 64; e++) {
+                if (g.rec) g.rec[in_record<DH>(y, lane + 64 * e)] = o1[e];
+                else store_out(a, out_at<DH>(a, q, rw, hk, G) + lane + 64 * e, sees ? o1[e] / l1 : 0.0f);
+            }
+        }
+    }
+    if (w0 + c32 >= last || ((again >> c32) & 1u)) return;
+    if (lim > bad_all) l = __builtin_nanf("");
+    if (g.rec) {
+        const int y = 32 * wave + c32;
+#pragma unroll
+        for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+            for (int n = 0; n < 4; n++)
+                *reinterpret_cast<float4*>(g.rec + in_record<DH>(y, 32 * d + 8 * n + 4 * h)) =
+                    make_float4(o[d][4 * n], o[d][4 * n + 1], o[d][4 * n + 2], o[d][4 * n + 3]);
+        if (h == 0) *reinterpret_cast<float2*>(rec_ml + 2 * y) = make_float2(m, l);
+        return;
+    }
+    const float inv = lim ? 1.0f / l : 0.0f;
+    const int64_t at = out_at<DH>(a, q, row, hk, G);
+#pragma unroll
+    for (int d = 0; d < DH / 32; d++)
+#pragma unroll
+        for (int n = 0; n < 4; n++)
+            store_out4(a, at + 32 * d + 8 * n + 4 * h, o[d][4 * n] * inv, o[d][4 * n + 1] * inv, o[d][4 * n + 2] * inv,
+                       o[d][4 * n + 3] * inv);
+}
+
+// The blocks that hold parts of the tile which cut j (1 .. pieces - 1) divides: the first one, and
+// how many. x0: the tile's beginning on the line.
+struct Parts {
+    int first, count;
+};
+__device__ __forceinline__ Parts parts_of(const TreeAttn& w, const Cuts& l, int j, double x0, int units, int rows) {
+    auto inside = [&](int i) {
+        if (i < 1 || i >= l.pieces) return false;
+        const int u = unit_at(w, l.at(i) - x0, units, rows);
+        return u > 0 && u < units;
+    };
+    const int lane = threadIdx.x & 63;
+    int from = j, to = j;  // the first and last cut inside
+    for (;;) {
+        const uint64_t out = __ballot(!inside(from - 1 - lane));
+        from -= out ? __ffsll((unsigned long long)out) - 1 : 64;
+        if (out) break;
+    }
+    for (;;) {
+        const uint64_t out = __ballot(!inside(to + 1 + lane));
+        to += out ? __ffsll((unsigned long long)out) - 1 : 64;
+        if (out) break;
+    }
+    return Parts{uniform(from - 1), uniform(to - from + 2)};
+}
+// Where records lie, in floats: of the tile that goes on in a block, and of the one that begins there.
+__device__ __forceinline__ int64_t record_at(const TreeAttn& w, int block, bool begins, int hk) {
+    return ((int64_t)(begins ? w.blocks + block : block) * w.a.Hk + hk) * w.size;
+}
+
+// What a block keeps of its piece while it works on a tile (in LDS: the tiles need all registers).
+struct Walk {
+    Cuts cuts;
+    Place at, end;
+};
+
+template <int DH, bool F16>
+__global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void tree_attn_kernel(TreeAttn w) {
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * 4 * 32 * DH * 2];  // 64 KB at a head_dim of 128
+    __shared__ Walk s_walk;
+    // (the grid's fastest axis: with 8 kv heads all blocks of a head share one XCD's L2)
+    const int hk = blockIdx.x, b = blockIdx.y;
+    {
+        const Line l = line_of(w);
+        if (b >= l.cuts.pieces) {
+            if (w.split && hk == 0 && threadIdx.x == 0) w.split[b].parts = 0;
+            return;
+        }
+        const Place at = place_of(w, l, l.cuts.at(b));
+        const Place end = b + 1 < l.cuts.pieces ? place_of(w, l, l.cuts.at(b + 1)) : Place{w.a.n_req, 0, 0, 0.0, Request{0, 0, 0}};
+        if (threadIdx.x == 0) s_walk = Walk{l.cuts, at, end};
+        if (w.split && hk == 0 && threadIdx.x == 0) w.split[b].parts = 0;
+    }
+    for (;;) {
+        __syncthreads();
+        const Place at = s_walk.at;
+        const struct {
+            int r, tile, unit;
+        } p = {uniform(at.r), uniform(at.tile), uniform(at.unit)};
+        const int end_r = uniform(s_walk.end.r), end_tile = uniform(s_walk.end.tile), end_unit = uniform(s_walk.end.unit);
+        if (p.r > end_r || (p.r == end_r && (p.tile > end_tile || (p.tile == end_tile && p.unit >= end_unit)))) return;
+        const Request q{uniform(at.q.start), uniform(at.q.n), uniform(at.q.kv)};
+        const Shape s = shape_of(q, w.G);
+        if (p.tile >= s.whole + s.rest_tiles) {
+            __syncthreads();
+            if (threadIdx.x == 0)
+                s_walk.at = Place{p.r + 1, 0, 0, at.begin + s.cost, p.r + 1 < w.a.n_req ? request(w.a, p.r + 1) : q};
+            continue;
+        }
+        bool all;
+        {
+            const Tile t = tile_of(s, p.tile);
+            const int to = p.r == end_r && p.tile == end_tile ? end_unit : s.units;
+            all = p.unit == 0 && to == s.units;
+            Segment g;
+            g.q = q, g.r = p.r, g.row0 = t.row0, g.rows = t.rows;
+            g.kb = p.unit * kUnit;
+            g.ke = uniform(min(reach_of_tile<true>(w.a, q, t.row0 + t.rows - 1, w.G), to * kUnit));
+            g.rec = all ? nullptr : w.part + record_at(w, b, p.unit == 0, hk);
+            int tid = threadIdx.x;
+            asm volatile("" : "+v"(tid));  // (what a tile makes of it is not kept for the next: registers are short)
+            if (t.kind == 32) rows32<DH, F16>(w, g, hk, lds, tid);
+            else if (t.kind == 64) rows_shared<DH, F16, 2>(w, g, hk, lds, tid);
+            else rows_shared<DH, F16, 4>(w, g, hk, lds, tid);
+        }
+        __syncthreads();
+        if (!all && hk == 0 && w.split) {  // the joining launch learns of a tile from the block that it begins in
+            const Place at = s_walk.at;
+            const Request q{uniform(at.q.start), uniform(at.q.n), uniform(at.q.kv)};
+            const Shape s = shape_of(q, w.G);
+            const Tile t = tile_of(s, uniform(at.tile));
+            const Parts parts = parts_of(w, s_walk.cuts, uniform(at.unit) > 0 ? b : b + 1, at.begin + t.at, s.units, t.rows);
+            if (parts.first == b && threadIdx.x == 0) w.split[b] = Split{parts.count, q, t.row0, t.rows};
+            __syncthreads();  // (all have read where the block is)
+        }
+        if (threadIdx.x == 0) s_walk.at.tile++, s_walk.at.unit = 0;
+    }
+}
+
+// The parts of a cut tile joined in their order. Block y: the y-th such tile. An item is 8 features
+// of 32 rows (in_record), 4 features of one row to a lane; a wave takes an item, or, where there are
+// more parts than it requests together, all four a quarter of the parts each.
+constexpr int kMergeWaves = 4, kJoin = 8;
+template <int DH>
+__global__ __launch_bounds__(64 * kMergeWaves) void tree_attn_merge_kernel(TreeAttn w) {
+    __shared__ float s_sums[kMergeWaves][6][64];
+    const PagedAttnArgs& a = w.a;
+    const int hk = blockIdx.x, lane = threadIdx.x & 63, wave = (int)threadIdx.x / 64;
+    int left = blockIdx.y, b = -1;
+    for (int b0 = 0; b0 < w.blocks && b < 0; b0 += 64) {
+        uint64_t cut = __ballot(b0 + lane < w.blocks && w.split[min(b0 + lane, w.blocks - 1)].parts > 0);
+        const int count = __popcll(cut);
+        if (left < count) {
+            for (; left > 0; left--) cut &= cut - 1;
+            b = b0 + __ffsll((unsigned long long)cut) - 1;
+        } else {
+            left -= count;
+        }
+    }
+    if (b < 0) return;
+    const Split t = w.split[b];
+    const bool shared = t.parts > kJoin;
+    const int items = (t.rows + 31) / 32 * (DH / 8), each = shared ? (t.parts + kMergeWaves - 1) / kMergeWaves : t.parts;
+    const int from = shared ? wave * each : 0, to = min(t.parts, from + each), step = shared ? 1 : kMergeWaves;
+    for (int item0 = blockIdx.z * step; item0 < items; item0 += gridDim.z * step) {
+        const int item = shared ? item0 : min(item0 + wave, items - 1);
+        const int x = item / (DH / 8) * 32 + (lane & 31), feature = item % (DH / 8) * 8 + (lane >> 5) * 4;
+        // (rows behind the last: what their places hold is not stored)
+        const float *const results = w.part + in_record<DH>(x, feature), *const ml = w.part + w.record * DH + 2 * x;
+        const bool sees = reach<true>(a, t.q, t.row0 + min(x, t.rows - 1), w.G) > 0;
+        float mx = ninf(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        auto join = [&](float2 u, float4 y) {
+            const float g = u.x == mx ? 1.0f : __builtin_amdgcn_exp2f(u.x - mx);
+            l = fmaf(u.y, g, l);
+            o[0] = fmaf(y.x, g, o[0]), o[1] = fmaf(y.y, g, o[1]);
+            o[2] = fmaf(y.z, g, o[2]), o[3] = fmaf(y.w, g, o[3]);
+        };
+        for (int s0 = from; s0 < to; s0 += kJoin) {
+            float2 u[kJoin];
+            float4 y[kJoin];
+            float top = mx;
+#pragma unroll
+            for (int i = 0; i < kJoin; i++) {
+                const int part = min(s0 + i, to - 1);
+                const int64_t at = record_at(w, b + part, part == 0, hk);
+                u[i] = *reinterpret_cast<const float2*>(ml + at);
+                y[i] = *reinterpret_cast<const float4*>(results + at);
+            }
+#pragma unroll
+            for (int i = 0; i < kJoin; i++) top = fmaxf(top, u[i].x);
+            const float g0 = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
+            l *= g0, o[0] *= g0, o[1] *= g0, o[2] *= g0, o[3] *= g0;
+            mx = top;
+#pragma unroll
+            for (int i = 0; i < kJoin; i++) {
+                if (s0 + i >= to) break;
+                join(u[i], y[i]);
+            }
+        }
+        if (shared) {
+            __syncthreads();  // (the item before is read)
+            float* const mine = &s_sums[wave][0][lane];
+            mine[0] = mx, mine[64] = l;
+#pragma unroll
+            for (int e = 0; e < 4; e++) mine[64 * (2 + e)] = o[e];
+            __syncthreads();
+            if (wave > 0) continue;
+#pragma unroll
+            for (int v = 1; v < kMergeWaves; v++) mx = fmaxf(mx, s_sums[v][0][lane]);
+            const float m0 = s_sums[0][0][lane], g0 = m0 == mx ? 1.0f : __builtin_amdgcn_exp2f(m0 - mx);
+            l *= g0, o[0] *= g0, o[1] *= g0, o[2] *= g0, o[3] *= g0;
+#pragma unroll
+            for (int v = 1; v < kMergeWaves; v++) {
+                const float* const q = &s_sums[v][0][lane];
+                join(make_float2(q[0], q[64]), make_float4(q[128], q[192], q[256], q[320]));
+            }
+        } else if (item0 + wave >= items) {
+            continue;
+        }
+        if (x >= t.rows) continue;
+        store_out4(a, out_at<DH>(a, t.q, t.row0 + x, hk, w.G) + feature, sees ? o[0] / l : 0.0f, sees ? o[1] / l : 0.0f,
+                   sees ? o[2] / l : 0.0f, sees ? o[3] / l : 0.0f);
+    }
+}
+
+struct Launch {
+    TreeAttn w;
+    int cut, shares;  // most tiles that are cut, and the blocks that join one
+    size_t records, bytes;
+};
+Launch plan_launch(const PagedAttnArgs& a, int num_cus) {
+    Launch L{};
+    const int64_t G = a.Hq / a.Hk, rows = (int64_t)a.n_rows * G;
+    L.w.a = a;
+    L.w.G = (int)G;
+    // blocks resident at once (LDS and registers)
+    const int64_t room = std::max<int64_t>(1, (int64_t)num_cus * (a.Dh == 256 ? 1 : 2) / a.Hk);
+    L.w.blocks = (int)room;
+    L.w.record = (int)(std::min<int64_t>(rows, kManyRows) + 31) / 32 * 32;
+    L.w.size = (L.w.record * (a.Dh + 2) + 31) / 32 * 32;
+    L.records = (size_t)2 * L.w.blocks * a.Hk * L.w.size * sizeof(float);
+    L.bytes = L.records + L.w.blocks * sizeof(Split);
+    const int64_t few = std::min<int64_t>((int64_t)a.max_new * G, rows);
+    // tiles: a request's whole ones and one more; a cut divides one tile
+    const int64_t tiles = std::min<int64_t>(a.n_req, a.n_rows) + rows / kManyRows;
+    L.cut = (int)std::min<int64_t>(L.w.blocks - 1, tiles);
+    // a block for every item (as the hint says), over about eight blocks to a CU
+    const int64_t items = (std::min<int64_t>(std::max<int64_t>(few, 1), kManyRows) + 31) / 32 * (a.Dh / 8);
+    L.shares = (int)std::max<int64_t>(1, std::min(items, 8 * (int64_t)num_cus / std::max<int64_t>(1, L.cut * a.Hk)));
+    return L;
+}
+
+}  // namespace
+
+size_t paged_tree_attn_workspace_bytes(const PagedAttnArgs& a, int num_cus) {
+    return plan_launch(a, num_cus).bytes;
+}
+
+Status launch_paged_tree_attn(const PagedAttnArgs& a, void* workspace, size_t workspace_bytes, int num_cus, hipStream_t st) {
+    Launch L = plan_launch(a, num_cus);
+    if (!a.whole && L.bytes > workspace_bytes)
+        return Status::fail(JH_ERR_INVALID, "jh_paged_tree_attention: the workspace does not hold the parts");
+    L.w.part = static_cast<float*>(workspace);
+    if (!a.whole) L.w.split = reinterpret_cast<Split*>(static_cast<char*>(workspace) + L.records);
+    const dim3 grid((unsigned)a.Hk, (unsigned)L.w.blocks);
+    auto with = [&](auto dh) {
+        constexpr int DH = decltype(dh)::value;
+        if (a.f16) hipLaunchKernelGGL((tree_attn_kernel<DH, true>), grid, dim3(256), 0, st, L.w);
+        else hipLaunchKernelGGL((tree_attn_kernel<DH, false>), grid, dim3(256), 0, st, L.w);
+        if (L.w.split && L.cut > 0)
+            hipLaunchKernelGGL(tree_attn_merge_kernel<DH>, dim3((unsigned)a.Hk, (unsigned)L.cut, (unsigned)L.shares),
+                               dim3(64 * kMergeWaves), 0, st, L.w);
+    };
+    if (a.Dh == 64) with(std::integral_constant<int, 64>{});
+    else if (a.Dh == 128) with(std::integral_constant<int, 128>{});
+    else with(std::integral_constant<int, 256>{});
+    return Status::ok();
+}
+
+}  // namespace jh

@@ -1310,12 +1310,16 @@ int paged_attention(jh_ctx* c, const char* op, const void* q, int64_t q_stride, 
     // the parts of split keys need a workspace; where it cannot grow (a stream under capture,
     // no memory) the keys stay whole
     int* const sync = xcd_sync(c) ? xcd_sync(c) + jh::kPagedSyncSlot : nullptr;
-    if (int r = ensure_workspace(c, jh::paged_attn_workspace_bytes(a, c->num_cus, sync), op)) {
+    const size_t need = mask ? jh::paged_tree_attn_workspace_bytes(a, c->num_cus)
+                             : jh::paged_attn_workspace_bytes(a, c->num_cus, sync);
+    if (int r = ensure_workspace(c, need, op)) {
         if (r != JH_ERR_INVALID && r != JH_ERR_OOM) return r;
         c->err.clear();
         a.whole = 1;
     }
-    if (int r = finish(c, jh::launch_paged_attn(a, c->ws, c->ws_bytes, c->num_cus, sync, c->stream), op)) return r;
+    const jh::Status st = mask ? jh::launch_paged_tree_attn(a, c->ws, c->ws_bytes, c->num_cus, c->stream)
+                               : jh::launch_paged_attn(a, c->ws, c->ws_bytes, c->num_cus, sync, c->stream);
+    if (int r = finish(c, st, op)) return r;
     const int64_t row = n_heads * head_dim;
     return check_values(c, op, out, out_dtype, used * row, from * row);
 }
