@@ -449,17 +449,8 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
         if (t >= n_tiles || k0 >= lim_hi) return;
         const uint8_t *const kt = lds + ((t + 1) & 1) * 2 * kTile, *const vt = lds + ((t & 1) * 2 + 1) * kTile;
         const float neg = mask_and_move<DH, F16, false, 2>(s, k0, lim, k0 + 64 > lim_lo, no_mask, c, m, l, o);
-        next[0] = scores32<DH, F16>(kt, qf);
-        next[1] = scores32<DH, F16>(kt + 32 * 2 * DH, qf);
-        weigh<2>(s, c, neg, l);
-#pragma unroll
-        for (int kk = 0; kk < 4; kk++) {
-            uint32_t p[4][kTerms];
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                split_pair<F16, kTerms>(s[kk >> 1][8 * (kk & 1) + 2 * e], s[kk >> 1][8 * (kk & 1) + 2 * e + 1], p[e]);
-            values16<DH, F16>(vt + kk * 16 * 2 * DH, p, o);
-        }
+        scores_and_weigh<DH, F16, 2>(kt, qf, next, s, c, neg, l, lane);
+        values<DH, F16, 2>(vt, s, o, lane);
     };
     floatx16 s0[2] = {scores32<DH, F16>(lds, qf), scores32<DH, F16>(lds + 32 * 2 * DH, qf)}, s1[2];
     for (int t = 0; t < n_steps; t += 2) {

@@ -414,6 +414,72 @@ __device__ __forceinline__ void weigh(floatx16 (&s)[N], float c, float neg, floa
     l += sum;
 }
 
+// Products and exponentials use different units, but only as far as their instructions
+// alternate; the order here is the source's (sched_barrier), with operands read two products ahead.
+// Left to the compiler, all products came first: a tree of 63 tokens (252 rows, head_dim 128) over
+// 30000 keys took 62 us for its parts instead of 58.
+__device__ __forceinline__ void in_order() { __builtin_amdgcn_sched_barrier(0); }
+
+// scores32 of a tile of 32 N keys into `next`, and weigh of the tile before it.
+template <int DH, bool F16, int N>
+__device__ __forceinline__ void scores_and_weigh(const uint8_t* kt, const uint4 (&qf)[DH / 16], floatx16 (&next)[N],
+                                                 floatx16 (&s)[N], float c, float neg, float& l, int lane) {
+    constexpr int kSteps = N * DH / 16, kEach = 16 * N / kSteps;
+    const int row = lane & 31, x = ((lane >> 5) ^ perm_k<DH>(row)) * 16;
+    const uint8_t* const at = kt + row * (2 * DH);
+    auto key = [&](int i) { return lds_read16(at + (i % N) * 64 * DH + (x ^ (32 * (i / N)))); };
+#pragma unroll
+    for (int n = 0; n < N; n++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) next[n][r] = 0.0f;
+    uint4 k[3] = {key(0), key(1), key(0)};
+    float sum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+        if (i + 2 < kSteps) k[(i + 2) % 3] = key(i + 2);
+        next[i % N] = mfma<F16>(k[i % 3], qf[i / N], next[i % N]);
+#pragma unroll
+        for (int e = i * kEach; e < (i + 1) * kEach; e++) {
+            s[e >> 4][e & 15] = __builtin_amdgcn_exp2f(fmaf(s[e >> 4][e & 15], c, neg));
+            sum += s[e >> 4][e & 15];
+        }
+        in_order();
+    }
+    l += sum;
+}
+// values16 over 32 N keys.
+template <int DH, bool F16, int N>
+__device__ __forceinline__ void values(const uint8_t* vt, const floatx16 (&s)[N], floatx16 (&o)[DH / 32], int lane) {
+    constexpr int kD = DH / 32, kSteps = 2 * N * kD;
+    const int i16 = lane & 15, x = perm_v<DH>(i16 >> 2) / 4;
+    const uint8_t* const at = vt + ((lane >> 5) * 4 + (i16 >> 2)) * (2 * DH) + ((lane >> 4) & 1) * 32 + (i16 & 3) * 8;
+    auto value = [&](int i) {
+        const uint8_t* const p = at + (i / kD) * 32 * DH + ((i % kD) ^ x) * 64;
+        const uint2 lo = lds_read_tr(p), hi = lds_read_tr(p + 16 * DH);
+        return make_uint4(lo.x, lo.y, hi.x, hi.y);
+    };
+    uint32_t p[2][4][kTerms];
+    auto split = [&](int kk, int e) {
+        split_pair<F16, kTerms>(s[kk >> 1][8 * (kk & 1) + 2 * e], s[kk >> 1][8 * (kk & 1) + 2 * e + 1], p[kk & 1][e]);
+    };
+    uint4 v[2] = {value(0), value(0)};
+#pragma unroll
+    for (int e = 0; e < 4; e++) split(0, e);
+    in_order();
+#pragma unroll
+    for (int i = 0; i < kSteps; i++) {
+        const int kk = i / kD, d = i % kD;
+        if (i + 1 < kSteps) v[(i + 1) & 1] = value(i + 1);
+#pragma unroll
+        for (int n = kTerms - 1; n >= 0; n--)
+            o[d] = mfma<F16>(v[i & 1], make_uint4(p[kk & 1][0][n], p[kk & 1][1][n], p[kk & 1][2][n], p[kk & 1][3][n]), o[d]);
+        if (kk + 1 < 2 * N)
+#pragma unroll
+            for (int e = d * 4 / kD; e < (d + 1) * 4 / kD; e++) split(kk + 1, e);
+        in_order();
+    }
+}
+
 // The wave's rows (bit lane % 32) whose results are not finite.
 template <int DH>
 __device__ __forceinline__ uint32_t rows_again(float l, const floatx16 (&o)[DH / 32], bool live) {
