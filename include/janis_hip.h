@@ -789,8 +789,9 @@ JH_API int jh_paged_tree_attention(jh_ctx *ctx, const void *q, int64_t q_stride,
                                    int64_t n_rows, int64_t max_new, int64_t n_heads, int64_t n_kv_heads,
                                    int64_t head_dim, float scale, void *out, jh_dtype out_dtype);
 
-/* The path that the large model agrees with, request by request, in at most one launch
- * for the bookkeeping and one for every 64 layers. The first known[r] rows of a request
+/* The path that the large model agrees with, request by request, in one launch to find
+ * it and one for every 64 layers (for a single request that is not updated in place
+ * without the first). What the first finds lies in the context's workspace. The first known[r] rows of a request
  * (held to 1 .. n; 1 where known is NULL) are tokens that are kept whatever the model
  * says, a chain whose parents are not looked at: the last token sampled, or a prompt's
  * end. From the last of them on, the row whose parent is the one before it and whose

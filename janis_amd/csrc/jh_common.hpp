@@ -524,7 +524,7 @@ struct TreePlanArgs {
 };
 Status launch_tree_plan(const TreePlanArgs& a, hipStream_t st);
 struct TreeCommitArgs {
-    const int32_t *parents, *tokens, *chosen;
+    const int32_t *parents, *tokens, *chosen, *slots;
     int64_t chosen_stride;
     const int32_t *known, *row_starts, *kv_lens;
     int n_req, n_rows, tree_rows, page_shift;  // tree_rows: a request of more is a run
@@ -534,17 +534,23 @@ struct TreeCommitArgs {
     int n_pages;
     const int32_t* free_count;
     int32_t *kv_out, *count_out, *accepted, *path, *next_tokens, *status;
+    // (the launch's, in the workspace)
+    int4* heads;
+    int2* moves;
+    int most;
 };
-Status launch_tree_commit(const TreeCommitArgs& a, hipStream_t st);
 // Pointers travel in the launch's arguments: so many layers a launch.
 constexpr int kMoveLayers = 64;
 struct TreeMoveArgs {
-    const int32_t *row_starts, *accepted, *path, *slots;
-    int n_req, n_rows, n_slots, page_shift, Hk, Dh, layers;
+    int n_slots, page_shift, Hk, Dh;
     int64_t page_stride;
+    // (the launch's)
+    int first, layers, each;
     uint16_t *k[kMoveLayers], *v[kMoveLayers];
 };
-Status launch_tree_move(const TreeMoveArgs& a, hipStream_t st);
+size_t tree_commit_workspace_bytes(const TreeCommitArgs& a);
+Status launch_tree_commit(TreeCommitArgs a, const TreeMoveArgs& move, void* const* k_pages, void* const* v_pages, int64_t layers,
+                          void* workspace, int num_cus, hipStream_t st);
 
 // ---- log probabilities (logprobs.hip) ----
 struct LogProbsArgs {

@@ -1423,26 +1423,19 @@ int jh_paged_tree_commit(jh_ctx* c, const int32_t* parents, const int32_t* token
     if (c->checks & JH_CHECK_INDICES)
         if (int r = checks_not_capturing(c, op)) return r;
     jh::TreeCommitArgs a{};
-    a.parents = parents, a.tokens = tokens, a.chosen = chosen, a.chosen_stride = chosen_stride, a.known = known;
+    a.parents = parents, a.tokens = tokens, a.chosen = chosen, a.chosen_stride = chosen_stride, a.slots = slots, a.known = known;
     a.row_starts = row_starts, a.kv_lens = kv_lens;
     a.n_req = (int)n_req, a.n_rows = (int)n_rows, a.tree_rows = (int)(32 * mask_words), a.page_shift = __builtin_ctzll(page_size);
     a.tables = block_tables, a.max_blocks = (int)max_blocks;
     a.free_pages = free_pages, a.n_pages = (int)n_pages, a.free_count = free_count;
     a.kv_out = kv_lens_out, a.count_out = free_count_out, a.accepted = accepted, a.path = path;
     a.next_tokens = next_tokens, a.status = status;
-    if (int r = finish(c, jh::launch_tree_commit(a, c->stream), op)) return r;
-    if (n_layers > 0 && n_req > 0 && n_rows > 0 && n_pages > 0) {
-        jh::TreeMoveArgs m{};
-        m.row_starts = row_starts, m.accepted = accepted, m.path = path, m.slots = slots;
-        m.n_req = (int)n_req, m.n_rows = (int)n_rows, m.n_slots = (int)(n_pages * page_size);
-        m.page_shift = a.page_shift, m.Hk = (int)n_kv_heads, m.Dh = (int)head_dim, m.page_stride = page_stride;
-        for (int64_t i = 0; i < n_layers; i += jh::kMoveLayers) {
-            m.layers = (int)std::min<int64_t>(jh::kMoveLayers, n_layers - i);
-            for (int j = 0; j < m.layers; j++)
-                m.k[j] = static_cast<uint16_t*>(k_pages[i + j]), m.v[j] = static_cast<uint16_t*>(v_pages[i + j]);
-            if (int r = finish(c, jh::launch_tree_move(m, c->stream), op)) return r;
-        }
-    }
+    jh::TreeMoveArgs m{};
+    m.n_slots = (int)(n_pages * page_size), m.page_shift = a.page_shift, m.Hk = (int)n_kv_heads, m.Dh = (int)head_dim;
+    m.page_stride = page_stride;
+    if (n_rows == 0 || n_pages == 0) n_layers = 0;
+    if (int r = ensure_workspace(c, jh::tree_commit_workspace_bytes(a), op)) return r;
+    if (int r = finish(c, jh::launch_tree_commit(a, m, k_pages, v_pages, n_layers, c->ws, c->num_cus, c->stream), op)) return r;
     if (c->checks & JH_CHECK_INDICES) {
         static const char* const why[] = {"", "a request of fewer keys than rows, or more than max_blocks pages",
                                           "row_starts that decrease or leave [0, n_rows]", "*free_count outside [0, n_pages]",

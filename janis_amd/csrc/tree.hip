@@ -1,6 +1,6 @@
 // Trees of drafted tokens over the paged cache: positions and masks, the path that the
 // model agrees with, and its keys and values moved together (attention:
-// paged_attention.hip).
+// paged_tree_attention.hip).
 #include "jh_common.hpp"
 
 namespace jh {
@@ -87,194 +87,227 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(TreePlanArgs a) {
 }
 
 // ---- the path that the model agrees with ----------------------------------------------
-// One workgroup: lengths and the stack are updated in place, so all that decides is read
-// before the barrier behind which anything is written. Rows (parents, tokens, choices)
-// come to LDS kRows at a time, all requested together; a thread walks its requests
-// there in one pass, since a child comes after its parent: row i is kept if its parent
-// is the last row kept and its token the choice there.
-constexpr int kCommitThreads = 1024, kRows = 8192;
-static_assert(kPlanMaxReq % kCommitThreads == 0, "requests per thread");
+// Two launches: the first finds every request's path and what is to be done, in the
+// workspace; the second does it. Nothing may be done if any request is wrong, lengths and
+// the stack are updated in place, and what a request gives back lies on the stack behind
+// what the ones before it give back: so all that decides comes before all that is written.
+// Both are chains of round trips: two to the path (lengths; rows, their slots and the pages
+// that may come back, all requested together), two to the writes (heads and moves; keys
+// and values). With the walk and the books in one workgroup, and path and slots looked up
+// by every block that moves, 64 requests of 8 to 32 rows in 36 layers took 33 us; so, 14.
+// A single request that is not updated in place needs no more than itself: there every
+// block of one launch finds the path (16 rows in 36 layers 7.1 us, with two launches 9.5).
+//
+// heads: per request {what is wrong with it or kFine, pages that come back, rows that move,
+// its length}, behind them {*free_count}. moves: [request][most rows of a tree] of slots.
+constexpr int kWalkThreads = 256, kTreeRows = 32 * JH_TREE_WORDS, kFine = 9;
+static_assert(JH_PLAN_TABLE < kFine, "of several faults the least is reported");
 
-__device__ __forceinline__ int scan_int(int v) {  // sum over the lanes up to this one
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const int u = __shfl_up(v, d, 64);
-        if ((int)(threadIdx.x & 63) >= d) v += u;
+// What a request's rows come to.
+struct Walk {
+    int4 head;       // as in heads
+    int kept, next;  // rows kept, and the choice after the last
+    int same;        // kept rows that stay where they are, the first ones
+};
+struct WalkRows {
+    int parent[kTreeRows], token[kTreeRows], chosen[kTreeRows], slot[kTreeRows];
+    int kept[kTreeRows];  // the kept rows
+    int end[3];
+};
+
+// By all threads of a block. A child comes after its parent, so the path goes up: from row i
+// on, the first row behind it whose parent is i and whose token the choice there, 64 rows to
+// a ballot.
+__device__ __forceinline__ Walk walk(const TreeCommitArgs& a, int r, WalkRows& s, bool write) {
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int64_t limit = min((int64_t)a.max_blocks << a.page_shift, (int64_t)0x7fffffff);
+    auto blocks = [&](int64_t kv) { return (int)((kv + (1 << a.page_shift) - 1) >> a.page_shift); };
+    const int start = a.row_starts[r], to = a.row_starts[r + 1], kv = a.kv_lens[r];
+    const int first = a.known ? a.known[r] : 1;
+    const bool wrong = start < 0 || to < start || to > a.n_rows;
+    const int n = wrong ? 0 : to - start;
+    const int fault = kv < n || kv > limit ? JH_PLAN_LENGTHS : wrong ? JH_PLAN_ROWS : kFine;
+    if (fault != kFine || n == 0) return Walk{make_int4(fault, 0, 0, kv), 0, -1, 0};
+    if (n > a.tree_rows) {
+        if (write)
+            for (int i = tid; i < n; i += kWalkThreads) a.path[start + i] = start + i;
+        return Walk{make_int4(kFine, 0, 0, kv), n, a.chosen[(start + n - 1) * a.chosen_stride], n};
     }
+    const int known = min(max(first, 1), n), b0 = blocks(kv - n + known), back = blocks(kv) - b0;
+    constexpr int kEach = kTreeRows / kWalkThreads;
+    int page[kEach];
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        const int i = e * kWalkThreads + tid;
+        page[e] = i < back ? a.tables[(int64_t)r * a.max_blocks + b0 + i] : 0;
+        if (i >= n) continue;
+        s.parent[i] = a.parents[start + i];
+        s.token[i] = a.tokens[start + i];
+        s.chosen[i] = a.chosen[(start + i) * a.chosen_stride];
+        s.slot[i] = a.slots[start + i];
+        s.kept[i] = i;
+    }
+    __syncthreads();
+    if (tid < 64) {
+        int at = known - 1, kept = known, same = known, want = s.chosen[at];
+        for (int g = at >> 6; g < (n + 63) >> 6; g++) {
+            const int i = min(64 * g + lane, n - 1);
+            const int parent = s.parent[i], token = s.token[i], choice = s.chosen[i];
+            for (;;) {
+                const uint64_t next = __ballot(64 * g + lane < n && i > at && parent == at && token == want);
+                if (!next) break;
+                const int l = __ffsll((unsigned long long)next) - 1;
+                at = 64 * g + l;
+                want = __builtin_amdgcn_readlane(choice, l);
+                same += at == kept;
+                if (lane == 0) s.kept[kept] = at;
+                kept++;
+            }
+        }
+        if (lane == 0) s.end[0] = kept, s.end[1] = want, s.end[2] = same;
+    }
+    __syncthreads();
+    const int kept = s.end[0], same = s.end[2], left = kv - n + kept, b = blocks(left) - b0;
+    bool outside = false;
+#pragma unroll
+    for (int e = 0; e < kEach; e++) {
+        const int i = e * kWalkThreads + tid;
+        outside |= i >= b && i < back && (uint32_t)page[e] >= (uint32_t)a.n_pages;
+        if (write && i < n) a.path[start + i] = i < kept ? start + s.kept[i] : -1;
+    }
+    outside = __syncthreads_or(outside);
+    return Walk{make_int4(outside ? JH_PLAN_TABLE : kFine, back - b, kept - same, left), kept, s.end[1], same};
+}
+
+// A block to a request.
+__global__ __launch_bounds__(kWalkThreads) void tree_walk_kernel(TreeCommitArgs a) {
+    __shared__ WalkRows s;
+    const int r = blockIdx.x;
+    if (r == 0 && threadIdx.x == 0) a.heads[a.n_req] = make_int4(*a.free_count, 0, 0, 0);
+    const Walk w = walk(a, r, s, true);
+    for (int i = threadIdx.x; i < w.head.z; i += kWalkThreads)
+        a.moves[(int64_t)r * a.most + i] = make_int2(s.slot[s.kept[w.same + i]], s.slot[w.same + i]);
+    if (threadIdx.x == 0) a.heads[r] = w.head, a.accepted[r] = w.kept, a.next_tokens[r] = w.next;
+}
+
+__device__ __forceinline__ int sum64(int v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v += __shfl_xor(v, d, 64);
+    return v;
+}
+__device__ __forceinline__ int least64(int v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = min(v, __shfl_xor(v, d, 64));
     return v;
 }
 
-__global__ __launch_bounds__(kCommitThreads) void tree_commit_kernel(TreeCommitArgs a) {
-    constexpr int kPer = kPlanMaxReq / kCommitThreads, kWaves = kCommitThreads / 64;
-    __shared__ int s_parent[kRows], s_token[kRows], s_chosen[kRows];
-    __shared__ int s_start[kPlanMaxReq + 1], s_kept[kPlanMaxReq];  // (~kept: of a run, kept whole)
-    __shared__ int s_known[kPlanMaxReq];
-    __shared__ int s_sum[kWaves];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, R = a.n_req, page = 1 << a.page_shift;
-    const int64_t limit = min((int64_t)a.max_blocks << a.page_shift, (int64_t)0x7fffffff);
-    auto blocks = [&](int64_t kv) { return (int)((kv + page - 1) >> a.page_shift); };
-    const int count = *a.free_count;
-    int start[kPer], n[kPer], kv[kPer], known[kPer];
-    bool lengths = false, rows = false;
-#pragma unroll
-    for (int e = 0; e < kPer; e++) {
-        const int r = tid * kPer + e;
-        start[e] = n[e] = kv[e] = known[e] = 0;
-        if (r >= R) continue;
-        start[e] = a.row_starts[r];
-        const int to = a.row_starts[r + 1];
-        kv[e] = a.kv_lens[r];
-        const bool wrong = start[e] < 0 || to < start[e] || to > a.n_rows;
-        rows |= wrong;
-        n[e] = wrong ? 0 : to - start[e];
-        lengths |= kv[e] < n[e] || kv[e] > limit;
-        known[e] = n[e] > a.tree_rows ? n[e] : min(max(a.known ? a.known[r] : 1, 1), n[e]);
-        s_start[r] = start[e];
-        s_known[r] = known[e];
-    }
-    if (tid == 0 && R > 0) s_start[R] = a.row_starts[R];
-    lengths = __syncthreads_or(lengths);
-    rows = __syncthreads_or(rows);
-    int status = lengths ? JH_PLAN_LENGTHS : rows ? JH_PLAN_ROWS : count < 0 || count > a.n_pages ? JH_PLAN_PAGES : JH_PLAN_OK;
-    int at[kPer], cur[kPer], want[kPer], kept[kPer];
-#pragma unroll
-    for (int e = 0; e < kPer; e++) at[e] = known[e] - 1, cur[e] = -1, want[e] = -1, kept[e] = known[e];
-    const int first = status == JH_PLAN_OK && R > 0 ? s_start[0] : 0, last = status == JH_PLAN_OK && R > 0 ? s_start[R] : 0;
-    for (int w0 = first; w0 < last; w0 += kRows) {
-        const int w1 = min(last, w0 + kRows);
-        if (w0 > first) __syncthreads();  // (the walks before have read)
-#pragma unroll
-        for (int e = 0; e < kRows / kCommitThreads; e++) {
-            const int t = w0 + e * kCommitThreads + tid;
-            if (t >= w1) continue;
-            s_parent[t - w0] = a.parents[t];
-            s_token[t - w0] = a.tokens[t];
-            s_chosen[t - w0] = a.chosen[t * a.chosen_stride];
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// Block (r, y): the books of request r (y 0, of the first launch), and its rows in the y-th part of
+// the layers, a thread to 16 bytes of a key's or value's heads. The j-th kept row moves to slot j of
+// the request, which is no kept row's behind it: so rows are read together, and written then. Every
+// wave finds out for itself whether anything is done, while its first rows are on their way.
+// ONE: a single request, whose path every block finds.
+template <bool ONE>
+__global__ __launch_bounds__(kWalkThreads) void tree_commit_kernel(TreeCommitArgs a, TreeMoveArgs m) {
+    __shared__ typename std::conditional<ONE, WalkRows, int>::type s;
+    const int r = blockIdx.x, R = a.n_req, tid = threadIdx.x, lane = tid & 63;
+    const bool books = m.first && blockIdx.y == 0;
+    const int l1 = min(m.layers, ((int)blockIdx.y + 1) * m.each);
+    Walk w;
+    if constexpr (ONE) w = walk(a, 0, s, books);
+    int4 mine = ONE ? w.head : R ? a.heads[r] : make_int4(kFine, 0, 0, 0);
+    if (m.layers == 0) mine.z = 0;
+    if (!books && mine.z == 0) return;
+    const int count = !ONE && R ? a.heads[R].x : *a.free_count;
+    int2 head = make_int2(kFine, 0);
+    if constexpr (ONE) head = make_int2(mine.x, lane == 0 ? mine.y : 0);
+    else if (lane < R) head = make_int2(a.heads[lane].x, a.heads[lane].y);
+    int status = -1, before = 0, total = 0;
+    auto verdict = [&]() {
+        int fault = head.x;
+        total = head.y, before = lane < r ? head.y : 0;
+        for (int i = lane + 64; !ONE && i < R; i += 64) {
+            const int4 h = a.heads[i];
+            fault = min(fault, h.x);
+            total += h.y;
+            if (i < r) before += h.y;
         }
-        __syncthreads();
+        fault = least64(fault), total = sum64(total), before = sum64(before);
+        if (count < 0 || count > a.n_pages) fault = min(fault, (int)JH_PLAN_PAGES);
+        else if ((int64_t)count + total > a.n_pages) fault = min(fault, (int)JH_PLAN_TABLE);
+        status = fault == kFine ? JH_PLAN_OK : fault;
+    };
+    const int pieces = m.Dh / 8, shift = __builtin_ctz(pieces | 1024), per = m.Hk * pieces;
+    for (int j0 = 0; j0 < mine.z; j0 += 64) {
+        const int count64 = min(64, mine.z - j0);
+        const int mv = j0 + min(lane, count64 - 1);
+        int2 slots;
+        if constexpr (ONE) slots = make_int2(s.slot[s.kept[w.same + mv]], s.slot[w.same + mv]);
+        else slots = a.moves[(int64_t)r * a.most + mv];
+        if ((uint32_t)slots.x >= (uint32_t)m.n_slots || (uint32_t)slots.y >= (uint32_t)m.n_slots) slots = make_int2(0, -1);
+        // Y layers from l on, E rows from j on; waves stay whole (verdict)
+        auto move = [&](auto layers, auto rows, int l, int j) {
+            constexpr int Y = decltype(layers)::value, E = decltype(rows)::value;
+            for (int i0 = tid - lane; i0 < 2 * per; i0 += kWalkThreads) {
+                const int i = min(i0 + lane, 2 * per - 1), x = i < per ? i : i - per, head = x >> shift, f = 8 * (x & (pieces - 1));
+                auto where = [&](int y, int slot) {
+                    uint16_t *const k = m.k[l + y], *const v = m.v[l + y];
+                    const int row = slot & ((1 << m.page_shift) - 1);
+                    return reinterpret_cast<u32x4*>((i < per ? k : v) + (slot >> m.page_shift) * m.page_stride +
+                                                    (((int64_t)head << m.page_shift) + row) * m.Dh + f);
+                };
+                u32x4 v[Y * E];
+                int to[E];
 #pragma unroll
-        for (int e = 0; e < kPer; e++) {
-            if (n[e] == 0) continue;
-            const int end = min(n[e], w1 - start[e]);
-            for (; at[e] < end; at[e]++) {
-                const int i = at[e], x = start[e] + i - w0;
-                if (i == known[e] - 1) {
-                    cur[e] = i, want[e] = s_chosen[x];
-                } else if (s_parent[x] == cur[e] && s_token[x] == want[e]) {
-                    a.path[start[e] + kept[e]] = start[e] + i;
-                    cur[e] = i, want[e] = s_chosen[x];
-                    kept[e]++;
+                for (int e = 0; e < E; e++) {
+                    const int at = min(j + e, count64 - 1), from = __builtin_amdgcn_readlane(slots.x, at);
+                    to[e] = j + e < count64 ? __builtin_amdgcn_readlane(slots.y, at) : -1;
+#pragma unroll
+                    for (int y = 0; y < Y; y++) v[e * Y + y] = *where(y, from);
                 }
+                if (status < 0) verdict();
+                if (status != JH_PLAN_OK) return;
+#pragma unroll
+                for (int e = 0; e < E; e++)
+#pragma unroll
+                    for (int y = 0; y < Y; y++)
+                        if (to[e] >= 0 && i0 + lane < 2 * per) *where(y, to[e]) = v[e * Y + y];
             }
-        }
+        };
+        using One = std::integral_constant<int, 1>;
+        using Two = std::integral_constant<int, 2>;
+        using Four = std::integral_constant<int, 4>;
+        for (int l = (int)blockIdx.y * m.each; l < l1; l += 2)
+            for (int j = 0; j < count64; j += 4) {
+                if (l + 1 == l1) move(One{}, Four{}, l, j);
+                else if (count64 - j == 1) move(Two{}, One{}, l, j);
+                else move(Two{}, Four{}, l, j);
+            }
     }
-    // pages that come back: a request's lie behind those of the requests before it
-    int back[kPer], run = 0;
-#pragma unroll
-    for (int e = 0; e < kPer; e++) {
-        back[e] = status == JH_PLAN_OK ? blocks(kv[e]) - blocks(kv[e] - n[e] + kept[e]) : 0;
-        run += back[e];
-    }
-    const int upto = scan_int(run);
-    if (lane == 63) s_sum[wave] = upto;
-    bool outside = false;
-#pragma unroll
-    for (int e = 0; e < kPer; e++) {
-        const int r = tid * kPer + e;
-        const int b = blocks(kv[e] - n[e] + kept[e]);
-        for (int j = 0; j < back[e]; j++) outside |= (uint32_t)a.tables[(int64_t)r * a.max_blocks + b + j] >= (uint32_t)a.n_pages;
-    }
-    outside = __syncthreads_or(outside);
-    int total = 0, to = count + upto - run;
-    for (int w = 0; w < kWaves; w++) {
-        if (w < wave) to += s_sum[w];
-        total += s_sum[w];
-    }
-    if (status == JH_PLAN_OK && (outside || (int64_t)count + total > a.n_pages)) status = JH_PLAN_TABLE;
+    if (!books) return;
+    if (status < 0) verdict();
     const bool ok = status == JH_PLAN_OK;
-#pragma unroll
-    for (int e = 0; e < kPer; e++) {
-        const int r = tid * kPer + e;
-        if (r >= R) continue;
-        const int left = kv[e] - n[e] + kept[e];
-        a.kv_out[r] = ok ? left : kv[e];
-        a.accepted[r] = ok ? kept[e] : 0;
-        a.next_tokens[r] = ok ? want[e] : -1;
-        s_kept[r] = kept[e];
-        if (ok)
-            for (int j = 0; j < back[e]; j++) a.free_pages[to++] = a.tables[(int64_t)r * a.max_blocks + blocks(left) + j];
-    }
-    if (tid == 0) {
+    if (r == 0 && tid == 0) {
         *a.status = status;
         *a.count_out = ok ? count + total : count;
     }
+    // rows that nobody has
+    const int first = ok && R ? a.row_starts[0] : a.n_rows, last = ok && R ? a.row_starts[R] : a.n_rows;
+    if (r == 0)
+        for (int t = tid; t < first; t += kWalkThreads) a.path[t] = -1;
+    if (r == R - 1)
+        for (int t = last + tid; t < a.n_rows; t += kWalkThreads) a.path[t] = -1;
+    if (R == 0) return;
     if (!ok) {
-        for (int t = tid; t < a.n_rows; t += kCommitThreads) a.path[t] = -1;
+        if (tid == 0) a.kv_out[r] = a.kv_lens[r], a.accepted[r] = 0, a.next_tokens[r] = -1;
         return;
     }
-    __syncthreads();
-    // the known rows' places, and those that no row has
-    for (int t = tid; t < a.n_rows; t += kCommitThreads) {
-        int v = -1;
-        if (t >= first && t < last) {
-            int lo = 0;
-            for (int len = R; len > 1;) {  // the last request that starts at or before t
-                const int half = len >> 1;
-                if (s_start[lo + half] <= t) lo += half;
-                len -= half;
-            }
-            const int i = t - s_start[lo];
-            if (i < s_known[lo]) v = t;
-            else if (i < s_kept[lo]) continue;  // (written by the walk)
-        }
-        a.path[t] = v;
-    }
-}
-
-// ---- keys and values of the path moved together ------------------------------------------
-// A block to a request and layer, a thread to 16 bytes of a key's or value's heads. Row j
-// of the path moves to slot j of the request, j <= path[j]: kTogether rows are read
-// before they are written, and what later rows read lies behind what is written.
-constexpr int kTogether = 8;
-__global__ __launch_bounds__(256) void tree_move_kernel(TreeMoveArgs a) {
-    const int r = blockIdx.x, layer = blockIdx.y, lane = threadIdx.x & 63;
-    const int start = a.row_starts[r], kept = a.accepted[r];
-    if (kept <= 0 || start < 0 || start > a.n_rows - kept) return;
-    const int32_t* const path = a.path + start;
-    if (path[kept - 1] == start + kept - 1) return;  // all are where they belong
-    const int pieces = a.Dh / 8, per = a.Hk * pieces;
-    for (int j0 = 0; j0 < kept; j0 += 64) {
-        // the lanes look up 64 rows
-        const int j = j0 + lane, from = j < kept ? path[j] : -1;
-        int src = -1, dst = -1;
-        if (from >= 0 && from < a.n_rows && from != start + j) src = a.slots[from], dst = a.slots[start + j];
-        const uint64_t moves = __ballot((uint32_t)src < (uint32_t)a.n_slots && (uint32_t)dst < (uint32_t)a.n_slots);
-        for (int i = threadIdx.x; i < 2 * per; i += 256) {
-            uint16_t* const pool = i < per ? a.k[layer] : a.v[layer];
-            const int x = i < per ? i : i - per, head = x / pieces, f = 8 * (x % pieces);
-            auto where = [&](int slot) {
-                const int row = slot & ((1 << a.page_shift) - 1);
-                return reinterpret_cast<uint4*>(pool + (slot >> a.page_shift) * a.page_stride +
-                                                (((int64_t)head << a.page_shift) + row) * a.Dh + f);
-            };
-            uint64_t left = moves;
-            while (left) {
-                uint4 v[kTogether];
-                int to[kTogether];
-#pragma unroll
-                for (int e = 0; e < kTogether; e++) {
-                    to[e] = -1;
-                    if (!left) continue;
-                    const int l = __ffsll((unsigned long long)left) - 1;
-                    left &= left - 1;
-                    v[e] = *where(__builtin_amdgcn_readlane(src, l));
-                    to[e] = __builtin_amdgcn_readlane(dst, l);
-                }
-#pragma unroll
-                for (int e = 0; e < kTogether; e++)
-                    if (to[e] >= 0) *where(to[e]) = v[e];
-            }
-        }
+    const int b = (int)(((int64_t)mine.w + (1 << a.page_shift) - 1) >> a.page_shift);
+    for (int j = tid; j < mine.y; j += kWalkThreads) a.free_pages[count + before + j] = a.tables[(int64_t)r * a.max_blocks + b + j];
+    if (tid == 0) {
+        a.kv_out[r] = mine.w;
+        if constexpr (ONE) a.accepted[0] = w.kept, a.next_tokens[0] = w.next;
     }
 }
 
@@ -290,13 +323,35 @@ Status launch_tree_plan(const TreePlanArgs& a, hipStream_t st) {
     return Status::ok();
 }
 
-Status launch_tree_commit(const TreeCommitArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(tree_commit_kernel, dim3(1), dim3(kCommitThreads), 0, st, a);
-    return Status::ok();
+size_t tree_commit_workspace_bytes(const TreeCommitArgs& a) {
+    return ((size_t)a.n_req + 1) * sizeof(int4) + (size_t)a.n_req * std::min(a.tree_rows, a.n_rows) * sizeof(int2);
 }
 
-Status launch_tree_move(const TreeMoveArgs& a, hipStream_t st) {
-    hipLaunchKernelGGL(tree_move_kernel, dim3((unsigned)a.n_req, (unsigned)a.layers), dim3(256), 0, st, a);
+Status launch_tree_commit(TreeCommitArgs a, const TreeMoveArgs& move, void* const* k_pages, void* const* v_pages, int64_t layers,
+                          void* workspace, int num_cus, hipStream_t st) {
+    a.heads = static_cast<int4*>(workspace);
+    a.moves = reinterpret_cast<int2*>(a.heads + a.n_req + 1);
+    a.most = std::min(a.tree_rows, a.n_rows);
+    // (in place, a block that begins late would find the length that another has written)
+    auto apart = [](const void* x, const void* y) {
+        const ptrdiff_t d = static_cast<const char*>(x) - static_cast<const char*>(y);
+        return d >= (ptrdiff_t)sizeof(int32_t) || d <= -(ptrdiff_t)sizeof(int32_t);
+    };
+    const bool one = a.n_req == 1 && apart(a.kv_out, a.kv_lens) && apart(a.count_out, a.free_count);
+    if (a.n_req && !one) hipLaunchKernelGGL(tree_walk_kernel, dim3((unsigned)a.n_req), dim3(kWalkThreads), 0, st, a);
+    for (int64_t i = 0; i == 0 || i < layers; i += kMoveLayers) {
+        TreeMoveArgs m = move;
+        m.first = i == 0;
+        m.layers = (int)std::min<int64_t>(kMoveLayers, layers - i);
+        for (int j = 0; j < m.layers; j++)
+            m.k[j] = static_cast<uint16_t*>(k_pages[i + j]), m.v[j] = static_cast<uint16_t*>(v_pages[i + j]);
+        // about eight blocks to a CU: with fewer requests fewer layers to a block
+        const int parts = std::max(1, std::min(m.layers, 8 * num_cus / std::max(1, a.n_req)));
+        m.each = std::max(1, (m.layers + parts - 1) / parts);
+        const unsigned y = (unsigned)std::max(1, (m.layers + m.each - 1) / m.each);
+        hipLaunchKernelGGL(one ? tree_commit_kernel<true> : tree_commit_kernel<false>, dim3((unsigned)std::max(1, a.n_req), y),
+                           dim3(kWalkThreads), 0, st, a, m);
+    }
     return Status::ok();
 }
 

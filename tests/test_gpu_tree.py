@@ -541,6 +541,44 @@ def test_commit_refused_on_the_device(hip, what, status, in_place):
         hip.SetChecks(False)
 
 
+@pytest.mark.parametrize("n,page,words,layers,Hk,D,known", [
+    (32, 16, 1, 2, 1, 64, None), (33, 16, 1, 2, 1, 64, None), (64, 4, 2, 70, 2, 64, 3), (512, 1, 16, 1, 3, 128, 40), (511, 64, 16, 2, 2, 256, 500),
+    (130, 8, 5, 0, 1, 64, 1), (0, 16, 1, 2, 1, 64, None), (700, 16, 16, 1, 1, 64, 9)])
+@pytest.mark.parametrize("in_place", ["", "kv", "count"])
+def test_commit_single_request(hip, n, page, words, layers, Hk, D, known, in_place):
+    """A request by itself takes one launch where nothing is updated in place."""
+    c = Step(n, [n], page, words, layers, Hk, D, known=None if known is None else [known], agree=0.97, front=1, far=300)
+    c.up(hip)
+    if in_place == "kv":
+        c.out[0] = c.d["kv"]
+    if in_place == "count":
+        c.out[1] = c.d["count"]
+    step(f"jh_paged_tree_commit n={n} page={page} words={words} layers={layers} known={known} in_place={in_place!r}")
+    want = c.ref()
+    c.call(hip)
+    same(c.got(hip), want)
+
+
+@pytest.mark.parametrize("what,status", [("kv below the rows", 1), ("starts leave", 2), ("count past", 3), ("page outside", 4), ("no room", 4)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_commit_single_request_refused_on_the_device(hip, what, status, in_place):
+    c = Step(11, [30], 4, 1, 2, agree=0.6)
+    want = c.ref()
+    back = want[1] - c.count
+    assert back > 1 and (np.diff(want[3][want[3] >= 0]) > 1).any()
+    if what == "kv below the rows": c.kv[0] = 29
+    if what == "starts leave": c.starts[1] = c.T + 1
+    if what == "count past": c.count = c.n_pages + 1
+    if what == "page outside": c.tables[0, -(-int(c.kv[0]) // 4) - 1] = c.n_pages
+    if what == "no room": c.count = c.n_pages - back + 1
+    c.up(hip)
+    if in_place:
+        c.out[0], c.out[1] = c.d["kv"], c.d["count"]
+    step(f"jh_paged_tree_commit of one request refuses: {what}")
+    c.call(hip)
+    same(c.got(hip), (c.kv, c.count, np.zeros(1), np.full(c.T, -1), np.full(1, -1), status, c.free, c.pools))
+
+
 def test_commit_slots_outside(hip):
     """Rows whose slot is outside the pages are not moved, and none is written there."""
     c = Step(21, [25] * 6, 16, 1, 2, agree=1.0)
