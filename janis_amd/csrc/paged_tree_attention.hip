@@ -12,7 +12,17 @@
 // the requests and walks it: the end of one tile, whole ones, the beginning of another. A
 // tile that is cut leaves parts, which a launch that follows joins in their order (joined by
 // the part that arrives last, the largest tiles, of 128 rows in 30 parts, held one block for
-// 170 us, and the launch is 4 to 9). A cut near a tile's end is moved there.
+// 170 us, and the launch is 4 to 20). A cut near a tile's end is moved there.
+//
+// What bounds it, bf16, 32 heads on 8 of 128 (MI355X):
+//   16 tokens of 700 keys    15 us: round trips (lengths, the line, tables, keys, records), 11
+//     of them the parts and 4 the launch that joins
+//   63 of 30000              66 us: 58 the parts, 8 the join; MFMA, two thirds of it the second
+//     product made twice, at a clock that the power holds to 1.8 GHz
+//   64 requests of 20 to 60 over 100 to 8000 212 us: 185 the parts (413 TFLOP/s of the formula's
+//     operations in all, tiles that are not full not counted), 19 the join, records to memory
+//     and back. The clock is 1.8 GHz of 2.4, by power, and the matrix pipes busy half of it
+//   tiles of 32 rows alone   HBM: 64 requests of 8 tokens over 4000 keys 169 us, 6.2 TB/s
 #include "paged_attention.hpp"
 
 namespace jh {
@@ -28,8 +38,8 @@ struct TreeAttn {
     struct Split* split;  // of block b: the tile that begins there and goes on in the next; nullptr: keys stay whole
     float* part;      // records: [blocks] of the tiles that go on in a block, [blocks] of those that begin there
 };
-// Cost of a unit of 64 keys, by the tile's rows: with all blocks at work one took 2.7, 3.1, 3.8 and
-// 4.3 us for tiles of 32, 64, 96 and 128 rows (bf16, head_dim 128). And of a tile (its queries, its
+// Cost of a unit of 64 keys, by the tile's rows: with all blocks at work one takes 2.7, 3.1, 3.6 and
+// 4.0 us for tiles of 32, 64, 96 and 128 rows (bf16, head_dim 128). And of a tile (its queries, its
 // results): 4 to 8 us.
 __device__ __forceinline__ int cost_of(int rows) { return 4 + (rows + 31) / 32; }
 constexpr int kCostTile = 12;
@@ -41,9 +51,8 @@ constexpr double kLeastPiece = 12;
 constexpr int kLeastUnits = 2;
 
 struct Split {
-    int parts;        // 0: no such tile
-    Request q;
-    int row0, rows;
+    int4 at;  // parts (0: no such tile), first row, rows
+    int4 q;   // the request
 };
 struct Shape {
     int whole, rest;     // tiles of 128 rows, and rows behind them
@@ -552,13 +561,13 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void tree_attn_kernel(TreeA
     {
         const Line l = line_of(w);
         if (b >= l.cuts.pieces) {
-            if (w.split && hk == 0 && threadIdx.x == 0) w.split[b].parts = 0;
+            if (w.split && hk == 0 && threadIdx.x == 0) w.split[b].at.x = 0;
             return;
         }
         const Place at = place_of(w, l, l.cuts.at(b));
         const Place end = b + 1 < l.cuts.pieces ? place_of(w, l, l.cuts.at(b + 1)) : Place{w.a.n_req, 0, 0, 0.0, Request{0, 0, 0}};
         if (threadIdx.x == 0) s_walk = Walk{l.cuts, at, end};
-        if (w.split && hk == 0 && threadIdx.x == 0) w.split[b].parts = 0;
+        if (w.split && hk == 0 && threadIdx.x == 0) w.split[b].at.x = 0;
     }
     for (;;) {
         __syncthreads();
@@ -599,7 +608,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void tree_attn_kernel(TreeA
             const Shape s = shape_of(q, w.G);
             const Tile t = tile_of(s, uniform(at.tile));
             const Parts parts = parts_of(w, s_walk.cuts, uniform(at.unit) > 0 ? b : b + 1, at.begin + t.at, s.units, t.rows);
-            if (parts.first == b && threadIdx.x == 0) w.split[b] = Split{parts.count, q, t.row0, t.rows};
+            if (parts.first == b && threadIdx.x == 0) w.split[b] = Split{make_int4(parts.count, t.row0, t.rows, 0), make_int4(q.start, q.n, q.kv, 0)};
             __syncthreads();  // (all have read where the block is)
         }
         if (threadIdx.x == 0) s_walk.at.tile++, s_walk.at.unit = 0;
@@ -607,88 +616,143 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void tree_attn_kernel(TreeA
 }
 
 // The parts of a cut tile joined in their order. Block y: the y-th such tile. An item is 8 features
-// of 32 rows (in_record), 4 features of one row to a lane; a wave takes an item, or, where there are
-// more parts than it requests together, all four a quarter of the parts each.
+// of 32 rows (in_record), 4 features of one row to a lane. A wave requests kJoin records of items
+// together: 4 items of 2 parts, 2 of 4, one of more (64 requests of 20 to 60 tokens, some 500 tiles and 70 MB of
+// records: 19 us, with one item at a time 25); beyond kJoin parts all four waves take a quarter of an item's parts each.
 constexpr int kMergeWaves = 4, kJoin = 8;
 template <int DH>
 __global__ __launch_bounds__(64 * kMergeWaves) void tree_attn_merge_kernel(TreeAttn w) {
     __shared__ float s_sums[kMergeWaves][6][64];
     const PagedAttnArgs& a = w.a;
     const int hk = blockIdx.x, lane = threadIdx.x & 63, wave = (int)threadIdx.x / 64;
+    // (a lane looks at two pieces, 128 are requested together)
     int left = blockIdx.y, b = -1;
-    for (int b0 = 0; b0 < w.blocks && b < 0; b0 += 64) {
-        uint64_t cut = __ballot(b0 + lane < w.blocks && w.split[min(b0 + lane, w.blocks - 1)].parts > 0);
-        const int count = __popcll(cut);
-        if (left < count) {
+    struct {
+        int parts, row0, rows;
+        Request q;
+    } t;
+    for (int b0 = 0; b0 < w.blocks && b < 0; b0 += 128) {
+        Split mine[2];
+#pragma unroll
+        for (int i = 0; i < 2; i++) mine[i] = w.split[min(b0 + 64 * i + lane, w.blocks - 1)];
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            uint64_t cut = __ballot(b0 + 64 * i + lane < w.blocks && mine[i].at.x > 0);
+            const int count = __popcll(cut);
+            if (b >= 0) continue;
+            if (left >= count) {
+                left -= count;
+                continue;
+            }
             for (; left > 0; left--) cut &= cut - 1;
-            b = b0 + __ffsll((unsigned long long)cut) - 1;
-        } else {
-            left -= count;
+            const int l = __ffsll((unsigned long long)cut) - 1;
+            auto of = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            b = b0 + 64 * i + l;
+            t.parts = of(mine[i].at.x), t.row0 = of(mine[i].at.y), t.rows = of(mine[i].at.z);
+            t.q = Request{of(mine[i].q.x), of(mine[i].q.y), of(mine[i].q.z)};
         }
     }
     if (b < 0) return;
-    const Split t = w.split[b];
-    const bool shared = t.parts > kJoin;
-    const int items = (t.rows + 31) / 32 * (DH / 8), each = shared ? (t.parts + kMergeWaves - 1) / kMergeWaves : t.parts;
-    const int from = shared ? wave * each : 0, to = min(t.parts, from + each), step = shared ? 1 : kMergeWaves;
-    for (int item0 = blockIdx.z * step; item0 < items; item0 += gridDim.z * step) {
-        const int item = shared ? item0 : min(item0 + wave, items - 1);
-        const int x = item / (DH / 8) * 32 + (lane & 31), feature = item % (DH / 8) * 8 + (lane >> 5) * 4;
-        // (rows behind the last: what their places hold is not stored)
-        const float *const results = w.part + in_record<DH>(x, feature), *const ml = w.part + w.record * DH + 2 * x;
-        const bool sees = reach<true>(a, t.q, t.row0 + min(x, t.rows - 1), w.G) > 0;
-        float mx = ninf(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        auto join = [&](float2 u, float4 y) {
-            const float g = u.x == mx ? 1.0f : __builtin_amdgcn_exp2f(u.x - mx);
+    const int items = (t.rows + 31) / 32 * (DH / 8);
+    struct Sums {
+        float m, l, o[4];
+        __device__ __forceinline__ void to(float top) {
+            const float g = m == top ? 1.0f : __builtin_amdgcn_exp2f(m - top);
+            m = top, l *= g, o[0] *= g, o[1] *= g, o[2] *= g, o[3] *= g;
+        }
+        __device__ __forceinline__ void join(float2 u, float4 y) {
+            const float g = u.x == m ? 1.0f : __builtin_amdgcn_exp2f(u.x - m);
             l = fmaf(u.y, g, l);
             o[0] = fmaf(y.x, g, o[0]), o[1] = fmaf(y.y, g, o[1]);
             o[2] = fmaf(y.z, g, o[2]), o[3] = fmaf(y.w, g, o[3]);
+        }
+    };
+    auto row_of = [&](int item) { return item / (DH / 8) * 32 + (lane & 31); };
+    auto feature_of = [&](int item) { return item % (DH / 8) * 8 + (lane >> 5) * 4; };
+    auto store = [&](int item, const Sums& s, bool sees) {
+        const int x = row_of(item);
+        if (item >= items || x >= t.rows) return;
+        store_out4(a, out_at<DH>(a, t.q, t.row0 + x, hk, w.G) + feature_of(item), sees ? s.o[0] / s.l : 0.0f,
+                   sees ? s.o[1] / s.l : 0.0f, sees ? s.o[2] / s.l : 0.0f, sees ? s.o[3] / s.l : 0.0f);
+    };
+    auto sees_any = [&](int item) { return reach<true>(a, t.q, t.row0 + min(row_of(item), t.rows - 1), w.G) > 0; };
+    // parts `from` on of I items, J parts together (rows behind the last: what their places hold is not stored)
+    auto parts = [&](auto each, auto together, const int (&item)[decltype(each)::value], Sums (&s)[decltype(each)::value],
+                     bool (&sees)[decltype(each)::value], int from, int to) {
+        constexpr int I = decltype(each)::value, J = decltype(together)::value;
+#pragma unroll
+        for (int i = 0; i < I; i++) s[i] = Sums{ninf(), 0.0f, {0.0f, 0.0f, 0.0f, 0.0f}};
+        for (int s0 = from; s0 < to; s0 += J) {
+            float2 u[I * J];
+            float4 y[I * J];
+#pragma unroll
+            for (int j = 0; j < J; j++) {
+                const int part = min(s0 + j, to - 1);
+                const float* const rec = w.part + record_at(w, b + part, part == 0, hk);
+#pragma unroll
+                for (int i = 0; i < I; i++) {
+                    const int x = row_of(item[i]);
+                    u[I * j + i] = *reinterpret_cast<const float2*>(rec + w.record * DH + 2 * x);
+                    y[I * j + i] = *reinterpret_cast<const float4*>(rec + in_record<DH>(x, feature_of(item[i])));
+                }
+            }
+            if (s0 == from)
+#pragma unroll
+                for (int i = 0; i < I; i++) sees[i] = sees_any(item[i]);  // (the records are on their way)
+#pragma unroll
+            for (int i = 0; i < I; i++) {
+                float top = s[i].m;
+#pragma unroll
+                for (int j = 0; j < J; j++) top = fmaxf(top, u[I * j + i].x);
+                s[i].to(top);
+#pragma unroll
+                for (int j = 0; j < J; j++)
+                    if (s0 + j < to) s[i].join(u[I * j + i], y[I * j + i]);
+            }
+        }
+    };
+    if (t.parts <= kJoin) {
+        auto run = [&](auto each, auto together) {
+            constexpr int I = decltype(each)::value;
+            for (int item0 = (blockIdx.z * kMergeWaves + wave) * I; item0 < items; item0 += gridDim.z * kMergeWaves * I) {
+                int item[I];
+                bool sees[I];
+                Sums s[I];
+#pragma unroll
+                for (int i = 0; i < I; i++) item[i] = min(item0 + i, items - 1);
+                parts(each, together, item, s, sees, 0, t.parts);
+#pragma unroll
+                for (int i = 0; i < I; i++) store(item0 + i, s[i], sees[i]);
+            }
         };
-        for (int s0 = from; s0 < to; s0 += kJoin) {
-            float2 u[kJoin];
-            float4 y[kJoin];
-            float top = mx;
+        if (t.parts <= 2) run(std::integral_constant<int, 4>{}, std::integral_constant<int, 2>{});
+        else if (t.parts <= 4) run(std::integral_constant<int, 2>{}, std::integral_constant<int, 4>{});
+        else run(std::integral_constant<int, 1>{}, std::integral_constant<int, kJoin>{});
+        return;
+    }
+    const int each = (t.parts + kMergeWaves - 1) / kMergeWaves, from = min(t.parts, wave * each);
+    for (int item = blockIdx.z; item < items; item += gridDim.z) {
+        const int one[1] = {item};
+        bool sees[1] = {false};
+        Sums s[1];
+        parts(std::integral_constant<int, 1>{}, std::integral_constant<int, kJoin>{}, one, s, sees, from, min(t.parts, from + each));
+        __syncthreads();  // (the item before is read)
+        float* const mine = &s_sums[wave][0][lane];
+        mine[0] = s[0].m, mine[64] = s[0].l;
 #pragma unroll
-            for (int i = 0; i < kJoin; i++) {
-                const int part = min(s0 + i, to - 1);
-                const int64_t at = record_at(w, b + part, part == 0, hk);
-                u[i] = *reinterpret_cast<const float2*>(ml + at);
-                y[i] = *reinterpret_cast<const float4*>(results + at);
-            }
+        for (int e = 0; e < 4; e++) mine[64 * (2 + e)] = s[0].o[e];
+        __syncthreads();
+        if (wave > 0) continue;
+        float top = s[0].m;
 #pragma unroll
-            for (int i = 0; i < kJoin; i++) top = fmaxf(top, u[i].x);
-            const float g0 = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
-            l *= g0, o[0] *= g0, o[1] *= g0, o[2] *= g0, o[3] *= g0;
-            mx = top;
+        for (int v = 1; v < kMergeWaves; v++) top = fmaxf(top, s_sums[v][0][lane]);
+        s[0].to(top);
 #pragma unroll
-            for (int i = 0; i < kJoin; i++) {
-                if (s0 + i >= to) break;
-                join(u[i], y[i]);
-            }
+        for (int v = 1; v < kMergeWaves; v++) {
+            const float* const q = &s_sums[v][0][lane];
+            s[0].join(make_float2(q[0], q[64]), make_float4(q[128], q[192], q[256], q[320]));
         }
-        if (shared) {
-            __syncthreads();  // (the item before is read)
-            float* const mine = &s_sums[wave][0][lane];
-            mine[0] = mx, mine[64] = l;
-#pragma unroll
-            for (int e = 0; e < 4; e++) mine[64 * (2 + e)] = o[e];
-            __syncthreads();
-            if (wave > 0) continue;
-#pragma unroll
-            for (int v = 1; v < kMergeWaves; v++) mx = fmaxf(mx, s_sums[v][0][lane]);
-            const float m0 = s_sums[0][0][lane], g0 = m0 == mx ? 1.0f : __builtin_amdgcn_exp2f(m0 - mx);
-            l *= g0, o[0] *= g0, o[1] *= g0, o[2] *= g0, o[3] *= g0;
-#pragma unroll
-            for (int v = 1; v < kMergeWaves; v++) {
-                const float* const q = &s_sums[v][0][lane];
-                join(make_float2(q[0], q[64]), make_float4(q[128], q[192], q[256], q[320]));
-            }
-        } else if (item0 + wave >= items) {
-            continue;
-        }
-        if (x >= t.rows) continue;
-        store_out4(a, out_at<DH>(a, t.q, t.row0 + x, hk, w.G) + feature, sees ? o[0] / l : 0.0f, sees ? o[1] / l : 0.0f,
-                   sees ? o[2] / l : 0.0f, sees ? o[3] / l : 0.0f);
+        store(item, s[0], sees[0]);
     }
 }
 
