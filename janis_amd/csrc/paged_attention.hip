@@ -33,11 +33,11 @@
 //     non-temporal: 32 of 8000 take 189 us without. Short ones are chains of
 //     round trips (lengths, tables, keys, records): 1 token of 64 keys 6 us, of 700 9 to 10;
 //     with a launch of its own for the join 9 and 11 us.
-//   many rows: 2000 tokens of 8000 bf16 keys 328 to 348 us, by device: 660 to 700 TFLOP/s
+//   many rows: 2000 tokens of 8000 bf16 keys 326 to 348 us, by device: 660 to 705 TFLOP/s
 //     of the formula's operations, and, the second product being made twice (kTerms), 990
 //     to 1050 of the matrix cores', where a large bf16 product of the library reaches 1180
 //     to 1350. By counters the MFMA pipes are busy 52 % of the time at 1.8 GHz and VALU
-//     47 %. Built with 256 registers, 8 of them spilled. 513 tokens of 513 24 us, of which
+//     47 %. Built with 256 registers. 513 tokens of 513 24 us, of which
 //     4 are a merge launch that finds nothing to join: 136 blocks walk five steps of keys.
 #include "paged_attention.hpp"
 
