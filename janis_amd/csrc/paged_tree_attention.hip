@@ -772,14 +772,14 @@ Launch plan_launch(const PagedAttnArgs& a, int num_cus) {
     L.w.record = (int)(std::min<int64_t>(rows, kManyRows) + 31) / 32 * 32;
     L.w.size = (L.w.record * (a.Dh + 2) + 31) / 32 * 32;
     L.records = (size_t)2 * L.w.blocks * a.Hk * L.w.size * sizeof(float);
-    L.bytes = L.records + L.w.blocks * sizeof(Split);
+    L.bytes = L.w.blocks > 1 ? L.records + L.w.blocks * sizeof(Split) : 0;  // (a line in one piece: nothing is cut)
     const int64_t few = std::min<int64_t>((int64_t)a.max_new * G, rows);
     // tiles: a request's whole ones and one more; a cut divides one tile
     const int64_t tiles = std::min<int64_t>(a.n_req, a.n_rows) + rows / kManyRows;
     L.cut = (int)std::min<int64_t>(L.w.blocks - 1, tiles);
     // a block for every item (as the hint says), over about eight blocks to a CU
     const int64_t items = (std::min<int64_t>(std::max<int64_t>(few, 1), kManyRows) + 31) / 32 * (a.Dh / 8);
-    L.shares = (int)std::max<int64_t>(1, std::min(items, 8 * (int64_t)num_cus / std::max<int64_t>(1, L.cut * a.Hk)));
+    L.shares = (int)std::max<int64_t>(1, std::min(items, 8 * (int64_t)num_cus / std::max<int64_t>(1, (int64_t)L.cut * a.Hk)));
     return L;
 }
 
@@ -794,7 +794,7 @@ Status launch_paged_tree_attn(const PagedAttnArgs& a, void* workspace, size_t wo
     if (!a.whole && L.bytes > workspace_bytes)
         return Status::fail(JH_ERR_INVALID, "jh_paged_tree_attention: the workspace does not hold the parts");
     L.w.part = static_cast<float*>(workspace);
-    if (!a.whole) L.w.split = reinterpret_cast<Split*>(static_cast<char*>(workspace) + L.records);
+    if (!a.whole && L.bytes) L.w.split = reinterpret_cast<Split*>(static_cast<char*>(workspace) + L.records);
     const dim3 grid((unsigned)a.Hk, (unsigned)L.w.blocks);
     auto with = [&](auto dh) {
         constexpr int DH = decltype(dh)::value;

@@ -5,7 +5,7 @@ Bars of the attention are those of tests/test_gpu_paged.py, from the same formul
 import numpy as np
 import pytest
 
-from janis_amd import _lib
+from janis_amd import _lib, synth
 from janis_amd.engine import BF16, F16, F32, I32, U32, HipBackend, JanisHipError, PagedLayers
 from tests.conftest import Graph, put, step
 from tests.test_gpu_paged import HALF, Paged, append_ref, ints, refused, rounded, up
@@ -315,6 +315,82 @@ def test_attention_bad_pages_and_lengths(hip):
         hip.Sync()
 
 
+def test_attention_many_requests(hip):
+    """More requests than a wave has lanes, most without rows or with one."""
+    rng = np.random.default_rng(17)
+    n = np.where(rng.random(300) < 0.5, 0, rng.integers(1, 21, 300))
+    lens = [(int(x), int(x + rng.integers(0, 300) * (rng.random() < 0.8))) for x in n]
+    c = Trees(hip, lens, 8, 8, 64, 16, BF16, words=1, pad=2)
+    step(f"jh_paged_tree_attention R=300 rows={c.T}")
+    got = c.run(F32)
+    near(got, c.ref(F32, rng.integers(0, int(n.sum()), 200)))
+    assert np.array_equal(got, c.run(F32))
+
+
+def test_attention_more_heads_than_blocks(hip):
+    """A block to a kv head, which walks all tiles: nothing is cut, no workspace."""
+    lens = [(9, 100), (0, 5), (33, 200), (1, 1)]
+    c = Trees(hip, lens, 600, 600, 64, 16, F16, words=2)
+    step("jh_paged_tree_attention Hk=600")
+    near(c.run(F16), c.ref(F16))
+
+
+def test_attention_two_contexts_and_streams():
+    """Two contexts at once, each with its stream and workspace, on calls whose tiles are cut."""
+    import torch
+    bs, stream = [HipBackend(0), HipBackend(0)], torch.cuda.Stream()
+    bs[1].SetStream(stream.cuda_stream)
+    cs = [Trees(b, [(30, 5000), (5, 700)], 32, 8, 128, 16, BF16, seed=i) for i, b in enumerate(bs)]
+    want = [c.run(F32) for c in cs]
+    outs = [up(b, np.zeros((c.T, c.Hq, c.D)), F32) for b, c in zip(bs, cs)]
+    for b in bs:
+        b.Sync()
+    step("jh_paged_tree_attention of two contexts at once")
+    for _ in range(20):
+        for b, c, o in zip(bs, cs, outs):
+            b.PagedTreeAttention(c.Q, c.K, c.V, c.TAB, c.ST, c.KV, c.M, c.scale, maxNew=30, out=o)
+    for b, c, o, w in zip(bs, cs, outs, want):
+        assert np.array_equal(b.Floats(o), w)
+        near(w, c.ref(F32))
+        b.Close()
+
+
+def far_pool(hip, pool, far):
+    """[P, Hk, page, D] bf16 bits with pages `far` elements apart: the buffer, the tensor and its pages."""
+    P, Hk, page, D = pool.shape
+    raw = hip.empty(BF16, (P - 1) * far + Hk * page * D)
+    pages = [hip._view(raw, (Hk, page, D), (page * D, D, 1), i * far) for i in range(P)]
+    for view, bits in zip(pages, pool):
+        put(hip, view, bits)
+    return raw, hip._view(raw, pool.shape, (far, page * D, D, 1)), pages
+
+
+def test_far_pages(hip):
+    """Pages that lie past 2^32 bytes: attention over them, and kept rows moved between them."""
+    far = (1 << 31) + 8
+    c = Trees(hip, [(12, 20)], 2, 1, 64, 8, BF16, words=1, extra_blocks=0)
+    m = Step(1, [12], 8, 1, 1, 1, 64, agree=1.0, far=9)
+    want = m.ref()
+    assert (np.diff(want[3][want[3] >= 0]) > 1).any()
+    try:
+        pools = [far_pool(hip, x, far) for x in (synth.f32_to_bf16_bits(c.pools[0]), synth.f32_to_bf16_bits(c.pools[1]), *m.pools[:, 0])]
+    except JanisHipError:
+        pytest.skip("no room")
+    step("jh_paged_tree_attention far pages")
+    near(c.run(F32, k=pools[0][1], v=pools[1][1]), c.ref(F32))
+    m.up(hip)
+    m.lay = PagedLayers([pools[2][1]], [pools[3][1]])
+    step("jh_paged_tree_commit far pages")
+    m.call(hip)
+    got = list(m.got(hip))
+    got[7] = np.array([[[np.frombuffer(hip.Bytes(hip._c(v)), np.uint16).reshape(v.shape) for v in pool[2]]] for pool in pools[2:]])
+    same(got, want)
+    hip.Sync()
+    m.lay = None
+    for raw, *_ in pools:
+        raw.free()
+
+
 def test_attention_graphs(hip):
     """Captured without a workspace (keys stay whole) and with one, replayed between eager
     calls of another size: each time the eager bits, or the formula's."""
@@ -577,6 +653,39 @@ def test_commit_single_request_refused_on_the_device(hip, what, status, in_place
     step(f"jh_paged_tree_commit of one request refuses: {what}")
     c.call(hip)
     same(c.got(hip), (c.kv, c.count, np.zeros(1), np.full(c.T, -1), np.full(1, -1), status, c.free, c.pools))
+
+
+def test_commit_captured_first():
+    """The workspace cannot grow in a capture: the same call goes before it. Replays find
+    other lengths, paths and pages."""
+    b = HipBackend(0)
+    c = Step(8, [20] * 40, 16, 4, 2, agree=0.9)
+    c.up(b)
+    step("jh_paged_tree_commit captured first")
+
+    def refused():
+        with pytest.raises(JanisHipError, match="make the same call once before"):
+            c.call(b)
+    Graph(b, refused).close()
+    c.call(b)
+    same(c.got(b), c.ref())
+    graph = Graph(b, lambda: c.call(b))
+    for seed in (9, 10, 11):  # other trees over the same slots
+        m = Step(seed, [20] * 40, 16, 4, 2, agree=0.9)
+        c.parents, c.tokens, c.chosen = m.parents, m.tokens, m.chosen
+        for name in ("parents", "tokens", "chosen", "free"):
+            put(b, c.d[name], getattr(c, name))
+        for ts, pool in zip((c.k, c.v), c.pools):
+            for t, bits in zip(ts, pool):
+                put(b, t, bits)
+        graph.replay()
+        same(c.got(b), c.ref())
+        other = Step(1, [3] * 5, 16, 1, 1)  # (another call's heads and moves in the same workspace)
+        other.up(b)
+        other.call(b)
+        same(other.got(b), other.ref())
+    graph.close()
+    b.Close()
 
 
 def test_commit_slots_outside(hip):
