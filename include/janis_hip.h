@@ -93,8 +93,8 @@ JH_API int jh_device_info(jh_ctx *ctx, char *name, size_t name_len, int *compute
 /* Enqueue on a caller-owned hipStream_t instead of the context's own stream
  * (NULL restores the context's stream). The caller keeps the stream alive.
  * The exchanges inside one launch (the attention merges of
- * jh_attention_decode, jh_qkv_attention_decode and jh_paged_attention, the split-K sums of
- * jh_quant_matmul's prefill product) need workgroups dealt to the 8 XCDs
+ * jh_attention_decode, jh_qkv_attention_decode and jh_paged_attention, the parts of rows in
+ * jh_token_logprobs, the split-K sums of jh_quant_matmul's prefill product) need workgroups dealt to the 8 XCDs
  * round-robin, which jh_create checks; a stream whose CU mask leaves any CU out
  * (hipExtStreamCreateWithCUMask) runs them as separate launches instead. */
 JH_API int jh_set_stream(jh_ctx *ctx, void *hip_stream);
@@ -120,11 +120,11 @@ JH_API void *jh_get_stream(const jh_ctx *ctx);
 
 /* Read-back checks, the equivalent of janis's JANIS_GGML_CHECK
  * (ggml/ggml.go:622-677), off by default. flags is a combination of:
- *   JH_CHECK_INDICES  jh_gather_quant_matmul, jh_moe_swiglu, jh_take_rows and the
- *                     operators of the paged cache
+ *   JH_CHECK_INDICES  jh_gather_quant_matmul, jh_moe_swiglu, jh_take_rows,
+ *                     jh_token_logprobs and the operators of the paged cache
  *                     copy their indices to the host and reject an out-of-range
- *                     one with JH_ERR_INVALID before launching (jh_paged_plan after
- *                     it, by its status). When off, an
+ *                     one with JH_ERR_INVALID before launching (jh_paged_plan and
+ *                     jh_paged_tree_commit after it, by their status). When off, an
  *                     out-of-range expert index yields a row of NaN (a row id,
  *                     a row of zeros) and no memory outside the table is read.
  *   JH_CHECK_VALUES   after each operator with a float result (the quantized
@@ -777,10 +777,14 @@ JH_API int jh_paged_tree_plan(jh_ctx *ctx, const int32_t *parents, const int32_t
  * sees no key (an empty mask and L <= n) is zeros. Requests of more than 32 *
  * mask_words new tokens are causal, as in jh_paged_attention.
  *   tree_mask  [n_rows, mask_words]
- * Everything else is as there: types, sizes, strides, precision, the workspace, splits
- * and their joining, max_new (a hint), rows without a request, checks. A row is NaN if
- * a page of its request that holds a key up to the last one that it sees lies outside
- * the pool. */
+ * Types, sizes, strides, precision, rows without a request and checks are as there. The work
+ * is cut into as many pieces as blocks are resident, wherever that divides a tile's keys,
+ * and the parts, which lie in the context's workspace, are joined by a second launch in a
+ * fixed order: the same call gives the same bits. Where the workspace cannot grow (a
+ * capture, no memory) keys stay whole, which is slower and sums in another order. max_new
+ * is a hint that sizes the second launch: a wrong one costs a few microseconds. A row is
+ * NaN if a page of its request that holds a key up to the last one that it sees lies
+ * outside the pool. */
 JH_API int jh_paged_tree_attention(jh_ctx *ctx, const void *q, int64_t q_stride, const void *k_pages,
                                    const void *v_pages, jh_dtype page_dtype, int64_t n_pages,
                                    int64_t page_size, int64_t page_stride, const int32_t *block_tables,
@@ -791,9 +795,10 @@ JH_API int jh_paged_tree_attention(jh_ctx *ctx, const void *q, int64_t q_stride,
 
 /* The path that the large model agrees with, request by request, in one launch to find
  * it and one for every 64 layers (for a single request that is not updated in place
- * without the first). What the first finds lies in the context's workspace. The first known[r] rows of a request
- * (held to 1 .. n; 1 where known is NULL) are tokens that are kept whatever the model
- * says, a chain whose parents are not looked at: the last token sampled, or a prompt's
+ * without the first). What the first finds lies in the context's workspace, 16 bytes a
+ * request and 8 for each row that a tree may have; it cannot grow in a capture, so make the
+ * call once before. The first known[r] rows of a request (held to 1 .. n; 1 where known
+ * is NULL) are tokens that are kept whatever the model says, a chain whose parents are not looked at: the last token sampled, or a prompt's
  * end. From the last of them on, the row whose parent is the one before it and whose
  * token is the model's choice there is kept too (of several the first), until there is
  * none. A run of more than 32 * mask_words rows is kept whole.
