@@ -166,15 +166,84 @@ __device__ __forceinline__ Work find_work(const Attn& w, int index) {
 
 constexpr auto no_mask = [](int) { return 0u; };
 
-// The rows of one tile of one kv head whose keys were split.
+// ---- joining the parts -----------------------------------------------------------------
+// Rows of one tile of one kv head whose keys were split, `first`, first + stride, ...
+// times the rows at once: groups of DH / 4 lanes, 4 features each, one to a row for every
+// 8 parts (all requested together); a row's groups meet in LDS in their order. L2: the
+// records were stored by this launch on this XCD (device-coherent loads: past the CU's L1).
+constexpr int kJoinBatch = 8;
 template <int DH, int NT, bool L2>
 __device__ __forceinline__ void join_rows(const Attn& w, const Work& k, int hk, int tile, int parts, int first, int stride,
                                           float4* s_o, float2* s_ml) {
-    const int tr = k.few ? kFewRows : kManyRows;
-    const int64_t step = (int64_t)w.a.Hk * w.size;
-    const float* const rec = w.part + ((int64_t)(k.slot + tile * k.splits) * w.a.Hk + hk) * w.size;
-    join_parts<DH, NT, L2, false>(w.a, k.q, w.G, hk, tile * tr, min(tr, k.q.n * w.G - tile * tr), parts, rec, w.record,
-                                  [&](int i) { return i * step; }, first, stride, s_o, s_ml);
+    constexpr int kLanes = DH / 4, kGroups = NT / kLanes, kBatch = kJoinBatch;
+    const PagedAttnArgs& a = w.a;
+    const int G = w.G, rows = k.q.n * G, tr = k.few ? kFewRows : kManyRows;
+    const int64_t step = (int64_t)a.Hk * w.size;
+    const float* const rec = w.part + ((int64_t)(k.slot + tile * k.splits) * a.Hk + hk) * w.size;
+    const auto rsrc = make_rsrc(rec, 0x7FFFFFFFu);  // (L2: the launch keeps the records below 2^31 bytes)
+    const int f = threadIdx.x % kLanes, group = threadIdx.x / kLanes, count = min(tr, rows - tile * tr);
+    // groups to a row: for its parts, as long as the block's rows find room beside each other
+    const int here = (count + stride - 1) / stride;
+    int each = 1;
+    while (each * kBatch < parts && 2 * each * here <= kGroups) each *= 2;
+    const int sub = group % each, at_once = kGroups / each;
+    for (int x0 = first * at_once; x0 < count; x0 += stride * at_once) {
+        const int x = min(x0 + group / each, count - 1);
+        // (a part without keys of the row: a maximum of -inf, a sum of 0)
+        float mx = ninf(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int s0 = sub; s0 < parts; s0 += each * kBatch) {
+            float2 u[kBatch];
+            float4 y[kBatch];
+            float top = mx;
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) {
+                const int64_t at = min(s0 + i * each, parts - 1) * step;
+                if constexpr (L2) {
+                    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+                    u[i] = __builtin_bit_cast(float2, (u32x2_t)__builtin_amdgcn_raw_buffer_load_b64(
+                                                          rsrc, (uint32_t)(at + w.record * DH + 2 * x) * 4, 0, kAuxSc1));
+                    y[i] = __builtin_bit_cast(float4, (u32x4_t)__builtin_amdgcn_raw_buffer_load_b128(
+                                                          rsrc, (uint32_t)(at + x * DH + 4 * f) * 4, 0, kAuxSc1));
+                } else {
+                    u[i] = *reinterpret_cast<const float2*>(rec + at + (int64_t)w.record * DH + 2 * x);
+                    y[i] = *reinterpret_cast<const float4*>(rec + at + (int64_t)x * DH + 4 * f);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) top = fmaxf(top, s0 + i * each < parts ? u[i].x : top);
+            const float g0 = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
+            l *= g0, o[0] *= g0, o[1] *= g0, o[2] *= g0, o[3] *= g0;
+            mx = top;
+#pragma unroll
+            for (int i = 0; i < kBatch; i++) {
+                if (s0 + i * each >= parts) break;
+                const float g = u[i].x == mx ? 1.0f : __builtin_amdgcn_exp2f(u[i].x - mx);
+                l = fmaf(u[i].y, g, l);
+                o[0] = fmaf(y[i].x, g, o[0]), o[1] = fmaf(y[i].y, g, o[1]);
+                o[2] = fmaf(y[i].z, g, o[2]), o[3] = fmaf(y[i].w, g, o[3]);
+            }
+        }
+        if (each > 1) {
+            __syncthreads();  // (the round before has read)
+            s_o[group * kLanes + f] = make_float4(o[0], o[1], o[2], o[3]);
+            if (f == 0) s_ml[group] = make_float2(mx, l);
+            __syncthreads();
+        }
+        if (sub != 0 || x0 + group / each >= count) continue;
+        for (int g = 1; g < each; g++) mx = fmaxf(mx, s_ml[group + g].x);
+        if (each > 1) l = o[0] = o[1] = o[2] = o[3] = 0.0f;
+        for (int g = 0; each > 1 && g < each; g++) {
+            const float2 u = s_ml[group + g];
+            const float4 y = s_o[(group + g) * kLanes + f];
+            const float h = u.x == mx ? 1.0f : __builtin_amdgcn_exp2f(u.x - mx);
+            l = fmaf(u.y, h, l);
+            o[0] = fmaf(y.x, h, o[0]), o[1] = fmaf(y.y, h, o[1]), o[2] = fmaf(y.z, h, o[2]), o[3] = fmaf(y.w, h, o[3]);
+        }
+        const int row = tile * tr + x;
+        const bool sees = seen(k.q, row, G) > 0;
+        store_out4(a, out_at<DH>(a, k.q, row, hk, G) + 4 * f, sees ? o[0] / l : 0.0f, sees ? o[1] / l : 0.0f,
+                   sees ? o[2] / l : 0.0f, sees ? o[3] / l : 0.0f);
+    }
 }
 
 // ---- few rows ------------------------------------------------------------------------

@@ -1,6 +1,6 @@
 // Parts of attention over a paged cache that its kernels share (paged_attention.hip,
 // paged_tree_attention.hip): loads into LDS, the two products, the online softmax, a row
-// computed again, the joining of split keys' parts.
+// computed again.
 #pragma once
 
 #include "jh_common.hpp"
@@ -144,34 +144,6 @@ __device__ __forceinline__ int seen(const Request& q, int row, int G) { return m
 // With TREE the new tokens of a request see each other by the bits of a mask (those of a
 // run longer than the mask's bits up to their own, as above): key kv - n + b by bit b.
 __device__ __forceinline__ bool is_tree(const PagedAttnArgs& a, const Request& q) { return q.n <= 32 * a.mask_words; }
-// Keys up to the last one that the row sees.
-template <bool TREE>
-__device__ __forceinline__ int reach(const PagedAttnArgs& a, const Request& q, int row, int G) {
-    if constexpr (TREE)
-        if (is_tree(a, q)) {
-            const uint32_t* const m = a.mask + (int64_t)(q.start + row / G) * a.mask_words;
-            int top = 0;
-            for (int w = (q.n - 1) / 32; w >= 0 && top == 0; w--) {
-                const uint32_t bits = q.n - 32 * w < 32 ? m[w] & ((1u << (q.n - 32 * w)) - 1) : m[w];
-                if (bits) top = 32 * w + 32 - __clz((int)bits);
-            }
-            return max(0, q.kv - q.n + top);
-        }
-    return seen(q, row, G);
-}
-// The same over rows up to `last` of a request, where their first `all` is what all see.
-template <bool TREE>
-__device__ __forceinline__ int reach_of_tile(const PagedAttnArgs& a, const Request& q, int last, int G) {
-    if constexpr (TREE)
-        if (is_tree(a, q)) return q.kv;
-    return seen(q, last, G);
-}
-template <bool TREE>
-__device__ __forceinline__ int seen_by_all(const PagedAttnArgs& a, const Request& q, int first, int G) {
-    if constexpr (TREE)
-        if (is_tree(a, q)) return max(0, q.kv - q.n);
-    return seen(q, first, G);
-}
 // Of the 32 keys from k0 on those that the row sees, as bits; `lim`: its reach.
 __device__ __forceinline__ uint32_t sees32(const PagedAttnArgs& a, const Request& q, int row, int G, int k0, int lim) {
     uint32_t bits = 0xFFFFFFFFu;
@@ -496,85 +468,6 @@ __device__ __forceinline__ int wave_min_int(int v) {
 #pragma unroll
     for (int d = 1; d < 64; d <<= 1) v = min(v, __shfl_xor(v, d, 64));
     return v;
-}
-
-// ---- joining the parts -----------------------------------------------------------------
-// Rows row0 .. row0 + count - 1 of a request and kv head whose keys were split, `first`,
-// first + stride, ... times the rows at once: groups of DH / 4 lanes, 4 features each, one
-// to a row for every 8 parts (all requested together); a row's groups meet in LDS in their
-// order. Part i lies at(i) floats from rec: [record][DH] results, then [record][2] maximum and
-// sum. L2: the records were stored by this launch on this XCD (device-coherent loads: past the
-// CU's L1; all lie within 2^31 bytes of rec).
-constexpr int kJoinBatch = 8;
-template <int DH, int NT, bool L2, bool TREE, class At>
-__device__ __forceinline__ void join_parts(const PagedAttnArgs& a, const Request& q, int G, int hk, int row0, int count, int parts,
-                                           const float* rec, int record, At part_at, int first, int stride, float4* s_o,
-                                           float2* s_ml) {
-    constexpr int kLanes = DH / 4, kGroups = NT / kLanes, kBatch = kJoinBatch;
-    const auto rsrc = make_rsrc(rec, 0x7FFFFFFFu);
-    const int f = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
-    // groups to a row: for its parts, as long as the block's rows find room beside each other
-    const int here = (count + stride - 1) / stride;
-    int each = 1;
-    while (each * kBatch < parts && 2 * each * here <= kGroups) each *= 2;
-    const int sub = group % each, at_once = kGroups / each;
-    for (int x0 = first * at_once; x0 < count; x0 += stride * at_once) {
-        const int x = min(x0 + group / each, count - 1);
-        // (a part without keys of the row: a maximum of -inf, a sum of 0)
-        float mx = ninf(), l = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int s0 = sub; s0 < parts; s0 += each * kBatch) {
-            float2 u[kBatch];
-            float4 y[kBatch];
-            float top = mx;
-#pragma unroll
-            for (int i = 0; i < kBatch; i++) {
-                const int64_t at = part_at(min(s0 + i * each, parts - 1));
-                if constexpr (L2) {
-                    typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
-                    u[i] = __builtin_bit_cast(float2, (u32x2_t)__builtin_amdgcn_raw_buffer_load_b64(
-                                                          rsrc, (uint32_t)(at + record * DH + 2 * x) * 4, 0, kAuxSc1));
-                    y[i] = __builtin_bit_cast(float4, (u32x4_t)__builtin_amdgcn_raw_buffer_load_b128(
-                                                          rsrc, (uint32_t)(at + x * DH + 4 * f) * 4, 0, kAuxSc1));
-                } else {
-                    u[i] = *reinterpret_cast<const float2*>(rec + at + (int64_t)record * DH + 2 * x);
-                    y[i] = *reinterpret_cast<const float4*>(rec + at + (int64_t)x * DH + 4 * f);
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < kBatch; i++) top = fmaxf(top, s0 + i * each < parts ? u[i].x : top);
-            const float g0 = mx == top ? 1.0f : __builtin_amdgcn_exp2f(mx - top);
-            l *= g0, o[0] *= g0, o[1] *= g0, o[2] *= g0, o[3] *= g0;
-            mx = top;
-#pragma unroll
-            for (int i = 0; i < kBatch; i++) {
-                if (s0 + i * each >= parts) break;
-                const float g = u[i].x == mx ? 1.0f : __builtin_amdgcn_exp2f(u[i].x - mx);
-                l = fmaf(u[i].y, g, l);
-                o[0] = fmaf(y[i].x, g, o[0]), o[1] = fmaf(y[i].y, g, o[1]);
-                o[2] = fmaf(y[i].z, g, o[2]), o[3] = fmaf(y[i].w, g, o[3]);
-            }
-        }
-        if (each > 1) {
-            __syncthreads();  // (the round before has read)
-            s_o[group * kLanes + f] = make_float4(o[0], o[1], o[2], o[3]);
-            if (f == 0) s_ml[group] = make_float2(mx, l);
-            __syncthreads();
-        }
-        if (sub != 0 || x0 + group / each >= count) continue;
-        for (int g = 1; g < each; g++) mx = fmaxf(mx, s_ml[group + g].x);
-        if (each > 1) l = o[0] = o[1] = o[2] = o[3] = 0.0f;
-        for (int g = 0; each > 1 && g < each; g++) {
-            const float2 u = s_ml[group + g];
-            const float4 y = s_o[(group + g) * kLanes + f];
-            const float h = u.x == mx ? 1.0f : __builtin_amdgcn_exp2f(u.x - mx);
-            l = fmaf(u.y, h, l);
-            o[0] = fmaf(y.x, h, o[0]), o[1] = fmaf(y.y, h, o[1]), o[2] = fmaf(y.z, h, o[2]), o[3] = fmaf(y.w, h, o[3]);
-        }
-        const int row = row0 + x;
-        const bool sees = reach<TREE>(a, q, row, G) > 0;
-        store_out4(a, out_at<DH>(a, q, row, hk, G) + 4 * f, sees ? o[0] / l : 0.0f, sees ? o[1] / l : 0.0f,
-                   sees ? o[2] / l : 0.0f, sees ? o[3] / l : 0.0f);
-    }
 }
 
 }  // namespace

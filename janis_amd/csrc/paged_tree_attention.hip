@@ -50,6 +50,25 @@ constexpr double kLeastPiece = 12;
 // tokens over 500 to 5000 keys took 60, 58 and 63 us with 1, 2 and 4.
 constexpr int kLeastUnits = 2;
 
+// Keys up to the last one that the row sees.
+__device__ __forceinline__ int reach(const PagedAttnArgs& a, const Request& q, int row, int G) {
+    if (!is_tree(a, q)) return seen(q, row, G);
+    const uint32_t* const m = a.mask + (int64_t)(q.start + row / G) * a.mask_words;
+    int top = 0;
+    for (int w = (q.n - 1) / 32; w >= 0 && top == 0; w--) {
+        const uint32_t bits = q.n - 32 * w < 32 ? m[w] & ((1u << (q.n - 32 * w)) - 1) : m[w];
+        if (bits) top = 32 * w + 32 - __clz((int)bits);
+    }
+    return max(0, q.kv - q.n + top);
+}
+// Of the rows up to `last`, and what all rows from `first` on see.
+__device__ __forceinline__ int reach_of_tile(const PagedAttnArgs& a, const Request& q, int last, int G) {
+    return is_tree(a, q) ? q.kv : seen(q, last, G);
+}
+__device__ __forceinline__ int seen_by_all(const PagedAttnArgs& a, const Request& q, int first, int G) {
+    return is_tree(a, q) ? max(0, q.kv - q.n) : seen(q, first, G);
+}
+
 struct Split {
     int4 at;  // parts (0: no such tile), first row, rows
     int4 q;   // the request
@@ -199,7 +218,7 @@ __device__ __forceinline__ void rows32(const TreeAttn& w, const Segment& g, int 
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int w0 = g.row0, n_rows = g.rows, kb = g.kb, ke = g.ke;
     const int row = w0 + min(c32, n_rows - 1);
-    const int lim = min(ke, reach<true>(a, q, row, G)), lim_lo = min(ke, seen_by_all<true>(a, q, w0, G));
+    const int lim = min(ke, reach(a, q, row, G)), lim_lo = min(ke, seen_by_all(a, q, w0, G));
     if (tid < n_rows) s_lim[tid] = lim;
     auto sees_from = [&](int k) { return sees32(a, q, row, G, k, lim); };
     uint4 qf[DH / 16];
@@ -404,8 +423,8 @@ __device__ __forceinline__ void rows_shared(const TreeAttn& w, const Segment& g,
     load(Vals{}, 0);
     load(Keys{}, 1);
     // (the first keys and values are on their way)
-    const int lim = min(ke, reach<true>(a, q, row, G)), lim_lo = min(ke, seen_by_all<true>(a, q, min(w0, last - 1), G));
-    const int lim_hi = w0 < last ? min(ke, reach_of_tile<true>(a, q, min(w0 + 31, last - 1), G)) : 0;
+    const int lim = min(ke, reach(a, q, row, G)), lim_lo = min(ke, seen_by_all(a, q, min(w0, last - 1), G));
+    const int lim_hi = w0 < last ? min(ke, reach_of_tile(a, q, min(w0 + 31, last - 1), G)) : 0;
     auto sees_from = [&](int k) { return sees32(a, q, row, G, k, lim); };
     uint4 qf[DH / 16];
     load_q<DH>(a, q, row, hk, G, qf, lane);
@@ -482,7 +501,7 @@ __device__ __forceinline__ void rows_shared(const TreeAttn& w, const Segment& g,
         for (int x = 0; x < min(32, last - w0); x++) {
             if (!((again >> x) & 1u)) continue;
             float m1, l1, o1[DH / 64];
-            const int rw = w0 + x, sees = min(ke, reach<true>(a, q, rw, G)), y = 32 * wave + x;
+            const int rw = w0 + x, sees = min(ke, reach(a, q, rw, G)), y = 32 * wave + x;
             row_again<DH, F16, true>(a, q, g.r, hk, hk * G + rw % G, q.start + rw / G, kb, sees, m1, l1, o1, lane);
             if (sees > bad_all) l1 = __builtin_nanf("");
             if (g.rec && lane == 0) *reinterpret_cast<float2*>(rec_ml + 2 * y) = make_float2(m1, l1);
@@ -593,7 +612,7 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void tree_attn_kernel(TreeA
             Segment g;
             g.q = q, g.r = p.r, g.row0 = t.row0, g.rows = t.rows;
             g.kb = p.unit * kUnit;
-            g.ke = uniform(min(reach_of_tile<true>(w.a, q, t.row0 + t.rows - 1, w.G), to * kUnit));
+            g.ke = uniform(min(reach_of_tile(w.a, q, t.row0 + t.rows - 1, w.G), to * kUnit));
             g.rec = all ? nullptr : w.part + record_at(w, b, p.unit == 0, hk);
             int tid = threadIdx.x;
             asm volatile("" : "+v"(tid));  // (what a tile makes of it is not kept for the next: registers are short)
@@ -675,7 +694,7 @@ __global__ __launch_bounds__(64 * kMergeWaves) void tree_attn_merge_kernel(TreeA
         store_out4(a, out_at<DH>(a, t.q, t.row0 + x, hk, w.G) + feature_of(item), sees ? s.o[0] / s.l : 0.0f,
                    sees ? s.o[1] / s.l : 0.0f, sees ? s.o[2] / s.l : 0.0f, sees ? s.o[3] / s.l : 0.0f);
     };
-    auto sees_any = [&](int item) { return reach<true>(a, t.q, t.row0 + min(row_of(item), t.rows - 1), w.G) > 0; };
+    auto sees_any = [&](int item) { return reach(a, t.q, t.row0 + min(row_of(item), t.rows - 1), w.G) > 0; };
     // parts `from` on of I items, J parts together (rows behind the last: what their places hold is not stored)
     auto parts = [&](auto each, auto together, const int (&item)[decltype(each)::value], Sums (&s)[decltype(each)::value],
                      bool (&sees)[decltype(each)::value], int from, int to) {
