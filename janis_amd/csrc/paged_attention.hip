@@ -33,7 +33,7 @@
 //     non-temporal: 32 of 8000 take 189 us without. Short ones are chains of
 //     round trips (lengths, tables, keys, records): 1 token of 64 keys 6 us, of 700 9 to 10;
 //     with a launch of its own for the join 9 and 11 us.
-//   many rows: 2000 tokens of 8000 bf16 keys 326 to 348 us, by device: 660 to 705 TFLOP/s
+//   many rows: 2000 tokens of 8000 bf16 keys 323 to 348 us, by device: 660 to 710 TFLOP/s
 //     of the formula's operations, and, the second product being made twice (kTerms), 990
 //     to 1050 of the matrix cores', where a large bf16 product of the library reaches 1180
 //     to 1350. By counters the MFMA pipes are busy 52 % of the time at 1.8 GHz and VALU
@@ -518,8 +518,25 @@ __device__ __forceinline__ void many_rows(const Attn& w, const Work& k, int hk, 
         if (t >= n_tiles || k0 >= lim_hi) return;
         const uint8_t *const kt = lds + ((t + 1) & 1) * 2 * kTile, *const vt = lds + ((t & 1) * 2 + 1) * kTile;
         const float neg = mask_and_move<DH, F16, false, 2>(s, k0, lim, k0 + 64 > lim_lo, no_mask, c, m, l, o);
-        scores_and_weigh<DH, F16, 2>(kt, qf, next, s, c, neg, l, lane);
-        values<DH, F16, 2>(vt, s, o, lane);
+        // In the source's order where four waves walk 128 rows of a head_dim of 128 or more (2000 tokens of
+        // 8000: 323 us, 339 in the compiler's); not with eight waves (22 tokens and two prompts' pieces 39.8
+        // and 40.9) or a head_dim of 64 (2000 of 8000 208 and 209).
+        if constexpr (NW == 4 && DH >= 128) {
+            scores_and_weigh<DH, F16, 2>(kt, qf, next, s, c, neg, l, lane);
+            values<DH, F16, 2>(vt, s, o, lane);
+        } else {
+            next[0] = scores32<DH, F16>(kt, qf);
+            next[1] = scores32<DH, F16>(kt + 32 * 2 * DH, qf);
+            weigh<2>(s, c, neg, l);
+#pragma unroll
+            for (int kk = 0; kk < 4; kk++) {
+                uint32_t p[4][kTerms];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    split_pair<F16, kTerms>(s[kk >> 1][8 * (kk & 1) + 2 * e], s[kk >> 1][8 * (kk & 1) + 2 * e + 1], p[e]);
+                values16<DH, F16>(vt + kk * 16 * 2 * DH, p, o);
+            }
+        }
     };
     floatx16 s0[2] = {scores32<DH, F16>(lds, qf), scores32<DH, F16>(lds + 32 * 2 * DH, qf)}, s1[2];
     for (int t = 0; t < n_steps; t += 2) {
