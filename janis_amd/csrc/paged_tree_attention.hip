@@ -589,6 +589,10 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void tree_attn_kernel(TreeA
         if (w.split && hk == 0 && threadIdx.x == 0) w.split[b].at.x = 0;
     }
     for (;;) {
+        // Thread 0's step at the loop's end is in LDS before the others read it. (The compiler leaves its own
+        // wait out at this barrier, with which the loop begins: without this one, in one call of 64 requests of
+        // 130 to 400, a wave went on from the place before and left wrong rows.)
+        wait_lds();
         __syncthreads();
         const Place at = s_walk.at;
         const struct {

@@ -327,6 +327,23 @@ def test_attention_many_requests(hip):
     assert np.array_equal(got, c.run(F32))
 
 
+@pytest.mark.parametrize("Hq,Hk,D,page,dt", [(8, 8, 64, 16, F16), (16, 8, 128, 16, BF16), (8, 4, 256, 32, BF16)])
+def test_attention_blocks_of_many_tiles(hip, Hq, Hk, D, page, dt):
+    """Blocks that walk several tiles of all kinds, over and over: the same bits each time."""
+    rng = np.random.default_rng(D)
+    lens = [(int(n), int(n + rng.integers(0, 600))) for n in rng.choice([1, 8, 20, 40, 64, 100], 128 if D < 256 else 64)]
+    c = Trees(hip, lens, Hq, Hk, D, page, dt, words=4, pad=1)
+    step(f"jh_paged_tree_attention blocks of many tiles R={len(lens)} rows={c.T} Hq={Hq} Hk={Hk} D={D}")
+    got = c.run(dt)
+    near(got, c.ref(dt, rng.integers(0, c.T - 1, 150)))
+    out = up(hip, np.zeros((c.T, Hq, D)), dt)
+    want = hip.Bytes(hip.PagedTreeAttention(c.Q, c.K, c.V, c.TAB, c.ST, c.KV, c.M, c.scale, maxNew=100, out=out))
+    assert np.array_equal(hip.Floats(out)[:-1], got[:-1])
+    for turn in range(60):
+        hip.PagedTreeAttention(c.Q, c.K, c.V, c.TAB, c.ST, c.KV, c.M, c.scale, maxNew=100, out=out)
+        assert hip.Bytes(out) == want, turn
+
+
 def test_attention_more_heads_than_blocks(hip):
     """A block to a kv head, which walks all tiles: nothing is cut, no workspace."""
     lens = [(9, 100), (0, 5), (33, 200), (1, 1)]
