@@ -107,6 +107,7 @@ static_assert(JH_PLAN_TABLE < kFine, "of several faults the least is reported");
 // What a request's rows come to.
 struct Walk {
     int4 head;       // as in heads
+    int rows;
     int kept, next;  // rows kept, and the choice after the last
     int same;        // kept rows that stay where they are, the first ones
 };
@@ -119,7 +120,7 @@ struct WalkRows {
 // By all threads of a block. A child comes after its parent, so the path goes up: from row i
 // on, the first row behind it whose parent is i and whose token the choice there, 64 rows to
 // a ballot.
-__device__ __forceinline__ Walk walk(const TreeCommitArgs& a, int r, WalkRows& s, bool write) {
+__device__ __forceinline__ Walk walk(const TreeCommitArgs& a, int r, WalkRows& s) {
     const int tid = threadIdx.x, lane = tid & 63;
     const int64_t limit = min((int64_t)a.max_blocks << a.page_shift, (int64_t)0x7fffffff);
     auto blocks = [&](int64_t kv) { return (int)((kv + (1 << a.page_shift) - 1) >> a.page_shift); };
@@ -128,12 +129,8 @@ __device__ __forceinline__ Walk walk(const TreeCommitArgs& a, int r, WalkRows& s
     const bool wrong = start < 0 || to < start || to > a.n_rows;
     const int n = wrong ? 0 : to - start;
     const int fault = kv < n || kv > limit ? JH_PLAN_LENGTHS : wrong ? JH_PLAN_ROWS : kFine;
-    if (fault != kFine || n == 0) return Walk{make_int4(fault, 0, 0, kv), 0, -1, 0};
-    if (n > a.tree_rows) {
-        if (write)
-            for (int i = tid; i < n; i += kWalkThreads) a.path[start + i] = start + i;
-        return Walk{make_int4(kFine, 0, 0, kv), n, a.chosen[(start + n - 1) * a.chosen_stride], n};
-    }
+    if (fault != kFine || n == 0) return Walk{make_int4(fault, 0, 0, kv), 0, 0, -1, 0};
+    if (n > a.tree_rows) return Walk{make_int4(kFine, 0, 0, kv), n, n, a.chosen[(start + n - 1) * a.chosen_stride], n};
     const int known = min(max(first, 1), n), b0 = blocks(kv - n + known), back = blocks(kv) - b0;
     constexpr int kEach = kTreeRows / kWalkThreads;
     int page[kEach];
@@ -174,10 +171,16 @@ __device__ __forceinline__ Walk walk(const TreeCommitArgs& a, int r, WalkRows& s
     for (int e = 0; e < kEach; e++) {
         const int i = e * kWalkThreads + tid;
         outside |= i >= b && i < back && (uint32_t)page[e] >= (uint32_t)a.n_pages;
-        if (write && i < n) a.path[start + i] = i < kept ? start + s.kept[i] : -1;
     }
     outside = __syncthreads_or(outside);
-    return Walk{make_int4(outside ? JH_PLAN_TABLE : kFine, back - b, kept - same, left), kept, s.end[1], same};
+    return Walk{make_int4(outside ? JH_PLAN_TABLE : kFine, back - b, kept - same, left), n, kept, s.end[1], same};
+}
+
+// The request's part of path, by all threads of a block.
+__device__ __forceinline__ void write_path(const TreeCommitArgs& a, int r, const Walk& w, const WalkRows& s) {
+    const int start = a.row_starts[r];
+    for (int i = threadIdx.x; i < w.rows; i += kWalkThreads)
+        a.path[start + i] = i >= w.kept ? -1 : start + (w.rows > a.tree_rows ? i : s.kept[i]);
 }
 
 // A block to a request.
@@ -185,7 +188,8 @@ __global__ __launch_bounds__(kWalkThreads) void tree_walk_kernel(TreeCommitArgs 
     __shared__ WalkRows s;
     const int r = blockIdx.x;
     if (r == 0 && threadIdx.x == 0) a.heads[a.n_req] = make_int4(*a.free_count, 0, 0, 0);
-    const Walk w = walk(a, r, s, true);
+    const Walk w = walk(a, r, s);
+    write_path(a, r, w, s);
     for (int i = threadIdx.x; i < w.head.z; i += kWalkThreads)
         a.moves[(int64_t)r * a.most + i] = make_int2(s.slot[s.kept[w.same + i]], s.slot[w.same + i]);
     if (threadIdx.x == 0) a.heads[r] = w.head, a.accepted[r] = w.kept, a.next_tokens[r] = w.next;
@@ -216,7 +220,7 @@ __global__ __launch_bounds__(kWalkThreads) void tree_commit_kernel(TreeCommitArg
     const bool books = m.first && blockIdx.y == 0;
     const int l1 = min(m.layers, ((int)blockIdx.y + 1) * m.each);
     Walk w;
-    if constexpr (ONE) w = walk(a, 0, s, books);
+    if constexpr (ONE) w = walk(a, 0, s);
     int4 mine = ONE ? w.head : R ? a.heads[r] : make_int4(kFine, 0, 0, 0);
     if (m.layers == 0) mine.z = 0;
     if (!books && mine.z == 0) return;
@@ -293,6 +297,9 @@ __global__ __launch_bounds__(kWalkThreads) void tree_commit_kernel(TreeCommitArg
         *a.status = status;
         *a.count_out = ok ? count + total : count;
     }
+    // (each row of path is written once: a refusal has nothing to take back)
+    if constexpr (ONE)
+        if (ok) write_path(a, 0, w, s);
     // rows that nobody has
     const int first = ok && R ? a.row_starts[0] : a.n_rows, last = ok && R ? a.row_starts[R] : a.n_rows;
     if (r == 0)

@@ -672,6 +672,33 @@ def test_commit_single_request_refused_on_the_device(hip, what, status, in_place
     same(c.got(hip), (c.kv, c.count, np.zeros(1), np.full(c.T, -1), np.full(1, -1), status, c.free, c.pools))
 
 
+@pytest.mark.parametrize("what,status", [("kv below the rows", 1), ("count below", 3), ("count past", 3)])
+@pytest.mark.parametrize("n,words,front", [(600, 1, 37), (90, 2, 100), (513, 16, 5)])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_commit_single_run_refused_on_the_device(hip, what, status, n, words, front, in_place):
+    """A request of more rows than bits, behind rows that nobody has: path is -1 everywhere."""
+    c = Step(n, [n], 16, words, 1, front=front, pad=70)
+    if what == "kv below the rows": c.kv[0] = n - 1
+    if what == "count below": c.count = -1
+    if what == "count past": c.count = c.n_pages + 1
+    c.up(hip)
+    if in_place:
+        c.out[0], c.out[1] = c.d["kv"], c.d["count"]
+    step(f"jh_paged_tree_commit of one run of {n} behind {front} rows refuses: {what}")
+    for _ in range(20):
+        c.call(hip)
+        same(c.got(hip), (c.kv, c.count, np.zeros(1), np.full(c.T, -1), np.full(1, -1), status, c.free, c.pools))
+
+
+@pytest.mark.parametrize("n,words,front", [(600, 1, 37), (90, 2, 100)])
+def test_commit_single_run(hip, n, words, front):
+    c = Step(n, [n], 16, words, 1, front=front, pad=70)
+    c.up(hip)
+    step(f"jh_paged_tree_commit of one run of {n} behind {front} rows")
+    c.call(hip)
+    same(c.got(hip), c.ref())
+
+
 def test_commit_captured_first():
     """The workspace cannot grow in a capture: the same call goes before it. Replays find
     other lengths, paths and pages."""
