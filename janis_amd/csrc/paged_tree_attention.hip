@@ -97,7 +97,7 @@ struct Place {
 };
 // The line's cuts: all a block keeps of it (in scalar registers).
 struct Cuts {
-    double each;   // cost of a piece
+    double each, total;  // cost of a piece, and of the line
     int pieces;
     // Where piece j (not the first behind the last) begins.
     __device__ __forceinline__ double at(int j) const { return floor(each * j); }
@@ -122,13 +122,13 @@ __device__ __forceinline__ Line line_of(const TreeAttn& w) {
     l.mine = 0.0;
     l.first = Request{0, 0, 0};
     float rows = 0.0f;
+#pragma unroll 4
     for (int e = 0; e < l.run; e++) {
         const int r = (threadIdx.x & 63) * l.run + e;
-        if (r >= a.n_req) break;
-        const Request q = request(a, r);
+        const Request q = request(a, min(r, a.n_req - 1));
         if (e == 0) l.first = q;
-        l.mine += shape_of(q, w.G).cost;
-        rows += (float)q.n;
+        l.mine += r < a.n_req ? shape_of(q, w.G).cost : 0.0;
+        rows += r < a.n_req ? (float)q.n : 0.0f;
     }
     const double upto = scan64(l.mine);
     l.before = upto - l.mine;
@@ -137,6 +137,7 @@ __device__ __forceinline__ Line line_of(const TreeAttn& w) {
     const double total = overlap ? 0.0 : lane_of(upto, 63);
     l.cuts.pieces = uniform(total > 0.0 ? max(1, (int)fmin((double)w.blocks, total / kLeastPiece)) : 0);
     l.cuts.each = uniform(total / max(1, l.cuts.pieces));
+    l.cuts.total = total;
     return l;
 }
 
@@ -170,18 +171,44 @@ __device__ __forceinline__ Place place_of(const TreeAttn& w, const Line& l, doub
     int r = at * l.run;
     Request q{__builtin_amdgcn_readlane(l.first.start, at), __builtin_amdgcn_readlane(l.first.n, at),
               __builtin_amdgcn_readlane(l.first.kv, at)};
-    Shape s = shape_of(q, w.G);
-    while (begin + s.cost <= x) {
-        begin += s.cost;
-        q = request(w.a, ++r);
-        s = shape_of(q, w.G);
+    // the lane's run, 64 requests side by side
+    for (int r0 = r; l.run > 1 && r0 < (at + 1) * l.run; r0 += 64) {
+        const int mine = r0 + (threadIdx.x & 63);
+        const Request of = request(w.a, min(mine, w.a.n_req - 1));
+        const double cost = mine < min((at + 1) * l.run, w.a.n_req) ? shape_of(of, w.G).cost : 0.0, upto = scan64(cost);
+        const uint64_t here = __ballot(begin + upto > x);
+        if (here) {
+            const int i = uniform(__ffsll((unsigned long long)here) - 1);
+            r = r0 + i, begin += lane_of(upto - cost, i);
+            q = Request{__builtin_amdgcn_readlane(of.start, i), __builtin_amdgcn_readlane(of.n, i), __builtin_amdgcn_readlane(of.kv, i)};
+            break;
+        }
+        begin += lane_of(upto, 63);
     }
+    const Shape s = shape_of(q, w.G);
     x -= begin;
     const int tiles = s.whole + s.rest_tiles, tile = tiles == 1 ? 0 : min(tiles - 1, (int)floor(x / s.tile));
     const Tile t = tile_of(s, tile);
     const int u = unit_at(w, x - t.at, s.units, t.rows);
     const bool next = u == s.units;
     return Place{uniform(r), uniform(next ? tile + 1 : tile), uniform(next ? 0 : u), uniform(begin), q};
+}
+
+// The first request behind r that has rows: lengths of 256 are requested together. (4 trees beside 252 idle slots
+// 31 us, beside 2044 45; one slot at a time took 125 and 805. Of the 31 9 are the join, whose blocks are
+// dealt out to as many tiles as requests could have.)
+__device__ __forceinline__ int next_with_rows(const PagedAttnArgs& a, int r) {
+    for (r++; r < a.n_req; r += 256) {
+        int n[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) n[i] = request(a, min(r + 64 * i + ((int)threadIdx.x & 63), a.n_req - 1)).n;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint64_t some = __ballot(n[i] > 0 && r + 64 * i + ((int)threadIdx.x & 63) < a.n_req);
+            if (some) return r + 64 * i + __ffsll((unsigned long long)some) - 1;
+        }
+    }
+    return a.n_req;
 }
 
 // A record holds results as the lanes have them: of 32 rows at a time and features 8 i .. + 7, the 4
@@ -603,9 +630,10 @@ __global__ __launch_bounds__(256, DH == 256 ? 1 : 2) void tree_attn_kernel(TreeA
         const Request q{uniform(at.q.start), uniform(at.q.n), uniform(at.q.kv)};
         const Shape s = shape_of(q, w.G);
         if (p.tile >= s.whole + s.rest_tiles) {
+            if (at.begin + s.cost >= s_walk.cuts.total) return;  // the line's end
+            const int r = uniform(next_with_rows(w.a, p.r));
             __syncthreads();
-            if (threadIdx.x == 0)
-                s_walk.at = Place{p.r + 1, 0, 0, at.begin + s.cost, p.r + 1 < w.a.n_req ? request(w.a, p.r + 1) : q};
+            if (threadIdx.x == 0) s_walk.at = Place{r, 0, 0, at.begin + s.cost, r < w.a.n_req ? request(w.a, r) : q};
             continue;
         }
         bool all;

@@ -344,6 +344,27 @@ def test_attention_blocks_of_many_tiles(hip, Hq, Hk, D, page, dt):
         assert hip.Bytes(out) == want, turn
 
 
+@pytest.mark.parametrize("where", ["behind", "between", "before", "around"])
+@pytest.mark.parametrize("idle", [1, 60, 252, 700, 2044])
+def test_attention_idle_slots(hip, where, idle):
+    """Requests without rows beside four with some change nothing: the line is the same, and its cuts."""
+    active = [(16, 700), (100, 1500), (3, 3000), (40, 200)]
+    c = Trees(hip, active, 16, 8, 64, 16, BF16, words=2)
+    want = c.run(F32)
+    near(want, c.ref(F32))
+    gaps = {"behind": [0, 0, 0, 0, idle], "between": [0, idle // 3, idle // 3, idle - 2 * (idle // 3), 0], "before": [idle, 0, 0, 0, 0],
+            "around": [idle // 2, 0, 1, 0, idle - idle // 2 - 1] if idle > 1 else [1, 0, 0, 0, 0]}[where]
+    starts, kv, tables = [0], [], []
+    for i, gap in enumerate(gaps):
+        for _ in range(gap):
+            starts.append(starts[-1]), kv.append(50), tables.append(np.full(c.tables.shape[1], -1, np.int32))
+        if i < 4:
+            starts.append(starts[-1] + active[i][0]), kv.append(active[i][1]), tables.append(c.tables[i])
+    c.ST, c.KV, c.TAB = ints(hip, starts), ints(hip, kv), ints(hip, np.array(tables))
+    step(f"jh_paged_tree_attention {idle} idle slots {where}")
+    assert np.array_equal(c.run(F32), want)
+
+
 def test_attention_more_heads_than_blocks(hip):
     """A block to a kv head, which walks all tiles: nothing is cut, no workspace."""
     lens = [(9, 100), (0, 5), (33, 200), (1, 1)]
