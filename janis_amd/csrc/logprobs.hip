@@ -562,11 +562,21 @@ Status launch_logprobs(const LogProbsArgs& a, void* workspace, int num_cus, int*
     Meeting w = meeting_of(a, num_cus);
     w.records = static_cast<char*>(workspace);
     if (w.parts > 1 && a.rows <= 8 * kLogProbsRows) w.arrivals = sync;
-    const int64_t rows = w.arrivals ? ((int64_t)a.rows + 7) / 8 * 8 : a.rows;
-    const dim3 grid((unsigned)(rows * w.parts));
+    // (a grid holds fewer than 2^32 threads; rows that are split are few)
+    constexpr int kMostRows = 1 << 23;
+    static_assert((int64_t)kMostRows * kThreads < ((int64_t)1 << 32), "rows of a launch");
     auto go = [&](auto f32, auto ent, auto top) {
-        hipLaunchKernelGGL((logprobs_kernel<decltype(f32)::value, decltype(ent)::value, decltype(top)::value>), grid,
-                           dim3(kThreads), 0, st, a, w);
+        for (int first = 0; first < a.rows; first += kMostRows) {
+            LogProbsArgs part = a;
+            part.rows = std::min(kMostRows, a.rows - first);
+            part.x = static_cast<const char*>(a.x) + first * a.stride * (a.f32 ? 4 : 2);
+            if (a.n_tokens) part.tokens += (int64_t)first * a.n_tokens, part.logprobs += (int64_t)first * a.n_tokens;
+            if (a.entropy) part.entropy += first;
+            if (a.top_k) part.top_ids += (int64_t)first * a.top_k, part.top_logprobs += (int64_t)first * a.top_k;
+            const int64_t rows = w.arrivals ? ((int64_t)part.rows + 7) / 8 * 8 : part.rows;
+            hipLaunchKernelGGL((logprobs_kernel<decltype(f32)::value, decltype(ent)::value, decltype(top)::value>),
+                               dim3((unsigned)(rows * w.parts)), dim3(kThreads), 0, st, part, w);
+        }
     };
     auto with = [&](auto f32, auto ent) { a.top_k ? go(f32, ent, std::true_type{}) : go(f32, ent, std::false_type{}); };
     auto typed = [&](auto f32) { a.entropy ? with(f32, std::true_type{}) : with(f32, std::false_type{}); };

@@ -282,6 +282,22 @@ def test_logprobs_far_rows(hip):
     X.free()
 
 
+@pytest.mark.parametrize("T", [(1 << 23) + 1, (1 << 24) - 1, 1 << 24])
+def test_logprobs_most_rows(hip, T):
+    """As many rows as there may be, in which 1009 rows come again and again."""
+    rng = np.random.default_rng(13)
+    x, t = some(rng, 1009, 5, BF16), rng.integers(0, 5, 1009).astype(np.int32)
+    want = ref(x, 1.0, t[:, None], 1)
+    at = np.arange(T) % 1009
+    X, tokens = up(hip, x[at], BF16), ints(hip, t[at])
+    step(f"jh_token_logprobs rows={T}")
+    lp, ent, ids, top = hip.TokenLogProbs(X, tokens, 1)
+    for got, w, bar in ((hip.Floats(lp), want[0][:, 0], want[1][:, 0]), (hip.Floats(ent), want[2], want[3]), (hip.Floats(top)[:, 0], want[5][:, 0], want[6][:, 0])):
+        assert (np.abs(got - w[at]) <= bar[at]).all()
+    assert np.array_equal(hip.Ints(ids)[:, 0], want[4][at, 0])
+    hip.Sync()
+
+
 def test_refusals(hip):
     INVALID, UNSUPPORTED = _lib.JH_ERR_INVALID, _lib.JH_ERR_UNSUPPORTED
     t = hip.empty(F32, 1 << 16)
