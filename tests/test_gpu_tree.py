@@ -209,6 +209,18 @@ def test_attention_joined(hip, lens, words, Hq, Hk, D, page, dt):
     assert np.array_equal(c.run(F32), c.run(F32))  # counters are left at zero, parts joined in order
 
 
+@pytest.mark.parametrize("Hq,Hk,D,page,dt", [(32, 8, 128, 16, BF16), (8, 8, 64, 64, F16), (24, 8, 128, 32, F16), (16, 8, 256, 16, BF16), (32, 4, 128, 16, F16)])
+def test_attention_joined_batch(hip, Hq, Hk, D, page, dt):
+    """A batch whose tiles are nearly all cut: parts in the workspace, joined by the second launch."""
+    c = Trees(hip, [(30, 900)] * 20, Hq, Hk, D, page, dt, words=1, pad=1)
+    tokens = np.random.default_rng(D).integers(0, 600, 90)
+    for out_dt in (dt, F32):
+        step(f"jh_paged_tree_attention 20 x 30 of 900 Hq={Hq} Hk={Hk} D={D} page={page} dt={dt} out={out_dt}")
+        got = c.run(out_dt)
+        near(got, c.ref(out_dt, tokens))
+        assert np.array_equal(got, c.run(out_dt))
+
+
 def test_attention_causal_masks_are_paged_attention(hip):
     """A chain's mask gives the results of jh_paged_attention (keys may be split elsewhere)."""
     for lens, Hq, Hk, D in (([(7, 900), (1, 60)], 32, 8, 128), ([(64, 900), (33, 40)], 8, 2, 128), ([(100, 100)], 4, 4, 64), ([(40, 300)], 4, 2, 256)):
