@@ -10,7 +10,7 @@
 // equal ones the lower token), so that all keys differ and the k largest are one set in
 // one order. The k-th largest of 64 groups' running maxima is a bound that a handful of the
 // logits read so far pass (64 ln (64 / (64 - k)) of random ones): it is made at chunks 0,
-// 1, 2, 4, 8 .. of a block's part of the row, and what passes it goes to a list in LDS,
+// 2, 4, 8 .. of a block's part of the row, and what passes it goes to a list in LDS,
 // which is sorted by counting at the end. A list that runs full (thousands of equal logits,
 // or rising ones) is made again from the lanes' largest keys.
 //

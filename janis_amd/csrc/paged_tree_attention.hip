@@ -8,21 +8,29 @@
 // over caches of very different lengths, which is too few tiles to fill the GPU and too
 // unequal to deal them out. So the work is dealt out instead: all tiles of a kv head, each
 // its 64-key units times what a unit of its kind costs, stand in one line, which is cut into
-// as many equal pieces as blocks are resident. A block finds its piece by running sums over
+// as many pieces of equal cost as blocks are resident. A block finds its piece by running sums over
 // the requests and walks it: the end of one tile, whole ones, the beginning of another. A
 // tile that is cut leaves parts, which a launch that follows joins in their order (joined by
 // the part that arrives last, the largest tiles, of 128 rows in 30 parts, held one block for
 // 170 us, and the launch is 4 to 20). A cut near a tile's end is moved there.
 //
+// Equal cost is not equal time: of the blocks of 63 tokens over 30000 keys, whose pieces are
+// alike, the fastest took 37 us, half of them 47 and the slowest 55; of those of 64 requests 105, 156 and
+// 190. And all tiles of a run (n > 32 * mask_words) are charged all of its keys, though an early
+// one ends at its rows' own: 2000 tokens of 2000 87 us, jh_paged_attention 70; of 8000 327 and 313.
+//
 // What bounds it, bf16, 32 heads on 8 of 128 (MI355X):
-//   16 tokens of 700 keys    15 us: round trips (lengths, the line, tables, keys, records), 11
+//   16 tokens of 700 keys    14.5 us: round trips (lengths, the line, tables, keys, records), 11
 //     of them the parts and 4 the launch that joins
-//   63 of 30000              66 us: 58 the parts, 8 the join; MFMA, two thirds of it the second
-//     product made twice, at a clock that the power holds to 1.8 GHz
-//   64 requests of 20 to 60 over 100 to 8000 212 us: 185 the parts (413 TFLOP/s of the formula's
-//     operations in all, tiles that are not full not counted), 19 the join, records to memory
-//     and back. The clock is 1.8 GHz of 2.4, by power, and the matrix pipes busy half of it
-//   tiles of 32 rows alone   HBM: 64 requests of 8 tokens over 4000 keys 169 us, 6.2 TB/s
+//   63 of 30000              66 to 73 us, by device: 58 the parts, 8 the join; MFMA, two thirds of it
+//     the second product made twice, at a clock that the power holds to 1.8 GHz
+//   64 requests of 20 to 60 over 100 to 8000 208 to 220 us, by device (413 TFLOP/s of the formula's
+//     operations in all, tiles that are not full not counted): 19 to 22 the join, records to memory
+//     and back, the rest the parts (182 at the least, more under a profiler). The clock is 1.8 GHz of
+//     2.4, by power, and the matrix pipes busy half of it
+//   tiles of 32 rows alone   HBM: 64 requests of 8 tokens over 4000 keys 173 us, 6.1 TB/s
+// head_dim 64 and 256: 16 requests of 32 tokens over 4000 keys 49 and 148 us (128: 78), 63 tokens over
+// 30000 45 and 123 us (65).
 #include "paged_attention.hpp"
 
 namespace jh {
@@ -39,8 +47,8 @@ struct TreeAttn {
     float* part;      // records: [blocks] of the tiles that go on in a block, [blocks] of those that begin there
 };
 // Cost of a unit of 64 keys, by the tile's rows: with all blocks at work one takes 2.7, 3.1, 3.6 and
-// 4.0 us for tiles of 32, 64, 96 and 128 rows (bf16, head_dim 128). And of a tile (its queries, its
-// results): 4 to 8 us.
+// 4.0 us for tiles of 32, 64, 96 and 128 rows (bf16, head_dim 128; used for f16, 64 and 256 too, where it
+// was not taken apart). And of a tile (its queries, its results): 4 to 8 us.
 __device__ __forceinline__ int cost_of(int rows) { return 4 + (rows + 31) / 32; }
 constexpr int kCostTile = 12;
 // The least cost of a piece, below which a block costs more to begin than it saves: 16 tokens over

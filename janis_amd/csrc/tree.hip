@@ -97,7 +97,7 @@ __global__ __launch_bounds__(64) void tree_plan_kernel(TreePlanArgs a) {
 // and values). With the walk and the books in one workgroup, and path and slots looked up
 // by every block that moves, 64 requests of 8 to 32 rows in 36 layers took 33 us; so, 14.
 // A single request that is not updated in place needs no more than itself: there every
-// block of one launch finds the path (16 rows in 36 layers 7.1 us, with two launches 9.5).
+// block of one launch finds the path (16 rows in 36 layers 6.7 us, with two launches 8.8).
 //
 // heads: per request {what is wrong with it or kFine, pages that come back, rows that move,
 // its length}, behind them {*free_count}. moves: [request][most rows of a tree] of slots.
