@@ -243,6 +243,34 @@ def test_logprobs_graphs_and_growth():
     b.Close()
 
 
+def test_logprobs_captured_first():
+    """Rows that are split need a workspace, which cannot grow in a capture: the call says so, and works
+    after one outside."""
+    b = HipBackend(0)
+    x = some(np.random.default_rng(14), 3, 50021, F32)
+    X = up(b, x, F32)
+    out = (None, up(b, np.zeros(3), F32), ints(b, np.zeros((3, 4))), up(b, np.zeros((3, 4)), F32))
+    call = lambda: b.TokenLogProbs(X, topK=4, out=out)  # noqa: E731
+    step("jh_token_logprobs captured first")
+
+    def refused_call():
+        with pytest.raises(JanisHipError, match="make the same call once before") as e:
+            call()
+        assert e.value.code == _lib.JH_ERR_INVALID
+    Graph(b, refused_call).close()
+    call()
+    graph = Graph(b, call)
+    want = ref(x, 1.0, None, 4)
+    for _ in range(3):
+        put(b, out[1], np.zeros(3, np.float32)), put(b, out[2], np.zeros((3, 4), np.int32))
+        graph.replay()
+        close(b.Floats(out[1]), want[2], want[3], "entropy")
+        assert np.array_equal(b.Ints(out[2]), want[4])
+        call()
+    graph.close()
+    b.Close()
+
+
 def test_logprobs_two_contexts_and_streams():
     import torch
 
